@@ -377,6 +377,183 @@ sage_status sage_forward_noalloc(const sage_attention* s, const sage_shape* shap
                                  const sage_tensor* q, const sage_tensor* k, const sage_tensor* v,
                                  const sage_tensor_mut* out, const sage_options* opts);
 
+/* ---- Positions along a sequence, a paged 4-bit key/value cache, and the attention over it ----
+ * No counterpart in the reference: what a program that answers token by token
+ * needs beside the attention of whole prompts. Every call enqueues on the
+ * context's stream, allocates nothing and does not synchronise, so it may be
+ * captured into a graph; lengths, starts, positions and the page table are
+ * read on the device when the work runs, so a captured step serves every step
+ * of its shape. The device of the context has to be the current one.
+ *
+ * Rotary positions: the rot / 2 pairs of a head's first rot channels (any even
+ * rot up to the head dim; the other channels pass) turn by an angle that the
+ * row's position and the pair give. HALF pairs channels (i, i + rot / 2),
+ * PAIRS (2 i, 2 i + 1). */
+typedef enum sage_rotary_layout { SAGE_ROTARY_HALF = 0, SAGE_ROTARY_PAIRS = 1 } sage_rotary_layout;
+
+/* Scaling for contexts longer than the model was trained on (`original`
+ * positions), by `factor` >= 1. With w_i = base^(-2 i / rot):
+ *   NONE    w_i
+ *   LINEAR  w_i / factor
+ *   NTK     base * factor^(rot / (rot - 2)) for the base (rot > 2)
+ *   YARN    g_i w_i + (1 - g_i) w_i / factor, where g_i rises from 0 at
+ *           beta_slow turns of the pair over `original` positions to 1 at
+ *           beta_fast turns (0 for either: 1 and 32).
+ * attention multiplies cos and sin; 0: 0.1 ln(factor) + 1 under YARN, else 1. */
+typedef enum sage_rotary_scaling_kind {
+    SAGE_ROTARY_NONE = 0,
+    SAGE_ROTARY_LINEAR = 1,
+    SAGE_ROTARY_NTK = 2,
+    SAGE_ROTARY_YARN = 3
+} sage_rotary_scaling_kind;
+typedef struct sage_rotary_scaling {
+    int32_t kind;
+    double factor;
+    double original;
+    double beta_fast;
+    double beta_slow;
+    double attention;
+} sage_rotary_scaling;
+
+/* Host only: cos and sin of position * w_i for `positions` positions, [positions][rot / 2][2]
+ * floats (computed in f64, rounded to f32) into `out`, which holds out_len floats.
+ * scaling == NULL is NONE. */
+sage_status sage_rotary_table(uint64_t rot, uint64_t positions, double base, const sage_rotary_scaling* scaling,
+                              float* out, uint64_t out_len);
+
+/* table: device floats, [table_len / rot][rot / 2][2], 16-byte aligned.
+ * positions: device int32 of each row, or NULL: the token's index
+ * (sage_rotary_apply), the token's slot (sage_cache_append). The rotated
+ * channels of a row whose position the table does not hold become NaN. */
+typedef struct sage_rotary {
+    const float* table;
+    uint64_t table_len;
+    uint64_t rot;
+    int32_t layout; /* sage_rotary_layout */
+    const int32_t* positions;
+    uint64_t positions_len;
+} sage_rotary;
+
+/* x rotated into out, [batch][token][head][head_dim] views of shape's batch,
+ * tokens and heads (kv_heads is not read), both of one type; positions holds
+ * batch * tokens entries. Each product and sum is rounded in fp32, the result
+ * once to the type. transpose != 0 turns the other way: the gradient of the
+ * rotation (its transpose, any attention factor included). out may be x itself
+ * (one address and strides) where no two rows of it share an element, else the
+ * two share no element. An empty shape is a no-op. */
+sage_status sage_rotary_apply(const sage_attention* s, const sage_shape* shape, const sage_rotary* rotary,
+                              const sage_tensor* x, const sage_tensor_mut* out, int32_t transpose);
+
+/* A batch of sequences over a pool of pages.
+ *   batch        sequences (at most 65535)
+ *   rows         rows of the packed q, k, v and out: the new tokens of all
+ *                sequences, one sequence behind the other, and any padding
+ *                behind the last
+ *   max_new      most rows of one sequence (sage_cache_attend leaves a sequence's
+ *                rows past it as they are; the other calls do not read it)
+ *   heads        query heads, a multiple of kv_heads
+ *   pages        pages of the pool
+ *   page_tokens  tokens a page: 16, 32, 64, 128 or 256
+ *   max_pages    columns of the page table; max_pages * page_tokens bounds a
+ *                sequence's length (at most 2^30) */
+typedef struct sage_cache_shape {
+    uint64_t batch;
+    uint64_t rows;
+    uint64_t max_new;
+    uint64_t heads;
+    uint64_t kv_heads;
+    uint64_t pages;
+    uint64_t page_tokens;
+    uint64_t max_pages;
+} sage_cache_shape;
+
+/* The pool, in the caller's device memory (16-byte aligned):
+ *   k_codes, v_codes    [pages][kv_heads][page_tokens][D / 2]: E2M1 codes (sign, two
+ *                       bits of exponent, one of mantissa: 0 .5 1 1.5 2 3 4 6), two a
+ *                       byte, the even channel low
+ *   k_scales, v_scales  [pages][kv_heads][page_tokens][D / 32]: the E8M0 scale of
+ *                       each 32 channels, 2^(byte - 127); 255: the block is NaN
+ * codes_len, scales_len: the bytes that each buffer holds. */
+typedef struct sage_cache {
+    uint8_t* k_codes;
+    uint8_t* k_scales;
+    uint8_t* v_codes;
+    uint8_t* v_scales;
+    uint64_t codes_len;
+    uint64_t scales_len;
+} sage_cache;
+
+/* Device int32 arrays: starts [batch + 1], nondecreasing, the first row of each
+ * sequence and the end of the last; lengths [batch], each sequence's tokens in
+ * the cache, this step's included; page_table [batch][max_pages]. A sequence
+ * of length L with n rows has them at slots L - n .. L - 1 (slot t: token
+ * t % page_tokens of page page_table[b][t / page_tokens]). Rows outside
+ * starts[0] .. starts[batch] are left as they are. Slots before 0 or past the
+ * page table, and pages that the pool does not have, hold nothing: nothing is
+ * written there, and their tokens are not attended to. */
+typedef struct sage_cache_index {
+    const int32_t* starts;
+    uint64_t starts_len;
+    const int32_t* lengths;
+    uint64_t lengths_len;
+    const int32_t* page_table;
+    uint64_t page_table_len;
+} sage_cache_index;
+
+/* Bytes of a pool's codes and scales (each, for K and for V). Host only. */
+sage_status sage_cache_sizes(const sage_cache_shape* shape, uint64_t head_dim, uint64_t* codes, uint64_t* scales);
+
+/* Writes the rows' keys and values to their slots. Under `rotary` (NULL:
+ * none) the keys turn first and are rounded to their 16-bit type, as
+ * sage_rotary_apply does, so that the two ways give the same codes. Each 32
+ * channels take the least scale 2^e, -126 <= e <= 126, with max |x| <= 6 * 2^e,
+ * and the codes nearest x / 2^e (ties to the even code); a block with an
+ * infinity or a NaN becomes NaN. q and q_out (both or neither): the step's
+ * queries, turned as the keys are, in the same launch (rotary required). k, v,
+ * q and q_out are views of [row][head][head_dim] (strides.batch is not read)
+ * of one type; q_out may be q itself, as in sage_rotary_apply. Two sequences
+ * of one call that write the same slot race. */
+sage_status sage_cache_append(const sage_attention* s, const sage_cache_shape* shape, const sage_cache* cache,
+                              const sage_cache_index* index, const sage_tensor* k, const sage_tensor* v,
+                              const sage_rotary* rotary, const sage_tensor* q, const sage_tensor_mut* q_out);
+
+/* The rows' keys and values back from their slots as 16-bit values (rounded
+ * once; fp16 overflows to infinity), zeros where a slot holds nothing: starts
+ * and lengths that cover whole sequences give the K and V that sage_forward
+ * takes. k and v are views of [row][head][head_dim] (strides.batch is not
+ * read), bf16 or fp16, of one type. */
+sage_status sage_cache_read(const sage_attention* s, const sage_cache_shape* shape, const sage_cache* cache,
+                            const sage_cache_index* index, const sage_tensor_mut* k, const sage_tensor_mut* v);
+
+/* What sage_cache_attend keeps between its kernels where a sequence's keys
+ * are split over workgroups. One call at a time may use it: order the calls
+ * (and graph replays) that share one on one stream. */
+typedef struct sage_cache_workspace sage_cache_workspace;
+sage_status sage_cache_workspace_new(const sage_attention* s, const sage_cache_shape* shape,
+                                     sage_cache_workspace** out);
+void sage_cache_workspace_destroy(sage_cache_workspace* ws);
+uint64_t sage_cache_workspace_bytes(const sage_cache_workspace* ws);
+
+/* has_softmax_scale = 0 means the default 1/sqrt(head_dim). */
+typedef struct sage_cache_options {
+    float softmax_scale;
+    int32_t has_softmax_scale;
+    int32_t causal;
+} sage_cache_options;
+
+/* Attention of the rows' queries over their sequence's cached keys: row i of a
+ * sequence's n rows sees the slots below its length, under `causal` up to its
+ * own, length - n + i (not causal: an encoder's states). q and out are views
+ * of [row][head][head_dim] (strides.batch is not read), bf16 or fp16, each its
+ * own type; out may be q itself (one address and strides, the same 16-bit
+ * size) where no two rows of it share an element, else the two share none.
+ * A row that sees nothing becomes zeros. The shape is the workspace's.
+ * Logits, softmax statistics and sums are fp32; cached values are exact, and
+ * the probabilities are rounded to bf16 for the second product. */
+sage_status sage_cache_attend(const sage_attention* s, const sage_cache_workspace* ws, const sage_cache* cache,
+                              const sage_cache_index* index, const sage_tensor* q, const sage_tensor_mut* out,
+                              const sage_cache_options* opts);
+
 /* Byte position of key k (0..63) of a 64-key block inside each channel row
  * of the v8 layout (the CDNA4 counterpart of sg_vpos, sage_common.cu:151-155):
  * the order in which the QK^T accumulator of the 32x32 MFMA hands keys to the

@@ -5,9 +5,9 @@
 Compiles every source under csrc/ with hipcc for gfx950 and links
 spl_sage/libsage_hip.so next to the Python mirror of the API. Objects go to
 _build/ (git-ignored). Packed FP32 instructions are disabled for all device
-code; the prologue is compiled with -ffp-contract=off so its fp32 arithmetic
-is exactly the written operation order, and the attention source twice
-(see UNITS).
+code; the prologue and the rotary and cache writes are compiled with
+-ffp-contract=off so their fp32 arithmetic is exactly the written operation
+order, and the attention source twice (see UNITS).
 """
 from __future__ import annotations
 
@@ -50,7 +50,10 @@ UNITS = [
     ("sage_attn_keys.hip", "sage_attn_keys.hip.o", []),
     ("sage_peak.hip", "sage_peak.hip.o", []),
     ("sage_noalloc.hip", "sage_noalloc.hip.o", []),
+    ("sage_cache.hip", "sage_cache.hip.o", ["-ffp-contract=off"]),
+    ("sage_cache_attn.hip", "sage_cache_attn.hip.o", []),
     ("sage_api.cpp", "sage_api.cpp.o", []),
+    ("sage_cache_api.cpp", "sage_cache_api.cpp.o", []),
 ]
 
 

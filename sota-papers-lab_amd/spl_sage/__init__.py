@@ -533,6 +533,38 @@ class SageAttention:
         _check(lib().sage_forward_noalloc(self._h, C.byref(shape._c()), C.byref(merge._c()), C.byref(q._c()),
                                           C.byref(k._c()), C.byref(v._c()), C.byref(out._c()), C.byref(o)))
 
+    def rotary(self, shape: Shape, rotary, x: Tensor, out: TensorMut, transpose: bool = False) -> None:
+        """x's heads turned by their rows' positions into out (spl_sage.rotary)."""
+        _check(lib().sage_rotary_apply(self._h, C.byref(shape._c()), C.byref(rotary._c()), C.byref(x._c()),
+                                       C.byref(out._c()), int(transpose)))
+
+    def cache_workspace(self, shape):
+        """The workspace of cache_attend for one CacheShape (spl_sage.cache)."""
+        from . import cache
+
+        return cache.CacheWorkspace(self, shape)
+
+    def cache_append(self, cache, index, k: Tensor, v: Tensor, rotary=None, q: Optional[Tensor] = None,
+                     q_out: Optional[TensorMut] = None) -> None:
+        """The step's keys (rotated) and values written to their slots of the
+        cache, and its queries rotated into q_out in the same launch."""
+        opt = lambda x: None if x is None else C.byref(x._c())  # noqa: E731
+        _check(lib().sage_cache_append(self._h, C.byref(cache.shape._c()), C.byref(cache._c()), C.byref(index._c()),
+                                       C.byref(k._c()), C.byref(v._c()), opt(rotary), opt(q), opt(q_out)))
+
+    def cache_read(self, cache, index, k: TensorMut, v: TensorMut) -> None:
+        """Cached rows back as 16-bit keys and values."""
+        _check(lib().sage_cache_read(self._h, C.byref(cache.shape._c()), C.byref(cache._c()), C.byref(index._c()),
+                                     C.byref(k._c()), C.byref(v._c())))
+
+    def cache_attend(self, ws, cache, index, q: Tensor, out: TensorMut, softmax_scale: Optional[float] = None,
+                     causal: bool = True) -> None:
+        """Attention of the rows' queries over the cached keys of their sequences."""
+        o = _abi.sage_cache_options(0.0 if softmax_scale is None else float(softmax_scale),
+                                    0 if softmax_scale is None else 1, int(causal))
+        _check(lib().sage_cache_attend(self._h, ws._h, C.byref(cache._c()), C.byref(index._c()), C.byref(q._c()),
+                                       C.byref(out._c()), C.byref(o)))
+
     def peak(self, which: int, iters: int = 2048) -> float:
         """Measured dense TOPS of one MFMA shape (0 INT8, 1 FP8, 2 BF16)."""
         t = C.c_double()

@@ -99,6 +99,45 @@ class sage_qkv_rope(C.Structure):
     _fields_ = [("table", C.c_void_p), ("table_len", u64), ("layout", i32), ("frame_len", u64)]
 
 
+class sage_rotary_scaling(C.Structure):
+    _fields_ = [
+        ("kind", i32), ("factor", C.c_double), ("original", C.c_double), ("beta_fast", C.c_double),
+        ("beta_slow", C.c_double), ("attention", C.c_double),
+    ]
+
+
+class sage_rotary(C.Structure):
+    _fields_ = [
+        ("table", C.c_void_p), ("table_len", u64), ("rot", u64), ("layout", i32), ("positions", C.c_void_p),
+        ("positions_len", u64),
+    ]
+
+
+class sage_cache_shape(C.Structure):
+    _fields_ = [
+        ("batch", u64), ("rows", u64), ("max_new", u64), ("heads", u64), ("kv_heads", u64), ("pages", u64),
+        ("page_tokens", u64), ("max_pages", u64),
+    ]
+
+
+class sage_cache(C.Structure):
+    _fields_ = [
+        ("k_codes", C.c_void_p), ("k_scales", C.c_void_p), ("v_codes", C.c_void_p), ("v_scales", C.c_void_p),
+        ("codes_len", u64), ("scales_len", u64),
+    ]
+
+
+class sage_cache_index(C.Structure):
+    _fields_ = [
+        ("starts", C.c_void_p), ("starts_len", u64), ("lengths", C.c_void_p), ("lengths_len", u64),
+        ("page_table", C.c_void_p), ("page_table_len", u64),
+    ]
+
+
+class sage_cache_options(C.Structure):
+    _fields_ = [("softmax_scale", C.c_float), ("has_softmax_scale", i32), ("causal", i32)]
+
+
 P = C.POINTER
 # name -> (restype, argtypes); every symbol include/sage_hip.h declares.
 SIGNATURES = {
@@ -146,6 +185,28 @@ SIGNATURES = {
         i32,
         [C.c_void_p, C.c_void_p, P(sage_qkv_in), P(sage_qkv_norm), P(sage_qkv_rope), P(sage_tensor_mut),
          P(sage_options)],
+    ),
+    "sage_rotary_table": (i32, [u64, u64, C.c_double, P(sage_rotary_scaling), C.c_void_p, u64]),
+    "sage_rotary_apply": (
+        i32, [C.c_void_p, P(sage_shape), P(sage_rotary), P(sage_tensor), P(sage_tensor_mut), i32],
+    ),
+    "sage_cache_sizes": (i32, [P(sage_cache_shape), u64, P(u64), P(u64)]),
+    "sage_cache_append": (
+        i32,
+        [C.c_void_p, P(sage_cache_shape), P(sage_cache), P(sage_cache_index), P(sage_tensor), P(sage_tensor),
+         P(sage_rotary), P(sage_tensor), P(sage_tensor_mut)],
+    ),
+    "sage_cache_read": (
+        i32,
+        [C.c_void_p, P(sage_cache_shape), P(sage_cache), P(sage_cache_index), P(sage_tensor_mut), P(sage_tensor_mut)],
+    ),
+    "sage_cache_workspace_new": (i32, [C.c_void_p, P(sage_cache_shape), P(C.c_void_p)]),
+    "sage_cache_workspace_destroy": (None, [C.c_void_p]),
+    "sage_cache_workspace_bytes": (u64, [C.c_void_p]),
+    "sage_cache_attend": (
+        i32,
+        [C.c_void_p, C.c_void_p, P(sage_cache), P(sage_cache_index), P(sage_tensor), P(sage_tensor_mut),
+         P(sage_cache_options)],
     ),
     "sage_v8_position": (i32, [i32]),
     "sage_peak": (i32, [C.c_void_p, i32, i32, P(C.c_double)]),

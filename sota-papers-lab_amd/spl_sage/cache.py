@@ -1,0 +1,120 @@
+"""spl_sage.cache -- a paged 4-bit key/value cache and the attention over it.
+
+The types of SageAttention.cache_append, cache_read, cache_workspace and
+cache_attend (sage_cache_* in include/sage_hip.h; no counterpart in the
+reference). Q, K, V and outputs are [1][row][head][head_dim] views (Tensor,
+TensorMut): the sequences' rows packed one behind the other. Device buffers are
+torch tensors.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from dataclasses import dataclass
+
+from . import SageError, _abi, _check
+from ._abi import lib
+from .rotary import _ints
+
+BLOCK = 32  # channels a scale
+
+
+@dataclass(frozen=True)
+class CacheShape:
+    """sage_cache_shape: sequences, packed rows, most rows of a sequence, query
+    and KV heads, pages of the pool, tokens a page, columns of the page table."""
+
+    batch: int
+    rows: int
+    max_new: int
+    heads: int
+    kv_heads: int
+    pages: int
+    page_tokens: int
+    max_pages: int
+
+    def _c(self) -> _abi.sage_cache_shape:
+        return _abi.sage_cache_shape(self.batch, self.rows, self.max_new, self.heads, self.kv_heads, self.pages,
+                                     self.page_tokens, self.max_pages)
+
+    def sizes(self, head_dim: int) -> tuple:
+        """Bytes of the codes and of the scales, each for K and for V."""
+        codes, scales = C.c_uint64(), C.c_uint64()
+        _check(lib().sage_cache_sizes(C.byref(self._c()), head_dim, C.byref(codes), C.byref(scales)))
+        return codes.value, scales.value
+
+
+def _bytes(t, what: str) -> tuple:
+    import torch
+
+    if t.dtype != torch.uint8 or not t.is_contiguous():
+        raise SageError(1, f"{what} must be a contiguous uint8 device tensor, got {t.dtype}")
+    return t.data_ptr(), t.numel()
+
+
+@dataclass
+class PagedCache:
+    """The pool: uint8 device tensors [pages][kv_heads][page_tokens][head_dim/2]
+    (codes) and [..][head_dim/32] (scales). One pool serves steps of any shape
+    with its pages, page_tokens and kv_heads (with_shape)."""
+
+    shape: CacheShape
+    k_codes: object
+    k_scales: object
+    v_codes: object
+    v_scales: object
+
+    @staticmethod
+    def new(shape: CacheShape, head_dim: int, device="cuda") -> "PagedCache":
+        """A pool of zeros."""
+        import torch
+
+        shape.sizes(head_dim)  # its refusals
+        dims = (shape.pages, shape.kv_heads, shape.page_tokens)
+        z = lambda n: torch.zeros(*dims, n, dtype=torch.uint8, device=device)  # noqa: E731
+        return PagedCache(shape, z(head_dim // 2), z(head_dim // BLOCK), z(head_dim // 2), z(head_dim // BLOCK))
+
+    def with_shape(self, shape: CacheShape) -> "PagedCache":
+        return PagedCache(shape, self.k_codes, self.k_scales, self.v_codes, self.v_scales)
+
+    def _c(self) -> _abi.sage_cache:
+        kc, ks = _bytes(self.k_codes, "cache K codes"), _bytes(self.k_scales, "cache K scales")
+        vc, vs = _bytes(self.v_codes, "cache V codes"), _bytes(self.v_scales, "cache V scales")
+        return _abi.sage_cache(kc[0], ks[0], vc[0], vs[0], min(kc[1], vc[1]), min(ks[1], vs[1]))
+
+
+@dataclass
+class CacheIndex:
+    """int32 device tensors: starts [batch + 1], lengths [batch] (this step's
+    rows included), page_table [batch][max_pages]."""
+
+    starts: object
+    lengths: object
+    page_table: object
+
+    def _c(self) -> _abi.sage_cache_index:
+        return _abi.sage_cache_index(*_ints(self.starts, "cache starts"), *_ints(self.lengths, "cache lengths"),
+                                     *_ints(self.page_table, "cache page table"))
+
+
+class CacheWorkspace:
+    """What cache_attend keeps between its kernels, for one shape; one call at a time uses it."""
+
+    def __init__(self, sa, shape: CacheShape):
+        h = C.c_void_p()
+        _check(lib().sage_cache_workspace_new(sa._h, C.byref(shape._c()), C.byref(h)))
+        self._h = h.value
+        self.shape = shape
+        # Bound now: at interpreter exit the module's globals may be gone before __del__ runs.
+        self._destroy = lib().sage_cache_workspace_destroy
+
+    def __del__(self):
+        h, self._h = getattr(self, "_h", None), None
+        destroy = getattr(self, "_destroy", None)
+        if h and destroy is not None:
+            destroy(h)
+
+    def bytes(self) -> int:
+        return lib().sage_cache_workspace_bytes(self._h)
+
+
+__all__ = ["BLOCK", "CacheShape", "PagedCache", "CacheIndex", "CacheWorkspace"]
