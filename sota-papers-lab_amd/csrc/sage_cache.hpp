@@ -60,7 +60,8 @@ struct CacheAttnArgs {
     CacheDev c;
     float* part_o;
     float* part_ml;
-    float qk_mul;  // softmax scale * log2(e)
+    float qk_mul;     // |softmax scale| * log2(e), over 0
+    uint32_t q_sign;  // 0x80008000 under a negative scale: the queries' signs
     int heads, group, max_new, causal, q_f16, out_f16;
     int splits;  // workgroups that a sequence's keys are split over, at most
 };

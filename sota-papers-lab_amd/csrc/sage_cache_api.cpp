@@ -347,7 +347,11 @@ sage_status sage_cache_attend(const sage_attention* s, const sage_cache_workspac
     a.q_f16 = q->dtype == SAGE_F16;
     a.out_f16 = out->dtype == SAGE_F16;
     const float scale = opts->has_softmax_scale ? opts->softmax_scale : (float)(1.0 / std::sqrt((double)d));
-    a.qk_mul = scale * 1.44269504088896340736f;
+    // A scale of 0 becomes the least normal float: every weight is 1 still, and
+    // the -infinity of a masked logit stays what it is.
+    a.qk_mul = std::max(std::fabs(scale) * 1.44269504088896340736f, 1.17549435e-38f);
+    if (scale != scale) a.qk_mul = scale;
+    a.q_sign = std::signbit(scale) ? 0x80008000u : 0u;
     a.splits = ws->splits;
     a.part_o = static_cast<float*>(ws->buf);
     a.part_ml = a.part_o + (uint64_t)ws->splits * h.rows * h.heads * d;

@@ -17,6 +17,9 @@
 // K Q^T gives each lane one column and four tokens of each 16-token tile, and
 // those four are the order in which O^T = V^T P^T takes its tokens, so P goes
 // from one MFMA to the next without leaving the lane's registers.
+#include <algorithm>
+#include <type_traits>
+
 #include "sage_cache.hpp"
 
 namespace sage {
@@ -30,6 +33,10 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr int COLS = 16;    // columns of a workgroup
 constexpr int TOKENS = 64;  // tokens of a wave's step
+constexpr int MAX_SPLITS = 256;
+// The reference m of the softmax follows the maximum only where that is 2^8
+// past it: the fp32 sums have room for that, and rescaling them becomes rare.
+constexpr float SLACK = 8.0f;
 constexpr float NEG_INF = -__builtin_inff();
 
 __device__ __forceinline__ uint32_t cvt2(uint32_t codes, float s, int which) {
@@ -46,6 +53,13 @@ __device__ __forceinline__ uint32_t cvt2(uint32_t codes, float s, int which) {
 // Eight channels of one code dword.
 __device__ __forceinline__ uint4 decode8(uint32_t codes, float s) {
     return make_uint4(cvt2(codes, s, 0), cvt2(codes, s, 1), cvt2(codes, s, 2), cvt2(codes, s, 3));
+}
+
+// Eight channels of a query, negated under a negative softmax scale (so that
+// the greatest logit is the greatest product).
+__device__ __forceinline__ uint4 load_q(const uint16_t* p, uint32_t sign) {
+    const uint4 x = *reinterpret_cast<const uint4*>(p);
+    return make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign);
 }
 
 // Maximum and sum over the four lanes of a column (lanes 16 apart).
@@ -75,6 +89,15 @@ __device__ __forceinline__ int split_tokens(int len, int splits) {
     return ((len + splits - 1) / splits + step - 1) / step * step;
 }
 
+// Byte of 16-channel unit u of a token's bf16 V row in LDS. The units of a row
+// are permuted by the token, so that what a transposing read takes at once
+// meets all banks: eight tokens of one unit (16x16), four of two (32x32).
+template <int D>
+__device__ __forceinline__ int unit_at(int tok, int u) {
+    const int f = D == 128 ? (tok & 3) << 1 | (tok >> 2 & 1) : (tok & 2) | (tok >> 2 & 1);
+    return tok * (D * 2) + ((u ^ f) << 5);
+}
+
 // One step's codes and scales of a wave, as loaded.
 template <int D>
 struct Step {
@@ -84,7 +107,8 @@ struct Step {
     int valid;  // bit i: the page of 16-token tile i is one of the pool's
 };
 
-template <int D>
+// QP, PP: bf16 parts of a query and of a probability.
+template <int D, int QP, int PP>
 __global__ __launch_bounds__(256, 2) void cache_attn(CacheAttnArgs a) {
     constexpr int G = D / 32;        // scale blocks of a row
     constexpr int VT = 64 / G;       // tokens of one V load
@@ -110,20 +134,21 @@ __global__ __launch_bounds__(256, 2) void cache_attn(CacheAttnArgs a) {
     const int end = min(t0 + chunk, seq.limit((min(c0 + COLS, cols) - 1) / a.group, a.causal));
 
     // Q^T, the second operand: column lane % 16, channels in K's order.
-    bf8 q[2][KS];
+    bf8 q[QP][KS];
     {
         const uint16_t* p = a.q.p + row * a.q.st + head * a.q.sh;
 #pragma unroll
         for (int s = 0; s < KS; s++) {
             uint4 x = make_uint4(0, 0, 0, 0);
-            if (have) x = *reinterpret_cast<const uint4*>(p + g * (D / 4) + 8 * s);
-            if (a.q_f16) {
-                float f[8], hi[8];
+            if (have) x = load_q(p + g * (D / 4) + 8 * s, a.q_sign);
+            if (QP == 2) {
+                float f[8];
                 unpack8(x, f, true);
 #pragma unroll
-                for (int i = 0; i < 8; i++) q[0][s][i] = (__bf16)f[i], hi[i] = (float)q[0][s][i];
-#pragma unroll
-                for (int i = 0; i < 8; i++) q[1][s][i] = (__bf16)(f[i] - hi[i]);
+                for (int i = 0; i < 8; i++) {
+                    q[0][s][i] = (__bf16)f[i];
+                    q[QP - 1][s][i] = (__bf16)(f[i] - (float)q[0][s][i]);
+                }
             } else {
                 q[0][s] = __builtin_bit_cast(bf8, x);
             }
@@ -167,12 +192,6 @@ __global__ __launch_bounds__(256, 2) void cache_attn(CacheAttnArgs a) {
     for (int u = 0; u < UNITS; u++) o[u] = f4{0, 0, 0, 0};
     float m = NEG_INF, l = 0.0f;
     uint8_t* vl = lds[wave];
-    // Where a lane's rows of V lie: 32-byte units permuted by the token, so
-    // that the eight tokens a transposing read takes at once meet all banks.
-    auto unit_at = [&](int tok, int u) {
-        const int f = D == 128 ? tok & 7 : (tok >> 1) & 3;
-        return tok * (D * 2) + ((u ^ f) << 5);
-    };
 
     Step<D> cur;
     const int t_first = t0 + wave * TOKENS;
@@ -190,8 +209,8 @@ __global__ __launch_bounds__(256, 2) void cache_attn(CacheAttnArgs a) {
 #pragma unroll
             for (int k = 0; k < KS; k++) {
                 const bf8 kk = __builtin_bit_cast(bf8, decode8(cur.k[i][k], s));
-                x[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, q[0][k], x[i], 0, 0, 0);
-                if (a.q_f16) x[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, q[1][k], x[i], 0, 0, 0);
+#pragma unroll
+                for (int p = 0; p < QP; p++) x[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, q[p][k], x[i], 0, 0, 0);
             }
         }
         // V into LDS as bf16. Blocks that are NaN go in as (almost) zeros and
@@ -206,7 +225,7 @@ __global__ __launch_bounds__(256, 2) void cache_attn(CacheAttnArgs a) {
             const uint32_t w[4] = {cur.v[i].x, cur.v[i].y, cur.v[i].z, cur.v[i].w};
 #pragma unroll
             for (int d = 0; d < 4; d++)
-                *reinterpret_cast<uint4*>(vl + unit_at(tok, (lane % G) * 2 + d / 2) + (d & 1) * 16) = decode8(w[d], s);
+                *reinterpret_cast<uint4*>(vl + unit_at<D>(tok, (lane % G) * 2 + d / 2) + (d & 1) * 16) = decode8(w[d], s);
         }
         // The softmax's step.
         const bool masked = t + TOKENS > least || cur.valid != 15;
@@ -215,19 +234,18 @@ __global__ __launch_bounds__(256, 2) void cache_attn(CacheAttnArgs a) {
         for (int i = 0; i < 4; i++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                x[i][r] *= a.qk_mul;
                 if (masked && (t + 16 * i + 4 * g + r >= limit || !(cur.valid >> i & 1))) x[i][r] = NEG_INF;
                 mx = fmaxf(mx, x[i][r]);
             }
         mx = fmaxf(m, col_max(mx));
-        const float base = mx == NEG_INF ? 0.0f : mx;
-        if (__any(mx > m)) {
-            const float scale = __builtin_amdgcn_exp2f(m - base);
+        if (__any((mx - m) * a.qk_mul > SLACK)) {
+            const float scale = __builtin_amdgcn_exp2f((m - (mx == NEG_INF ? 0.0f : mx)) * a.qk_mul);
+            m = mx;
             l *= scale;
 #pragma unroll
             for (int u = 0; u < UNITS; u++) o[u] *= scale;
         }
-        m = mx;
+        const float base = m == NEG_INF ? 0.0f : m * a.qk_mul;
         uint32_t hit = 0;  // blocks of NaN that this lane's tokens bring to its column
         uint64_t any_bad = 0;
 #pragma unroll
@@ -247,24 +265,30 @@ __global__ __launch_bounds__(256, 2) void cache_attn(CacheAttnArgs a) {
         for (int i = 0; i < 4; i++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                x[i][r] = __builtin_amdgcn_exp2f(x[i][r] - base);
+                x[i][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][r], a.qk_mul, -base));
                 l += x[i][r];
             }
         // O^T += V^T P^T, 32 tokens a step: the lane's tokens of two tiles.
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
-            bf8 p;
+            bf8 p[PP];
 #pragma unroll
-            for (int r = 0; r < 4; r++) p[r] = (__bf16)x[i][r], p[4 + r] = (__bf16)x[i + 1][r];
+            for (int r = 0; r < 8; r++) {
+                const float e = x[i + r / 4][r % 4];
+                p[0][r] = (__bf16)e;
+                if (PP == 2) p[PP - 1][r] = (__bf16)(e - (float)p[0][r]);
+            }
 #pragma unroll
             for (int u = 0; u < UNITS; u++) {
                 typedef __attribute__((address_space(3))) s4* lp;
                 const int tok = 16 * i + 4 * g + (col >> 2);
-                const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vl + unit_at(tok, u) + (col & 3) * 8));
-                const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vl + unit_at(tok + 16, u) + (col & 3) * 8));
+                const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vl + unit_at<D>(tok, u) + (col & 3) * 8));
+                const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vl + unit_at<D>(tok + 16, u) + (col & 3) * 8));
                 typedef short s8 __attribute__((ext_vector_type(8)));
                 const s8 vv = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                o[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, vv), p, o[u], 0, 0, 0);
+#pragma unroll
+                for (int k = 0; k < PP; k++)
+                    o[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, vv), p[k], o[u], 0, 0, 0);
             }
         }
         if (any_bad)
@@ -283,7 +307,7 @@ __global__ __launch_bounds__(256, 2) void cache_attn(CacheAttnArgs a) {
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < UNITS; u++) *reinterpret_cast<f4*>(ol + (wave * COLS + col) * PAD + 16 * u + 4 * g) = o[u];
-    if (g == 0) wm[wave][col] = m, wl[wave][col] = l;
+    if (g == 0) wm[wave][col] = m * a.qk_mul, wl[wave][col] = l;
     __syncthreads();
     constexpr int TPC = D / 8;  // threads a column, eight channels each
     const int oc = threadIdx.x / TPC, ch = (threadIdx.x % TPC) * 8;
@@ -324,52 +348,351 @@ __global__ __launch_bounds__(256, 2) void cache_attn(CacheAttnArgs a) {
     }
 }
 
-// The splits' parts of one (row, head) joined, in the order of the splits: a
-// wave a pair, D / 64 channels a lane.
+// ---- Chunks of rows ----
+//
+// 128 columns a workgroup, 32 a wave, over tiles of 64 tokens. Each thread
+// loads 16 (D = 64: 8) bytes of K's and V's codes two tiles ahead; V goes into
+// LDS as bf16, K as the codes, which every wave converts for itself: as bf16,
+// K would double what the waves read from LDS, which is then what bounds the
+// kernel, while the conversion is two instructions for 64 lanes' four codes.
+constexpr int CCOLS = 128;
+typedef float f16v __attribute__((ext_vector_type(16)));
+
+template <int D>
+struct ChunkLds {
+    uint8_t v[2][TOKENS * D * 2];
+    uint8_t k[2][TOKENS * D / 2];
+    uint32_t ks[2][TOKENS];      // the token's scale bytes
+    uint64_t bad[2][4];          // V blocks that are NaN, bit (token % 16) * 4 + block, by 16 tokens
+    int flags[2][4];             // by 16 tokens: 1 bad blocks, 2 no page
+};
+
+// QP, PP: bf16 parts of a query and of a probability.
+template <int D, int QP, int PP>
+__global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
+    constexpr int G = D / 32, KS = D / 16, CT = D / 32, WORDS = D / 32;  // WORDS: code dwords a thread loads
+    __shared__ __align__(16) ChunkLds<D> lds;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, half = lane >> 5;
+    const int split = blockIdx.x % a.splits, kvh = blockIdx.y, b = blockIdx.z;
+    const int tile = gridDim.x / a.splits - 1 - blockIdx.x / a.splits;  // the last rows see most: first
+    const CacheDev& c = a.c;
+    const SequenceIndex seq = sequence_index(c, b, a.max_new);
+    const int first = tile * CCOLS, cols = seq.n * a.group;
+    if (first >= cols) return;
+    const int chunk = split_tokens(seq.len, a.splits), t0 = split * chunk;
+    if (split && t0 >= seq.len) return;
+    const int c0 = first + 32 * wave;  // this wave's columns
+    const int j = (c0 + col) / a.group, head = kvh * a.group + (c0 + col) - j * a.group;
+    const long long row = seq.start + j;
+    const bool have = c0 + col < cols && row >= 0 && row < c.rows;
+    const int limit = seq.limit(j, a.causal);
+    const int least = seq.limit(c0 / a.group, a.causal);
+    const int most = c0 < cols ? seq.limit((min(c0 + 32, cols) - 1) / a.group, a.causal) : 0;
+    const int end = min(t0 + chunk, seq.limit((min(first + CCOLS, cols) - 1) / a.group, a.causal));
+
+    bf8 q[QP][KS];
+    {
+        const uint16_t* p = a.q.p + row * a.q.st + head * a.q.sh + half * (D / 2);
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (have) x = load_q(p + 8 * s, a.q_sign);
+            if (QP == 2) {
+                float f[8];
+                unpack8(x, f, true);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    q[0][s][i] = (__bf16)f[i];
+                    q[QP - 1][s][i] = (__bf16)(f[i] - (float)q[0][s][i]);
+                }
+            } else {
+                q[0][s] = __builtin_bit_cast(bf8, x);
+            }
+        }
+    }
+
+    // This thread's part of a tile: token tok, 4 * WORDS bytes of codes.
+    const int tok = threadIdx.x >> 2, part = threadIdx.x & 3;
+    uint32_t kw[WORDS], vw[WORDS], ksc = 0, vsc = 0;
+    int there = 0;
+    auto load = [&](int t) {
+        const int page = cache_page(c, b, t + 16 * wave);
+        there = page >= 0;
+        const long long r = cache_row(c, max(page, 0), kvh, (t + 16 * wave) & ((1 << c.page_shift) - 1)) + (tok & 15);
+        const uint8_t *kp = c.k_codes + r * (D / 2) + part * (D / 8), *vp = c.v_codes + r * (D / 2) + part * (D / 8);
+        if constexpr (D == 128) {
+            const uint4 x = *reinterpret_cast<const uint4*>(kp), y = *reinterpret_cast<const uint4*>(vp);
+            kw[0] = x.x, kw[1] = x.y, kw[2] = x.z, kw[3] = x.w;
+            vw[0] = y.x, vw[1] = y.y, vw[2] = y.z, vw[3] = y.w;
+            ksc = *reinterpret_cast<const uint32_t*>(c.k_scales + r * G);
+        } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(kp), y = *reinterpret_cast<const uint2*>(vp);
+            kw[0] = x.x, kw[1] = x.y;
+            vw[0] = y.x, vw[1] = y.y;
+            ksc = *reinterpret_cast<const uint16_t*>(c.k_scales + r * G);
+        }
+        vsc = c.v_scales[r * G + part * G / 4];
+    };
+    auto store = [&](int buf) {
+        // K: the row's 16-byte (D = 64: 8-byte) units permuted by the token.
+        if constexpr (D == 128) {
+            *reinterpret_cast<uint4*>(lds.k[buf] + tok * 64 + ((part ^ (tok >> 1 & 3)) << 4)) = make_uint4(kw[0], kw[1], kw[2], kw[3]);
+        } else {
+            *reinterpret_cast<uint2*>(lds.k[buf] + tok * 32 + (((part >> 1) ^ (tok >> 2 & 1)) << 4) + (part & 1) * 8) = make_uint2(kw[0], kw[1]);
+        }
+        if (part == 0) lds.ks[buf][tok] = ksc;
+        const bool nan = vsc == 255;
+        const uint64_t bad = __ballot(D == 128 ? nan : nan && !(part & 1));
+        if (lane == 0) {
+            lds.bad[buf][wave] = bad;
+            lds.flags[buf][wave] = (bad != 0) | (there ? 0 : 2);
+        }
+        const float s = __uint_as_float(nan ? 0 : vsc << 23);
+#pragma unroll
+        for (int w = 0; w < WORDS; w++) {
+            const int ch = part * (D / 4) + 8 * w;
+            *reinterpret_cast<uint4*>(lds.v[buf] + unit_at<D>(tok, ch / 16) + (ch & 8) * 2) = decode8(vw[w], s);
+        }
+    };
+
+    f16v o[CT];
+#pragma unroll
+    for (int u = 0; u < CT; u++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[u][i] = 0.0f;
+    float m = NEG_INF, l = 0.0f;
+    // A transposing read's place in a tile: lanes 0-15 and 32-47 the first 16
+    // of 32 channels, tokens 4 * half + (lane % 16) / 4.
+    const int vtok = 4 * half + (lane >> 2 & 3), vunit = lane >> 4 & 1, vbyte = (lane & 3) * 8;
+
+    if (t0 < end) {
+        load(t0);
+        store(0);
+        if (t0 + TOKENS < end) load(t0 + TOKENS);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int t = t0; t < end; t += TOKENS, buf ^= 1) {
+        if (t + TOKENS < end) {
+            store(buf ^ 1);
+            if (t + 2 * TOKENS < end) load(t + 2 * TOKENS);
+        }
+        if (t < most) {
+            f16v x[2];
+#pragma unroll
+            for (int sub = 0; sub < 2; sub++) {
+                const int tk = 32 * sub + col;
+#pragma unroll
+                for (int i = 0; i < 16; i++) x[sub][i] = 0.0f;
+                uint32_t w[KS];
+#pragma unroll
+                for (int u = 0; u < KS / 4; u++) {
+                    const uint4 y = D == 128
+                        ? *reinterpret_cast<const uint4*>(lds.k[buf] + tk * 64 + (((half * 2 + u) ^ (tk >> 1 & 3)) << 4))
+                        : *reinterpret_cast<const uint4*>(lds.k[buf] + tk * 32 + ((half ^ (tk >> 2 & 1)) << 4));
+                    w[4 * u] = y.x, w[4 * u + 1] = y.y, w[4 * u + 2] = y.z, w[4 * u + 3] = y.w;
+                }
+                const uint32_t sc = lds.ks[buf][tk] >> (half * (KS / 4) * 8);
+#pragma unroll
+                for (int s = 0; s < KS; s++) {
+                    const bf8 kk = __builtin_bit_cast(bf8, decode8(w[s], __uint_as_float((sc >> (s / 4 * 8) & 255) << 23)));
+#pragma unroll
+                    for (int p = 0; p < QP; p++) x[sub] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kk, q[p][s], x[sub], 0, 0, 0);
+                }
+            }
+            const int4 fl = *reinterpret_cast<const int4*>(lds.flags[buf]);
+            const int flags = __builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w);
+            uint32_t hit = 0;
+            if (flags || t + TOKENS > least) {
+                const int fi[4] = {fl.x, fl.y, fl.z, fl.w};
+#pragma unroll
+                for (int sub = 0; sub < 2; sub++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const int k = 32 * sub + 8 * (i / 4) + 4 * half + i % 4, six = 2 * sub + i / 8;
+                        const bool seen = t + k < limit && !(fi[six] & 2);
+                        if (!seen) x[sub][i] = NEG_INF;
+                        if (flags & 1) {
+                            const uint32_t blocks = (uint32_t)(lds.bad[buf][six] >> ((k & 15) * 4)) & 15;
+                            if (seen) hit |= blocks;
+                        }
+                    }
+                if (flags & 1) {
+                    auto r = __builtin_amdgcn_permlane32_swap(hit, hit, false, false);
+                    hit = r[0] | r[1];
+                }
+            }
+            float mx = NEG_INF;
+#pragma unroll
+            for (int sub = 0; sub < 2; sub++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) mx = fmaxf(mx, x[sub][i]);
+            {
+                auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+                mx = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+            }
+            mx = fmaxf(m, mx);
+            if (__any((mx - m) * a.qk_mul > SLACK)) {
+                const float scale = __builtin_amdgcn_exp2f((m - (mx == NEG_INF ? 0.0f : mx)) * a.qk_mul);
+                m = mx;
+                l *= scale;
+#pragma unroll
+                for (int u = 0; u < CT; u++) o[u] *= scale;
+            }
+            const float base = m == NEG_INF ? 0.0f : m * a.qk_mul;
+#pragma unroll
+            for (int sub = 0; sub < 2; sub++)
+#pragma unroll
+                for (int st = 0; st < 2; st++) {
+                    bf8 p[PP];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[sub][8 * st + i], a.qk_mul, -base));
+                        l += e;
+                        p[0][i] = (__bf16)e;
+                        if (PP == 2) p[PP - 1][i] = (__bf16)(e - (float)p[0][i]);
+                    }
+#pragma unroll
+                    for (int u = 0; u < CT; u++) {
+                        typedef __attribute__((address_space(3))) s4* lp;
+                        typedef short s8 __attribute__((ext_vector_type(8)));
+                        const uint8_t* v = lds.v[buf] + (32 * sub + 16 * st) * (D * 2) + unit_at<D>(vtok, 2 * u + vunit) + vbyte;
+                        const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(v));
+                        const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(v + 8 * (D * 2)));
+                        const s8 vv = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                        for (int k = 0; k < PP; k++)
+                            o[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, vv), p[k], o[u], 0, 0, 0);
+                    }
+                }
+            if (flags & 1)
+#pragma unroll
+                for (int u = 0; u < CT; u++)
+                    if (hit >> (D == 128 ? u : 2 * u) & 1)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) o[u][i] = __builtin_nanf("");
+        }
+        __syncthreads();
+    }
+    {
+        auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+        l = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    if (!have) return;
+    // A lane holds four channels of each eight of its column.
+    if (a.splits == 1) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        uint16_t* out = a.out.p + row * a.out.st + head * a.out.sh;
+#pragma unroll
+        for (int u = 0; u < CT; u++)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const f4 f = f4{o[u][i], o[u][i + 1], o[u][i + 2], o[u][i + 3]} * inv;
+                const uint2 w = a.out_f16 ? make_uint2(pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]))
+                                          : make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
+                *reinterpret_cast<uint2*>(out + 32 * u + 2 * i + 4 * half) = w;
+            }
+    } else {
+        const long long at = ((long long)split * c.rows + row) * a.heads + head;
+#pragma unroll
+        for (int u = 0; u < CT; u++)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<f4*>(a.part_o + at * D + 32 * u + 2 * i + 4 * half) = f4{o[u][i], o[u][i + 1], o[u][i + 2], o[u][i + 3]};
+        if (half == 0) {
+            a.part_ml[at * 2] = m * a.qk_mul;
+            a.part_ml[at * 2 + 1] = l;
+        }
+    }
+}
+
+// The splits' parts of one (row, head) joined by a workgroup: every group of
+// D / 8 lanes sums the splits that fall to it, eight channels a lane, and the
+// groups' sums are added in their order, so the same call gives the same bits.
 template <int D>
 __global__ __launch_bounds__(256) void cache_attn_join(CacheAttnArgs a) {
+    constexpr int LANES = D / 8, GROUPS = 256 / LANES;
+    __shared__ float ws[MAX_SPLITS], sums[GROUPS][D + 4];
     const CacheDev& c = a.c;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = blockIdx.z;
+    const int b = blockIdx.z, j = blockIdx.x / a.heads, h = blockIdx.x - j * a.heads;
     const SequenceIndex seq = sequence_index(c, b, a.max_new);
-    const int i = blockIdx.x * 4 + wave, j = i / a.heads, h = i - j * a.heads;
     const long long row = seq.start + j;
     if (j >= seq.n || row < 0 || row >= c.rows) return;
     const int chunk = split_tokens(seq.len, a.splits), parts = seq.len ? (seq.len + chunk - 1) / chunk : 1;
     const long long at = row * a.heads + h, step = (long long)c.rows * a.heads;
+    // Maximum over the splits, and their weights (every wave for itself).
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float m = NEG_INF, l = 0.0f;
-    float f[D / 64] = {};
-    for (int p = 0; p < parts; p++) {
-        const float pm = a.part_ml[(at + p * step) * 2], pl = a.part_ml[(at + p * step) * 2 + 1];
-        const float mx = fmaxf(m, pm), base = mx == NEG_INF ? 0.0f : mx;
-        const float s0 = __builtin_amdgcn_exp2f(m - base), s1 = __builtin_amdgcn_exp2f(pm - base);
-        l = l * s0 + pl * s1;
-#pragma unroll
-        for (int k = 0; k < D / 64; k++) f[k] = f[k] * s0 + a.part_o[(at + p * step) * D + lane * (D / 64) + k] * s1;
-        m = mx;
+    for (int p = lane; p < parts; p += 64) m = fmaxf(m, a.part_ml[(at + p * step) * 2]);
+    m = wave_max(m);
+    const float base = m == NEG_INF ? 0.0f : m;
+    for (int p = lane; p < parts; p += 64) {
+        const float w = __builtin_amdgcn_exp2f(a.part_ml[(at + p * step) * 2] - base);
+        l += w * a.part_ml[(at + p * step) * 2 + 1];
+        if (wave == 0) ws[p] = w;
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    uint16_t* out = a.out.p + row * a.out.st + h * a.out.sh + lane * (D / 64);
 #pragma unroll
-    for (int k = 0; k < D / 64; k++)
-        out[k] = (uint16_t)(a.out_f16 ? pack_f16x2(f[k] * inv, 0.0f) : pack_bf16x2(f[k] * inv, 0.0f));
+    for (int i = 32; i; i >>= 1) l += __shfl_xor(l, i);
+    __syncthreads();
+    const int grp = threadIdx.x / LANES, ch = (threadIdx.x % LANES) * 8;
+    f4 f[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
+#pragma unroll 4
+    for (int p = grp; p < parts; p += GROUPS) {
+        const f4* o = reinterpret_cast<const f4*>(a.part_o + (at + p * step) * D + ch);
+        f[0] += o[0] * ws[p];
+        f[1] += o[1] * ws[p];
+    }
+    *reinterpret_cast<f4*>(&sums[grp][ch]) = f[0];
+    *reinterpret_cast<f4*>(&sums[grp][ch + 4]) = f[1];
+    __syncthreads();
+    if (threadIdx.x >= D / 2) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    float x = 0.0f, y = 0.0f;
+#pragma unroll
+    for (int g = 0; g < GROUPS; g++) x += sums[g][2 * threadIdx.x], y += sums[g][2 * threadIdx.x + 1];
+    *reinterpret_cast<uint32_t*>(a.out.p + row * a.out.st + h * a.out.sh + 2 * threadIdx.x) =
+        a.out_f16 ? pack_f16x2(x * inv, y * inv) : pack_bf16x2(x * inv, y * inv);
 }
 
 }  // namespace
 
+#ifndef SPLIT_TARGET
+#define SPLIT_TARGET 4096
+#endif
+// Whether a call runs the chunk kernel.
+static bool in_chunks(int max_new, int group) { return (long long)max_new * group > 64; }
+
 int cache_splits(int head_dim, int batch, int kv_heads, int group, int max_new, int max_tokens) {
     (void)head_dim;
-    const long long tiles = ((long long)max_new * group + COLS - 1) / COLS;
+    const int per = in_chunks(max_new, group) ? CCOLS : COLS;
+    const long long tiles = ((long long)max_new * group + per - 1) / per;
     const long long units = tiles * kv_heads * batch;
     const long long most = (max_tokens + 511) / 512;
-    return (int)std::max(1ll, std::min({most, 4096 / std::max(units, 1ll), 256ll}));
+    if (per == CCOLS) return (int)std::max(1ll, std::min({most, 512 / std::max(units, 1ll), (long long)MAX_SPLITS}));
+    return (int)std::max(1ll, std::min({most, SPLIT_TARGET / std::max(units, 1ll), (long long)MAX_SPLITS}));
 }
 
 template <int D>
 static hipError_t launch(const CacheAttnArgs& a, hipStream_t s) {
-    const unsigned tiles = (unsigned)(((long long)a.max_new * a.group + COLS - 1) / COLS);
-    hipLaunchKernelGGL((cache_attn<D>), dim3(tiles * a.splits, a.c.kv_heads, a.c.batch), dim3(256), 0, s, a);
+    const int per = in_chunks(a.max_new, a.group) ? CCOLS : COLS;
+    const unsigned tiles = (unsigned)(((long long)a.max_new * a.group + per - 1) / per);
+    const dim3 grid(tiles * a.splits, a.c.kv_heads, a.c.batch), block(256);
+    const auto go = [&](auto qp, auto pp) {
+        constexpr int QP = decltype(qp)::value, PP = decltype(pp)::value;
+        if (per == COLS)
+            hipLaunchKernelGGL((cache_attn<D, QP, PP>), grid, block, 0, s, a);
+        else
+            hipLaunchKernelGGL((cache_attn_chunk<D, QP, PP>), grid, block, 0, s, a);
+    };
+    constexpr std::integral_constant<int, 1> one;
+    constexpr std::integral_constant<int, 2> two;
+    if (a.q_f16)
+        a.out_f16 ? go(two, two) : go(two, one);
+    else
+        a.out_f16 ? go(one, two) : go(one, one);
     if (a.splits > 1)
-        hipLaunchKernelGGL((cache_attn_join<D>), dim3((unsigned)(((long long)a.max_new * a.heads + 3) / 4), 1, a.c.batch), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((cache_attn_join<D>), dim3((unsigned)a.max_new * a.heads, 1, a.c.batch), block, 0, s, a);
     return hipGetLastError();
 }
 

@@ -139,9 +139,9 @@ def attend(q, kv, vv, starts, lengths, page_table, page_tokens, causal, scale, o
 
 def attend_tolerance(want, size, reach, d, out_type):
     """How far an element may be: each probability is rounded to bf16 once (half a step of it; the sum of the
-    probabilities is not), each logit is an fp32 sum of d products (and of a second part of the query) in base 2, the
+    probabilities is not), for an fp16 output to two bf16 parts (half a step of half a step), each logit is an fp32 sum of d products (and of a second part of the query) in base 2, the
     output is an fp32 sum and is rounded once to its type."""
     logit = 4 * d * 2.0 ** -24 * reach  # absolute error of a logit; p is off by its exponential, and so is their sum
-    p = HALF_STEP["bf16"] + 2 * logit + 2.0 ** -20
+    p = (HALF_STEP["bf16"] if out_type == "bf16" else HALF_STEP["bf16"] ** 2) + 2 * logit + 2.0 ** -20
     least = 2.0 ** -24 if out_type == "f16" else 0.0  # half an fp16 subnormal's step
     return p * size + HALF_STEP[out_type] * (np.abs(want) + p * size) + least + 1e-30

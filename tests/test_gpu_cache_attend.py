@@ -52,8 +52,9 @@ def test_single_tokens(torch_gpu, d, t, kv, group):
 
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("t,out_t", [("bf16", "bf16"), ("bf16", "f16"), ("f16", "f16"), ("f16", "bf16")])
 @pytest.mark.parametrize("kv,group", [(2, 1), (1, 5), (1, 8)])
-def test_chunks(torch_gpu, d, causal, kv, group):
+def test_chunks(torch_gpu, d, causal, t, out_t, kv, group):
     """Several new rows a sequence: none, a few, more than a tile; the first of them the sequence's first tokens; rows
     behind the last sequence stay."""
     rng = np.random.default_rng(d + group)
@@ -63,8 +64,8 @@ def test_chunks(torch_gpu, d, causal, kv, group):
     if not causal:
         lengths = [33, 0, 129, 1, 64, 0]
     p = Pool(torch_gpu, d, starts, lengths, kv, 32, kv * group, starts[-1] + 5, seed=group)
-    q, qv = draw16(torch_gpu, rng, (1, starts[-1] + 5, kv * group, d), "bf16")
-    out = check(torch_gpu, p, q, qv, "f16", causal)
+    q, qv = draw16(torch_gpu, rng, (1, starts[-1] + 5, kv * group, d), t)
+    out = check(torch_gpu, p, q, qv, out_t, causal)
     assert (out[0, starts[-1]:] == 3.0).all()
 
 
@@ -79,12 +80,23 @@ def test_long_sequences(torch_gpu, d):
     assert torch_gpu.equal(a, run(torch_gpu, p, q, "bf16"))  # the same bits again
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_long_prefix_under_a_few_rows(torch_gpu, d):
+    """Chunks whose keys are split over workgroups, and more rows than a workgroup's columns."""
+    rng = np.random.default_rng(d)
+    p = Pool(torch_gpu, d, [0, 33, 34, 200], [6001, 700, 1500], 1, 128, 3, seed=1)
+    q, qv = draw16(torch_gpu, rng, (1, 200, 3, d), "f16", 2.0)
+    a = check(torch_gpu, p, q, qv, "f16")
+    assert torch_gpu.equal(a, run(torch_gpu, p, q, "f16"))
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 3.0])
 def test_softmax_scale(torch_gpu, scale):
     rng = np.random.default_rng(2)
-    p = Pool(torch_gpu, 128, [0, 3, 5], [70, 200], 2, 16, 4, seed=1)
-    q, qv = draw16(torch_gpu, rng, (1, 5, 4, 128), "f16")
-    check(torch_gpu, p, q, qv, "f16", scale=scale)
+    for more in (0, 60):  # few columns, and a chunk
+        p = Pool(torch_gpu, 128, [0, 3 + more, 5 + more], [70, 200], 2, 16, 4, seed=1)
+        q, qv = draw16(torch_gpu, rng, (1, 5 + more, 4, 128), "f16")
+        check(torch_gpu, p, q, qv, "f16", scale=scale)
 
 
 def test_views_in_place_and_types(torch_gpu):
