@@ -3,6 +3,8 @@
 // Compiled with -ffp-contract=off: every product and sum of the rotation is
 // rounded in fp32 as written, and its result once to the 16-bit type, so that
 // sage_cache_append's keys are those of sage_rotary_apply bit for bit.
+#include <algorithm>
+
 #include "sage_cache.hpp"
 
 namespace sage {
@@ -96,6 +98,14 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
     }
 }
 
+// Workgroups in y that share the heads of a row among them: all the parts
+// (steps of a workgroup's heads) where there are few rows, and fewer as the
+// rows fill the chip by themselves, so that what a thread looks up for its row
+// serves several heads. blocks: workgroups of the rows.
+unsigned share_heads(long long blocks, long long parts) {
+    return (unsigned)std::min(parts, std::max(1ll, (4096 + blocks - 1) / blocks));
+}
+
 // ---- append and read ----
 
 // Four lanes' 32 channels -> their scale byte and each lane's four code bytes.
@@ -123,76 +133,105 @@ __device__ __forceinline__ uint32_t encode(const float (&x)[8], uint32_t& scale)
     return codes;
 }
 
-// Grid: x = rows in steps of a workgroup's, y = KV heads of K, then of V, then
-// the query heads. A workgroup's rows are consecutive and of one head: their
-// code rows are consecutive too, so the stores fill whole lines.
+// The place of a row in the pool. Every thread of a workgroup asks; up to
+// STARTS - 1 sequences are looked through in LDS, one load instead of a chain.
+constexpr int STARTS = 1024;
+struct Place {
+    int b, slot, page;
+    long long at;  // the slot's code row for KV head 0
+};
+__device__ __forceinline__ Place place_of(CacheDev c, int row, int* starts) {
+    if (c.batch < STARTS) {
+        for (int i = threadIdx.x; i <= c.batch; i += blockDim.x) starts[i] = c.starts[i];
+        __syncthreads();
+        c.starts = starts;
+    }
+    Place p{-1, -1, -1, 0};
+    if (row >= c.rows) return p;
+    p.b = sequence_of(c, row);
+    if (p.b < 0) return p;
+    p.slot = slot_of(c, p.b, row);
+    p.page = cache_page(c, p.b, p.slot);
+    p.at = cache_row(c, max(p.page, 0), 0, p.slot & ((1 << c.page_shift) - 1));
+    return p;
+}
+
+// Grid: x = rows in steps of a workgroup's; y = shares of the parts, which are
+// the KV heads of K, then of V, then the query heads. A workgroup's rows are
+// consecutive and of one head at a time: their code rows are consecutive
+// too, so the stores fill whole lines.
 template <int D>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     constexpr int CH = D / 8, ROWS = 256 / CH;
-    const int c0 = ((int)threadIdx.x % CH) * 8, head = blockIdx.y;
-    const int row = blockIdx.x * ROWS + threadIdx.x / CH;
-    if (row >= a.c.rows) return;
-    const int b = sequence_of(a.c, row);
-    if (b < 0) return;
-    const int slot = slot_of(a.c, b, row);
-    const int kv = a.c.kv_heads, part = head < kv ? 0 : head < 2 * kv ? 1 : 2;
-    const int h = part == 0 ? head : part == 1 ? head - kv : head - 2 * kv;
-    const RowView& in = part == 0 ? a.k : part == 1 ? a.v : a.q;
-    const uint16_t* p = in.p + row * in.st + h * in.sh;
-    float x[8];
-    unpack8(*reinterpret_cast<const uint4*>(p + c0), x, a.f16);
-    if (part != 1 && a.r.table) {
-        f2 cs[8];
-        load_turns(a.r, a.r.positions ? a.r.positions[row] : slot, c0, cs);
-        turn(a.r, p, c0, cs, a.f16, x);
-        const uint4 y = pack8(x, a.f16);
-        if (part == 2) {
-            *reinterpret_cast<uint4*>(a.q_out.p + row * a.q_out.st + h * a.q_out.sh + c0) = y;
-            return;
+    __shared__ int starts[STARTS];
+    const int c0 = ((int)threadIdx.x % CH) * 8, row = blockIdx.x * ROWS + threadIdx.x / CH;
+    const int kv = a.c.kv_heads, parts = 2 * kv + (a.q.p ? a.heads : 0);
+    const Place place = place_of(a.c, row, starts);
+    if (place.b < 0) return;
+    f2 cs[8];
+    if (a.r.table) load_turns(a.r, a.r.positions ? a.r.positions[row] : place.slot, c0, cs);
+    for (int part = blockIdx.y; part < parts; part += gridDim.y) {
+        const bool is_v = part >= kv && part < 2 * kv, is_q = part >= 2 * kv;
+        const int h = is_q ? part - 2 * kv : is_v ? part - kv : part;
+        const RowView& in = is_q ? a.q : is_v ? a.v : a.k;
+        const uint16_t* p = in.p + row * in.st + h * in.sh;
+        float x[8];
+        unpack8(*reinterpret_cast<const uint4*>(p + c0), x, a.f16);
+        if (!is_v && a.r.table) {
+            turn(a.r, p, c0, cs, a.f16, x);
+            const uint4 y = pack8(x, a.f16);
+            if (is_q) {
+                *reinterpret_cast<uint4*>(a.q_out.p + row * a.q_out.st + h * a.q_out.sh + c0) = y;
+                continue;
+            }
+            unpack8(y, x, a.f16);
         }
-        unpack8(y, x, a.f16);
+        uint32_t scale;
+        const uint32_t codes = encode(x, scale);
+        if (place.page < 0) continue;
+        const long long at = place.at + ((long long)h << a.c.page_shift);
+        uint8_t* code = is_v ? a.c.v_codes : a.c.k_codes;
+        uint8_t* sc = is_v ? a.c.v_scales : a.c.k_scales;
+        *reinterpret_cast<uint32_t*>(code + at * (D / 2) + c0 / 2) = codes;
+        if (c0 % CACHE_BLOCK == 0) sc[at * (D / CACHE_BLOCK) + c0 / CACHE_BLOCK] = (uint8_t)scale;
     }
-    uint32_t scale;
-    const uint32_t codes = encode(x, scale);
-    const int page = cache_page(a.c, b, slot);
-    if (page < 0) return;
-    const long long at = cache_row(a.c, page, h, slot & ((1 << a.c.page_shift) - 1));
-    uint8_t* code = part ? a.c.v_codes : a.c.k_codes;
-    uint8_t* sc = part ? a.c.v_scales : a.c.k_scales;
-    *reinterpret_cast<uint32_t*>(code + at * (D / 2) + c0 / 2) = codes;
-    if (c0 % CACHE_BLOCK == 0) sc[at * (D / CACHE_BLOCK) + c0 / CACHE_BLOCK] = (uint8_t)scale;
 }
 
 template <int D>
 __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
     constexpr int CH = D / 8, ROWS = 256 / CH;
-    const int c0 = ((int)threadIdx.x % CH) * 8, part = blockIdx.y >= (unsigned)a.c.kv_heads;
-    const int h = blockIdx.y - part * a.c.kv_heads, row = blockIdx.x * ROWS + threadIdx.x / CH;
-    if (row >= a.c.rows) return;
-    const int b = sequence_of(a.c, row);
-    if (b < 0) return;
-    const int slot = slot_of(a.c, b, row), page = cache_page(a.c, b, slot);
-    float x[8] = {};
-    if (page >= 0) {
-        const long long at = cache_row(a.c, page, h, slot & ((1 << a.c.page_shift) - 1));
-        const uint32_t codes =
-            *reinterpret_cast<const uint32_t*>((part ? a.c.v_codes : a.c.k_codes) + at * (D / 2) + c0 / 2);
-        const uint32_t sc = (part ? a.c.v_scales : a.c.k_scales)[at * (D / CACHE_BLOCK) + c0 / CACHE_BLOCK];
-        const float s = __uint_as_float(sc << 23);  // 255: infinity, which the conversion turns into NaN
-        const f2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 1),
-                         __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 2), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 3)};
+    __shared__ int starts[STARTS];
+    const int c0 = ((int)threadIdx.x % CH) * 8, row = blockIdx.x * ROWS + threadIdx.x / CH, kv = a.c.kv_heads;
+    const Place place = place_of(a.c, row, starts);
+    if (place.b < 0) return;
+    for (int part = blockIdx.y; part < 2 * kv; part += gridDim.y) {
+        const bool is_v = part >= kv;
+        const int h = is_v ? part - kv : part;
+        float x[8] = {};
+        if (place.page >= 0) {
+            const long long at = place.at + ((long long)h << a.c.page_shift);
+            const uint32_t codes =
+                *reinterpret_cast<const uint32_t*>((is_v ? a.c.v_codes : a.c.k_codes) + at * (D / 2) + c0 / 2);
+            const uint32_t sc = (is_v ? a.c.v_scales : a.c.k_scales)[at * (D / CACHE_BLOCK) + c0 / CACHE_BLOCK];
+            const float s = __uint_as_float(sc << 23);  // 255: infinity, which the conversion turns into NaN
+            const f2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 0),
+                             __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 1),
+                             __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 2),
+                             __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 3)};
 #pragma unroll
-        for (int k = 0; k < 4; k++) x[2 * k] = v[k].x, x[2 * k + 1] = v[k].y;
+            for (int k = 0; k < 4; k++) x[2 * k] = v[k].x, x[2 * k + 1] = v[k].y;
+        }
+        const RowView& o = is_v ? a.v : a.k;
+        *reinterpret_cast<uint4*>(o.p + row * o.st + h * o.sh + c0) = pack8(x, a.f16);
     }
-    const RowView& o = part ? a.v : a.k;
-    *reinterpret_cast<uint4*>(o.p + row * o.st + h * o.sh + c0) = pack8(x, a.f16);
 }
 
 }  // namespace
 
 hipError_t launch_rotary(int head_dim, const RotaryArgs& a, hipStream_t s) {
-    const long long rows = (long long)a.batch * a.tokens;
-    const dim3 grid((unsigned)((rows + 3) / 4), 1);
+    const long long blocks = ((long long)a.batch * a.tokens + 3) / 4;
+    const int slots = 64 / (head_dim / 8);
+    const dim3 grid((unsigned)blocks, share_heads(blocks, std::min(65535, (a.heads + slots - 1) / slots)));
     if (head_dim == 64)
         hipLaunchKernelGGL(rotary_kernel<64>, grid, dim3(256), 0, s, a);
     else
@@ -202,7 +241,8 @@ hipError_t launch_rotary(int head_dim, const RotaryArgs& a, hipStream_t s) {
 
 hipError_t launch_cache_append(int head_dim, const AppendArgs& a, hipStream_t s) {
     const int rows = 256 / (head_dim / 8);
-    const dim3 grid((unsigned)((a.c.rows + rows - 1) / rows), (unsigned)(2 * a.c.kv_heads + (a.q.p ? a.heads : 0)));
+    const long long blocks = ((long long)a.c.rows + rows - 1) / rows;
+    const dim3 grid((unsigned)blocks, share_heads(blocks, 2 * a.c.kv_heads + (a.q.p ? a.heads : 0)));
     if (head_dim == 64)
         hipLaunchKernelGGL(append_kernel<64>, grid, dim3(256), 0, s, a);
     else
@@ -212,7 +252,8 @@ hipError_t launch_cache_append(int head_dim, const AppendArgs& a, hipStream_t s)
 
 hipError_t launch_cache_read(int head_dim, const ReadArgs& a, hipStream_t s) {
     const int rows = 256 / (head_dim / 8);
-    const dim3 grid((unsigned)((a.c.rows + rows - 1) / rows), (unsigned)(2 * a.c.kv_heads));
+    const long long blocks = ((long long)a.c.rows + rows - 1) / rows;
+    const dim3 grid((unsigned)blocks, share_heads(blocks, 2 * a.c.kv_heads));
     if (head_dim == 64)
         hipLaunchKernelGGL(read_kernel<64>, grid, dim3(256), 0, s, a);
     else

@@ -29,6 +29,7 @@ namespace {
 typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
+typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr int COLS = 16;    // columns of a workgroup
@@ -75,12 +76,49 @@ __device__ __forceinline__ float col_sum(float v) {
     r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+// Maximum over the aligned LANES (8 or 16) lanes of a row, in each of them.
+template <int LANES>
+__device__ __forceinline__ float row_max(float v) {
+    v = fmaxf(v, dpp<0xB1>(v));
+    v = fmaxf(v, dpp<0x4E>(v));
+    v = fmaxf(v, dpp<0x141>(v));
+    return LANES > 8 ? fmaxf(v, dpp<0x140>(v)) : v;
+}
 __device__ __forceinline__ uint32_t col_or(uint32_t v) {
     auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     v = r[0] | r[1];
     r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
     return r[0] | r[1];
 }
+
+// A sequence's pages as a wave walks it: 64 columns of the page table, one a
+// lane, loaded at once and read by lane index. Looked up one by one, each id is
+// a load in front of the loads that need it, and waiting for it waits for
+// all that are in flight (chunks of 2048 rows behind 8190 tokens, 32/8 heads of
+// 128: 550 us against 313 with the window).
+struct Pages {
+    const int* table;  // the sequence's row
+    int cols, pages, shift, lane;
+    int base, ids;
+    __device__ __forceinline__ Pages(const CacheDev& c, int b, int lane_, int t)
+        : table(c.page_table + (long long)b * c.max_pages), cols(c.max_pages), pages(c.pages), shift(c.page_shift),
+          lane(lane_) {
+        fill(t >> shift);
+    }
+    __device__ __forceinline__ void fill(int col) {
+        base = col;
+        const int at = col + lane;
+        const int id = at < cols ? table[at] : -1;
+        ids = (unsigned)id < (unsigned)pages ? id : -1;
+        asm volatile("" : "+v"(ids));  // waited for here, once a window, not at every use
+    }
+    // The page of slot t (of the window's first column or behind it), or -1.
+    __device__ __forceinline__ int of(int t) {
+        const int col = t >> shift;
+        if (col - base >= 64) fill(col);
+        return __builtin_amdgcn_readlane(ids, col - base);
+    }
+};
 
 // Tokens of one split of a sequence of len tokens: whole steps of the
 // workgroup's four waves.
@@ -98,23 +136,17 @@ __device__ __forceinline__ int unit_at(int tok, int u) {
     return tok * (D * 2) + ((u ^ f) << 5);
 }
 
-// One step's codes and scales of a wave, as loaded.
-template <int D>
-struct Step {
-    uint32_t k[4][D / 32];     // [16-token tile][dwords]: token lane % 16, channels (lane / 16) * D / 4 ..
-    uint4 v[D / 32];           // token lane / (D / 32) + i * 2048 / D, channels (lane % (D / 32)) * 32 ..
-    uint32_t ks[4], vs[D / 32];
-    int valid;  // bit i: the page of 16-token tile i is one of the pool's
-};
-
 // QP, PP: bf16 parts of a query and of a probability.
 template <int D, int QP, int PP>
-__global__ __launch_bounds__(256, 2) void cache_attn(CacheAttnArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void cache_attn(CacheAttnArgs a) {
     constexpr int G = D / 32;        // scale blocks of a row
     constexpr int VT = 64 / G;       // tokens of one V load
     constexpr int UNITS = D / 16;    // 32-byte units of a V row in LDS
     constexpr int KS = D / 32;       // MFMA steps over the channels
-    __shared__ __align__(16) uint8_t lds[4][TOKENS * D * 2];
+    constexpr int PAD = D + 4;       // floats of a column where the waves' parts meet
+    constexpr int HALF = TOKENS / 2; // tokens of V in LDS at a time, per wave
+    constexpr int LDS = 4 * (HALF * D * 2 > COLS * PAD * 4 ? HALF * D * 2 : COLS * PAD * 4);
+    __shared__ __align__(16) uint8_t lds[LDS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
     const int split = blockIdx.x % a.splits, tile = blockIdx.x / a.splits, kvh = blockIdx.y, b = blockIdx.z;
@@ -155,18 +187,32 @@ __global__ __launch_bounds__(256, 2) void cache_attn(CacheAttnArgs a) {
         }
     }
 
-    auto load = [&](int t, Step<D>& st) {
+    const int t_first = t0 + wave * TOKENS;
+    Pages pages(c, b, lane, t_first);
+    // One step's codes and scales: K's token lane % 16 of each 16-token tile,
+    // channels (lane / 16) * D / 4 on; V's token lane / G + i * VT, block lane % G.
+    struct Step {
+        uint32_t k[4][KS], ks[4];
+        uint4 v[G];
+        uint32_t vs[G];
+        int valid;
+    };
+    // valid: bit i: the page of 16-token tile i is one of the pool's
+    auto row_of = [&](int t, int page) {
+        return cache_row(c, max(page, 0), kvh, t & ((1 << c.page_shift) - 1));
+    };
+    auto load = [&](int t, Step& st) {
         st.valid = 0;
-        long long rows[4];  // code row of each 16-token tile
+        long long rows[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int page = cache_page(c, b, t + 16 * i);
+            const int page = pages.of(t + 16 * i);
             st.valid |= (page >= 0) << i;
-            rows[i] = cache_row(c, max(page, 0), kvh, (t + 16 * i) & ((1 << c.page_shift) - 1));
+            rows[i] = row_of(t + 16 * i, page);
         }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const uint8_t* p = c.k_codes + (rows[i] + col) * (D / 2) + g * (D / 8);
+            const uint8_t* p = c.k_codes + rows[i] * (D / 2) + (uint32_t)(col * (D / 2) + g * (D / 8));
             if constexpr (D == 128) {
                 const uint4 x = *reinterpret_cast<const uint4*>(p);
                 st.k[i][0] = x.x, st.k[i][1] = x.y, st.k[i][2] = x.z, st.k[i][3] = x.w;
@@ -174,14 +220,13 @@ __global__ __launch_bounds__(256, 2) void cache_attn(CacheAttnArgs a) {
                 const uint2 x = *reinterpret_cast<const uint2*>(p);
                 st.k[i][0] = x.x, st.k[i][1] = x.y;
             }
-            st.ks[i] = c.k_scales[(rows[i] + col) * G + g * G / 4];
+            st.ks[i] = (c.k_scales + rows[i] * G)[(uint32_t)(col * G + g * G / 4)];
         }
 #pragma unroll
         for (int i = 0; i < G; i++) {
-            const int tok = lane / G + i * VT;
             long long r = rows[(i * VT) / 16];
             if (VT == 32 && lane >= 32) r = rows[(i * VT) / 16 + 1];
-            r += tok & 15;
+            r += lane / G & 15;
             st.v[i] = *reinterpret_cast<const uint4*>(c.v_codes + r * (D / 2) + (lane % G) * 16);
             st.vs[i] = c.v_scales[r * G + lane % G];
         }
@@ -191,50 +236,38 @@ __global__ __launch_bounds__(256, 2) void cache_attn(CacheAttnArgs a) {
 #pragma unroll
     for (int u = 0; u < UNITS; u++) o[u] = f4{0, 0, 0, 0};
     float m = NEG_INF, l = 0.0f;
-    uint8_t* vl = lds[wave];
+    uint8_t* vl = lds + wave * (HALF * D * 2);
 
-    Step<D> cur;
-    const int t_first = t0 + wave * TOKENS;
-    if (t_first < end) load(t_first, cur);
-    for (int t = t_first; t < end; t += 4 * TOKENS) {
-        Step<D> nxt;
-        const bool more = t + 4 * TOKENS < end;
-        if (more) load(t + 4 * TOKENS, nxt);
+    // Two steps in registers, taken in turns: the loop does both.
+    Step one, two;
+    auto step = [&](int t, const Step& st) __attribute__((always_inline)) {
         // S^T, tile by tile.
         f4 x[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             x[i] = f4{0, 0, 0, 0};
-            const float s = __uint_as_float(cur.ks[i] << 23);
+            const float s = __uint_as_float(st.ks[i] << 23);
 #pragma unroll
-            for (int k = 0; k < KS; k++) {
-                const bf8 kk = __builtin_bit_cast(bf8, decode8(cur.k[i][k], s));
+            for (int n = 0; n < KS; n++) {
+                const bf8 kk = __builtin_bit_cast(bf8, decode8(st.k[i][n], s));
 #pragma unroll
-                for (int p = 0; p < QP; p++) x[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, q[p][k], x[i], 0, 0, 0);
+                for (int p = 0; p < QP; p++) x[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, q[p][n], x[i], 0, 0, 0);
             }
         }
-        // V into LDS as bf16. Blocks that are NaN go in as (almost) zeros and
-        // are noted: a masked token's must not reach a row through 0 * NaN.
+        const int there = st.valid;
+        // Blocks of V that are NaN go into LDS as (almost) zeros and are noted:
+        // a masked token's must not reach a row through 0 * NaN.
         uint64_t bad[G];
 #pragma unroll
-        for (int i = 0; i < G; i++) {
-            const int tok = lane / G + i * VT;
-            const bool nan = cur.vs[i] == 255;
-            bad[i] = __ballot(nan);
-            const float s = __uint_as_float(nan ? 0 : cur.vs[i] << 23);
-            const uint32_t w[4] = {cur.v[i].x, cur.v[i].y, cur.v[i].z, cur.v[i].w};
-#pragma unroll
-            for (int d = 0; d < 4; d++)
-                *reinterpret_cast<uint4*>(vl + unit_at<D>(tok, (lane % G) * 2 + d / 2) + (d & 1) * 16) = decode8(w[d], s);
-        }
+        for (int i = 0; i < G; i++) bad[i] = __ballot(st.vs[i] == 255);
         // The softmax's step.
-        const bool masked = t + TOKENS > least || cur.valid != 15;
+        const bool masked = t + TOKENS > least || there != 15;
         float mx = NEG_INF;
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                if (masked && (t + 16 * i + 4 * g + r >= limit || !(cur.valid >> i & 1))) x[i][r] = NEG_INF;
+                if (masked && (t + 16 * i + 4 * g + r >= limit || !(there >> i & 1))) x[i][r] = NEG_INF;
                 mx = fmaxf(mx, x[i][r]);
             }
         mx = fmaxf(m, col_max(mx));
@@ -257,7 +290,7 @@ __global__ __launch_bounds__(256, 2) void cache_attn(CacheAttnArgs a) {
                 for (int r = 0; r < 4; r++) {
                     const int tok = 16 * i + 4 * g + r;
                     const uint32_t blocks = (uint32_t)(bad[16 * i / VT] >> (tok % VT * G)) & ((1u << G) - 1);
-                    if (t + tok < limit && (cur.valid >> i & 1)) hit |= blocks;
+                    if (t + tok < limit && (there >> i & 1)) hit |= blocks;
                 }
             hit = col_or(hit);
         }
@@ -268,9 +301,19 @@ __global__ __launch_bounds__(256, 2) void cache_attn(CacheAttnArgs a) {
                 x[i][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][r], a.qk_mul, -base));
                 l += x[i][r];
             }
-        // O^T += V^T P^T, 32 tokens a step: the lane's tokens of two tiles.
+        // O^T += V^T P^T, 32 tokens a step: V into the wave's part of LDS as
+        // bf16, then the lane's tokens of two tiles.
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
+#pragma unroll
+            for (int n = i * G / 4; n < (i + 2) * G / 4; n++) {
+                const float s = __uint_as_float(st.vs[n] == 255 ? 0 : st.vs[n] << 23);
+                const uint32_t w[4] = {st.v[n].x, st.v[n].y, st.v[n].z, st.v[n].w};
+#pragma unroll
+                for (int d = 0; d < 4; d++)
+                    *reinterpret_cast<uint4*>(vl + unit_at<D>((lane / G + n * VT) % HALF, (lane % G) * 2 + d / 2) +
+                                              (d & 1) * 16) = decode8(w[d], s);
+            }
             bf8 p[PP];
 #pragma unroll
             for (int r = 0; r < 8; r++) {
@@ -281,7 +324,7 @@ __global__ __launch_bounds__(256, 2) void cache_attn(CacheAttnArgs a) {
 #pragma unroll
             for (int u = 0; u < UNITS; u++) {
                 typedef __attribute__((address_space(3))) s4* lp;
-                const int tok = 16 * i + 4 * g + (col >> 2);
+                const int tok = 4 * g + (col >> 2);
                 const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vl + unit_at<D>(tok, u) + (col & 3) * 8));
                 const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vl + unit_at<D>(tok + 16, u) + (col & 3) * 8));
                 typedef short s8 __attribute__((ext_vector_type(8)));
@@ -291,19 +334,27 @@ __global__ __launch_bounds__(256, 2) void cache_attn(CacheAttnArgs a) {
                     o[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, vv), p[k], o[u], 0, 0, 0);
             }
         }
-        if (any_bad)
+        if (any_bad) {
+            asm volatile("" : "+v"(hit));  // a branch, not a select of every sum in every step
 #pragma unroll
             for (int u = 0; u < UNITS; u++)
                 if (hit >> (u / 2) & 1) o[u] = f4{1, 1, 1, 1} * __builtin_nanf("");
-        if (more) cur = nxt;
+        }
+    };
+    constexpr int STRIDE = 4 * TOKENS;
+    if (t_first < end) load(t_first, one);
+    for (int t = t_first; t < end; t += 2 * STRIDE) {
+        if (t + STRIDE < end) load(t + STRIDE, two);
+        step(t, one);
+        if (t + STRIDE >= end) break;
+        if (t + 2 * STRIDE < end) load(t + 2 * STRIDE, one);
+        step(t + STRIDE, two);
     }
     l = col_sum(l);
 
     // The four waves' parts meet in LDS.
-    constexpr int PAD = D + 4;
     __shared__ float wm[4][COLS], wl[4][COLS];
-    float* ol = reinterpret_cast<float*>(lds[0]);  // [4][COLS][PAD]
-    static_assert(4 * COLS * PAD * 4 <= sizeof lds, "");
+    float* ol = reinterpret_cast<float*>(lds);  // [4][COLS][PAD]
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < UNITS; u++) *reinterpret_cast<f4*>(ol + (wave * COLS + col) * PAD + 16 * u + 4 * g) = o[u];
@@ -383,14 +434,12 @@ __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
     const int chunk = split_tokens(seq.len, a.splits), t0 = split * chunk;
     if (split && t0 >= seq.len) return;
     const int c0 = first + 32 * wave;  // this wave's columns
+    const int least = seq.limit(c0 / a.group, a.causal);
+    const int end = min(t0 + chunk, seq.limit((min(first + CCOLS, cols) - 1) / a.group, a.causal));
     const int j = (c0 + col) / a.group, head = kvh * a.group + (c0 + col) - j * a.group;
     const long long row = seq.start + j;
     const bool have = c0 + col < cols && row >= 0 && row < c.rows;
-    const int limit = seq.limit(j, a.causal);
-    const int least = seq.limit(c0 / a.group, a.causal);
-    const int most = c0 < cols ? seq.limit((min(c0 + 32, cols) - 1) / a.group, a.causal) : 0;
-    const int end = min(t0 + chunk, seq.limit((min(first + CCOLS, cols) - 1) / a.group, a.causal));
-
+    const int limit = seq.limit(j, a.causal);  // this column sees slots below it
     bf8 q[QP][KS];
     {
         const uint16_t* p = a.q.p + row * a.q.st + head * a.q.sh + half * (D / 2);
@@ -412,47 +461,62 @@ __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
         }
     }
 
-    // This thread's part of a tile: token tok, 4 * WORDS bytes of codes.
+    // This thread's part of a tile: token tok of the tile, 4 * WORDS bytes of
+    // codes. A wave's sixteen tokens are of one page: its place is scalar, and
+    // the thread's offset in it never changes.
     const int tok = threadIdx.x >> 2, part = threadIdx.x & 3;
-    uint32_t kw[WORDS], vw[WORDS], ksc = 0, vsc = 0;
-    int there = 0;
-    auto load = [&](int t) {
-        const int page = cache_page(c, b, t + 16 * wave);
-        there = page >= 0;
-        const long long r = cache_row(c, max(page, 0), kvh, (t + 16 * wave) & ((1 << c.page_shift) - 1)) + (tok & 15);
-        const uint8_t *kp = c.k_codes + r * (D / 2) + part * (D / 8), *vp = c.v_codes + r * (D / 2) + part * (D / 8);
+    const uint32_t code_at = (tok & 15) * (D / 2) + part * (D / 8);
+    const uint32_t in_page = (1u << c.page_shift) - 1;
+    struct Part {
+        uint32_t w[WORDS], sc;
+    } kr, vr;
+    bool v_there = false;
+    Pages pages(c, b, lane, t0 + 16 * wave);
+    auto page_of = [&](int t) { return t < end ? pages.of(t + 16 * wave) : -1; };
+    auto load_codes = [&](const uint8_t* codes, Part& r, long long row0) {
+        const uint8_t* p = codes + row0 * (D / 2) + code_at;
         if constexpr (D == 128) {
-            const uint4 x = *reinterpret_cast<const uint4*>(kp), y = *reinterpret_cast<const uint4*>(vp);
-            kw[0] = x.x, kw[1] = x.y, kw[2] = x.z, kw[3] = x.w;
-            vw[0] = y.x, vw[1] = y.y, vw[2] = y.z, vw[3] = y.w;
-            ksc = *reinterpret_cast<const uint32_t*>(c.k_scales + r * G);
+            const uint4 x = *reinterpret_cast<const uint4*>(p);
+            r.w[0] = x.x, r.w[1] = x.y, r.w[2] = x.z, r.w[3] = x.w;
         } else {
-            const uint2 x = *reinterpret_cast<const uint2*>(kp), y = *reinterpret_cast<const uint2*>(vp);
-            kw[0] = x.x, kw[1] = x.y;
-            vw[0] = y.x, vw[1] = y.y;
-            ksc = *reinterpret_cast<const uint16_t*>(c.k_scales + r * G);
+            const uint2 x = *reinterpret_cast<const uint2*>(p);
+            r.w[0] = x.x, r.w[1] = x.y;
         }
-        vsc = c.v_scales[r * G + part * G / 4];
     };
-    auto store = [&](int buf) {
-        // K: the row's 16-byte (D = 64: 8-byte) units permuted by the token.
-        if constexpr (D == 128) {
-            *reinterpret_cast<uint4*>(lds.k[buf] + tok * 64 + ((part ^ (tok >> 1 & 3)) << 4)) = make_uint4(kw[0], kw[1], kw[2], kw[3]);
-        } else {
-            *reinterpret_cast<uint2*>(lds.k[buf] + tok * 32 + (((part >> 1) ^ (tok >> 2 & 1)) << 4) + (part & 1) * 8) = make_uint2(kw[0], kw[1]);
-        }
-        if (part == 0) lds.ks[buf][tok] = ksc;
-        const bool nan = vsc == 255;
+    auto row_of = [&](int t, int page) { return cache_row(c, max(page, 0), kvh, (t + 16 * wave) & in_page); };
+    auto load_k = [&](int t, int page) {
+        const long long row0 = row_of(t, page);
+        load_codes(c.k_codes, kr, row0);
+        const uint8_t* p = c.k_scales + row0 * G + (tok & 15) * G;
+        kr.sc = D == 128 ? *reinterpret_cast<const uint32_t*>(p) : *reinterpret_cast<const uint16_t*>(p);
+    };
+    auto load_v = [&](int t, int page) {
+        const long long row0 = row_of(t, page);
+        load_codes(c.v_codes, vr, row0);
+        vr.sc = (c.v_scales + row0 * G)[(tok & 15) * G + part * G / 4];
+        v_there = page >= 0;
+    };
+    const int k_at = D == 128 ? tok * 64 + ((part ^ (tok >> 1 & 3)) << 4)
+                              : tok * 32 + (((part >> 1) ^ (tok >> 2 & 1)) << 4) + (part & 1) * 8;
+    auto store_k = [&](int buf) {  // the row's 16-byte units permuted by the token
+        if constexpr (D == 128)
+            *reinterpret_cast<uint4*>(lds.k[buf] + k_at) = make_uint4(kr.w[0], kr.w[1], kr.w[2], kr.w[3]);
+        else
+            *reinterpret_cast<uint2*>(lds.k[buf] + k_at) = make_uint2(kr.w[0], kr.w[1]);
+        if (part == 0) lds.ks[buf][tok] = kr.sc;
+    };
+    auto store_v = [&](int buf) {
+        const bool nan = vr.sc == 255;
         const uint64_t bad = __ballot(D == 128 ? nan : nan && !(part & 1));
         if (lane == 0) {
             lds.bad[buf][wave] = bad;
-            lds.flags[buf][wave] = (bad != 0) | (there ? 0 : 2);
+            lds.flags[buf][wave] = (bad != 0) | (v_there ? 0 : 2);
         }
-        const float s = __uint_as_float(nan ? 0 : vsc << 23);
+        const float s = __uint_as_float(nan ? 0 : vr.sc << 23);
 #pragma unroll
         for (int w = 0; w < WORDS; w++) {
             const int ch = part * (D / 4) + 8 * w;
-            *reinterpret_cast<uint4*>(lds.v[buf] + unit_at<D>(tok, ch / 16) + (ch & 8) * 2) = decode8(vw[w], s);
+            *reinterpret_cast<uint4*>(lds.v[buf] + unit_at<D>(tok, ch / 16) + (ch & 8) * 2) = decode8(vr.w[w], s);
         }
     };
 
@@ -462,116 +526,125 @@ __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; i++) o[u][i] = 0.0f;
     float m = NEG_INF, l = 0.0f;
-    // A transposing read's place in a tile: lanes 0-15 and 32-47 the first 16
-    // of 32 channels, tokens 4 * half + (lane % 16) / 4.
+    // Where a lane reads K's codes, and the place of a transposing read of V:
+    // lanes 0-15 and 32-47 the first 16 of 32 channels, tokens 4 * half +
+    // (lane % 16) / 4.
+    const int kx = D == 128 ? (col >> 1 & 3) : (col >> 2 & 1);
+    const int kr_at = col * (D / 2), ks_shift = half * (KS / 4) * 8;
     const int vtok = 4 * half + (lane >> 2 & 3), vunit = lane >> 4 & 1, vbyte = (lane & 3) * 8;
+    auto scores = [&](int buf, int sub, f16v& y) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) y[i] = 0.0f;
+        uint32_t w[KS];
+#pragma unroll
+        for (int u = 0; u < KS / 4; u++) {
+            const uint4 z = *reinterpret_cast<const uint4*>(lds.k[buf] + sub * 32 * (D / 2) + kr_at +
+                                                            (((D == 128 ? half * 2 + u : half) ^ kx) << 4));
+            w[4 * u] = z.x, w[4 * u + 1] = z.y, w[4 * u + 2] = z.z, w[4 * u + 3] = z.w;
+        }
+        const uint32_t sc = lds.ks[buf][32 * sub + col] >> ks_shift;
+        const float sf[2] = {__uint_as_float((sc & 255) << 23), __uint_as_float((sc >> 8 & 255) << 23)};
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            const bf8 kk = __builtin_bit_cast(bf8, decode8(w[s], sf[s / 4]));
+#pragma unroll
+            for (int p = 0; p < QP; p++) y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kk, q[p][s], y, 0, 0, 0);
+        }
+    };
 
     if (t0 < end) {
-        load(t0);
-        store(0);
-        if (t0 + TOKENS < end) load(t0 + TOKENS);
+        const int page = page_of(t0);
+        load_k(t0, page);
+        load_v(t0, page);
+        store_k(0);
+        store_v(0);
+        const int next = page_of(t0 + TOKENS);
+        load_k(t0 + TOKENS, next);
+        load_v(t0 + TOKENS, next);
     }
     __syncthreads();
     int buf = 0;
     for (int t = t0; t < end; t += TOKENS, buf ^= 1) {
         if (t + TOKENS < end) {
-            store(buf ^ 1);
-            if (t + 2 * TOKENS < end) load(t + 2 * TOKENS);
+            store_k(buf ^ 1);
+            store_v(buf ^ 1);
+            const int page = page_of(t + 2 * TOKENS);
+            load_k(t + 2 * TOKENS, page);
+            load_v(t + 2 * TOKENS, page);
         }
-        if (t < most) {
-            f16v x[2];
-#pragma unroll
-            for (int sub = 0; sub < 2; sub++) {
-                const int tk = 32 * sub + col;
-#pragma unroll
-                for (int i = 0; i < 16; i++) x[sub][i] = 0.0f;
-                uint32_t w[KS];
-#pragma unroll
-                for (int u = 0; u < KS / 4; u++) {
-                    const uint4 y = D == 128
-                        ? *reinterpret_cast<const uint4*>(lds.k[buf] + tk * 64 + (((half * 2 + u) ^ (tk >> 1 & 3)) << 4))
-                        : *reinterpret_cast<const uint4*>(lds.k[buf] + tk * 32 + ((half ^ (tk >> 2 & 1)) << 4));
-                    w[4 * u] = y.x, w[4 * u + 1] = y.y, w[4 * u + 2] = y.z, w[4 * u + 3] = y.w;
-                }
-                const uint32_t sc = lds.ks[buf][tk] >> (half * (KS / 4) * 8);
-#pragma unroll
-                for (int s = 0; s < KS; s++) {
-                    const bf8 kk = __builtin_bit_cast(bf8, decode8(w[s], __uint_as_float((sc >> (s / 4 * 8) & 255) << 23)));
-#pragma unroll
-                    for (int p = 0; p < QP; p++) x[sub] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kk, q[p][s], x[sub], 0, 0, 0);
-                }
-            }
-            const int4 fl = *reinterpret_cast<const int4*>(lds.flags[buf]);
-            const int flags = __builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w);
-            uint32_t hit = 0;
-            if (flags || t + TOKENS > least) {
-                const int fi[4] = {fl.x, fl.y, fl.z, fl.w};
-#pragma unroll
-                for (int sub = 0; sub < 2; sub++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const int k = 32 * sub + 8 * (i / 4) + 4 * half + i % 4, six = 2 * sub + i / 8;
-                        const bool seen = t + k < limit && !(fi[six] & 2);
-                        if (!seen) x[sub][i] = NEG_INF;
-                        if (flags & 1) {
-                            const uint32_t blocks = (uint32_t)(lds.bad[buf][six] >> ((k & 15) * 4)) & 15;
-                            if (seen) hit |= blocks;
-                        }
-                    }
-                if (flags & 1) {
-                    auto r = __builtin_amdgcn_permlane32_swap(hit, hit, false, false);
-                    hit = r[0] | r[1];
-                }
-            }
-            float mx = NEG_INF;
+        f16v x[2];
+        scores(buf, 0, x[0]);
+        scores(buf, 1, x[1]);
+        const int4 fl = *reinterpret_cast<const int4*>(lds.flags[buf]);
+        const int flags = __builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w);
+        uint32_t hit = 0;
+        if (flags || t + TOKENS > least) {
+            const int fi[4] = {fl.x, fl.y, fl.z, fl.w};
 #pragma unroll
             for (int sub = 0; sub < 2; sub++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) mx = fmaxf(mx, x[sub][i]);
-            {
-                auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-                mx = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-            }
-            mx = fmaxf(m, mx);
-            if (__any((mx - m) * a.qk_mul > SLACK)) {
-                const float scale = __builtin_amdgcn_exp2f((m - (mx == NEG_INF ? 0.0f : mx)) * a.qk_mul);
-                m = mx;
-                l *= scale;
-#pragma unroll
-                for (int u = 0; u < CT; u++) o[u] *= scale;
-            }
-            const float base = m == NEG_INF ? 0.0f : m * a.qk_mul;
-#pragma unroll
-            for (int sub = 0; sub < 2; sub++)
-#pragma unroll
-                for (int st = 0; st < 2; st++) {
-                    bf8 p[PP];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[sub][8 * st + i], a.qk_mul, -base));
-                        l += e;
-                        p[0][i] = (__bf16)e;
-                        if (PP == 2) p[PP - 1][i] = (__bf16)(e - (float)p[0][i]);
-                    }
-#pragma unroll
-                    for (int u = 0; u < CT; u++) {
-                        typedef __attribute__((address_space(3))) s4* lp;
-                        typedef short s8 __attribute__((ext_vector_type(8)));
-                        const uint8_t* v = lds.v[buf] + (32 * sub + 16 * st) * (D * 2) + unit_at<D>(vtok, 2 * u + vunit) + vbyte;
-                        const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(v));
-                        const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(v + 8 * (D * 2)));
-                        const s8 vv = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-                        for (int k = 0; k < PP; k++)
-                            o[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, vv), p[k], o[u], 0, 0, 0);
+                for (int i = 0; i < 16; i++) {
+                    const int k = 32 * sub + 8 * (i / 4) + 4 * half + i % 4, six = 2 * sub + i / 8;
+                    const bool seen = t + k < limit && !(fi[six] & 2);
+                    if (!seen) x[sub][i] = NEG_INF;
+                    if (flags & 1) {
+                        const uint32_t blocks = (uint32_t)(lds.bad[buf][six] >> ((k & 15) * 4)) & 15;
+                        if (seen) hit |= blocks;
                     }
                 }
-            if (flags & 1)
+            if (flags & 1) {
+                auto r = __builtin_amdgcn_permlane32_swap(hit, hit, false, false);
+                hit = r[0] | r[1];
+            }
+        }
+        float mx = NEG_INF;
 #pragma unroll
-                for (int u = 0; u < CT; u++)
-                    if (hit >> (D == 128 ? u : 2 * u) & 1)
+        for (int sub = 0; sub < 2; sub++)
 #pragma unroll
-                        for (int i = 0; i < 16; i++) o[u][i] = __builtin_nanf("");
+            for (int i = 0; i < 16; i++) mx = fmaxf(mx, x[sub][i]);
+        {
+            auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+            mx = fmaxf(m, fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+        }
+        if (__any((mx - m) * a.qk_mul > SLACK)) {
+            const float scale = __builtin_amdgcn_exp2f((m - (mx == NEG_INF ? 0.0f : mx)) * a.qk_mul);
+            m = mx;
+            l *= scale;
+#pragma unroll
+            for (int u = 0; u < CT; u++) o[u] *= scale;
+        }
+        const float base = m == NEG_INF ? 0.0f : m * a.qk_mul;
+#pragma unroll
+        for (int sub = 0; sub < 2; sub++)
+#pragma unroll
+            for (int st = 0; st < 2; st++) {
+                bf8 p[PP];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[sub][8 * st + i], a.qk_mul, -base));
+                    l += e;
+                    p[0][i] = (__bf16)e;
+                    if (PP == 2) p[PP - 1][i] = (__bf16)(e - (float)p[0][i]);
+                }
+#pragma unroll
+                for (int u = 0; u < CT; u++) {
+                    typedef __attribute__((address_space(3))) s4* lp;
+                    typedef short s8 __attribute__((ext_vector_type(8)));
+                    const uint8_t* v = lds.v[buf] + (32 * sub + 16 * st) * (D * 2) + unit_at<D>(vtok, 2 * u + vunit) + vbyte;
+                    const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(v));
+                    const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(v + 8 * (D * 2)));
+                    const bf8 vv = __builtin_bit_cast(bf8, (s8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                    for (int k = 0; k < PP; k++) o[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv, p[k], o[u], 0, 0, 0);
+                }
+            }
+        if (flags & 1) {
+            asm volatile("" : "+v"(hit));  // a branch, not a select of every sum in every step
+#pragma unroll
+            for (int u = 0; u < CT; u++)
+                if (hit >> (D == 128 ? u : 2 * u) & 1)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) o[u][i] = __builtin_nanf("");
         }
         __syncthreads();
     }
@@ -599,7 +672,8 @@ __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
         for (int u = 0; u < CT; u++)
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<f4*>(a.part_o + at * D + 32 * u + 2 * i + 4 * half) = f4{o[u][i], o[u][i + 1], o[u][i + 2], o[u][i + 3]};
+                *reinterpret_cast<f4*>(a.part_o + at * D + 32 * u + 2 * i + 4 * half) =
+                    f4{o[u][i], o[u][i + 1], o[u][i + 2], o[u][i + 3]};
         if (half == 0) {
             a.part_ml[at * 2] = m * a.qk_mul;
             a.part_ml[at * 2 + 1] = l;
@@ -607,75 +681,84 @@ __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
     }
 }
 
-// The splits' parts of one (row, head) joined by a workgroup: every group of
-// D / 8 lanes sums the splits that fall to it, eight channels a lane, and the
-// groups' sums are added in their order, so the same call gives the same bits.
-template <int D>
+// The splits' parts joined, every (row, head) by as many groups of D / 8 lanes
+// (eight channels a lane) as SHARE says: all of a workgroup's where there are
+// many splits of few rows, else one. A group sums the splits that fall to it
+// in their order and the groups' sums are added in theirs: the same call gives
+// the same bits.
+template <int D, bool SHARE>
 __global__ __launch_bounds__(256) void cache_attn_join(CacheAttnArgs a) {
     constexpr int LANES = D / 8, GROUPS = 256 / LANES;
-    __shared__ float ws[MAX_SPLITS], sums[GROUPS][D + 4];
+    __shared__ float sums[SHARE ? GROUPS : 1][D + 4], ls[GROUPS];
     const CacheDev& c = a.c;
-    const int b = blockIdx.z, j = blockIdx.x / a.heads, h = blockIdx.x - j * a.heads;
+    const int b = blockIdx.z, grp = threadIdx.x / LANES, ch = (threadIdx.x % LANES) * 8;
+    const int pair = SHARE ? blockIdx.x : blockIdx.x * GROUPS + grp, j = pair / a.heads, h = pair - j * a.heads;
     const SequenceIndex seq = sequence_index(c, b, a.max_new);
     const long long row = seq.start + j;
-    if (j >= seq.n || row < 0 || row >= c.rows) return;
+    if (j >= seq.n || row < 0 || row >= c.rows) return;  // (SHARE: all threads or none)
     const int chunk = split_tokens(seq.len, a.splits), parts = seq.len ? (seq.len + chunk - 1) / chunk : 1;
     const long long at = row * a.heads + h, step = (long long)c.rows * a.heads;
-    // Maximum over the splits, and their weights (every wave for itself).
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const f2* ml = reinterpret_cast<const f2*>(a.part_ml) + at;
+    // The maximum over all splits, then this group's share of the sums.
     float m = NEG_INF, l = 0.0f;
-    for (int p = lane; p < parts; p += 64) m = fmaxf(m, a.part_ml[(at + p * step) * 2]);
-    m = wave_max(m);
+    for (int p = threadIdx.x % LANES; p < parts; p += LANES) m = fmaxf(m, ml[p * step].x);
+    m = row_max<LANES>(m);
     const float base = m == NEG_INF ? 0.0f : m;
-    for (int p = lane; p < parts; p += 64) {
-        const float w = __builtin_amdgcn_exp2f(a.part_ml[(at + p * step) * 2] - base);
-        l += w * a.part_ml[(at + p * step) * 2 + 1];
-        if (wave == 0) ws[p] = w;
-    }
-#pragma unroll
-    for (int i = 32; i; i >>= 1) l += __shfl_xor(l, i);
-    __syncthreads();
-    const int grp = threadIdx.x / LANES, ch = (threadIdx.x % LANES) * 8;
     f4 f[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
 #pragma unroll 4
-    for (int p = grp; p < parts; p += GROUPS) {
+    for (int p = SHARE ? grp : 0; p < parts; p += SHARE ? GROUPS : 1) {
+        const f2 s = ml[p * step];
         const f4* o = reinterpret_cast<const f4*>(a.part_o + (at + p * step) * D + ch);
-        f[0] += o[0] * ws[p];
-        f[1] += o[1] * ws[p];
+        const float w = __builtin_amdgcn_exp2f(s.x - base);
+        l += w * s.y;
+        f[0] += o[0] * w;
+        f[1] += o[1] * w;
     }
-    *reinterpret_cast<f4*>(&sums[grp][ch]) = f[0];
-    *reinterpret_cast<f4*>(&sums[grp][ch + 4]) = f[1];
-    __syncthreads();
-    if (threadIdx.x >= D / 2) return;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    float x = 0.0f, y = 0.0f;
+    if (SHARE) {
+        *reinterpret_cast<f4*>(&sums[grp][ch]) = f[0];
+        *reinterpret_cast<f4*>(&sums[grp][ch + 4]) = f[1];
+        ls[grp] = l;
+        __syncthreads();
+        if (grp) return;
+        l = 0.0f, f[0] = f[1] = f4{0, 0, 0, 0};
 #pragma unroll
-    for (int g = 0; g < GROUPS; g++) x += sums[g][2 * threadIdx.x], y += sums[g][2 * threadIdx.x + 1];
-    *reinterpret_cast<uint32_t*>(a.out.p + row * a.out.st + h * a.out.sh + 2 * threadIdx.x) =
-        a.out_f16 ? pack_f16x2(x * inv, y * inv) : pack_bf16x2(x * inv, y * inv);
+        for (int g = 0; g < GROUPS; g++) {
+            l += ls[g];
+            f[0] += *reinterpret_cast<const f4*>(&sums[SHARE ? g : 0][ch]);
+            f[1] += *reinterpret_cast<const f4*>(&sums[SHARE ? g : 0][ch + 4]);
+        }
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float x = f[i / 2][i % 2 * 2] * inv, y = f[i / 2][i % 2 * 2 + 1] * inv;
+        w[i] = a.out_f16 ? pack_f16x2(x, y) : pack_bf16x2(x, y);
+    }
+    *reinterpret_cast<uint4*>(a.out.p + row * a.out.st + h * a.out.sh + ch) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 }  // namespace
 
-#ifndef SPLIT_TARGET
-#define SPLIT_TARGET 4096
-#endif
 // Whether a call runs the chunk kernel.
-static bool in_chunks(int max_new, int group) { return (long long)max_new * group > 64; }
+static bool in_chunks(int batch, int kv_heads, int group, int max_new, int max_tokens) {
+    const long long cols = (long long)max_new * group;
+    return cols > 64 && (max_tokens > 2048 || (cols + CCOLS - 1) / CCOLS * kv_heads * batch >= 512);
+}
 
 int cache_splits(int head_dim, int batch, int kv_heads, int group, int max_new, int max_tokens) {
     (void)head_dim;
-    const int per = in_chunks(max_new, group) ? CCOLS : COLS;
+    const int per = in_chunks(batch, kv_heads, group, max_new, max_tokens) ? CCOLS : COLS;
     const long long tiles = ((long long)max_new * group + per - 1) / per;
     const long long units = tiles * kv_heads * batch;
     const long long most = (max_tokens + 511) / 512;
-    if (per == CCOLS) return (int)std::max(1ll, std::min({most, 512 / std::max(units, 1ll), (long long)MAX_SPLITS}));
-    return (int)std::max(1ll, std::min({most, SPLIT_TARGET / std::max(units, 1ll), (long long)MAX_SPLITS}));
+    if (per != COLS) return (int)std::max(1ll, std::min({most, 512 / std::max(units, 1ll), (long long)MAX_SPLITS}));
+    return (int)std::max(1ll, std::min({most, 2048 / std::max(units, 1ll), (long long)MAX_SPLITS}));
 }
 
 template <int D>
 static hipError_t launch(const CacheAttnArgs& a, hipStream_t s) {
-    const int per = in_chunks(a.max_new, a.group) ? CCOLS : COLS;
+    const int per = in_chunks(a.c.batch, a.c.kv_heads, a.group, a.max_new, a.c.max_pages << a.c.page_shift) ? CCOLS : COLS;
     const unsigned tiles = (unsigned)(((long long)a.max_new * a.group + per - 1) / per);
     const dim3 grid(tiles * a.splits, a.c.kv_heads, a.c.batch), block(256);
     const auto go = [&](auto qp, auto pp) {
@@ -691,8 +774,14 @@ static hipError_t launch(const CacheAttnArgs& a, hipStream_t s) {
         a.out_f16 ? go(two, two) : go(two, one);
     else
         a.out_f16 ? go(one, two) : go(one, one);
-    if (a.splits > 1)
-        hipLaunchKernelGGL((cache_attn_join<D>), dim3((unsigned)a.max_new * a.heads, 1, a.c.batch), block, 0, s, a);
+    if (a.splits > 1) {
+        const long long pairs = (long long)a.max_new * a.heads;
+        constexpr int PER = 256 / (D / 8);
+        if (a.splits > 8 && pairs * a.c.batch <= 4096)
+            hipLaunchKernelGGL((cache_attn_join<D, true>), dim3((unsigned)pairs, 1, a.c.batch), block, 0, s, a);
+        else
+            hipLaunchKernelGGL((cache_attn_join<D, false>), dim3((unsigned)((pairs + PER - 1) / PER), 1, a.c.batch), block, 0, s, a);
+    }
     return hipGetLastError();
 }
 
