@@ -315,6 +315,8 @@ sage_status set_error(sage_status st, const char* fmt, ...) {
     return st;
 }
 
+sage_status succeeded() { return ok(); }
+
 sage_status workspace_layout(const sage_attention* s, const sage_shape* shape, const sage_kv_merge* merge,
                              sage_plan* plan_out, WsSizes* n) {
     sage_kv_merge dense{};

@@ -10,6 +10,7 @@
 #include "sage_internal.hpp"
 
 using sage::set_error;
+using sage::succeeded;
 
 struct sage_cache_workspace {
     sage_cache_shape shape;
@@ -29,7 +30,7 @@ sage_status hip_failed(hipError_t e, const char* what) {
 
 sage_status done(hipError_t e, const char* what) {
     if (e != hipSuccess) return hip_failed(e, what);
-    return set_error(SAGE_OK, "%s", "");
+    return succeeded();
 }
 
 // The kernels run on the current device; the context's stream and the memory
@@ -194,13 +195,13 @@ sage_status sage_rotary_table(uint64_t rot, uint64_t positions, double base, con
             out[(p * (rot / 2) + i) * 2 + 1] = (float)(attention * std::sin(a));
         }
     }
-    return set_error(SAGE_OK, "%s", "");
+    return succeeded();
 }
 
 sage_status sage_rotary_apply(const sage_attention* s, const sage_shape* shape, const sage_rotary* rotary,
                               const sage_tensor* x, const sage_tensor_mut* out, int32_t transpose) {
     if (!s || !shape || !rotary || !x || !out) return set_error(SAGE_ERR_INVALID, "null argument");
-    if (shape->batch == 0 || shape->tokens == 0 || shape->heads == 0) return set_error(SAGE_OK, "%s", "");
+    if (shape->batch == 0 || shape->tokens == 0 || shape->heads == 0) return succeeded();
     uint64_t rows;
     if (__builtin_mul_overflow(shape->batch, shape->tokens, &rows) || rows > I32 || shape->heads > I32)
         return set_error(SAGE_ERR_INVALID, "rotary: %llu x %llu rows of %llu heads do not fit in i32", (u64)shape->batch,
@@ -232,7 +233,7 @@ sage_status sage_cache_sizes(const sage_cache_shape* shape, uint64_t head_dim, u
     if (st != SAGE_OK) return st;
     *codes = code_rows(*shape) * (head_dim / 2);
     *scales = code_rows(*shape) * (head_dim / sage::CACHE_BLOCK);
-    return set_error(SAGE_OK, "%s", "");
+    return succeeded();
 }
 
 sage_status sage_cache_append(const sage_attention* s, const sage_cache_shape* shape, const sage_cache* cache,
@@ -253,7 +254,7 @@ sage_status sage_cache_append(const sage_attention* s, const sage_cache_shape* s
     if (st == SAGE_OK && rotary) st = rotary_checked(rotary, d, shape->rows, 0, &a.r);
     if (st == SAGE_OK) st = on_device(s);
     if (st != SAGE_OK) return st;
-    if (shape->rows == 0 || shape->batch == 0) return set_error(SAGE_OK, "%s", "");
+    if (shape->rows == 0 || shape->batch == 0) return succeeded();
     a.k = rows_of(k);
     a.v = rows_of(v);
     if (q) {
@@ -276,7 +277,7 @@ sage_status sage_cache_read(const sage_attention* s, const sage_cache_shape* sha
     if (st == SAGE_OK && k->dtype != v->dtype) st = set_error(SAGE_ERR_INVALID, "K and V must share one element type");
     if (st == SAGE_OK) st = on_device(s);
     if (st != SAGE_OK) return st;
-    if (shape->rows == 0 || shape->batch == 0) return set_error(SAGE_OK, "%s", "");
+    if (shape->rows == 0 || shape->batch == 0) return succeeded();
     a.k = rows_of(k);
     a.v = rows_of(v);
     a.f16 = k->dtype == SAGE_F16;
@@ -309,7 +310,7 @@ sage_status sage_cache_workspace_new(const sage_attention* s, const sage_cache_s
         }
     }
     *out = w;
-    return set_error(SAGE_OK, "%s", "");
+    return succeeded();
 }
 
 void sage_cache_workspace_destroy(sage_cache_workspace* ws) {
@@ -337,7 +338,7 @@ sage_status sage_cache_attend(const sage_attention* s, const sage_cache_workspac
     if (st == SAGE_OK) st = view(out, h.rows, h.heads, d, "output");
     if (st == SAGE_OK) st = on_device(s);
     if (st != SAGE_OK) return st;
-    if (h.rows == 0 || h.batch == 0 || h.max_new == 0) return set_error(SAGE_OK, "%s", "");
+    if (h.rows == 0 || h.batch == 0 || h.max_new == 0) return succeeded();
     a.q = rows_of(q);
     a.out = rows_of(out);
     a.heads = (int)h.heads;

@@ -112,6 +112,8 @@ sage_status noalloc_init(int device);
 
 // Sets this thread's sage_last_error() text; returns st.
 sage_status set_error(sage_status st, const char* fmt, ...);
+// Clears it; returns SAGE_OK.
+sage_status succeeded();
 
 // Plan::new plus the buffer sizes of SageAttention::workspace for shape and
 // merge (NULL = dense), with the same refusals.

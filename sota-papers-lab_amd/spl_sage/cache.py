@@ -32,9 +32,13 @@ class CacheShape:
     page_tokens: int
     max_pages: int
 
+    def __post_init__(self):
+        c = _abi.sage_cache_shape(self.batch, self.rows, self.max_new, self.heads, self.kv_heads, self.pages,
+                                  self.page_tokens, self.max_pages)
+        object.__setattr__(self, "_struct", c)
+
     def _c(self) -> _abi.sage_cache_shape:
-        return _abi.sage_cache_shape(self.batch, self.rows, self.max_new, self.heads, self.kv_heads, self.pages,
-                                     self.page_tokens, self.max_pages)
+        return self._struct
 
     def sizes(self, head_dim: int) -> tuple:
         """Bytes of the codes and of the scales, each for K and for V."""
@@ -51,11 +55,12 @@ def _bytes(t, what: str) -> tuple:
     return t.data_ptr(), t.numel()
 
 
-@dataclass
+@dataclass(frozen=True)
 class PagedCache:
     """The pool: uint8 device tensors [pages][kv_heads][page_tokens][head_dim/2]
-    (codes) and [..][head_dim/32] (scales). One pool serves steps of any shape
-    with its pages, page_tokens and kv_heads (with_shape)."""
+    (codes) and [..][head_dim/32] (scales). Made once for its tensors; one pool
+    serves steps of any shape with its pages, page_tokens and kv_heads
+    (with_shape)."""
 
     shape: CacheShape
     k_codes: object
@@ -76,24 +81,33 @@ class PagedCache:
     def with_shape(self, shape: CacheShape) -> "PagedCache":
         return PagedCache(shape, self.k_codes, self.k_scales, self.v_codes, self.v_scales)
 
-    def _c(self) -> _abi.sage_cache:
+    def __post_init__(self):
         kc, ks = _bytes(self.k_codes, "cache K codes"), _bytes(self.k_scales, "cache K scales")
         vc, vs = _bytes(self.v_codes, "cache V codes"), _bytes(self.v_scales, "cache V scales")
-        return _abi.sage_cache(kc[0], ks[0], vc[0], vs[0], min(kc[1], vc[1]), min(ks[1], vs[1]))
+        c = _abi.sage_cache(kc[0], ks[0], vc[0], vs[0], min(kc[1], vc[1]), min(ks[1], vs[1]))
+        object.__setattr__(self, "_struct", c)
+
+    def _c(self) -> _abi.sage_cache:
+        return self._struct
 
 
-@dataclass
+@dataclass(frozen=True)
 class CacheIndex:
     """int32 device tensors: starts [batch + 1], lengths [batch] (this step's
-    rows included), page_table [batch][max_pages]."""
+    rows included), page_table [batch][max_pages]. Made once for its tensors,
+    whose contents change from step to step."""
 
     starts: object
     lengths: object
     page_table: object
 
+    def __post_init__(self):
+        c = _abi.sage_cache_index(*_ints(self.starts, "cache starts"), *_ints(self.lengths, "cache lengths"),
+                                  *_ints(self.page_table, "cache page table"))
+        object.__setattr__(self, "_struct", c)
+
     def _c(self) -> _abi.sage_cache_index:
-        return _abi.sage_cache_index(*_ints(self.starts, "cache starts"), *_ints(self.lengths, "cache lengths"),
-                                     *_ints(self.page_table, "cache page table"))
+        return self._struct
 
 
 class CacheWorkspace:

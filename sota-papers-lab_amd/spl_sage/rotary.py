@@ -79,23 +79,28 @@ def _ints(t, what: str) -> tuple:
     return t.data_ptr(), t.numel()
 
 
-@dataclass
+@dataclass(frozen=True)
 class Rotary:
     """An uploaded RotaryTable with its layout, and the rows' positions (int32
-    device tensor; None: the token's index, or its slot in cache_append)."""
+    device tensor; None: the token's index, or its slot in cache_append). Made
+    once for its tensors, whose contents may change."""
 
     table: object
     rot: int
     layout: RotaryLayout = RotaryLayout.Half
     positions: object = None
 
-    def _c(self) -> _abi.sage_rotary:
+    def __post_init__(self):
         import torch
 
         if self.table.dtype != torch.float32 or not self.table.is_contiguous():
             raise SageError(1, f"the rotary table must be a contiguous float32 device tensor, got {self.table.dtype}")
         p, n = (None, 0) if self.positions is None else _ints(self.positions, "rotary positions")
-        return _abi.sage_rotary(self.table.data_ptr(), self.table.numel(), self.rot, int(self.layout), p, n)
+        c = _abi.sage_rotary(self.table.data_ptr(), self.table.numel(), self.rot, int(self.layout), p, n)
+        object.__setattr__(self, "_struct", c)
+
+    def _c(self) -> _abi.sage_rotary:
+        return self._struct
 
 
 __all__ = ["RotaryLayout", "ScalingKind", "RotaryScaling", "RotaryTable", "Rotary"]

@@ -91,18 +91,17 @@ def test_wrong_types_are_refused():
     from spl_sage import rotary as R
 
     with pytest.raises(SageError, match="float32"):
-        R.Rotary(torch.zeros(8, dtype=torch.float64), 4)._c()
+        R.Rotary(torch.zeros(8, dtype=torch.float64), 4)
     with pytest.raises(SageError, match="int32"):
-        R.Rotary(torch.zeros(8), 4, positions=torch.zeros(4, dtype=torch.int64))._c()
+        R.Rotary(torch.zeros(8), 4, positions=torch.zeros(4, dtype=torch.int64))
     i = torch.zeros(4, dtype=torch.int32)
     with pytest.raises(SageError, match="int32"):
-        K.CacheIndex(i, i, i.view(2, 2).t())._c()
+        K.CacheIndex(i, i, i.view(2, 2).t())
     shape = K.CacheShape(1, 1, 1, 1, 1, 1, 16, 1)
     assert shape.sizes(64) == (512, 32)
     c = K.PagedCache.new(shape, 64, device="cpu")
-    c.k_codes = c.k_codes.to(torch.int8)
     with pytest.raises(SageError, match="uint8"):
-        c._c()
+        K.PagedCache(shape, c.k_codes.to(torch.int8), c.k_scales, c.v_codes, c.v_scales)
     with pytest.raises(SageError, match="pages of 17 tokens"):
         K.PagedCache.new(K.CacheShape(1, 1, 1, 1, 1, 1, 17, 1), 64, device="cpu")
 
