@@ -53,8 +53,8 @@ struct ReadArgs {
     int f16;
 };
 
-// One attention call. part: the partial outputs of split sequences, [split]
-// [row][head] of D floats, then [split][row][head] of (maximum, sum) pairs.
+// One attention call. part_o, part_ml: the partial outputs of split sequences,
+// D floats and a (maximum, sum) pair each.
 struct CacheAttnArgs {
     RowView q, out;
     CacheDev c;
@@ -63,16 +63,24 @@ struct CacheAttnArgs {
     float qk_mul;     // |softmax scale| * log2(e), over 0
     uint32_t q_sign;  // 0x80008000 under a negative scale: the queries' signs
     int heads, group, max_new, causal, q_f16, out_f16;
-    int splits;  // workgroups that a sequence's keys are split over, at most
+    int splits;  // chunks: workgroups that a sequence's keys are split over, at most
+    int whole;   // few rows: a workgroup a unit
 };
 
 hipError_t launch_rotary(int head_dim, const RotaryArgs& a, hipStream_t s);
 hipError_t launch_cache_append(int head_dim, const AppendArgs& a, hipStream_t s);
 hipError_t launch_cache_read(int head_dim, const ReadArgs& a, hipStream_t s);
-hipError_t launch_cache_attend(int head_dim, const CacheAttnArgs& a, hipStream_t s);
-// Workgroups that launch_cache_attend splits a sequence's keys over (1: none;
-// no partial outputs). max_tokens: most tokens that the page table holds.
-int cache_splits(int head_dim, int batch, int kv_heads, int group, int max_new, int max_tokens);
+// How an attention call of these sizes runs: the chunk kernel, its keys split
+// over wgs workgroups at most, or the one for few rows, in whole units or on
+// wgs workgroups; and the partial outputs that the workspace holds. max_tokens: most tokens that
+// the page table holds.
+struct CachePlan {
+    bool chunks, whole;
+    int wgs;
+    uint64_t part_rows;
+};
+CachePlan cache_plan(int head_dim, int batch, int rows, int heads, int kv_heads, int max_new, int max_tokens);
+hipError_t launch_cache_attend(int head_dim, const CacheAttnArgs& a, const CachePlan& plan, hipStream_t s);
 
 // The index lookups, host and device: tests/cpp/cache_host.cpp runs them on bad
 // indexes on the CPU.

@@ -15,7 +15,8 @@ using sage::succeeded;
 struct sage_cache_workspace {
     sage_cache_shape shape;
     uint64_t head_dim, bytes;
-    int device, splits;
+    int device;
+    sage::CachePlan plan;
     void* buf;
 };
 
@@ -293,14 +294,13 @@ sage_status sage_cache_workspace_new(const sage_attention* s, const sage_cache_s
     if (st == SAGE_OK) st = on_device(s);
     if (st != SAGE_OK) return st;
     const sage_cache_shape& h = *shape;
-    const int splits = sage::cache_splits((int)s->head_dim, (int)h.batch, (int)h.kv_heads, (int)(h.heads / h.kv_heads),
-                                          (int)h.max_new, (int)(h.max_pages * h.page_tokens));
-    // Splits of rows x heads partial rows: D floats, a maximum and a sum.
+    const sage::CachePlan plan = sage::cache_plan((int)s->head_dim, (int)h.batch, (int)h.rows, (int)h.heads,
+                                                  (int)h.kv_heads, (int)h.max_new, (int)(h.max_pages * h.page_tokens));
+    // A partial row: D floats, a maximum and a sum.
     uint64_t bytes = 0;
-    if (splits > 1 && (__builtin_mul_overflow(h.rows * h.heads, (uint64_t)splits * (s->head_dim + 2) * 4, &bytes) ||
-                       bytes > 1ull << 62))
+    if (__builtin_mul_overflow(plan.part_rows, (s->head_dim + 2) * 4, &bytes) || bytes > 1ull << 62)
         return set_error(SAGE_ERR_INVALID, "cache workspace needs more than 2^62 bytes");
-    sage_cache_workspace* w = new (std::nothrow) sage_cache_workspace{h, s->head_dim, bytes, s->device, splits, nullptr};
+    sage_cache_workspace* w = new (std::nothrow) sage_cache_workspace{h, s->head_dim, bytes, s->device, plan, nullptr};
     if (!w) return set_error(SAGE_ERR_DEVICE, "out of host memory");
     if (bytes) {
         const hipError_t e = hipMalloc(&w->buf, bytes);
@@ -353,11 +353,11 @@ sage_status sage_cache_attend(const sage_attention* s, const sage_cache_workspac
     a.qk_mul = std::max(std::fabs(scale) * 1.44269504088896340736f, 1.17549435e-38f);
     if (scale != scale) a.qk_mul = scale;
     a.q_sign = std::signbit(scale) ? 0x80008000u : 0u;
-    a.splits = ws->splits;
+    a.splits = ws->plan.chunks ? ws->plan.wgs : 1;
+    a.whole = ws->plan.whole;
     a.part_o = static_cast<float*>(ws->buf);
-    a.part_ml = a.part_o + (uint64_t)ws->splits * h.rows * h.heads * d;
-    if (!ws->buf) a.part_ml = nullptr;
-    return done(sage::launch_cache_attend((int)d, a, s->stream), "launch cache attention");
+    a.part_ml = ws->buf ? a.part_o + ws->plan.part_rows * d : nullptr;
+    return done(sage::launch_cache_attend((int)d, a, ws->plan, s->stream), "launch cache attention");
 }
 
 }  // extern "C"

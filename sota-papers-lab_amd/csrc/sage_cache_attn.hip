@@ -136,6 +136,115 @@ __device__ __forceinline__ int unit_at(int tok, int u) {
     return tok * (D * 2) + ((u ^ f) << 5);
 }
 
+// Eight channels of an output row: the sums over the softmax's.
+__device__ __forceinline__ void store_row(const CacheAttnArgs& a, long long row, int head, int ch, const float* f,
+                                          float sum) {
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float x = f[2 * i] * inv, y = f[2 * i + 1] * inv;
+        w[i] = a.out_f16 ? pack_f16x2(x, y) : pack_bf16x2(x, y);
+    }
+    *reinterpret_cast<uint4*>(a.out.p + row * a.out.st + head * a.out.sh + ch) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Parts first .. first + parts - 1 of one column joined by a group of D / 8
+// lanes, eight channels a lane (ch); or, with SHARE, by all the groups of a
+// workgroup together (the first has the result): each sums the parts that fall
+// to it in their order and the groups' sums are added in theirs, so the same
+// call gives the same bits. at(p): part p's place. Returns the softmax's sum.
+template <int D, bool SHARE, class At>
+__device__ __forceinline__ float join_parts(const CacheAttnArgs& a, int parts, int ch, At at, float (&out)[8]) {
+    constexpr int LANES = D / 8, GROUPS = 256 / LANES;
+    __shared__ float sums[SHARE ? GROUPS : 1][D + 4], ls[GROUPS];
+    const f2* ml = reinterpret_cast<const f2*>(a.part_ml);
+    const int grp = threadIdx.x / LANES;
+    // The maximum over all parts, then this group's share of the sums.
+    float m = NEG_INF, l = 0.0f;
+    for (int p = threadIdx.x % LANES; p < parts; p += LANES) m = fmaxf(m, ml[at(p)].x);
+    m = row_max<LANES>(m);
+    const float base = m == NEG_INF ? 0.0f : m;
+    f4 f[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
+#pragma unroll 4
+    for (int p = SHARE ? grp : 0; p < parts; p += SHARE ? GROUPS : 1) {
+        const f2 s = ml[at(p)];
+        const f4* o = reinterpret_cast<const f4*>(a.part_o + at(p) * D + ch);
+        const float w = __builtin_amdgcn_exp2f(s.x - base);
+        l += w * s.y;
+        f[0] += o[0] * w;
+        f[1] += o[1] * w;
+    }
+    if (SHARE) {
+        *reinterpret_cast<f4*>(&sums[SHARE ? grp : 0][ch]) = f[0];
+        *reinterpret_cast<f4*>(&sums[SHARE ? grp : 0][ch + 4]) = f[1];
+        ls[grp] = l;
+        __syncthreads();
+        l = 0.0f, f[0] = f[1] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int g = 0; g < GROUPS; g++) {
+            l += ls[g];
+            f[0] += *reinterpret_cast<const f4*>(&sums[SHARE ? g : 0][ch]);
+            f[1] += *reinterpret_cast<const f4*>(&sums[SHARE ? g : 0][ch + 4]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) out[i] = f[i / 4][i % 4];
+    return l;
+}
+
+// ---- Few rows ----
+//
+// The work of a call is a line of units, one for each (sequence, KV head, tile
+// of 16 columns), and a unit is a step for each 256 of the sequence's tokens,
+// after one more for its beginning and end. The line is cut into equal
+// shares, one a workgroup, as many as the chip holds at once: sequences of any
+// lengths end together, and only the units that a cut goes through leave
+// partial outputs, two a workgroup at most. (Cut into equal parts of each
+// sequence instead, 64 sequences of up to 16384 tokens, 32/8 heads of 128, took
+// 137 us at the best number of parts.)
+constexpr int STEP = 4 * TOKENS;
+
+struct Units {
+    int steps, tiles;  // of the sequence: steps of a unit's tokens, column tiles (0: no rows)
+    __device__ __forceinline__ Units(const CacheAttnArgs& a, const SequenceIndex& s) {
+        steps = max(1, (s.len + STEP - 1) / STEP);
+        tiles = (s.n * a.group + COLS - 1) / COLS;
+    }
+    __device__ __forceinline__ long long cost(const CacheDev& c) const {
+        return (long long)c.kv_heads * tiles * (steps + 1);
+    }
+};
+
+// A lane's value, scalar.
+__device__ __forceinline__ long long uniform(long long v, int lane) {
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, lane), hi = __builtin_amdgcn_readlane((uint32_t)(v >> 32), lane);
+    return (long long)((uint64_t)hi << 32 | lo);
+}
+
+// The line as every wave sums it: each lane a run of sequences, `before` the
+// runs before the lane's.
+struct Line {
+    long long before, total;
+    int run;
+    __device__ __forceinline__ Line(const CacheAttnArgs& a, int lane) {
+        const CacheDev& c = a.c;
+        run = (c.batch + 63) / 64;
+        const int b0 = min(c.batch, lane * run), b1 = min(c.batch, b0 + run);
+        long long sum = 0;
+        for (int b = b0; b < b1; b++) sum += Units(a, sequence_index(c, b, a.max_new)).cost(c);
+        long long upto = sum;
+        for (int d = 1; d < min(64, c.batch); d *= 2) {
+            const long long v = __shfl_up(upto, d);
+            if (lane >= d) upto += v;
+        }
+        before = upto - sum;
+        total = uniform(upto, (c.batch - 1) / run);
+    }
+};
+// Steps of a share; at least two, so that a share is more than a unit's first step.
+__device__ __forceinline__ long long share_of(long long total, int wgs) { return max(2ll, (total + wgs - 1) / wgs); }
+
 // QP, PP: bf16 parts of a query and of a probability.
 template <int D, int QP, int PP>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void cache_attn(CacheAttnArgs a) {
@@ -149,21 +258,65 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void cache_attn(CacheAttnArgs
     __shared__ __align__(16) uint8_t lds[LDS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
-    const int split = blockIdx.x % a.splits, tile = blockIdx.x / a.splits, kvh = blockIdx.y, b = blockIdx.z;
     const CacheDev& c = a.c;
 
-    // The sequence's rows and tokens.
-    const SequenceIndex seq = sequence_index(c, b, a.max_new);
-    const int c0 = tile * COLS, cols = seq.n * a.group;
-    if (c0 >= cols) return;
-    const int chunk = split_tokens(seq.len, a.splits), t0 = split * chunk;
-    if (split && t0 >= seq.len) return;
+    // This workgroup's share [pos, stop) of the line, and the sequence b that it
+    // begins in, whose part of the line begins at base_b. Or one whole unit.
+    int b;
+    long long pos, stop, base_b;
+    SequenceIndex seq;
+    if (a.whole) {
+        b = blockIdx.z, base_b = 0;
+        seq = sequence_index(c, b, a.max_new);
+        const Units units(a, seq);
+        if ((int)blockIdx.x >= units.tiles) return;
+        pos = (long long)(blockIdx.y * units.tiles + blockIdx.x) * (units.steps + 1);
+        stop = pos + units.steps + 1;
+    } else {
+        const Line line(a, lane);
+        const long long share = share_of(line.total, gridDim.x);
+        pos = blockIdx.x * share;
+        stop = min(line.total, pos + share);
+        if (pos >= stop) return;
+        // The last lane whose run begins at pos or before has it in its run.
+        const int at = 63 - __builtin_clzll(__ballot(line.before <= pos && lane * line.run < c.batch));
+        base_b = uniform(line.before, at);
+        b = at * line.run;
+        while (true) {
+            seq = sequence_index(c, b, a.max_new);
+            const long long cost = Units(a, seq).cost(c);
+            if (pos < base_b + cost || b >= c.batch - 1) break;
+            base_b += cost;
+            b++;
+        }
+    }
+    while (pos < stop) {
+    const Units units(a, seq);
+    if (units.tiles == 0) return;
+    const long long idx = (pos - base_b) / (units.steps + 1), begin = base_b + idx * (units.steps + 1);
+    const long long next = begin + units.steps + 1;
+    const int kvh = (int)(idx / units.tiles), tile = (int)(idx - (long long)kvh * units.tiles);
+    const int s0 = (int)max(0ll, pos - begin - 1), s1 = (int)(min(stop, next) - begin - 1);
+    const SequenceIndex now = seq;
+    const int b_now = b;
+    pos = next;
+    if (next >= base_b + units.cost(c)) {  // on to the next sequence that has rows
+        base_b = next;
+        while (pos < stop && b < c.batch - 1) {
+            seq = sequence_index(c, ++b, a.max_new);
+            if (seq.n) break;
+        }
+    }
+    if (s1 <= s0) continue;  // no more than the unit's beginning
+    const bool whole = s0 == 0 && s1 == units.steps;
+    const long long part = 2ll * blockIdx.x + (s0 == 0);
+    const int c0 = tile * COLS, cols = now.n * a.group, t0 = s0 * STEP;
     const int j = (c0 + col) / a.group, head = kvh * a.group + (c0 + col) - j * a.group;
-    const long long row = seq.start + j;
+    const long long row = now.start + j;
     const bool have = c0 + col < cols && row >= 0 && row < c.rows;
-    const int limit = seq.limit(j, a.causal);              // this column sees slots below it
-    const int least = seq.limit(c0 / a.group, a.causal);   // every column sees these
-    const int end = min(t0 + chunk, seq.limit((min(c0 + COLS, cols) - 1) / a.group, a.causal));
+    const int limit = now.limit(j, a.causal);              // this column sees slots below it
+    const int least = now.limit(c0 / a.group, a.causal);   // every column sees these
+    const int end = min(s1 * STEP, now.limit((min(c0 + COLS, cols) - 1) / a.group, a.causal));
 
     // Q^T, the second operand: column lane % 16, channels in K's order.
     bf8 q[QP][KS];
@@ -188,7 +341,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void cache_attn(CacheAttnArgs
     }
 
     const int t_first = t0 + wave * TOKENS;
-    Pages pages(c, b, lane, t_first);
+    Pages pages(c, b_now, lane, t_first);
     // One step's codes and scales: K's token lane % 16 of each 16-token tile,
     // channels (lane / 16) * D / 4 on; V's token lane / G + i * VT, block lane % G.
     struct Step {
@@ -362,40 +515,31 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void cache_attn(CacheAttnArgs
     __syncthreads();
     constexpr int TPC = D / 8;  // threads a column, eight channels each
     const int oc = threadIdx.x / TPC, ch = (threadIdx.x % TPC) * 8;
-    if (oc >= COLS || c0 + oc >= cols) return;
-    const int oj = (c0 + oc) / a.group, oh = kvh * a.group + (c0 + oc) - oj * a.group;
-    const long long orow = seq.start + oj;
-    if (orow < 0 || orow >= c.rows) return;
-    float top = NEG_INF, sum = 0.0f, f[8] = {};
+    if (oc < COLS && c0 + oc < cols) {
+        const int oj = (c0 + oc) / a.group, oh = kvh * a.group + (c0 + oc) - oj * a.group;
+        const long long orow = now.start + oj;
+        float top = NEG_INF, sum = 0.0f, f[8] = {};
 #pragma unroll
-    for (int w = 0; w < 4; w++) top = fmaxf(top, wm[w][oc]);
-    const float base = top == NEG_INF ? 0.0f : top;
+        for (int w = 0; w < 4; w++) top = fmaxf(top, wm[w][oc]);
+        const float base = top == NEG_INF ? 0.0f : top;
 #pragma unroll
-    for (int w = 0; w < 4; w++) {
-        const float s = __builtin_amdgcn_exp2f(wm[w][oc] - base);
-        sum += wl[w][oc] * s;
-        const float* p = ol + (w * COLS + oc) * PAD + ch;
+        for (int w = 0; w < 4; w++) {
+            const float s = __builtin_amdgcn_exp2f(wm[w][oc] - base);
+            sum += wl[w][oc] * s;
+            const float* p = ol + (w * COLS + oc) * PAD + ch;
 #pragma unroll
-        for (int i = 0; i < 8; i++) f[i] += p[i] * s;
-    }
-    if (a.splits == 1) {
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-        for (int i = 0; i < 8; i++) f[i] *= inv;
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            w[i] = a.out_f16 ? pack_f16x2(f[2 * i], f[2 * i + 1]) : pack_bf16x2(f[2 * i], f[2 * i + 1]);
-        *reinterpret_cast<uint4*>(a.out.p + orow * a.out.st + oh * a.out.sh + ch) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
-        const long long at = ((long long)split * c.rows + orow) * a.heads + oh;
-        float* p = a.part_o + at * D + ch;
-        *reinterpret_cast<f4*>(p) = f4{f[0], f[1], f[2], f[3]};
-        *reinterpret_cast<f4*>(p + 4) = f4{f[4], f[5], f[6], f[7]};
-        if (ch == 0) {
-            a.part_ml[at * 2] = top;
-            a.part_ml[at * 2 + 1] = sum;
+            for (int i = 0; i < 8; i++) f[i] += p[i] * s;
         }
+        if (!whole) {
+            float* p = a.part_o + (part * COLS + oc) * D + ch;
+            *reinterpret_cast<f4*>(p) = f4{f[0], f[1], f[2], f[3]};
+            *reinterpret_cast<f4*>(p + 4) = f4{f[4], f[5], f[6], f[7]};
+            if (ch == 0) reinterpret_cast<f2*>(a.part_ml)[part * COLS + oc] = f2{top, sum};
+        } else if (orow >= 0 && orow < c.rows) {
+            store_row(a, orow, oh, ch, f, sum);
+        }
+    }
+    __syncthreads();  // LDS is the next unit's
     }
 }
 
@@ -681,15 +825,10 @@ __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
     }
 }
 
-// The splits' parts joined, every (row, head) by as many groups of D / 8 lanes
-// (eight channels a lane) as SHARE says: all of a workgroup's where there are
-// many splits of few rows, else one. A group sums the splits that fall to it
-// in their order and the groups' sums are added in theirs: the same call gives
-// the same bits.
+// The splits of chunks joined, a group of D / 8 lanes a (row, head); SHARE: a workgroup.
 template <int D, bool SHARE>
-__global__ __launch_bounds__(256) void cache_attn_join(CacheAttnArgs a) {
+__global__ __launch_bounds__(256) void cache_chunk_join(CacheAttnArgs a) {
     constexpr int LANES = D / 8, GROUPS = 256 / LANES;
-    __shared__ float sums[SHARE ? GROUPS : 1][D + 4], ls[GROUPS];
     const CacheDev& c = a.c;
     const int b = blockIdx.z, grp = threadIdx.x / LANES, ch = (threadIdx.x % LANES) * 8;
     const int pair = SHARE ? blockIdx.x : blockIdx.x * GROUPS + grp, j = pair / a.heads, h = pair - j * a.heads;
@@ -697,45 +836,38 @@ __global__ __launch_bounds__(256) void cache_attn_join(CacheAttnArgs a) {
     const long long row = seq.start + j;
     if (j >= seq.n || row < 0 || row >= c.rows) return;  // (SHARE: all threads or none)
     const int chunk = split_tokens(seq.len, a.splits), parts = seq.len ? (seq.len + chunk - 1) / chunk : 1;
-    const long long at = row * a.heads + h, step = (long long)c.rows * a.heads;
-    const f2* ml = reinterpret_cast<const f2*>(a.part_ml) + at;
-    // The maximum over all splits, then this group's share of the sums.
-    float m = NEG_INF, l = 0.0f;
-    for (int p = threadIdx.x % LANES; p < parts; p += LANES) m = fmaxf(m, ml[p * step].x);
-    m = row_max<LANES>(m);
-    const float base = m == NEG_INF ? 0.0f : m;
-    f4 f[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
-#pragma unroll 4
-    for (int p = SHARE ? grp : 0; p < parts; p += SHARE ? GROUPS : 1) {
-        const f2 s = ml[p * step];
-        const f4* o = reinterpret_cast<const f4*>(a.part_o + (at + p * step) * D + ch);
-        const float w = __builtin_amdgcn_exp2f(s.x - base);
-        l += w * s.y;
-        f[0] += o[0] * w;
-        f[1] += o[1] * w;
-    }
-    if (SHARE) {
-        *reinterpret_cast<f4*>(&sums[grp][ch]) = f[0];
-        *reinterpret_cast<f4*>(&sums[grp][ch + 4]) = f[1];
-        ls[grp] = l;
-        __syncthreads();
-        if (grp) return;
-        l = 0.0f, f[0] = f[1] = f4{0, 0, 0, 0};
-#pragma unroll
-        for (int g = 0; g < GROUPS; g++) {
-            l += ls[g];
-            f[0] += *reinterpret_cast<const f4*>(&sums[SHARE ? g : 0][ch]);
-            f[1] += *reinterpret_cast<const f4*>(&sums[SHARE ? g : 0][ch + 4]);
-        }
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float x = f[i / 2][i % 2 * 2] * inv, y = f[i / 2][i % 2 * 2 + 1] * inv;
-        w[i] = a.out_f16 ? pack_f16x2(x, y) : pack_bf16x2(x, y);
-    }
-    *reinterpret_cast<uint4*>(a.out.p + row * a.out.st + h * a.out.sh + ch) = make_uint4(w[0], w[1], w[2], w[3]);
+    const long long first = row * a.heads + h, step = (long long)c.rows * a.heads;
+    float f[8];
+    const float l = join_parts<D, SHARE>(a, parts, ch, [&](int p) { return first + p * step; }, f);
+    if (!SHARE || grp == 0) store_row(a, row, h, ch, f, l);
+}
+
+// The units that more than one share has joined: grid x column tiles (SHARE:
+// columns) of a sequence, y KV heads, z sequences. wgs: cache_attn's grid.
+template <int D, bool SHARE>
+__global__ __launch_bounds__(256) void cache_attn_join(CacheAttnArgs a, int wgs) {
+    constexpr int LANES = D / 8;
+    const CacheDev& c = a.c;
+    const int b = blockIdx.z, kvh = blockIdx.y, grp = threadIdx.x / LANES, ch = (threadIdx.x % LANES) * 8;
+    const SequenceIndex seq = sequence_index(c, b, a.max_new);
+    const Units units(a, seq);
+    const int tile = SHARE ? blockIdx.x / COLS : blockIdx.x;
+    if (tile >= units.tiles) return;
+    const Line line(a, threadIdx.x & 63);
+    const long long share = share_of(line.total, wgs);
+    long long begin = uniform(line.before, b / line.run);
+    for (int i = b / line.run * line.run; i < b; i++) begin += Units(a, sequence_index(c, i, a.max_new)).cost(c);
+    begin += (long long)(kvh * units.tiles + tile) * (units.steps + 1) + 1;  // its first token step
+    const long long w0 = begin / share, w1 = (begin + units.steps - 1) / share;
+    if (w0 == w1) return;  // one share had it all and wrote its rows
+    const int col = SHARE ? blockIdx.x % COLS : grp, at = tile * COLS + col, j = at / a.group;
+    if (col >= COLS || at >= seq.n * a.group) return;  // (SHARE: all threads or none)
+    const long long row = seq.start + j;
+    float f[8];
+    // The first share's part is its tail, every other's its head.
+    const float l = join_parts<D, SHARE>(
+        a, (int)(w1 - w0 + 1), ch, [&](int p) { return (2 * (w0 + p) + (p == 0)) * COLS + col; }, f);
+    if (row >= 0 && row < c.rows && (!SHARE || grp == 0)) store_row(a, row, kvh * a.group + at - j * a.group, ch, f, l);
 }
 
 }  // namespace
@@ -746,27 +878,41 @@ static bool in_chunks(int batch, int kv_heads, int group, int max_new, int max_t
     return cols > 64 && (max_tokens > 2048 || (cols + CCOLS - 1) / CCOLS * kv_heads * batch >= 512);
 }
 
-int cache_splits(int head_dim, int batch, int kv_heads, int group, int max_new, int max_tokens) {
-    (void)head_dim;
-    const int per = in_chunks(batch, kv_heads, group, max_new, max_tokens) ? CCOLS : COLS;
-    const long long tiles = ((long long)max_new * group + per - 1) / per;
-    const long long units = tiles * kv_heads * batch;
-    const long long most = (max_tokens + 511) / 512;
-    if (per != COLS) return (int)std::max(1ll, std::min({most, 512 / std::max(units, 1ll), (long long)MAX_SPLITS}));
-    return (int)std::max(1ll, std::min({most, 2048 / std::max(units, 1ll), (long long)MAX_SPLITS}));
+CachePlan cache_plan(int head_dim, int batch, int rows, int heads, int kv_heads, int max_new, int max_tokens) {
+    CachePlan p{};
+    const int group = heads / kv_heads;
+    p.chunks = in_chunks(batch, kv_heads, group, max_new, max_tokens);
+    const long long per = p.chunks ? CCOLS : COLS, units = ((long long)max_new * group + per - 1) / per * kv_heads * batch;
+    if (p.chunks) {
+        // Two workgroups a CU fill the chip; a split is 512 tokens at least.
+        const long long most = (max_tokens + 511) / 512;
+        p.wgs = (int)std::max(1ll, std::min({most, 512 / std::max(units, 1ll), (long long)MAX_SPLITS}));
+        p.part_rows = p.wgs > 1 ? (uint64_t)p.wgs * rows * heads : 0;
+    } else {
+        // As many shares as the chip holds workgroups (three a CU, two at head
+        // dim 128), no more than the steps that there can be.
+        const long long steps = units * ((max_tokens + STEP - 1) / STEP + 1);
+        p.wgs = (int)std::max(1ll, std::min<long long>(head_dim == 64 ? 768 : 512, (steps + 1) / 2));
+        // Units of a few steps that fill the chip run whole, a workgroup each
+        // (a decoder's 448 rows of 16 heads over 1500 states, six sequences: 34 us
+        // against 43 in shares); so do units of four steps at most, which a second
+        // kernel would not shorten (16 heads over 778 tokens: 10.6 us against 14).
+        p.whole = max_tokens <= 4 * STEP || (max_tokens <= 8 * STEP && units >= p.wgs);
+        p.part_rows = p.whole ? 0 : 2ull * p.wgs * COLS;
+    }
+    return p;
 }
 
 template <int D>
-static hipError_t launch(const CacheAttnArgs& a, hipStream_t s) {
-    const int per = in_chunks(a.c.batch, a.c.kv_heads, a.group, a.max_new, a.c.max_pages << a.c.page_shift) ? CCOLS : COLS;
-    const unsigned tiles = (unsigned)(((long long)a.max_new * a.group + per - 1) / per);
-    const dim3 grid(tiles * a.splits, a.c.kv_heads, a.c.batch), block(256);
+static hipError_t launch(const CacheAttnArgs& a, const CachePlan& plan, hipStream_t s) {
+    const dim3 block(256);
+    const unsigned per = plan.chunks ? CCOLS : COLS, tiles = (unsigned)(((long long)a.max_new * a.group + per - 1) / per);
     const auto go = [&](auto qp, auto pp) {
         constexpr int QP = decltype(qp)::value, PP = decltype(pp)::value;
-        if (per == COLS)
-            hipLaunchKernelGGL((cache_attn<D, QP, PP>), grid, block, 0, s, a);
+        if (plan.chunks)
+            hipLaunchKernelGGL((cache_attn_chunk<D, QP, PP>), dim3(tiles * a.splits, a.c.kv_heads, a.c.batch), block, 0, s, a);
         else
-            hipLaunchKernelGGL((cache_attn_chunk<D, QP, PP>), grid, block, 0, s, a);
+            hipLaunchKernelGGL((cache_attn<D, QP, PP>), a.whole ? dim3(tiles, a.c.kv_heads, a.c.batch) : dim3(plan.wgs), block, 0, s, a);
     };
     constexpr std::integral_constant<int, 1> one;
     constexpr std::integral_constant<int, 2> two;
@@ -774,19 +920,25 @@ static hipError_t launch(const CacheAttnArgs& a, hipStream_t s) {
         a.out_f16 ? go(two, two) : go(two, one);
     else
         a.out_f16 ? go(one, two) : go(one, one);
-    if (a.splits > 1) {
+    // Many parts of few columns are joined by a workgroup a column.
+    if (plan.chunks && a.splits > 1) {
         const long long pairs = (long long)a.max_new * a.heads;
         constexpr int PER = 256 / (D / 8);
         if (a.splits > 8 && pairs * a.c.batch <= 4096)
-            hipLaunchKernelGGL((cache_attn_join<D, true>), dim3((unsigned)pairs, 1, a.c.batch), block, 0, s, a);
+            hipLaunchKernelGGL((cache_chunk_join<D, true>), dim3((unsigned)pairs, 1, a.c.batch), block, 0, s, a);
         else
-            hipLaunchKernelGGL((cache_attn_join<D, false>), dim3((unsigned)((pairs + PER - 1) / PER), 1, a.c.batch), block, 0, s, a);
+            hipLaunchKernelGGL((cache_chunk_join<D, false>), dim3((unsigned)((pairs + PER - 1) / PER), 1, a.c.batch), block, 0, s, a);
+    } else if (!plan.chunks && !a.whole) {
+        if ((long long)tiles * a.c.kv_heads * a.c.batch <= 64)
+            hipLaunchKernelGGL((cache_attn_join<D, true>), dim3(tiles * COLS, a.c.kv_heads, a.c.batch), block, 0, s, a, plan.wgs);
+        else
+            hipLaunchKernelGGL((cache_attn_join<D, false>), dim3(tiles, a.c.kv_heads, a.c.batch), block, 0, s, a, plan.wgs);
     }
     return hipGetLastError();
 }
 
-hipError_t launch_cache_attend(int head_dim, const CacheAttnArgs& a, hipStream_t s) {
-    return head_dim == 64 ? launch<64>(a, s) : launch<128>(a, s);
+hipError_t launch_cache_attend(int head_dim, const CacheAttnArgs& a, const CachePlan& plan, hipStream_t s) {
+    return head_dim == 64 ? launch<64>(a, plan, s) : launch<128>(a, plan, s);
 }
 
 }  // namespace sage

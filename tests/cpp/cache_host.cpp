@@ -163,9 +163,10 @@ static void refusals() {
         struct {
             sage_cache_shape shape;
             uint64_t head_dim, bytes;
-            int device, splits;
+            int device;
+            sage::CachePlan plan;
             void* buf;
-        } ws{h, 128, 0, -2, 1, nullptr};
+        } ws{h, 128, 0, -2, {false, true, 1, 0}, nullptr};
         const sage_cache_options o{0, 0, 1};
         return sage_cache_attend(&ctx, reinterpret_cast<sage_cache_workspace*>(&ws), &c, &i, &q, &qo, &o);
     };

@@ -81,6 +81,22 @@ def test_long_sequences(torch_gpu, d):
 
 
 @pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("batch", [63, 64, 65, 200])
+def test_many_sequences(torch_gpu, d, batch):
+    """Sequences without rows or tokens among others of up to 1500: the shares of the work begin and end everywhere."""
+    rng = np.random.default_rng(batch)
+    news = rng.integers(0, 3, batch)
+    news[:2] = 0
+    starts = np.concatenate([[0], np.cumsum(news)]).tolist()
+    lengths = np.where(rng.random(batch) < 0.3, rng.integers(0, 4, batch), rng.integers(0, 1500, batch)).tolist()
+    lengths[5] = 1500
+    p = Pool(torch_gpu, d, starts, lengths, 2, 64, 4, seed=batch)
+    q, qv = draw16(torch_gpu, rng, (1, starts[-1], 4, d), "bf16")
+    a = check(torch_gpu, p, q, qv, "bf16")
+    assert torch_gpu.equal(a, run(torch_gpu, p, q, "bf16"))
+
+
+@pytest.mark.parametrize("d", [64, 128])
 def test_a_long_prefix_under_a_few_rows(torch_gpu, d):
     """Chunks whose keys are split over workgroups, and more rows than a workgroup's columns."""
     rng = np.random.default_rng(d)
