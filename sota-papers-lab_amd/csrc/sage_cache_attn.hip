@@ -127,13 +127,15 @@ __device__ __forceinline__ int split_tokens(int len, int splits) {
     return ((len + splits - 1) / splits + step - 1) / step * step;
 }
 
-// Byte of 16-channel unit u of a token's bf16 V row in LDS. The units of a row
-// are permuted by the token, so that what a transposing read takes at once
-// meets all banks: eight tokens of one unit (16x16), four of two (32x32).
+// Byte of half h (eight channels) of 16-channel unit u of a token's bf16 V row
+// in LDS. LDS serves 128 bytes a clock: the units of a row are permuted by the
+// token, so that the four tokens that 16 lanes of a transposing read take meet
+// all of them, and the halves of some are swapped, so that what eight lanes
+// write at once does too.
 template <int D>
-__device__ __forceinline__ int unit_at(int tok, int u) {
-    const int f = D == 128 ? (tok & 3) << 1 | (tok >> 2 & 1) : (tok & 2) | (tok >> 2 & 1);
-    return tok * (D * 2) + ((u ^ f) << 5);
+__device__ __forceinline__ int unit_at(int tok, int u, int h) {
+    const int f = D == 128 ? tok & 7 : tok & 3, s = D == 128 ? u >> 2 & 1 : (tok ^ tok >> 1) & 1;
+    return tok * (D * 2) + ((u ^ f) << 5) + ((h ^ s) << 4);
 }
 
 // Eight channels of an output row: the sums over the softmax's.
@@ -464,8 +466,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void cache_attn(CacheAttnArgs
                 const uint32_t w[4] = {st.v[n].x, st.v[n].y, st.v[n].z, st.v[n].w};
 #pragma unroll
                 for (int d = 0; d < 4; d++)
-                    *reinterpret_cast<uint4*>(vl + unit_at<D>((lane / G + n * VT) % HALF, (lane % G) * 2 + d / 2) +
-                                              (d & 1) * 16) = decode8(w[d], s);
+                    *reinterpret_cast<uint4*>(vl + unit_at<D>((lane / G + n * VT) % HALF, (lane % G) * 2 + d / 2, d & 1)) =
+                        decode8(w[d], s);
             }
             bf8 p[PP];
 #pragma unroll
@@ -478,8 +480,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void cache_attn(CacheAttnArgs
             for (int u = 0; u < UNITS; u++) {
                 typedef __attribute__((address_space(3))) s4* lp;
                 const int tok = 4 * g + (col >> 2);
-                const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vl + unit_at<D>(tok, u) + (col & 3) * 8));
-                const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vl + unit_at<D>(tok + 16, u) + (col & 3) * 8));
+                const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vl + unit_at<D>(tok, u, col >> 1 & 1) + (col & 1) * 8));
+                const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vl + unit_at<D>(tok + 16, u, col >> 1 & 1) + (col & 1) * 8));
                 typedef short s8 __attribute__((ext_vector_type(8)));
                 const s8 vv = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
@@ -609,35 +611,31 @@ __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
     // codes. A wave's sixteen tokens are of one page: its place is scalar, and
     // the thread's offset in it never changes.
     const int tok = threadIdx.x >> 2, part = threadIdx.x & 3;
-    const uint32_t code_at = (tok & 15) * (D / 2) + part * (D / 8);
-    const uint32_t in_page = (1u << c.page_shift) - 1;
+    const uint32_t code_at = (tok & 15) * (D / 2) + part * (D / 8), scale_at = (tok & 15) * G;
+    const int in_page = (1 << c.page_shift) - 1, head0 = kvh << c.page_shift, page_rows = c.kv_heads << c.page_shift;
     struct Part {
         uint32_t w[WORDS], sc;
     } kr, vr;
     bool v_there = false;
     Pages pages(c, b, lane, t0 + 16 * wave);
     auto page_of = [&](int t) { return t < end ? pages.of(t + 16 * wave) : -1; };
-    auto load_codes = [&](const uint8_t* codes, Part& r, long long row0) {
-        const uint8_t* p = codes + row0 * (D / 2) + code_at;
+    auto load_codes = [&](const uint8_t* p, Part& r) {
         if constexpr (D == 128) {
-            const uint4 x = *reinterpret_cast<const uint4*>(p);
+            const uint4 x = *reinterpret_cast<const uint4*>(p + code_at);
             r.w[0] = x.x, r.w[1] = x.y, r.w[2] = x.z, r.w[3] = x.w;
         } else {
-            const uint2 x = *reinterpret_cast<const uint2*>(p);
+            const uint2 x = *reinterpret_cast<const uint2*>(p + code_at);
             r.w[0] = x.x, r.w[1] = x.y;
         }
     };
-    auto row_of = [&](int t, int page) { return cache_row(c, max(page, 0), kvh, (t + 16 * wave) & in_page); };
-    auto load_k = [&](int t, int page) {
-        const long long row0 = row_of(t, page);
-        load_codes(c.k_codes, kr, row0);
-        const uint8_t* p = c.k_scales + row0 * G + (tok & 15) * G;
-        kr.sc = D == 128 ? *reinterpret_cast<const uint32_t*>(p) : *reinterpret_cast<const uint16_t*>(p);
-    };
-    auto load_v = [&](int t, int page) {
-        const long long row0 = row_of(t, page);
-        load_codes(c.v_codes, vr, row0);
-        vr.sc = (c.v_scales + row0 * G)[(tok & 15) * G + part * G / 4];
+    auto load = [&](int t) {
+        const int page = page_of(t);
+        const long long row0 = (long long)max(page, 0) * page_rows + (head0 + ((t + 16 * wave) & in_page));
+        load_codes(c.k_codes + row0 * (D / 2), kr);
+        load_codes(c.v_codes + row0 * (D / 2), vr);
+        const uint8_t* p = c.k_scales + row0 * G;
+        kr.sc = D == 128 ? *reinterpret_cast<const uint32_t*>(p + scale_at) : *reinterpret_cast<const uint16_t*>(p + scale_at);
+        vr.sc = (c.v_scales + row0 * G)[scale_at + part * G / 4];
         v_there = page >= 0;
     };
     const int k_at = D == 128 ? tok * 64 + ((part ^ (tok >> 1 & 3)) << 4)
@@ -647,20 +645,18 @@ __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
             *reinterpret_cast<uint4*>(lds.k[buf] + k_at) = make_uint4(kr.w[0], kr.w[1], kr.w[2], kr.w[3]);
         else
             *reinterpret_cast<uint2*>(lds.k[buf] + k_at) = make_uint2(kr.w[0], kr.w[1]);
-        if (part == 0) lds.ks[buf][tok] = kr.sc;
+        lds.ks[buf][tok] = kr.sc;  // (four threads, one value)
     };
     auto store_v = [&](int buf) {
         const bool nan = vr.sc == 255;
         const uint64_t bad = __ballot(D == 128 ? nan : nan && !(part & 1));
-        if (lane == 0) {
-            lds.bad[buf][wave] = bad;
-            lds.flags[buf][wave] = (bad != 0) | (v_there ? 0 : 2);
-        }
+        if (bad) lds.bad[buf][wave] = bad;
+        lds.flags[buf][wave] = (bad != 0) | (v_there ? 0 : 2);
         const float s = __uint_as_float(nan ? 0 : vr.sc << 23);
 #pragma unroll
         for (int w = 0; w < WORDS; w++) {
             const int ch = part * (D / 4) + 8 * w;
-            *reinterpret_cast<uint4*>(lds.v[buf] + unit_at<D>(tok, ch / 16) + (ch & 8) * 2) = decode8(vr.w[w], s);
+            *reinterpret_cast<uint4*>(lds.v[buf] + unit_at<D>(tok, ch / 16, ch >> 3 & 1)) = decode8(vr.w[w], s);
         }
     };
 
@@ -675,7 +671,7 @@ __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
     // (lane % 16) / 4.
     const int kx = D == 128 ? (col >> 1 & 3) : (col >> 2 & 1);
     const int kr_at = col * (D / 2), ks_shift = half * (KS / 4) * 8;
-    const int vtok = 4 * half + (lane >> 2 & 3), vunit = lane >> 4 & 1, vbyte = (lane & 3) * 8;
+    const int vtok = 4 * half + (lane >> 2 & 3), vunit = lane >> 4 & 1;
     auto scores = [&](int buf, int sub, f16v& y) {
 #pragma unroll
         for (int i = 0; i < 16; i++) y[i] = 0.0f;
@@ -697,29 +693,23 @@ __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
     };
 
     if (t0 < end) {
-        const int page = page_of(t0);
-        load_k(t0, page);
-        load_v(t0, page);
+        load(t0);
         store_k(0);
         store_v(0);
-        const int next = page_of(t0 + TOKENS);
-        load_k(t0 + TOKENS, next);
-        load_v(t0 + TOKENS, next);
+        load(t0 + TOKENS);
     }
     __syncthreads();
     int buf = 0;
     for (int t = t0; t < end; t += TOKENS, buf ^= 1) {
+        const int4 fl = *reinterpret_cast<const int4*>(lds.flags[buf]);
         if (t + TOKENS < end) {
             store_k(buf ^ 1);
             store_v(buf ^ 1);
-            const int page = page_of(t + 2 * TOKENS);
-            load_k(t + 2 * TOKENS, page);
-            load_v(t + 2 * TOKENS, page);
+            load(t + 2 * TOKENS);
         }
         f16v x[2];
         scores(buf, 0, x[0]);
         scores(buf, 1, x[1]);
-        const int4 fl = *reinterpret_cast<const int4*>(lds.flags[buf]);
         const int flags = __builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w);
         uint32_t hit = 0;
         if (flags || t + TOKENS > least) {
@@ -733,7 +723,7 @@ __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
                     if (!seen) x[sub][i] = NEG_INF;
                     if (flags & 1) {
                         const uint32_t blocks = (uint32_t)(lds.bad[buf][six] >> ((k & 15) * 4)) & 15;
-                        if (seen) hit |= blocks;
+                        if (seen && (fi[six] & 1)) hit |= blocks;
                     }
                 }
             if (flags & 1) {
@@ -774,7 +764,7 @@ __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
                 for (int u = 0; u < CT; u++) {
                     typedef __attribute__((address_space(3))) s4* lp;
                     typedef short s8 __attribute__((ext_vector_type(8)));
-                    const uint8_t* v = lds.v[buf] + (32 * sub + 16 * st) * (D * 2) + unit_at<D>(vtok, 2 * u + vunit) + vbyte;
+                    const uint8_t* v = lds.v[buf] + (32 * sub + 16 * st) * (D * 2) + unit_at<D>(vtok, 2 * u + vunit, lane >> 1 & 1) + (lane & 1) * 8;
                     const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(v));
                     const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(v + 8 * (D * 2)));
                     const bf8 vv = __builtin_bit_cast(bf8, (s8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
