@@ -64,7 +64,8 @@ sage_status view(const void* data, uint64_t len, const sage_strides& st, int32_t
                  uint64_t heads, uint64_t d, const char* what) {
     sage_status r = sage_strides_check(&st, what);
     if (r != SAGE_OK) return r;
-    if (dtype != SAGE_BF16 && dtype != SAGE_F16) return set_error(SAGE_ERR_INVALID, "%s: unknown dtype %d", what, dtype);
+    if (dtype != SAGE_BF16 && dtype != SAGE_F16)
+        return set_error(SAGE_ERR_INVALID, "%s: unknown dtype %d", what, dtype);
     if (st.token >= 1ull << 62 || st.head >= 1ull << 62 || (batch > 1 && st.batch >= 1ull << 62))
         return set_error(SAGE_ERR_INVALID, "%s: strides exceed 2^62 elements", what);
     return buffer(data, len, sage_strides_extent(&st, batch, tokens, heads, d), 16, what);
@@ -155,7 +156,8 @@ sage_status sage_rotary_table(uint64_t rot, uint64_t positions, double base, con
     if (!out) return set_error(SAGE_ERR_INVALID, "null argument");
     if (rot < 2 || rot % 2 || rot > 1u << 16)
         return set_error(SAGE_ERR_INVALID, "rotary: %llu rotated channels: an even number from 2", (u64)rot);
-    if (!(base > 1.0) || !std::isfinite(base)) return set_error(SAGE_ERR_INVALID, "rotary: base %g is not over 1", base);
+    if (!(base > 1.0) || !std::isfinite(base))
+        return set_error(SAGE_ERR_INVALID, "rotary: base %g is not over 1", base);
     sage_status st = in_i32(positions, "rotary positions");
     if (st == SAGE_OK && out_len < positions * rot)
         st = set_error(SAGE_ERR_INVALID, "rotary table: buffer holds %llu elements, needs %llu", (u64)out_len,
@@ -165,7 +167,8 @@ sage_status sage_rotary_table(uint64_t rot, uint64_t positions, double base, con
     const double f = kind == SAGE_ROTARY_NONE ? 1.0 : scaling->factor, pi = 3.14159265358979323846;
     if (kind < SAGE_ROTARY_NONE || kind > SAGE_ROTARY_YARN)
         return set_error(SAGE_ERR_INVALID, "rotary: unknown scaling %d", kind);
-    if (!(f >= 1.0) || !std::isfinite(f)) return set_error(SAGE_ERR_INVALID, "rotary: scaling factor %g is not 1 or more", f);
+    if (!(f >= 1.0) || !std::isfinite(f))
+        return set_error(SAGE_ERR_INVALID, "rotary: scaling factor %g is not 1 or more", f);
     double attention = scaling && scaling->attention != 0.0 ? scaling->attention : 1.0, fast = 0, slow = 0;
     if (!std::isfinite(attention)) return set_error(SAGE_ERR_INVALID, "rotary: attention factor %g", attention);
     if (kind == SAGE_ROTARY_NTK) {
@@ -208,9 +211,10 @@ sage_status sage_rotary_apply(const sage_attention* s, const sage_shape* shape, 
         return set_error(SAGE_ERR_INVALID, "rotary: %llu x %llu rows of %llu heads do not fit in i32", (u64)shape->batch,
                          (u64)shape->tokens, (u64)shape->heads);
     const uint64_t d = s->head_dim;
-    sage_status st = view(x->data, x->len, x->strides, x->dtype, shape->batch, shape->tokens, shape->heads, d, "rotary input");
+    const sage_shape& h = *shape;
+    sage_status st = view(x->data, x->len, x->strides, x->dtype, h.batch, h.tokens, h.heads, d, "rotary input");
     if (st == SAGE_OK)
-        st = view(out->data, out->len, out->strides, out->dtype, shape->batch, shape->tokens, shape->heads, d, "rotary output");
+        st = view(out->data, out->len, out->strides, out->dtype, h.batch, h.tokens, h.heads, d, "rotary output");
     if (st == SAGE_OK && x->dtype != out->dtype)
         st = set_error(SAGE_ERR_INVALID, "rotary input and output must share one element type");
     sage::RotaryArgs a{};

@@ -8,7 +8,8 @@
 // and their scale in one instruction (v_cvt_scalef32_pk_bf16_fp4), so both
 // products run on the bf16 MFMA with fp32 sums: K and V enter exactly, bf16
 // queries too, fp16 ones as two bf16 parts; the probabilities are rounded to
-// bf16 (half a step: 2^-8 of each). The scaled FP8 x FP4 MFMA would take K's
+// bf16 (half a step: 2^-8 of each), or, where the output is fp16, to two bf16
+// parts. The scaled FP8 x FP4 MFMA would take K's
 // codes as they are, but it drops the terms of a dot product that lie some
 // 2^-12 below its largest: under a channel of K with a large offset, which the
 // softmax cancels, that is more than the differences between the keys.
@@ -29,6 +30,7 @@ namespace {
 typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
+typedef short s8 __attribute__((ext_vector_type(8)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
@@ -94,8 +96,8 @@ __device__ __forceinline__ uint32_t col_or(uint32_t v) {
 // A sequence's pages as a wave walks it: 64 columns of the page table, one a
 // lane, loaded at once and read by lane index. Looked up one by one, each id is
 // a load in front of the loads that need it, and waiting for it waits for
-// all that are in flight (chunks of 2048 rows behind 8190 tokens, 32/8 heads of
-// 128: 550 us against 313 with the window).
+// all that are in flight (64 ragged sequences of up to 16384 tokens, 32/8 heads
+// of 128: 173 us, with the window 152).
 struct Pages {
     const int* table;  // the sequence's row
     int cols, pages, shift, lane;
@@ -136,6 +138,15 @@ template <int D>
 __device__ __forceinline__ int unit_at(int tok, int u, int h) {
     const int f = D == 128 ? tok & 7 : tok & 3, s = D == 128 ? u >> 2 & 1 : (tok ^ tok >> 1) & 1;
     return tok * (D * 2) + ((u ^ f) << 5) + ((h ^ s) << 4);
+}
+
+// Eight tokens of a lane's channel from two transposing reads, of four tokens
+// each, at v and `on` bytes behind it.
+__device__ __forceinline__ bf8 read_v(const uint8_t* v, int on) {
+    typedef __attribute__((address_space(3))) s4* lds_ptr;
+    const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(v));
+    const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(v + on));
+    return __builtin_bit_cast(bf8, (s8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
 // Eight channels of an output row: the sums over the softmax's.
@@ -220,7 +231,8 @@ struct Units {
 
 // A lane's value, scalar.
 __device__ __forceinline__ long long uniform(long long v, int lane) {
-    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, lane), hi = __builtin_amdgcn_readlane((uint32_t)(v >> 32), lane);
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, lane);
+    const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(v >> 32), lane);
     return (long long)((uint64_t)hi << 32 | lo);
 }
 
@@ -234,6 +246,7 @@ struct Line {
         run = (c.batch + 63) / 64;
         const int b0 = min(c.batch, lane * run), b1 = min(c.batch, b0 + run);
         long long sum = 0;
+#pragma unroll 4
         for (int b = b0; b < b1; b++) sum += Units(a, sequence_index(c, b, a.max_new)).cost(c);
         long long upto = sum;
         for (int d = 1; d < min(64, c.batch); d *= 2) {
@@ -272,7 +285,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void cache_attn(CacheAttnArgs
         seq = sequence_index(c, b, a.max_new);
         const Units units(a, seq);
         if ((int)blockIdx.x >= units.tiles) return;
-        pos = (long long)(blockIdx.y * units.tiles + blockIdx.x) * (units.steps + 1);
+        pos = ((long long)blockIdx.y * units.tiles + blockIdx.x) * (units.steps + 1);
         stop = pos + units.steps + 1;
     } else {
         const Line line(a, lane);
@@ -293,255 +306,251 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void cache_attn(CacheAttnArgs
         }
     }
     while (pos < stop) {
-    const Units units(a, seq);
-    if (units.tiles == 0) return;
-    const long long idx = (pos - base_b) / (units.steps + 1), begin = base_b + idx * (units.steps + 1);
-    const long long next = begin + units.steps + 1;
-    const int kvh = (int)(idx / units.tiles), tile = (int)(idx - (long long)kvh * units.tiles);
-    const int s0 = (int)max(0ll, pos - begin - 1), s1 = (int)(min(stop, next) - begin - 1);
-    const SequenceIndex now = seq;
-    const int b_now = b;
-    pos = next;
-    if (next >= base_b + units.cost(c)) {  // on to the next sequence that has rows
-        base_b = next;
-        while (pos < stop && b < c.batch - 1) {
-            seq = sequence_index(c, ++b, a.max_new);
-            if (seq.n) break;
+        const Units units(a, seq);
+        if (units.tiles == 0) return;
+        const long long idx = (pos - base_b) / (units.steps + 1), begin = base_b + idx * (units.steps + 1);
+        const long long next = begin + units.steps + 1;
+        const int kvh = (int)(idx / units.tiles), tile = (int)(idx - (long long)kvh * units.tiles);
+        const int s0 = (int)max(0ll, pos - begin - 1), s1 = (int)(min(stop, next) - begin - 1);
+        const SequenceIndex now = seq;
+        const int b_now = b;
+        pos = next;
+        if (next >= base_b + units.cost(c)) {  // on to the next sequence that has rows
+            base_b = next;
+            while (pos < stop && b < c.batch - 1) {
+                seq = sequence_index(c, ++b, a.max_new);
+                if (seq.n) break;
+            }
         }
-    }
-    if (s1 <= s0) continue;  // no more than the unit's beginning
-    const bool whole = s0 == 0 && s1 == units.steps;
-    const long long part = 2ll * blockIdx.x + (s0 == 0);
-    const int c0 = tile * COLS, cols = now.n * a.group, t0 = s0 * STEP;
-    const int j = (c0 + col) / a.group, head = kvh * a.group + (c0 + col) - j * a.group;
-    const long long row = now.start + j;
-    const bool have = c0 + col < cols && row >= 0 && row < c.rows;
-    const int limit = now.limit(j, a.causal);              // this column sees slots below it
-    const int least = now.limit(c0 / a.group, a.causal);   // every column sees these
-    const int end = min(s1 * STEP, now.limit((min(c0 + COLS, cols) - 1) / a.group, a.causal));
+        if (s1 <= s0) continue;  // no more than the unit's beginning
+        const bool whole = s0 == 0 && s1 == units.steps;
+        const long long part = 2ll * blockIdx.x + (s0 == 0);
+        const int c0 = tile * COLS, cols = now.n * a.group, t0 = s0 * STEP;
+        const int j = (c0 + col) / a.group, head = kvh * a.group + (c0 + col) - j * a.group;
+        const long long row = now.start + j;
+        const bool have = c0 + col < cols && row >= 0 && row < c.rows;
+        const int limit = now.limit(j, a.causal);              // this column sees slots below it
+        const int least = now.limit(c0 / a.group, a.causal);   // every column sees these
+        const int end = min(s1 * STEP, now.limit((min(c0 + COLS, cols) - 1) / a.group, a.causal));
 
-    // Q^T, the second operand: column lane % 16, channels in K's order.
-    bf8 q[QP][KS];
-    {
-        const uint16_t* p = a.q.p + row * a.q.st + head * a.q.sh;
+        // Q^T, the second operand: column lane % 16, channels in K's order.
+        bf8 q[QP][KS];
+        {
+            const uint16_t* p = a.q.p + row * a.q.st + head * a.q.sh;
 #pragma unroll
-        for (int s = 0; s < KS; s++) {
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (have) x = load_q(p + g * (D / 4) + 8 * s, a.q_sign);
-            if (QP == 2) {
-                float f[8];
-                unpack8(x, f, true);
+            for (int s = 0; s < KS; s++) {
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (have) x = load_q(p + g * (D / 4) + 8 * s, a.q_sign);
+                if (QP == 2) {
+                    float f[8];
+                    unpack8(x, f, true);
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    q[0][s][i] = (__bf16)f[i];
-                    q[QP - 1][s][i] = (__bf16)(f[i] - (float)q[0][s][i]);
+                    for (int i = 0; i < 8; i++) {
+                        q[0][s][i] = (__bf16)f[i];
+                        q[QP - 1][s][i] = (__bf16)(f[i] - (float)q[0][s][i]);
+                    }
+                } else {
+                    q[0][s] = __builtin_bit_cast(bf8, x);
                 }
-            } else {
-                q[0][s] = __builtin_bit_cast(bf8, x);
             }
         }
-    }
 
-    const int t_first = t0 + wave * TOKENS;
-    Pages pages(c, b_now, lane, t_first);
-    // One step's codes and scales: K's token lane % 16 of each 16-token tile,
-    // channels (lane / 16) * D / 4 on; V's token lane / G + i * VT, block lane % G.
-    struct Step {
-        uint32_t k[4][KS], ks[4];
-        uint4 v[G];
-        uint32_t vs[G];
-        int valid;
-    };
-    // valid: bit i: the page of 16-token tile i is one of the pool's
-    auto row_of = [&](int t, int page) {
-        return cache_row(c, max(page, 0), kvh, t & ((1 << c.page_shift) - 1));
-    };
-    auto load = [&](int t, Step& st) {
-        st.valid = 0;
-        long long rows[4];
+        const int t_first = t0 + wave * TOKENS;
+        Pages pages(c, b_now, lane, t_first);
+        // One step's codes and scales: K's token lane % 16 of each 16-token tile,
+        // channels (lane / 16) * D / 4 on; V's token lane / G + i * VT, block lane % G.
+        struct Step {
+            uint32_t k[4][KS], ks[4];
+            uint4 v[G];
+            uint32_t vs[G];
+            int valid;  // bit i: the page of 16-token tile i is one of the pool's
+        };
+        auto row_of = [&](int t, int page) {
+            return cache_row(c, max(page, 0), kvh, t & ((1 << c.page_shift) - 1));
+        };
+        auto load = [&](int t, Step& st) {
+            st.valid = 0;
+            long long rows[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int page = pages.of(t + 16 * i);
-            st.valid |= (page >= 0) << i;
-            rows[i] = row_of(t + 16 * i, page);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint8_t* p = c.k_codes + rows[i] * (D / 2) + (uint32_t)(col * (D / 2) + g * (D / 8));
-            if constexpr (D == 128) {
-                const uint4 x = *reinterpret_cast<const uint4*>(p);
-                st.k[i][0] = x.x, st.k[i][1] = x.y, st.k[i][2] = x.z, st.k[i][3] = x.w;
-            } else {
-                const uint2 x = *reinterpret_cast<const uint2*>(p);
-                st.k[i][0] = x.x, st.k[i][1] = x.y;
+            for (int i = 0; i < 4; i++) {
+                const int page = pages.of(t + 16 * i);
+                st.valid |= (page >= 0) << i;
+                rows[i] = row_of(t + 16 * i, page);
             }
-            st.ks[i] = (c.k_scales + rows[i] * G)[(uint32_t)(col * G + g * G / 4)];
-        }
 #pragma unroll
-        for (int i = 0; i < G; i++) {
-            long long r = rows[(i * VT) / 16];
-            if (VT == 32 && lane >= 32) r = rows[(i * VT) / 16 + 1];
-            r += lane / G & 15;
-            st.v[i] = *reinterpret_cast<const uint4*>(c.v_codes + r * (D / 2) + (lane % G) * 16);
-            st.vs[i] = c.v_scales[r * G + lane % G];
-        }
-    };
+            for (int i = 0; i < 4; i++) {
+                const uint8_t* p = c.k_codes + rows[i] * (D / 2) + (uint32_t)(col * (D / 2) + g * (D / 8));
+                if constexpr (D == 128) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(p);
+                    st.k[i][0] = x.x, st.k[i][1] = x.y, st.k[i][2] = x.z, st.k[i][3] = x.w;
+                } else {
+                    const uint2 x = *reinterpret_cast<const uint2*>(p);
+                    st.k[i][0] = x.x, st.k[i][1] = x.y;
+                }
+                st.ks[i] = (c.k_scales + rows[i] * G)[(uint32_t)(col * G + g * G / 4)];
+            }
+#pragma unroll
+            for (int i = 0; i < G; i++) {
+                long long r = rows[(i * VT) / 16];
+                if (VT == 32 && lane >= 32) r = rows[(i * VT) / 16 + 1];
+                r += lane / G & 15;
+                st.v[i] = *reinterpret_cast<const uint4*>(c.v_codes + r * (D / 2) + (lane % G) * 16);
+                st.vs[i] = c.v_scales[r * G + lane % G];
+            }
+        };
 
-    f4 o[UNITS];
+        f4 o[UNITS];
 #pragma unroll
-    for (int u = 0; u < UNITS; u++) o[u] = f4{0, 0, 0, 0};
-    float m = NEG_INF, l = 0.0f;
-    uint8_t* vl = lds + wave * (HALF * D * 2);
+        for (int u = 0; u < UNITS; u++) o[u] = f4{0, 0, 0, 0};
+        float m = NEG_INF, l = 0.0f;
+        uint8_t* vl = lds + wave * (HALF * D * 2);
 
-    // Two steps in registers, taken in turns: the loop does both.
-    Step one, two;
-    auto step = [&](int t, const Step& st) __attribute__((always_inline)) {
-        // S^T, tile by tile.
-        f4 x[4];
+        // Two steps in registers, taken in turns: the loop does both.
+        Step one, two;
+        auto step = [&](int t, const Step& st) __attribute__((always_inline)) {
+            // S^T, tile by tile.
+            f4 x[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            x[i] = f4{0, 0, 0, 0};
-            const float s = __uint_as_float(st.ks[i] << 23);
+            for (int i = 0; i < 4; i++) {
+                x[i] = f4{0, 0, 0, 0};
+                const float s = __uint_as_float(st.ks[i] << 23);
 #pragma unroll
-            for (int n = 0; n < KS; n++) {
-                const bf8 kk = __builtin_bit_cast(bf8, decode8(st.k[i][n], s));
+                for (int n = 0; n < KS; n++) {
+                    const bf8 kk = __builtin_bit_cast(bf8, decode8(st.k[i][n], s));
 #pragma unroll
-                for (int p = 0; p < QP; p++) x[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, q[p][n], x[i], 0, 0, 0);
+                    for (int p = 0; p < QP; p++)
+                        x[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, q[p][n], x[i], 0, 0, 0);
+                }
             }
-        }
-        const int there = st.valid;
-        // Blocks of V that are NaN go into LDS as (almost) zeros and are noted:
-        // a masked token's must not reach a row through 0 * NaN.
-        uint64_t bad[G];
+            const int there = st.valid;
+            // Blocks of V that are NaN go into LDS as (almost) zeros and are noted:
+            // a masked token's must not reach a row through 0 * NaN.
+            uint64_t bad[G];
 #pragma unroll
-        for (int i = 0; i < G; i++) bad[i] = __ballot(st.vs[i] == 255);
-        // The softmax's step.
-        const bool masked = t + TOKENS > least || there != 15;
-        float mx = NEG_INF;
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                if (masked && (t + 16 * i + 4 * g + r >= limit || !(there >> i & 1))) x[i][r] = NEG_INF;
-                mx = fmaxf(mx, x[i][r]);
-            }
-        mx = fmaxf(m, col_max(mx));
-        if (__any((mx - m) * a.qk_mul > SLACK)) {
-            const float scale = __builtin_amdgcn_exp2f((m - (mx == NEG_INF ? 0.0f : mx)) * a.qk_mul);
-            m = mx;
-            l *= scale;
-#pragma unroll
-            for (int u = 0; u < UNITS; u++) o[u] *= scale;
-        }
-        const float base = m == NEG_INF ? 0.0f : m * a.qk_mul;
-        uint32_t hit = 0;  // blocks of NaN that this lane's tokens bring to its column
-        uint64_t any_bad = 0;
-#pragma unroll
-        for (int i = 0; i < G; i++) any_bad |= bad[i];
-        if (any_bad) {
+            for (int i = 0; i < G; i++) bad[i] = __ballot(st.vs[i] == 255);
+            // The softmax's step.
+            const bool masked = t + TOKENS > least || there != 15;
+            float mx = NEG_INF;
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const int tok = 16 * i + 4 * g + r;
-                    const uint32_t blocks = (uint32_t)(bad[16 * i / VT] >> (tok % VT * G)) & ((1u << G) - 1);
-                    if (t + tok < limit && (there >> i & 1)) hit |= blocks;
+                    if (masked && (t + 16 * i + 4 * g + r >= limit || !(there >> i & 1))) x[i][r] = NEG_INF;
+                    mx = fmaxf(mx, x[i][r]);
                 }
-            hit = col_or(hit);
+            mx = fmaxf(m, col_max(mx));
+            if (__any((mx - m) * a.qk_mul > SLACK)) {
+                const float scale = __builtin_amdgcn_exp2f((m - (mx == NEG_INF ? 0.0f : mx)) * a.qk_mul);
+                m = mx;
+                l *= scale;
+#pragma unroll
+                for (int u = 0; u < UNITS; u++) o[u] *= scale;
+            }
+            const float base = m == NEG_INF ? 0.0f : m * a.qk_mul;
+            uint32_t hit = 0;  // blocks of NaN that this lane's tokens bring to its column
+            uint64_t any_bad = 0;
+#pragma unroll
+            for (int i = 0; i < G; i++) any_bad |= bad[i];
+            if (any_bad) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const int tok = 16 * i + 4 * g + r;
+                        const uint32_t blocks = (uint32_t)(bad[16 * i / VT] >> (tok % VT * G)) & ((1u << G) - 1);
+                        if (t + tok < limit && (there >> i & 1)) hit |= blocks;
+                    }
+                hit = col_or(hit);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    x[i][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][r], a.qk_mul, -base));
+                    l += x[i][r];
+                }
+            // O^T += V^T P^T, 32 tokens a step: V into the wave's part of LDS as
+            // bf16, then the lane's tokens of two tiles.
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+#pragma unroll
+                for (int n = i * G / 4; n < (i + 2) * G / 4; n++) {
+                    const float s = __uint_as_float(st.vs[n] == 255 ? 0 : st.vs[n] << 23);
+                    const uint32_t w[4] = {st.v[n].x, st.v[n].y, st.v[n].z, st.v[n].w};
+#pragma unroll
+                    for (int d = 0; d < 4; d++)
+                        *reinterpret_cast<uint4*>(
+                            vl + unit_at<D>((lane / G + n * VT) % HALF, (lane % G) * 2 + d / 2, d & 1)) = decode8(w[d], s);
+                }
+                bf8 p[PP];
+#pragma unroll
+                for (int r = 0; r < 8; r++) {
+                    const float e = x[i + r / 4][r % 4];
+                    p[0][r] = (__bf16)e;
+                    if (PP == 2) p[PP - 1][r] = (__bf16)(e - (float)p[0][r]);
+                }
+#pragma unroll
+                for (int u = 0; u < UNITS; u++) {
+                    const uint8_t* at = vl + unit_at<D>(4 * g + (col >> 2), u, col >> 1 & 1) + (col & 1) * 8;
+                    const bf8 vv = read_v(at, 16 * (D * 2));
+#pragma unroll
+                    for (int k = 0; k < PP; k++)
+                        o[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, p[k], o[u], 0, 0, 0);
+                }
+            }
+            if (any_bad) {
+                asm volatile("" : "+v"(hit));  // a branch, not a select of every sum in every step
+#pragma unroll
+                for (int u = 0; u < UNITS; u++)
+                    if (hit >> (u / 2) & 1) o[u] = f4{1, 1, 1, 1} * __builtin_nanf("");
+            }
+        };
+        constexpr int STRIDE = 4 * TOKENS;
+        if (t_first < end) load(t_first, one);
+        for (int t = t_first; t < end; t += 2 * STRIDE) {
+            if (t + STRIDE < end) load(t + STRIDE, two);
+            step(t, one);
+            if (t + STRIDE >= end) break;
+            if (t + 2 * STRIDE < end) load(t + 2 * STRIDE, one);
+            step(t + STRIDE, two);
         }
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                x[i][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][r], a.qk_mul, -base));
-                l += x[i][r];
-            }
-        // O^T += V^T P^T, 32 tokens a step: V into the wave's part of LDS as
-        // bf16, then the lane's tokens of two tiles.
-#pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-#pragma unroll
-            for (int n = i * G / 4; n < (i + 2) * G / 4; n++) {
-                const float s = __uint_as_float(st.vs[n] == 255 ? 0 : st.vs[n] << 23);
-                const uint32_t w[4] = {st.v[n].x, st.v[n].y, st.v[n].z, st.v[n].w};
-#pragma unroll
-                for (int d = 0; d < 4; d++)
-                    *reinterpret_cast<uint4*>(vl + unit_at<D>((lane / G + n * VT) % HALF, (lane % G) * 2 + d / 2, d & 1)) =
-                        decode8(w[d], s);
-            }
-            bf8 p[PP];
-#pragma unroll
-            for (int r = 0; r < 8; r++) {
-                const float e = x[i + r / 4][r % 4];
-                p[0][r] = (__bf16)e;
-                if (PP == 2) p[PP - 1][r] = (__bf16)(e - (float)p[0][r]);
-            }
-#pragma unroll
-            for (int u = 0; u < UNITS; u++) {
-                typedef __attribute__((address_space(3))) s4* lp;
-                const int tok = 4 * g + (col >> 2);
-                const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vl + unit_at<D>(tok, u, col >> 1 & 1) + (col & 1) * 8));
-                const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vl + unit_at<D>(tok + 16, u, col >> 1 & 1) + (col & 1) * 8));
-                typedef short s8 __attribute__((ext_vector_type(8)));
-                const s8 vv = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-                for (int k = 0; k < PP; k++)
-                    o[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, vv), p[k], o[u], 0, 0, 0);
-            }
-        }
-        if (any_bad) {
-            asm volatile("" : "+v"(hit));  // a branch, not a select of every sum in every step
-#pragma unroll
-            for (int u = 0; u < UNITS; u++)
-                if (hit >> (u / 2) & 1) o[u] = f4{1, 1, 1, 1} * __builtin_nanf("");
-        }
-    };
-    constexpr int STRIDE = 4 * TOKENS;
-    if (t_first < end) load(t_first, one);
-    for (int t = t_first; t < end; t += 2 * STRIDE) {
-        if (t + STRIDE < end) load(t + STRIDE, two);
-        step(t, one);
-        if (t + STRIDE >= end) break;
-        if (t + 2 * STRIDE < end) load(t + 2 * STRIDE, one);
-        step(t + STRIDE, two);
-    }
-    l = col_sum(l);
+        l = col_sum(l);
 
-    // The four waves' parts meet in LDS.
-    __shared__ float wm[4][COLS], wl[4][COLS];
-    float* ol = reinterpret_cast<float*>(lds);  // [4][COLS][PAD]
-    __syncthreads();
+        // The four waves' parts meet in LDS.
+        __shared__ float wm[4][COLS], wl[4][COLS];
+        float* ol = reinterpret_cast<float*>(lds);  // [4][COLS][PAD]
+        __syncthreads();
 #pragma unroll
-    for (int u = 0; u < UNITS; u++) *reinterpret_cast<f4*>(ol + (wave * COLS + col) * PAD + 16 * u + 4 * g) = o[u];
-    if (g == 0) wm[wave][col] = m * a.qk_mul, wl[wave][col] = l;
-    __syncthreads();
-    constexpr int TPC = D / 8;  // threads a column, eight channels each
-    const int oc = threadIdx.x / TPC, ch = (threadIdx.x % TPC) * 8;
-    if (oc < COLS && c0 + oc < cols) {
-        const int oj = (c0 + oc) / a.group, oh = kvh * a.group + (c0 + oc) - oj * a.group;
-        const long long orow = now.start + oj;
-        float top = NEG_INF, sum = 0.0f, f[8] = {};
+        for (int u = 0; u < UNITS; u++) *reinterpret_cast<f4*>(ol + (wave * COLS + col) * PAD + 16 * u + 4 * g) = o[u];
+        if (g == 0) wm[wave][col] = m * a.qk_mul, wl[wave][col] = l;
+        __syncthreads();
+        constexpr int TPC = D / 8;  // threads a column, eight channels each
+        const int oc = threadIdx.x / TPC, ch = (threadIdx.x % TPC) * 8;
+        if (oc < COLS && c0 + oc < cols) {
+            const int oj = (c0 + oc) / a.group, oh = kvh * a.group + (c0 + oc) - oj * a.group;
+            const long long orow = now.start + oj;
+            float top = NEG_INF, sum = 0.0f, f[8] = {};
 #pragma unroll
-        for (int w = 0; w < 4; w++) top = fmaxf(top, wm[w][oc]);
-        const float base = top == NEG_INF ? 0.0f : top;
+            for (int w = 0; w < 4; w++) top = fmaxf(top, wm[w][oc]);
+            const float base = top == NEG_INF ? 0.0f : top;
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
-            const float s = __builtin_amdgcn_exp2f(wm[w][oc] - base);
-            sum += wl[w][oc] * s;
-            const float* p = ol + (w * COLS + oc) * PAD + ch;
+            for (int w = 0; w < 4; w++) {
+                const float s = __builtin_amdgcn_exp2f(wm[w][oc] - base);
+                sum += wl[w][oc] * s;
+                const float* p = ol + (w * COLS + oc) * PAD + ch;
 #pragma unroll
-            for (int i = 0; i < 8; i++) f[i] += p[i] * s;
+                for (int i = 0; i < 8; i++) f[i] += p[i] * s;
+            }
+            if (!whole) {
+                float* p = a.part_o + (part * COLS + oc) * D + ch;
+                *reinterpret_cast<f4*>(p) = f4{f[0], f[1], f[2], f[3]};
+                *reinterpret_cast<f4*>(p + 4) = f4{f[4], f[5], f[6], f[7]};
+                if (ch == 0) reinterpret_cast<f2*>(a.part_ml)[part * COLS + oc] = f2{top, sum};
+            } else if (orow >= 0 && orow < c.rows) {
+                store_row(a, orow, oh, ch, f, sum);
+            }
         }
-        if (!whole) {
-            float* p = a.part_o + (part * COLS + oc) * D + ch;
-            *reinterpret_cast<f4*>(p) = f4{f[0], f[1], f[2], f[3]};
-            *reinterpret_cast<f4*>(p + 4) = f4{f[4], f[5], f[6], f[7]};
-            if (ch == 0) reinterpret_cast<f2*>(a.part_ml)[part * COLS + oc] = f2{top, sum};
-        } else if (orow >= 0 && orow < c.rows) {
-            store_row(a, orow, oh, ch, f, sum);
-        }
-    }
-    __syncthreads();  // LDS is the next unit's
+        __syncthreads();  // LDS is the next unit's
     }
 }
 
@@ -551,7 +560,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void cache_attn(CacheAttnArgs
 // loads 16 (D = 64: 8) bytes of K's and V's codes two tiles ahead; V goes into
 // LDS as bf16, K as the codes, which every wave converts for itself: as bf16,
 // K would double what the waves read from LDS, which is then what bounds the
-// kernel, while the conversion is two instructions for 64 lanes' four codes.
+// kernel, while the conversion (one instruction for two codes) runs beside the
+// MFMAs of the logits. Chunks of 2048 rows behind 8190 tokens, 32/8 heads of 128
+// (425 GFLOP): 482 us, 0.88 PFLOP/s; the chip's clock falls to 1.9 GHz under
+// it, with the MFMA pipe busy 44% of the time.
 constexpr int CCOLS = 128;
 typedef float f16v __attribute__((ext_vector_type(16)));
 
@@ -634,7 +646,8 @@ __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
         load_codes(c.k_codes + row0 * (D / 2), kr);
         load_codes(c.v_codes + row0 * (D / 2), vr);
         const uint8_t* p = c.k_scales + row0 * G;
-        kr.sc = D == 128 ? *reinterpret_cast<const uint32_t*>(p + scale_at) : *reinterpret_cast<const uint16_t*>(p + scale_at);
+        kr.sc = D == 128 ? *reinterpret_cast<const uint32_t*>(p + scale_at)
+                         : *reinterpret_cast<const uint16_t*>(p + scale_at);
         vr.sc = (c.v_scales + row0 * G)[scale_at + part * G / 4];
         v_there = page >= 0;
     };
@@ -762,14 +775,12 @@ __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
                 }
 #pragma unroll
                 for (int u = 0; u < CT; u++) {
-                    typedef __attribute__((address_space(3))) s4* lp;
-                    typedef short s8 __attribute__((ext_vector_type(8)));
-                    const uint8_t* v = lds.v[buf] + (32 * sub + 16 * st) * (D * 2) + unit_at<D>(vtok, 2 * u + vunit, lane >> 1 & 1) + (lane & 1) * 8;
-                    const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(v));
-                    const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(v + 8 * (D * 2)));
-                    const bf8 vv = __builtin_bit_cast(bf8, (s8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                    const uint8_t* at = lds.v[buf] + (32 * sub + 16 * st) * (D * 2) +
+                                        unit_at<D>(vtok, 2 * u + vunit, lane >> 1 & 1) + (lane & 1) * 8;
+                    const bf8 vv = read_v(at, 8 * (D * 2));
 #pragma unroll
-                    for (int k = 0; k < PP; k++) o[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv, p[k], o[u], 0, 0, 0);
+                    for (int k = 0; k < PP; k++)
+                        o[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv, p[k], o[u], 0, 0, 0);
                 }
             }
         if (flags & 1) {
@@ -872,7 +883,8 @@ CachePlan cache_plan(int head_dim, int batch, int rows, int heads, int kv_heads,
     CachePlan p{};
     const int group = heads / kv_heads;
     p.chunks = in_chunks(batch, kv_heads, group, max_new, max_tokens);
-    const long long per = p.chunks ? CCOLS : COLS, units = ((long long)max_new * group + per - 1) / per * kv_heads * batch;
+    const long long per = p.chunks ? CCOLS : COLS;
+    const long long units = ((long long)max_new * group + per - 1) / per * kv_heads * batch;
     if (p.chunks) {
         // Two workgroups a CU fill the chip; a split is 512 tokens at least.
         const long long most = (max_tokens + 511) / 512;
@@ -886,8 +898,10 @@ CachePlan cache_plan(int head_dim, int batch, int rows, int heads, int kv_heads,
         // Units of a few steps that fill the chip run whole, a workgroup each
         // (a decoder's 448 rows of 16 heads over 1500 states, six sequences: 34 us
         // against 43 in shares); so do units of four steps at most, which a second
-        // kernel would not shorten (16 heads over 778 tokens: 10.6 us against 14).
-        p.whole = max_tokens <= 4 * STEP || (max_tokens <= 8 * STEP && units >= p.wgs);
+        // kernel would not shorten (16 heads over 778 tokens: 10.6 us against 14),
+        // and more sequences than the shares are cheap to find among, which fill
+        // the chip whatever their lengths.
+        p.whole = max_tokens <= 4 * STEP || batch > 512 || (max_tokens <= 8 * STEP && units >= p.wgs);
         p.part_rows = p.whole ? 0 : 2ull * p.wgs * COLS;
     }
     return p;
@@ -896,13 +910,15 @@ CachePlan cache_plan(int head_dim, int batch, int rows, int heads, int kv_heads,
 template <int D>
 static hipError_t launch(const CacheAttnArgs& a, const CachePlan& plan, hipStream_t s) {
     const dim3 block(256);
-    const unsigned per = plan.chunks ? CCOLS : COLS, tiles = (unsigned)(((long long)a.max_new * a.group + per - 1) / per);
+    const unsigned per = plan.chunks ? CCOLS : COLS, heads = a.c.kv_heads, batch = a.c.batch;
+    const unsigned tiles = (unsigned)(((long long)a.max_new * a.group + per - 1) / per);
     const auto go = [&](auto qp, auto pp) {
         constexpr int QP = decltype(qp)::value, PP = decltype(pp)::value;
         if (plan.chunks)
-            hipLaunchKernelGGL((cache_attn_chunk<D, QP, PP>), dim3(tiles * a.splits, a.c.kv_heads, a.c.batch), block, 0, s, a);
+            hipLaunchKernelGGL((cache_attn_chunk<D, QP, PP>), dim3(tiles * a.splits, heads, batch), block, 0, s, a);
         else
-            hipLaunchKernelGGL((cache_attn<D, QP, PP>), a.whole ? dim3(tiles, a.c.kv_heads, a.c.batch) : dim3(plan.wgs), block, 0, s, a);
+            hipLaunchKernelGGL((cache_attn<D, QP, PP>), a.whole ? dim3(tiles, heads, batch) : dim3(plan.wgs), block, 0,
+                               s, a);
     };
     constexpr std::integral_constant<int, 1> one;
     constexpr std::integral_constant<int, 2> two;
@@ -914,15 +930,16 @@ static hipError_t launch(const CacheAttnArgs& a, const CachePlan& plan, hipStrea
     if (plan.chunks && a.splits > 1) {
         const long long pairs = (long long)a.max_new * a.heads;
         constexpr int PER = 256 / (D / 8);
-        if (a.splits > 8 && pairs * a.c.batch <= 4096)
-            hipLaunchKernelGGL((cache_chunk_join<D, true>), dim3((unsigned)pairs, 1, a.c.batch), block, 0, s, a);
+        if (a.splits > 8 && pairs * batch <= 4096)
+            hipLaunchKernelGGL((cache_chunk_join<D, true>), dim3((unsigned)pairs, 1, batch), block, 0, s, a);
         else
-            hipLaunchKernelGGL((cache_chunk_join<D, false>), dim3((unsigned)((pairs + PER - 1) / PER), 1, a.c.batch), block, 0, s, a);
+            hipLaunchKernelGGL((cache_chunk_join<D, false>), dim3((unsigned)((pairs + PER - 1) / PER), 1, batch), block, 0,
+                               s, a);
     } else if (!plan.chunks && !a.whole) {
-        if ((long long)tiles * a.c.kv_heads * a.c.batch <= 64)
-            hipLaunchKernelGGL((cache_attn_join<D, true>), dim3(tiles * COLS, a.c.kv_heads, a.c.batch), block, 0, s, a, plan.wgs);
+        if ((long long)tiles * heads * batch <= 64)
+            hipLaunchKernelGGL((cache_attn_join<D, true>), dim3(tiles * COLS, heads, batch), block, 0, s, a, plan.wgs);
         else
-            hipLaunchKernelGGL((cache_attn_join<D, false>), dim3(tiles, a.c.kv_heads, a.c.batch), block, 0, s, a, plan.wgs);
+            hipLaunchKernelGGL((cache_attn_join<D, false>), dim3(tiles, heads, batch), block, 0, s, a, plan.wgs);
     }
     return hipGetLastError();
 }
