@@ -511,4 +511,128 @@ inline void prepare_qkv(const SageAttention& sa, Workspace& ws, const QkvIn& in,
 
 }  // namespace qkv
 
+// ---------------------------------------------------------------- rotary, cache
+// No counterpart in the reference: positions along a sequence, and a paged
+// 4-bit key/value cache with the attention over it (sage_hip.h has the
+// semantics). Device pointers with their element counts, as above.
+namespace rotary {
+
+enum class Layout : int32_t { Half = SAGE_ROTARY_HALF, Pairs = SAGE_ROTARY_PAIRS };
+enum class ScalingKind : int32_t {
+    None = SAGE_ROTARY_NONE,
+    Linear = SAGE_ROTARY_LINEAR,
+    Ntk = SAGE_ROTARY_NTK,
+    Yarn = SAGE_ROTARY_YARN
+};
+struct Scaling {
+    ScalingKind kind = ScalingKind::None;
+    double factor = 1.0, original = 0.0, beta_fast = 0.0, beta_slow = 0.0, attention = 0.0;
+    sage_rotary_scaling raw() const {
+        return sage_rotary_scaling{static_cast<int32_t>(kind), factor, original, beta_fast, beta_slow, attention};
+    }
+};
+
+// cos and sin per (position, pair), host memory: positions x rot / 2 x 2.
+struct Table {
+    std::size_t rot = 0, positions = 0;
+    std::vector<float> cos_sin;
+    static Table create(std::size_t rot, std::size_t positions, double base = 10000.0, const Scaling& scaling = {}) {
+        Table t{rot, positions, std::vector<float>(rot * positions)};
+        const sage_rotary_scaling sc = scaling.raw();
+        check(sage_rotary_table(rot, positions, base, &sc, t.cos_sin.data(), t.cos_sin.size()));
+        return t;
+    }
+};
+
+// The uploaded table and the rows' positions (null: the token's index, or its slot in cache::append).
+struct Rotary {
+    const float* table = nullptr;
+    std::size_t table_len = 0, rot = 0;
+    Layout layout = Layout::Half;
+    const int32_t* positions = nullptr;
+    std::size_t positions_len = 0;
+    sage_rotary raw() const {
+        return sage_rotary{table, table_len, rot, static_cast<int32_t>(layout), positions, positions_len};
+    }
+};
+
+inline void apply(const SageAttention& sa, const Shape& shape, const Rotary& r, const Tensor& x, const TensorMut& out,
+                  bool transpose = false) {
+    const sage_shape sh = shape.raw();
+    const sage_rotary ro = r.raw();
+    const sage_tensor tx = x.raw();
+    const sage_tensor_mut to = out.raw();
+    check(sage_rotary_apply(sa.handle(), &sh, &ro, &tx, &to, transpose));
+}
+
+}  // namespace rotary
+
+namespace cache {
+
+constexpr std::size_t BLOCK = 32;  // channels a scale
+
+using CacheShape = sage_cache_shape;  // batch, rows, max_new, heads, kv_heads, pages, page_tokens, max_pages
+using Pool = sage_cache;              // k_codes, k_scales, v_codes, v_scales, codes_len, scales_len
+using Index = sage_cache_index;       // starts, lengths, page_table, each with its count
+
+struct Sizes {
+    uint64_t codes, scales;  // bytes, each for K and for V
+};
+inline Sizes sizes(const CacheShape& shape, std::size_t head_dim) {
+    Sizes s{};
+    check(sage_cache_sizes(&shape, head_dim, &s.codes, &s.scales));
+    return s;
+}
+
+inline void append(const SageAttention& sa, const CacheShape& shape, const Pool& pool, const Index& index,
+                   const Tensor& k, const Tensor& v, const rotary::Rotary* rotary = nullptr, const Tensor* q = nullptr,
+                   const TensorMut* q_out = nullptr) {
+    const sage_tensor tk = k.raw(), tv = v.raw(), tq = q ? q->raw() : sage_tensor{};
+    const sage_tensor_mut to = q_out ? q_out->raw() : sage_tensor_mut{};
+    const sage_rotary r = rotary ? rotary->raw() : sage_rotary{};
+    check(sage_cache_append(sa.handle(), &shape, &pool, &index, &tk, &tv, rotary ? &r : nullptr, q ? &tq : nullptr,
+                            q_out ? &to : nullptr));
+}
+
+inline void read(const SageAttention& sa, const CacheShape& shape, const Pool& pool, const Index& index,
+                 const TensorMut& k, const TensorMut& v) {
+    const sage_tensor_mut tk = k.raw(), tv = v.raw();
+    check(sage_cache_read(sa.handle(), &shape, &pool, &index, &tk, &tv));
+}
+
+// attend's workspace for one shape; one call at a time uses it.
+class CacheWorkspace {
+public:
+    CacheWorkspace(const SageAttention& sa, const CacheShape& shape) {
+        check(sage_cache_workspace_new(sa.handle(), &shape, &h_));
+    }
+    ~CacheWorkspace() { sage_cache_workspace_destroy(h_); }
+    CacheWorkspace(CacheWorkspace&& o) noexcept : h_(std::exchange(o.h_, nullptr)) {}
+    CacheWorkspace& operator=(CacheWorkspace&& o) noexcept {
+        std::swap(h_, o.h_);
+        return *this;
+    }
+    CacheWorkspace(const CacheWorkspace&) = delete;
+    CacheWorkspace& operator=(const CacheWorkspace&) = delete;
+    std::size_t bytes() const { return sage_cache_workspace_bytes(h_); }
+    const sage_cache_workspace* handle() const { return h_; }
+
+private:
+    sage_cache_workspace* h_ = nullptr;
+};
+
+struct AttendOptions {
+    std::optional<float> softmax_scale;
+    bool causal = true;
+};
+inline void attend(const SageAttention& sa, const CacheWorkspace& ws, const Pool& pool, const Index& index,
+                   const Tensor& q, const TensorMut& out, const AttendOptions& opts = {}) {
+    const sage_tensor tq = q.raw();
+    const sage_tensor_mut to = out.raw();
+    const sage_cache_options o{opts.softmax_scale.value_or(0.0f), opts.softmax_scale.has_value(), opts.causal};
+    check(sage_cache_attend(sa.handle(), ws.handle(), &pool, &index, &tq, &to, &o));
+}
+
+}  // namespace cache
+
 }  // namespace spl_sage

@@ -5,6 +5,8 @@ into graphs, and calls on several streams."""
 from __future__ import annotations
 
 import math
+import subprocess
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -246,3 +248,11 @@ def test_refused_on_the_gpu(torch_gpu):
     assert (out == 3.0).all()
     sa.cache_attend(ws, p.cache, p.index, S.Tensor(q), S.TensorMut(out))
     assert (out != 3.0).any(-1).all()  # every row is written
+
+
+def test_cpp_calls(torch_gpu):
+    """The same calls through include/spl_sage.hpp (tests/cpp/gpu_cache.cpp)."""
+    exe = Path(__file__).resolve().parent / "cpp" / "bin" / "gpu_cache"
+    assert exe.exists(), f"{exe} is not built; run `python __graft_entry__.py` (build)"
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0 and "0 failure(s)" in r.stdout, r.stdout + r.stderr
