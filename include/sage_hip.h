@@ -549,7 +549,12 @@ typedef struct sage_cache_options {
  * size) where no two rows of it share an element, else the two share none.
  * A row that sees nothing becomes zeros. The shape is the workspace's.
  * Logits, softmax statistics and sums are fp32; cached values are exact, and
- * the probabilities are rounded to bf16 for the second product. */
+ * the probabilities are rounded to bf16 for the second product, for an fp16
+ * out to two bf16 parts. The sums are of weights up to 2^8, so values of V
+ * past 2^100 can overflow them; V blocks of scale 2^126 and up (bytes 253 and
+ * 254), which hold infinities, count as NaN. The same call gives the same bits;
+ * the order of a row's sums, and so its last bits, depend on the shape and on
+ * the lengths of the whole batch. */
 sage_status sage_cache_attend(const sage_attention* s, const sage_cache_workspace* ws, const sage_cache* cache,
                               const sage_cache_index* index, const sage_tensor* q, const sage_tensor_mut* out,
                               const sage_cache_options* opts);

@@ -41,6 +41,10 @@ constexpr int MAX_SPLITS = 256;
 // past it: the fp32 sums have room for that, and rescaling them becomes rare.
 constexpr float SLACK = 8.0f;
 constexpr float NEG_INF = -__builtin_inff();
+// V's blocks from this scale on (2^126: a code of 4 is past every 16- and 32-bit
+// type) are NaN as 255 is: an infinity of a masked token would reach the
+// rows that do not see it as 0 * inf.
+constexpr uint32_t V_NAN = 253;
 
 __device__ __forceinline__ uint32_t cvt2(uint32_t codes, float s, int which) {
     bf2 r;
@@ -427,7 +431,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void cache_attn(CacheAttnArgs
             // a masked token's must not reach a row through 0 * NaN.
             uint64_t bad[G];
 #pragma unroll
-            for (int i = 0; i < G; i++) bad[i] = __ballot(st.vs[i] == 255);
+            for (int i = 0; i < G; i++) bad[i] = __ballot(st.vs[i] >= V_NAN);
             // The softmax's step.
             const bool masked = t + TOKENS > least || there != 15;
             float mx = NEG_INF;
@@ -475,12 +479,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void cache_attn(CacheAttnArgs
             for (int i = 0; i < 4; i += 2) {
 #pragma unroll
                 for (int n = i * G / 4; n < (i + 2) * G / 4; n++) {
-                    const float s = __uint_as_float(st.vs[n] == 255 ? 0 : st.vs[n] << 23);
+                    const float s = __uint_as_float(st.vs[n] >= V_NAN ? 0 : st.vs[n] << 23);
                     const uint32_t w[4] = {st.v[n].x, st.v[n].y, st.v[n].z, st.v[n].w};
 #pragma unroll
                     for (int d = 0; d < 4; d++)
-                        *reinterpret_cast<uint4*>(
-                            vl + unit_at<D>((lane / G + n * VT) % HALF, (lane % G) * 2 + d / 2, d & 1)) = decode8(w[d], s);
+                        *reinterpret_cast<uint4*>(vl + unit_at<D>((lane / G + n * VT) % HALF, (lane % G) * 2 + d / 2,
+                                                                  d & 1)) = decode8(w[d], s);
                 }
                 bf8 p[PP];
 #pragma unroll
@@ -661,7 +665,7 @@ __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
         lds.ks[buf][tok] = kr.sc;  // (four threads, one value)
     };
     auto store_v = [&](int buf) {
-        const bool nan = vr.sc == 255;
+        const bool nan = vr.sc >= V_NAN;
         const uint64_t bad = __ballot(D == 128 ? nan : nan && !(part & 1));
         if (bad) lds.bad[buf][wave] = bad;
         lds.flags[buf][wave] = (bad != 0) | (v_there ? 0 : 2);
@@ -933,8 +937,8 @@ static hipError_t launch(const CacheAttnArgs& a, const CachePlan& plan, hipStrea
         if (a.splits > 8 && pairs * batch <= 4096)
             hipLaunchKernelGGL((cache_chunk_join<D, true>), dim3((unsigned)pairs, 1, batch), block, 0, s, a);
         else
-            hipLaunchKernelGGL((cache_chunk_join<D, false>), dim3((unsigned)((pairs + PER - 1) / PER), 1, batch), block, 0,
-                               s, a);
+            hipLaunchKernelGGL((cache_chunk_join<D, false>), dim3((unsigned)((pairs + PER - 1) / PER), 1, batch), block,
+                               0, s, a);
     } else if (!plan.chunks && !a.whole) {
         if ((long long)tiles * heads * batch <= 64)
             hipLaunchKernelGGL((cache_attn_join<D, true>), dim3(tiles * COLS, heads, batch), block, 0, s, a, plan.wgs);

@@ -168,6 +168,30 @@ def test_nan_and_infinity_stay_where_they_are_seen(torch_gpu, d, new):
     assert 0 < torch_gpu.isnan(out).sum() < out.numel() // 2
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new", [1, 40])
+def test_scales_past_the_range(torch_gpu, d, new):
+    """V blocks of 2^126 and 2^127, whose values can be infinities: nothing where they are masked (memory that was never
+    written holds them), NaN to the rows that see them."""
+    rng = np.random.default_rng(d)
+    lengths = [100, 300, 90]
+    p = Pool(torch_gpu, d, [0, new, 2 * new, 3 * new], lengths, 2, 16, 6, seed=5)
+    for b, n in enumerate(lengths):
+        for slot in range(n, p.table.shape[1] * 16):
+            for side in "kv":
+                block = p.host[side + "_scales"][p.table[b, slot // 16], :, slot % 16]
+                block[:] = rng.integers(253, 255, block.shape)
+    p.host["v_scales"][p.table[0, 99 // 16], 1, 99 % 16, 1] = 254  # only the last row sees it
+    p.upload()
+    q, qv = draw16(torch_gpu, rng, (1, 3 * new, 6, d), "bf16")
+    out = run(torch_gpu, p, q, "bf16")
+    p.host["v_scales"][p.host["v_scales"] >= 253] = 255
+    p.upload()
+    want = check(torch_gpu, p, q, qv, "bf16")
+    assert torch_gpu.equal(torch_gpu.isnan(out), torch_gpu.isnan(want)) and 0 < torch_gpu.isnan(out).sum() <= 3 * 32
+    assert torch_gpu.equal(out.nan_to_num(7.0), want.nan_to_num(7.0))
+
+
 def test_pages_that_the_pool_does_not_have(torch_gpu):
     """Their tokens are not attended to; a sequence with no other page gives zeros."""
     rng = np.random.default_rng(1)
