@@ -435,9 +435,9 @@ typedef struct sage_rotary {
 } sage_rotary;
 
 /* x rotated into out, [batch][token][head][head_dim] views of shape's batch,
- * tokens and heads (kv_heads is not read), both of one type; positions holds
- * batch * tokens entries. Each product and sum is rounded in fp32, the result
- * once to the type. transpose != 0 turns the other way: the gradient of the
+ * tokens and heads (kv_heads is not read), fewer than 2^26 rows (batch *
+ * tokens), both of one type; positions holds an entry a row. Each product and
+ * sum is rounded in fp32, the result once to the type. transpose != 0 turns the other way: the gradient of the
  * rotation (its transpose, any attention factor included). out may be x itself
  * (one address and strides) where no two rows of it share an element, else the
  * two share no element. An empty shape is a no-op. */
@@ -446,9 +446,9 @@ sage_status sage_rotary_apply(const sage_attention* s, const sage_shape* shape, 
 
 /* A batch of sequences over a pool of pages.
  *   batch        sequences (at most 65535)
- *   rows         rows of the packed q, k, v and out: the new tokens of all
- *                sequences, one sequence behind the other, and any padding
- *                behind the last
+ *   rows         rows of the packed q, k, v and out (below 2^26): the new tokens
+ *                of all sequences, one sequence behind the other, and any
+ *                padding behind the last
  *   max_new      most rows of one sequence (sage_cache_attend leaves a sequence's
  *                rows past it as they are; the other calls do not read it)
  *   heads        query heads, a multiple of kv_heads

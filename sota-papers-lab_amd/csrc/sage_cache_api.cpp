@@ -24,6 +24,8 @@ namespace {
 
 using u64 = unsigned long long;
 constexpr uint64_t I32 = 2147483647ull;
+// Rows below it: at most 64 threads a row in a grid's x, of which a launch takes less than 2^32.
+constexpr uint64_t ROWS = 1ull << 26;
 
 sage_status hip_failed(hipError_t e, const char* what) {
     return set_error(SAGE_ERR_DEVICE, "%s: %s (%s)", what, hipGetErrorName(e), hipGetErrorString(e));
@@ -89,8 +91,9 @@ sage_status rotary_checked(const sage_rotary* r, uint64_t d, uint64_t rows, int 
     if (r->layout != SAGE_ROTARY_HALF && r->layout != SAGE_ROTARY_PAIRS)
         return set_error(SAGE_ERR_INVALID, "rotary: unknown layout %d", r->layout);
     if (r->rot < 2 || r->rot % 2 || r->rot > d)
-        return set_error(SAGE_ERR_INVALID, "rotary: %llu rotated channels of head dim %llu: an even number from 2 to it",
-                         (u64)r->rot, (u64)d);
+        return set_error(SAGE_ERR_INVALID,
+                         "rotary: %llu rotated channels of head dim %llu: an even number from 2 to it", (u64)r->rot,
+                         (u64)d);
     sage_status st = buffer(r->table, r->table_len, r->rot, 16, "rotary table");
     if (st == SAGE_OK) st = in_i32(r->table_len / r->rot, "rotary positions");
     if (st == SAGE_OK && r->positions) st = buffer(r->positions, r->positions_len, rows, 4, "rotary positions");
@@ -107,14 +110,16 @@ sage_status shape_checked(const sage_cache_shape& h) {
         return set_error(SAGE_ERR_INVALID, "cache: pages of %llu tokens (16, 32, 64, 128 or 256 are supported)",
                          (u64)h.page_tokens);
     if (h.pages == 0 || h.max_pages == 0)
-        return set_error(SAGE_ERR_INVALID, "cache: %llu pages in the pool, %llu columns in the page table", (u64)h.pages,
-                         (u64)h.max_pages);
+        return set_error(SAGE_ERR_INVALID, "cache: %llu pages in the pool, %llu columns in the page table",
+                         (u64)h.pages, (u64)h.max_pages);
     sage_status st = in_i32(h.pages, "cache pages");
     if (st == SAGE_OK) st = in_i32(h.rows, "cache rows");
     if (st != SAGE_OK) return st;
     if (h.max_pages > (1ull << 30) / h.page_tokens)
         return set_error(SAGE_ERR_INVALID, "cache: %llu pages of %llu tokens exceed 2^30 tokens a sequence",
                          (u64)h.max_pages, (u64)h.page_tokens);
+    if (h.rows >= ROWS)
+        return set_error(SAGE_ERR_INVALID, "cache: %llu rows exceed the launch grid", (u64)h.rows);
     // Launch grids: the KV heads (append: K, V and query heads) in y, the batch in z.
     if (h.batch > 65535 || h.heads > 65535 || 2 * h.kv_heads + h.heads > 65535)
         return set_error(SAGE_ERR_INVALID, "cache: %llu sequences of %llu and %llu heads exceed the launch grid",
@@ -208,8 +213,11 @@ sage_status sage_rotary_apply(const sage_attention* s, const sage_shape* shape, 
     if (shape->batch == 0 || shape->tokens == 0 || shape->heads == 0) return succeeded();
     uint64_t rows;
     if (__builtin_mul_overflow(shape->batch, shape->tokens, &rows) || rows > I32 || shape->heads > I32)
-        return set_error(SAGE_ERR_INVALID, "rotary: %llu x %llu rows of %llu heads do not fit in i32", (u64)shape->batch,
-                         (u64)shape->tokens, (u64)shape->heads);
+        return set_error(SAGE_ERR_INVALID, "rotary: %llu x %llu rows of %llu heads do not fit in i32",
+                         (u64)shape->batch, (u64)shape->tokens, (u64)shape->heads);
+    if (rows >= ROWS || shape->heads > 1ull << 30)
+        return set_error(SAGE_ERR_INVALID, "rotary: %llu rows of %llu heads exceed the launch grid", (u64)rows,
+                         (u64)shape->heads);
     const uint64_t d = s->head_dim;
     const sage_shape& h = *shape;
     sage_status st = view(x->data, x->len, x->strides, x->dtype, h.batch, h.tokens, h.heads, d, "rotary input");

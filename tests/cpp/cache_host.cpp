@@ -92,6 +92,9 @@ static void refusals() {
     CHECK(sage_rotary_apply(&ctx, &none, &r, &x, &o, 0) == SAGE_OK);
     CHECK(refused(sage_rotary_apply(&ctx, &wide, &r, &x, &o, 0), "do not fit in i32"));
     CHECK(refused(sage_rotary_apply(&ctx, &wraps, &r, &x, &o, 0), "do not fit in i32"));
+    const sage_shape tall{1ull << 6, 1, 1ull << 20, 0}, broad{1, (1ull << 30) + 1, 1, 0};
+    CHECK(refused(sage_rotary_apply(&ctx, &tall, &r, &x, &o, 0), "exceed the launch grid"));
+    CHECK(refused(sage_rotary_apply(&ctx, &broad, &r, &x, &o, 0), "exceed the launch grid"));
     auto rot = [&](auto change, const char* text) {
         sage_rotary q = r;
         change(q);
@@ -212,6 +215,7 @@ static void refusals() {
     all([](H h, C, I) { h.max_pages = 0; }, "0 columns in the page table");
     all([](H h, C, I) { h.pages = 1ull << 31; }, "does not fit in i32");
     all([](H h, C, I) { h.rows = 1ull << 31; }, "does not fit in i32");
+    all([](H h, C, I) { h.rows = 1ull << 26; }, "exceed the launch grid");
     all([](H h, C, I) { h.max_pages = (1ull << 26) + 1; }, "exceed 2^30 tokens");
     all([](H h, C, I) { h.max_pages = ~0ull; }, "exceed 2^30 tokens");
     all([](H h, C, I) { h.batch = 65536; }, "exceed the launch grid");
