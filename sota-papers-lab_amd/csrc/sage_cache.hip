@@ -12,6 +12,7 @@ namespace sage {
 namespace {
 
 typedef float f2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ uint4 pack8(const float* f, bool f16) {
     uint32_t w[4];
@@ -20,18 +21,27 @@ __device__ __forceinline__ uint4 pack8(const float* f, bool f16) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Eight channels that nothing reads again before the call's end: the hint keeps
+// them from driving out the table and the lines being written (a rotation of
+// 5003 rows of 96 heads of 64, 124 MB: 26 us, 30.5 without it; 14879 rows of 16
+// KV heads of 64 appended and read back: 40 us, 47 without it).
+__device__ __forceinline__ uint4 load_once(const uint16_t* p) {
+    return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u4*>(p)));
+}
+
 __device__ __forceinline__ float load1(const uint16_t* p, bool f16) {
     return f16 ? f16_to_f32(*p) : __uint_as_float((uint32_t)*p << 16);
 }
 
-// The turns of a lane's eight channels c0 .. c0 + 7 and the rows they apply to.
+// The turns of a lane's eight channels c0 .. c0 + 7.
 // VEC: rot is a multiple of 16, so that the lane's pairs are whole vectors of
-// the table and its partners (HALF) one vector of the row; other rots go
-// channel by channel (9.7 us against 4.2 for 8 rows of 40 heads).
+// the table and its partners (HALF) those that one lane of the head holds. Other
+// rots go channel by channel and load the partners one by one (5003 rows of
+// 96 heads of 64, HALF: rot 64 26 us, 62 57 us; pairs of neighbours: 26 us both).
 template <bool VEC>
 struct Turns {
     f2 cs[8];   // channel c0 + k's pair
-    int at;     // HALF: where the lane's partners begin
+    int from;   // HALF: the lane of the wave that holds the lane's partners
     bool on;    // whether any of its channels turns
 
     // At position pos; NaN where the table has no such position.
@@ -40,7 +50,7 @@ struct Turns {
         const f2* row = reinterpret_cast<const f2*>(r.table) + (long long)(in ? pos : 0) * (r.rot >> 1);
         const int half = r.rot >> 1;
         on = c0 < r.rot;
-        at = c0 < half ? c0 + half : c0 - half;
+        from = (threadIdx.x & 63) + (c0 < half ? half : -half) / 8;
         if (!on) return;
         if (VEC) {
             const int i = r.layout ? c0 >> 1 : c0 < half ? c0 : c0 - half;
@@ -71,14 +81,11 @@ struct Turns {
         }
     }
 
-    // The partners of the channels of the row at p, as loaded (VEC, HALF).
-    __device__ __forceinline__ uint4 partners(const RotaryDev& r, const uint16_t* p) const {
-        return VEC && on && !r.layout ? *reinterpret_cast<const uint4*>(p + at) : make_uint4(0, 0, 0, 0);
-    }
-
-    // x, the row's channels, turned; y as partners() gave it.
-    __device__ __forceinline__ void apply(const RotaryDev& r, const uint16_t* p, int c0, bool f16, uint4 y,
+    // The lane's channels raw of the row at p, turned, in x. All lanes of the
+    // head call together: they exchange their channels.
+    __device__ __forceinline__ void apply(const RotaryDev& r, const uint16_t* p, int c0, bool f16, uint4 raw,
                                           float (&x)[8]) const {
+        unpack8(raw, x, f16);
         if (!on) return;
         if (r.layout) {
 #pragma unroll
@@ -93,7 +100,8 @@ struct Turns {
         const int half = r.rot >> 1;
         float z[8];
         if (VEC) {
-            unpack8(y, z, f16);
+            unpack8(make_uint4(__shfl(raw.x, from), __shfl(raw.y, from), __shfl(raw.z, from), __shfl(raw.w, from)), z,
+                    f16);
         } else {
 #pragma unroll
             for (int k = 0; k < 8; k++)
@@ -113,6 +121,9 @@ __device__ __forceinline__ int run_of(int parts) { return (parts + gridDim.y - 1
 
 // ---- rotary ----
 //
+// y_a = x_a cos - x_b sin, y_b = x_b cos + x_a sin for each pair (a, b) of
+// channels: 16 bits in and out and six operations a pair, so the memory bounds
+// it (16126 rows of 40 heads of 128, 334 MB: 68 us, 4.9 TB/s, a large copy's rate).
 // A wave holds one row's heads, D / 8 lanes a head and eight channels a lane,
 // so the turns of a lane's channels are loaded once and serve every head.
 // A head's loads come before its stores, all in one wave: out may be x.
@@ -131,20 +142,15 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
     uint16_t* po = a.out.p + b * a.out.sb + t * a.out.st;
     const int run = run_of((a.heads + SLOTS - 1) / SLOTS) * SLOTS, end = min(a.heads, (int)(blockIdx.y + 1) * run);
     for (int h = blockIdx.y * run + lane / CH; h < end; h += AHEAD * SLOTS) {
-        uint4 x[AHEAD], y[AHEAD];
+        uint4 x[AHEAD];
 #pragma unroll
         for (int i = 0; i < AHEAD; i++)
-            if (h + i * SLOTS < end) {
-                const uint16_t* p = px + (h + i * SLOTS) * a.x.sh;
-                x[i] = *reinterpret_cast<const uint4*>(p + c0);
-                y[i] = turns.partners(a.r, p);
-            }
+            if (h + i * SLOTS < end) x[i] = load_once(px + (h + i * SLOTS) * a.x.sh + c0);
 #pragma unroll
         for (int i = 0; i < AHEAD; i++)
             if (h + i * SLOTS < end) {
                 float f[8];
-                unpack8(x[i], f, a.f16);
-                turns.apply(a.r, px + (h + i * SLOTS) * a.x.sh, c0, a.f16, y[i], f);
+                turns.apply(a.r, px + (h + i * SLOTS) * a.x.sh, c0, a.f16, x[i], f);
                 *reinterpret_cast<uint4*>(po + (h + i * SLOTS) * a.out.sh + c0) = pack8(f, a.f16);
             }
     }
@@ -154,7 +160,11 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
 // each: all the parts (a workgroup's heads at a time) where there are few
 // rows, and fewer as the rows fill the chip by themselves, so that what a
 // thread looks up for its row serves several heads. blocks: workgroups of the
-// rows; fill: workgroups that are enough.
+// rows; fill: workgroups that are enough. 1024 for the rotation (the 5003 rows
+// above, before the hint: 30.8 us, 32 with 2048, 45 with 8192) and the append
+// (the 14879 rows: 40 us, 44 with 2048), 4096 for the read, whose loads are a
+// quarter as wide (46875 rows of 8 KV heads of
+// 128: 57 us, 63 with 1024, 62 with 8192).
 unsigned share_heads(long long blocks, long long parts, long long fill) {
     return (unsigned)std::min(parts, std::max(1ll, (fill + blocks - 1) / blocks));
 }
@@ -209,13 +219,17 @@ __device__ __forceinline__ Place place_of(CacheDev c, int row, int* starts) {
     return p;
 }
 
+// The append reads 16-bit rows and writes 17/64 of their bytes; the memory
+// bounds it (14879 rows of 16 KV heads of 64, 77 MB in 23 us: 3.3 TB/s), and a
+// step's 64 rows the launch and four loads in a row (the sequence, its length,
+// its page and the table): 5.5 us.
 // Grid: x = rows in steps of a workgroup's; y = shares of the parts, which are
 // the KV heads of K, then of V, then the query heads. A workgroup's rows are
 // consecutive and of one head at a time: their code rows are consecutive
 // too, so the stores fill whole lines.
 template <int D, bool VEC>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
-    constexpr int CH = D / 8, ROWS = 256 / CH, AHEAD = VEC ? 4 : 1;
+    constexpr int CH = D / 8, ROWS = 256 / CH, AHEAD = VEC ? 2 : 1;
     __shared__ int starts[STARTS];
     const int c0 = ((int)threadIdx.x % CH) * 8, row = blockIdx.x * ROWS + threadIdx.x / CH;
     const int kv = a.c.kv_heads, parts = 2 * kv + (a.q.p ? a.heads : 0);
@@ -231,14 +245,12 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     };
     const int run = run_of(parts), end = min(parts, (int)(blockIdx.y + 1) * run);
     for (int first = blockIdx.y * run; first < end; first += AHEAD) {
-        uint4 raw[AHEAD], beside[AHEAD];
+        uint4 raw[AHEAD];
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) {
             const int part = first + i;
             if (part >= end) break;
-            const uint16_t* p = row_of(part);
-            raw[i] = *reinterpret_cast<const uint4*>(p + c0);
-            if (!is_v(part)) beside[i] = turns.partners(a.r, p);
+            raw[i] = load_once(row_of(part) + c0);
         }
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) {
@@ -246,8 +258,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
             if (part >= end) break;
             float x[8];
             if (!is_v(part) && turns.on) {
-                unpack8(raw[i], x, a.f16);
-                turns.apply(a.r, row_of(part), c0, a.f16, beside[i], x);
+                turns.apply(a.r, row_of(part), c0, a.f16, raw[i], x);
                 raw[i] = pack8(x, a.f16);
             }
             if (part >= 2 * kv) {
@@ -267,6 +278,8 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     }
 }
 
+// The other way, a part at a time in the same grid: 17/64 of the bytes in, the
+// rest out (46875 rows of 8 KV heads of 128, 243 MB: 56 us, 4.3 TB/s).
 template <int D>
 __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
     constexpr int CH = D / 8, ROWS = 256 / CH;

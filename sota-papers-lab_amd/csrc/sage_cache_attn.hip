@@ -126,11 +126,9 @@ struct Pages {
     }
 };
 
-// Tokens of one split of a sequence of len tokens: whole steps of the
-// workgroup's four waves.
+// Tokens of one of the chunk kernel's splits of a sequence of len tokens: whole tiles.
 __device__ __forceinline__ int split_tokens(int len, int splits) {
-    const int step = 4 * TOKENS;
-    return ((len + splits - 1) / splits + step - 1) / step * step;
+    return ((len + splits - 1) / splits + TOKENS - 1) / TOKENS * TOKENS;
 }
 
 // Byte of half h (eight channels) of 16-channel unit u of a token's bf16 V row
@@ -217,9 +215,12 @@ __device__ __forceinline__ float join_parts(const CacheAttnArgs& a, int parts, i
 // after one more for its beginning and end. The line is cut into equal
 // shares, one a workgroup, as many as the chip holds at once: sequences of any
 // lengths end together, and only the units that a cut goes through leave
-// partial outputs, two a workgroup at most. (Cut into equal parts of each
-// sequence instead, 64 sequences of up to 16384 tokens, 32/8 heads of 128, took
-// 137 us at the best number of parts.)
+// partial outputs, two a workgroup at most.
+// The cache is read once, at one pass's worth of MFMA and conversions beside
+// it: the memory bounds it. 63 sequences of up to 16384 tokens (532542 in all),
+// 32/8 heads of 128, one row each: 564 MB in 119 us, 4.7 TB/s. (Cut into
+// equal parts of each sequence instead: 137 us at the best number of parts; in
+// twice as many shares as the chip holds: 132.)
 constexpr int STEP = 4 * TOKENS;
 
 struct Units {
@@ -877,7 +878,13 @@ __global__ __launch_bounds__(256) void cache_attn_join(CacheAttnArgs a, int wgs)
 
 }  // namespace
 
-// Whether a call runs the chunk kernel.
+// Whether a call runs the chunk kernel: above 64 columns, over which the other
+// kernel would read a tile's keys more than four times, and with keys to split
+// or tiles that fill the chip. Behind 20000 tokens, 32/8 heads of 128, chunk
+// kernel and the other: 12 rows (48 columns) 50 and 62 us, 24 rows 78 and 95,
+// 64 rows 55 and 80 (8 sequences: 139 and 256); 448 rows of 16 heads over 1500
+// states, 6 sequences: head dim 64 36 and 32, fp16 48 and 35, head dim 128 52
+// and 52; 100 rows of them 28 and 22.
 static bool in_chunks(int batch, int kv_heads, int group, int max_new, int max_tokens) {
     const long long cols = (long long)max_new * group;
     return cols > 64 && (max_tokens > 2048 || (cols + CCOLS - 1) / CCOLS * kv_heads * batch >= 512);
@@ -890,7 +897,9 @@ CachePlan cache_plan(int head_dim, int batch, int rows, int heads, int kv_heads,
     const long long per = p.chunks ? CCOLS : COLS;
     const long long units = ((long long)max_new * group + per - 1) / per * kv_heads * batch;
     if (p.chunks) {
-        // Two workgroups a CU fill the chip; a split is 512 tokens at least.
+        // Two workgroups a CU fill the chip (four sequences' 64 rows behind 20000
+        // tokens, 32/8 heads of 128: 116 us, 131 with half as many, 127 with twice);
+        // a split is 512 tokens at least.
         const long long most = (max_tokens + 511) / 512;
         p.wgs = (int)std::max(1ll, std::min({most, 512 / std::max(units, 1ll), (long long)MAX_SPLITS}));
         p.part_rows = p.wgs > 1 ? (uint64_t)p.wgs * rows * heads : 0;
@@ -930,17 +939,19 @@ static hipError_t launch(const CacheAttnArgs& a, const CachePlan& plan, hipStrea
         a.out_f16 ? go(two, two) : go(two, one);
     else
         a.out_f16 ? go(one, two) : go(one, one);
-    // Many parts of few columns are joined by a workgroup a column.
+    // Many parts of few columns are joined by a workgroup a column (20000 tokens,
+    // 32/8 heads of 128: one row each of 2 sequences 21.5 us against 24, of 8 47.7
+    // against 46.8; chunks of 32 rows 37.4 against 39.3, of 128 76 against 70).
     if (plan.chunks && a.splits > 1) {
         const long long pairs = (long long)a.max_new * a.heads;
         constexpr int PER = 256 / (D / 8);
-        if (a.splits > 8 && pairs * batch <= 4096)
+        if (a.splits > 8 && pairs * batch <= 2048)
             hipLaunchKernelGGL((cache_chunk_join<D, true>), dim3((unsigned)pairs, 1, batch), block, 0, s, a);
         else
             hipLaunchKernelGGL((cache_chunk_join<D, false>), dim3((unsigned)((pairs + PER - 1) / PER), 1, batch), block,
                                0, s, a);
     } else if (!plan.chunks && !a.whole) {
-        if ((long long)tiles * heads * batch <= 64)
+        if ((long long)tiles * heads * batch <= 32)
             hipLaunchKernelGGL((cache_attn_join<D, true>), dim3(tiles * COLS, heads, batch), block, 0, s, a, plan.wgs);
         else
             hipLaunchKernelGGL((cache_attn_join<D, false>), dim3(tiles, heads, batch), block, 0, s, a, plan.wgs);
