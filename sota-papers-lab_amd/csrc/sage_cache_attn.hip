@@ -62,6 +62,21 @@ __device__ __forceinline__ uint4 decode8(uint32_t codes, float s) {
     return make_uint4(cvt2(codes, s, 0), cvt2(codes, s, 1), cvt2(codes, s, 2), cvt2(codes, s, 3));
 }
 
+// Eight values as bf16, or as two bf16 parts: the nearest and the rest's.
+template <int PARTS>
+__device__ __forceinline__ void parts_of(const float* f, bf8 (&p)[PARTS]) {
+    uint32_t w[PARTS][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        w[0][i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
+        if (PARTS == 2)
+            w[PARTS - 1][i] = pack_bf16x2(f[2 * i] - __uint_as_float(w[0][i] << 16),
+                                          f[2 * i + 1] - __uint_as_float(w[0][i] & 0xffff0000u));
+    }
+#pragma unroll
+    for (int k = 0; k < PARTS; k++) p[k] = __builtin_bit_cast(bf8, make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]));
+}
+
 // Eight channels of a query, negated under a negative softmax scale (so that
 // the greatest logit is the greatest product).
 __device__ __forceinline__ uint4 load_q(const uint16_t* p, uint32_t sign) {
@@ -349,11 +364,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void cache_attn(CacheAttnArgs
                 if (QP == 2) {
                     float f[8];
                     unpack8(x, f, true);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        q[0][s][i] = (__bf16)f[i];
-                        q[QP - 1][s][i] = (__bf16)(f[i] - (float)q[0][s][i]);
-                    }
+                    bf8 two[2];
+                    parts_of<2>(f, two);
+                    q[0][s] = two[0], q[QP - 1][s] = two[1];
                 } else {
                     q[0][s] = __builtin_bit_cast(bf8, x);
                 }
@@ -487,13 +500,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void cache_attn(CacheAttnArgs
                         *reinterpret_cast<uint4*>(vl + unit_at<D>((lane / G + n * VT) % HALF, (lane % G) * 2 + d / 2,
                                                                   d & 1)) = decode8(w[d], s);
                 }
-                bf8 p[PP];
+                float e[8];
 #pragma unroll
-                for (int r = 0; r < 8; r++) {
-                    const float e = x[i + r / 4][r % 4];
-                    p[0][r] = (__bf16)e;
-                    if (PP == 2) p[PP - 1][r] = (__bf16)(e - (float)p[0][r]);
-                }
+                for (int r = 0; r < 8; r++) e[r] = x[i + r / 4][r % 4];
+                bf8 p[PP];
+                parts_of<PP>(e, p);
 #pragma unroll
                 for (int u = 0; u < UNITS; u++) {
                     const uint8_t* at = vl + unit_at<D>(4 * g + (col >> 2), u, col >> 1 & 1) + (col & 1) * 8;
@@ -613,11 +624,9 @@ __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
             if (QP == 2) {
                 float f[8];
                 unpack8(x, f, true);
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    q[0][s][i] = (__bf16)f[i];
-                    q[QP - 1][s][i] = (__bf16)(f[i] - (float)q[0][s][i]);
-                }
+                bf8 two[2];
+                parts_of<2>(f, two);
+                q[0][s] = two[0], q[QP - 1][s] = two[1];
             } else {
                 q[0][s] = __builtin_bit_cast(bf8, x);
             }
@@ -770,14 +779,14 @@ __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
         for (int sub = 0; sub < 2; sub++)
 #pragma unroll
             for (int st = 0; st < 2; st++) {
-                bf8 p[PP];
+                float e[8];
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[sub][8 * st + i], a.qk_mul, -base));
-                    l += e;
-                    p[0][i] = (__bf16)e;
-                    if (PP == 2) p[PP - 1][i] = (__bf16)(e - (float)p[0][i]);
+                    e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[sub][8 * st + i], a.qk_mul, -base));
+                    l += e[i];
                 }
+                bf8 p[PP];
+                parts_of<PP>(e, p);
 #pragma unroll
                 for (int u = 0; u < CT; u++) {
                     const uint8_t* at = lds.v[buf] + (32 * sub + 16 * st) * (D * 2) +
