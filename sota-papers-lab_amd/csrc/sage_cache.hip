@@ -163,8 +163,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
 // rows; fill: workgroups that are enough. 1024 for the rotation (the 5003 rows
 // above, before the hint: 30.8 us, 32 with 2048, 45 with 8192) and the append
 // (the 14879 rows: 40 us, 44 with 2048), 4096 for the read, whose loads are a
-// quarter as wide (46875 rows of 8 KV heads of
-// 128: 57 us, 63 with 1024, 62 with 8192).
+// quarter as wide (46875 rows of 8 KV heads of 128: 51.6 us, 53.5 with 2048 and
+// with 8192).
 unsigned share_heads(long long blocks, long long parts, long long fill) {
     return (unsigned)std::min(parts, std::max(1ll, (fill + blocks - 1) / blocks));
 }
@@ -278,35 +278,46 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     }
 }
 
-// The other way, a part at a time in the same grid: 17/64 of the bytes in, the
-// rest out (46875 rows of 8 KV heads of 128, 243 MB: 56 us, 4.3 TB/s).
+// The other way in the same grid: 17/64 of the bytes in, the rest out. Four
+// parts' loads, of four bytes and one a lane, are in flight together (46875 rows of
+// 8 KV heads of 128, 243 MB: 51.6 us, 4.7 TB/s; one part at a time 57).
 template <int D>
 __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
-    constexpr int CH = D / 8, ROWS = 256 / CH;
+    constexpr int CH = D / 8, ROWS = 256 / CH, AHEAD = 4;
     __shared__ int starts[STARTS];
     const int c0 = ((int)threadIdx.x % CH) * 8, row = blockIdx.x * ROWS + threadIdx.x / CH, kv = a.c.kv_heads;
     const Place place = place_of(a.c, row, starts);
     if (place.b < 0) return;
     const int run = run_of(2 * kv), end = min(2 * kv, (int)(blockIdx.y + 1) * run);
-    for (int part = blockIdx.y * run; part < end; part++) {
-        const bool is_v = part >= kv;
-        const int h = is_v ? part - kv : part;
-        float x[8] = {};
-        if (place.page >= 0) {
-            const long long at = place.at + ((long long)h << a.c.page_shift);
-            const uint32_t codes =
-                *reinterpret_cast<const uint32_t*>((is_v ? a.c.v_codes : a.c.k_codes) + at * (D / 2) + c0 / 2);
-            const uint32_t sc = (is_v ? a.c.v_scales : a.c.k_scales)[at * (D / CACHE_BLOCK) + c0 / CACHE_BLOCK];
-            const float s = __uint_as_float(sc << 23);  // 255: infinity, which the conversion turns into NaN
-            const f2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 0),
-                             __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 1),
-                             __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 2),
-                             __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 3)};
+    for (int first = blockIdx.y * run; first < end; first += AHEAD) {
+        uint32_t codes[AHEAD], scales[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            const int part = first + i;
+            if (part >= end) break;
+            const bool is_v = part >= kv;
+            codes[i] = scales[i] = 0;  // a slot that holds nothing: zeros
+            if (place.page < 0) continue;
+            const long long at = place.at + ((long long)(is_v ? part - kv : part) << a.c.page_shift);
+            codes[i] = *reinterpret_cast<const uint32_t*>((is_v ? a.c.v_codes : a.c.k_codes) + at * (D / 2) + c0 / 2);
+            scales[i] = (is_v ? a.c.v_scales : a.c.k_scales)[at * (D / CACHE_BLOCK) + c0 / CACHE_BLOCK];
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            const int part = first + i;
+            if (part >= end) break;
+            const bool is_v = part >= kv;
+            const float s = __uint_as_float(scales[i] << 23);  // 255: infinity, which the conversion turns into NaN
+            const f2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[i], s, 0),
+                             __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[i], s, 1),
+                             __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[i], s, 2),
+                             __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[i], s, 3)};
+            float x[8];
 #pragma unroll
             for (int k = 0; k < 4; k++) x[2 * k] = v[k].x, x[2 * k + 1] = v[k].y;
+            const RowView& o = is_v ? a.v : a.k;
+            *reinterpret_cast<uint4*>(o.p + row * o.st + (is_v ? part - kv : part) * o.sh + c0) = pack8(x, a.f16);
         }
-        const RowView& o = is_v ? a.v : a.k;
-        *reinterpret_cast<uint4*>(o.p + row * o.st + h * o.sh + c0) = pack8(x, a.f16);
     }
 }
 
