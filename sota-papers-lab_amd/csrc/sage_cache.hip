@@ -161,9 +161,9 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
 // rows, and fewer as the rows fill the chip by themselves, so that what a
 // thread looks up for its row serves several heads. blocks: workgroups of the
 // rows; fill: workgroups that are enough. 1024 for the rotation (the 5003 rows
-// above, before the hint: 30.8 us, 32 with 2048, 45 with 8192) and the append
-// (the 14879 rows: 40 us, 44 with 2048), 4096 for the read, whose loads are a
-// quarter as wide (46875 rows of 8 KV heads of 128: 51.6 us, 53.5 with 2048 and
+// above, before the hint: 30.8 us, 32 with 2048, 45 with 8192), 1536 for the
+// append (6000 rows of 40 KV heads of 128, with the read: 70 us, 76 with 1024,
+// 73 with 2048), 4096 for the read, whose loads are a quarter as wide (46875 rows of 8 KV heads of 128: 51.6 us, 53.5 with 2048 and
 // with 8192).
 unsigned share_heads(long long blocks, long long parts, long long fill) {
     return (unsigned)std::min(parts, std::max(1ll, (fill + blocks - 1) / blocks));
@@ -220,38 +220,44 @@ __device__ __forceinline__ Place place_of(CacheDev c, int row, int* starts) {
 }
 
 // The append reads 16-bit rows and writes 17/64 of their bytes; the memory
-// bounds it (14879 rows of 16 KV heads of 64, 77 MB in 23 us: 3.3 TB/s), and a
+// bounds it (14879 rows of 16 KV heads of 64, 77 MB in 23 us: 3.3 TB/s; a part's
+// code rows come from pieces of one head, 128 bytes of each row), and a
 // step's 64 rows the launch and four loads in a row (the sequence, its length,
 // its page and the table): 5.5 us.
 // Grid: x = rows in steps of a workgroup's; y = shares of the parts, which are
 // the KV heads of K, then of V, then the query heads. A workgroup's rows are
 // consecutive and of one head at a time: their code rows are consecutive
-// too, so the stores fill whole lines.
+// too, so the stores fill whole lines. Two parts' loads are ahead of the two at
+// work, the first two ahead of the lookups.
 template <int D, bool VEC>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     constexpr int CH = D / 8, ROWS = 256 / CH, AHEAD = VEC ? 2 : 1;
     __shared__ int starts[STARTS];
     const int c0 = ((int)threadIdx.x % CH) * 8, row = blockIdx.x * ROWS + threadIdx.x / CH;
     const int kv = a.c.kv_heads, parts = 2 * kv + (a.q.p ? a.heads : 0);
-    const Place place = place_of(a.c, row, starts);
-    if (place.b < 0) return;
-    Turns<VEC> turns;
-    turns.on = false;
-    if (a.r.table) turns.load(a.r, a.r.positions ? a.r.positions[row] : place.slot, c0);
+    const int run = run_of(parts), end = min(parts, (int)(blockIdx.y + 1) * run);
     auto is_v = [&](int part) { return part >= kv && part < 2 * kv; };
     auto row_of = [&](int part) {
         const RowView& in = part >= 2 * kv ? a.q : is_v(part) ? a.v : a.k;
         return in.p + row * in.st + (part >= 2 * kv ? part - 2 * kv : is_v(part) ? part - kv : part) * in.sh;
     };
-    const int run = run_of(parts), end = min(parts, (int)(blockIdx.y + 1) * run);
+    uint4 next[AHEAD];
+    auto load = [&](int first) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++)
+            if (row < a.c.rows && first + i < end) next[i] = load_once(row_of(first + i) + c0);
+    };
+    load(blockIdx.y * run);
+    const Place place = place_of(a.c, row, starts);
+    if (place.b < 0) return;
+    Turns<VEC> turns;
+    turns.on = false;
+    if (a.r.table) turns.load(a.r, a.r.positions ? a.r.positions[row] : place.slot, c0);
     for (int first = blockIdx.y * run; first < end; first += AHEAD) {
         uint4 raw[AHEAD];
 #pragma unroll
-        for (int i = 0; i < AHEAD; i++) {
-            const int part = first + i;
-            if (part >= end) break;
-            raw[i] = load_once(row_of(part) + c0);
-        }
+        for (int i = 0; i < AHEAD; i++) raw[i] = next[i];
+        load(first + AHEAD);
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) {
             const int part = first + i;
@@ -338,7 +344,7 @@ hipError_t launch_rotary(int head_dim, const RotaryArgs& a, hipStream_t s) {
 hipError_t launch_cache_append(int head_dim, const AppendArgs& a, hipStream_t s) {
     const int rows = 256 / (head_dim / 8);
     const long long blocks = ((long long)a.c.rows + rows - 1) / rows;
-    const dim3 grid((unsigned)blocks, share_heads(blocks, 2 * a.c.kv_heads + (a.q.p ? a.heads : 0), 1024));
+    const dim3 grid((unsigned)blocks, share_heads(blocks, 2 * a.c.kv_heads + (a.q.p ? a.heads : 0), 1536));
     const bool vec = a.r.rot % 16 == 0;  // (no rotation: 0)
     if (head_dim == 64)
         hipLaunchKernelGGL((vec ? append_kernel<64, true> : append_kernel<64, false>), grid, dim3(256), 0, s, a);
