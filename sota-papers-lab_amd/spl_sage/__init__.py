@@ -432,6 +432,12 @@ def _stream_handle(stream) -> int:
     return int(stream.cuda_stream)
 
 
+def _current_device() -> int:
+    import torch
+
+    return torch.cuda.current_device()
+
+
 class SageAttention:
     """Kernels for one head dim and Config on one stream (mod.rs:509-901).
     Every call enqueues work and returns without synchronising."""
@@ -442,6 +448,7 @@ class SageAttention:
         _check(lib().sage_new(_stream_handle(stream), head_dim, cfg, C.byref(h)))
         self._h = h.value
         self._stream = stream
+        self._device = _current_device()
         self._destroy = lib().sage_destroy
 
     @classmethod
@@ -533,10 +540,36 @@ class SageAttention:
         _check(lib().sage_forward_noalloc(self._h, C.byref(shape._c()), C.byref(merge._c()), C.byref(q._c()),
                                           C.byref(k._c()), C.byref(v._c()), C.byref(out._c()), C.byref(o)))
 
+    # The structs of the rotary and cache calls' arguments, which refuse what an
+    # address alone does not tell from a good tensor: one of another device or in
+    # host memory, or with its channels apart.
+    def _handle(self, h):
+        if h._device != self._device:
+            raise self._out_of_reach(h._device)
+        return C.byref(h._struct)
+
+    def _view(self, cls, x):
+        t, s = x.data, x.strides
+        if t.get_device() != self._device:
+            raise self._out_of_reach(t.get_device())
+        if s is None:
+            st = t.stride()
+            if st[-1] != 1:
+                raise SageError(1, "the channels of a tensor's rows must be contiguous")
+            st = (st[0], st[1], st[2])
+        else:
+            st = (s.batch, s.token, s.head)
+        return C.byref(cls(t.data_ptr(), _elems_from(t), st, _dtype_code(t)))
+
+    def _out_of_reach(self, device: int) -> SageError:
+        where = "in host memory" if device < 0 else f"on device {device}"
+        return SageError(1, f"a tensor is {where}, the context on device {self._device}")
+
     def rotary(self, shape: Shape, rotary, x: Tensor, out: TensorMut, transpose: bool = False) -> None:
         """x's heads turned by their rows' positions into out (spl_sage.rotary)."""
-        _check(lib().sage_rotary_apply(self._h, C.byref(shape._c()), C.byref(rotary._c()), C.byref(x._c()),
-                                       C.byref(out._c()), int(transpose)))
+        _check(lib().sage_rotary_apply(self._h, C.byref(shape._c()), self._handle(rotary),
+                                       self._view(_abi.sage_tensor, x), self._view(_abi.sage_tensor_mut, out),
+                                       int(transpose)))
 
     def cache_workspace(self, shape):
         """The workspace of cache_attend for one CacheShape (spl_sage.cache)."""
@@ -548,22 +581,25 @@ class SageAttention:
                      q_out: Optional[TensorMut] = None) -> None:
         """The step's keys (rotated) and values written to their slots of the
         cache, and its queries rotated into q_out in the same launch."""
-        opt = lambda x: None if x is None else C.byref(x._c())  # noqa: E731
-        _check(lib().sage_cache_append(self._h, C.byref(cache.shape._c()), C.byref(cache._c()), C.byref(index._c()),
-                                       C.byref(k._c()), C.byref(v._c()), opt(rotary), opt(q), opt(q_out)))
+        _check(lib().sage_cache_append(self._h, C.byref(cache.shape._c()), self._handle(cache), self._handle(index),
+                                       self._view(_abi.sage_tensor, k), self._view(_abi.sage_tensor, v),
+                                       None if rotary is None else self._handle(rotary),
+                                       None if q is None else self._view(_abi.sage_tensor, q),
+                                       None if q_out is None else self._view(_abi.sage_tensor_mut, q_out)))
 
     def cache_read(self, cache, index, k: TensorMut, v: TensorMut) -> None:
         """Cached rows back as 16-bit keys and values."""
-        _check(lib().sage_cache_read(self._h, C.byref(cache.shape._c()), C.byref(cache._c()), C.byref(index._c()),
-                                     C.byref(k._c()), C.byref(v._c())))
+        _check(lib().sage_cache_read(self._h, C.byref(cache.shape._c()), self._handle(cache), self._handle(index),
+                                     self._view(_abi.sage_tensor_mut, k), self._view(_abi.sage_tensor_mut, v)))
 
     def cache_attend(self, ws, cache, index, q: Tensor, out: TensorMut, softmax_scale: Optional[float] = None,
                      causal: bool = True) -> None:
         """Attention of the rows' queries over the cached keys of their sequences."""
         o = _abi.sage_cache_options(0.0 if softmax_scale is None else float(softmax_scale),
                                     0 if softmax_scale is None else 1, int(causal))
-        _check(lib().sage_cache_attend(self._h, ws._h, C.byref(cache._c()), C.byref(index._c()), C.byref(q._c()),
-                                       C.byref(out._c()), C.byref(o)))
+        _check(lib().sage_cache_attend(self._h, ws._h, self._handle(cache), self._handle(index),
+                                       self._view(_abi.sage_tensor, q), self._view(_abi.sage_tensor_mut, out),
+                                       C.byref(o)))
 
     def peak(self, which: int, iters: int = 2048) -> float:
         """Measured dense TOPS of one MFMA shape (0 INT8, 1 FP8, 2 BF16)."""

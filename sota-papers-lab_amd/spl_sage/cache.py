@@ -13,7 +13,7 @@ from dataclasses import dataclass
 
 from . import SageError, _abi, _check
 from ._abi import lib
-from .rotary import _ints
+from .rotary import _device_of, _ints
 
 BLOCK = 32  # channels a scale
 
@@ -86,9 +86,8 @@ class PagedCache:
         vc, vs = _bytes(self.v_codes, "cache V codes"), _bytes(self.v_scales, "cache V scales")
         c = _abi.sage_cache(kc[0], ks[0], vc[0], vs[0], min(kc[1], vc[1]), min(ks[1], vs[1]))
         object.__setattr__(self, "_struct", c)
-
-    def _c(self) -> _abi.sage_cache:
-        return self._struct
+        object.__setattr__(self, "_device", _device_of("the cache's buffers", self.k_codes, self.k_scales, self.v_codes,
+                                                       self.v_scales))
 
 
 @dataclass(frozen=True)
@@ -105,9 +104,7 @@ class CacheIndex:
         c = _abi.sage_cache_index(*_ints(self.starts, "cache starts"), *_ints(self.lengths, "cache lengths"),
                                   *_ints(self.page_table, "cache page table"))
         object.__setattr__(self, "_struct", c)
-
-    def _c(self) -> _abi.sage_cache_index:
-        return self._struct
+        object.__setattr__(self, "_device", _device_of("the cache's index", self.starts, self.lengths, self.page_table))
 
 
 class CacheWorkspace:

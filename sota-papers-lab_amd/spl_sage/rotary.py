@@ -79,6 +79,13 @@ def _ints(t, what: str) -> tuple:
     return t.data_ptr(), t.numel()
 
 
+def _device_of(what: str, *tensors) -> int:
+    """The device that all the tensors are on; -1: host memory."""
+    if any(t.device != tensors[0].device for t in tensors):
+        raise SageError(1, f"{what} are on different devices")
+    return tensors[0].get_device()
+
+
 @dataclass(frozen=True)
 class Rotary:
     """An uploaded RotaryTable with its layout, and the rows' positions (int32
@@ -98,9 +105,8 @@ class Rotary:
         p, n = (None, 0) if self.positions is None else _ints(self.positions, "rotary positions")
         c = _abi.sage_rotary(self.table.data_ptr(), self.table.numel(), self.rot, int(self.layout), p, n)
         object.__setattr__(self, "_struct", c)
-
-    def _c(self) -> _abi.sage_rotary:
-        return self._struct
+        at = (self.table,) if self.positions is None else (self.table, self.positions)
+        object.__setattr__(self, "_device", _device_of("the rotary table and positions", *at))
 
 
 __all__ = ["RotaryLayout", "ScalingKind", "RotaryScaling", "RotaryTable", "Rotary"]

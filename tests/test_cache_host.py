@@ -106,6 +106,67 @@ def test_wrong_types_are_refused():
         K.PagedCache.new(K.CacheShape(1, 1, 1, 1, 1, 1, 17, 1), 64, device="cpu")
 
 
+class _Far:
+    """A handle or tensor of device 1, as far as the check sees it."""
+
+    _device, strides = 1, None
+    data = property(lambda self: self)
+
+    def get_device(self):
+        return 1
+
+
+def test_tensors_out_of_reach_are_refused():
+    """Host memory, another device's and channels apart: refused before the library is called, whichever tensor it is."""
+    import torch
+
+    import spl_sage as S
+    from spl_sage import cache as K
+    from spl_sage import rotary as R
+
+    sa = object.__new__(S.SageAttention)  # no GPU here: the checks come before the handle's use
+    sa._h = None
+    i = torch.zeros(2, dtype=torch.int32)
+    shape = K.CacheShape(1, 1, 1, 1, 1, 1, 16, 1)
+    pool, index, r = K.PagedCache.new(shape, 64, device="cpu"), K.CacheIndex(i, i, i), R.Rotary(torch.zeros(8), 4)
+    x = torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16)
+    t, m = S.Tensor(x), S.TensorMut(x)
+    ws = type("", (), {"_h": None})
+
+    class Far(_Far):
+        shape = pool.shape
+
+    calls = [((pool, index, t, m), lambda *a: sa.cache_attend(ws, *a)),
+             ((r, t, m), lambda *a: sa.rotary(S.Shape(1, 1, 1), *a)),
+             ((pool, index, t, t, r, t, m), sa.cache_append),
+             ((pool, index, t, t), sa.cache_append),
+             ((pool, index, m, m), sa.cache_read)]
+    for args, call in calls:
+        sa._device = 0
+        with pytest.raises(S.SageError, match="in host memory, the context on device 0"):
+            call(*args)
+        sa._device = -1  # host memory passes for the device's
+        for n in range(len(args)):
+            with pytest.raises(S.SageError, match="on device 1, the context on device -1"):
+                call(*args[:n], Far(), *args[n + 1:])
+    with pytest.raises(S.SageError, match="channels"):
+        sa.cache_read(pool, index, m, S.TensorMut(torch.zeros(1, 1, 64, 8, dtype=torch.bfloat16).transpose(2, 3)))
+
+
+def test_handles_of_one_device():
+    import torch
+
+    from spl_sage import SageError
+    from spl_sage import cache as K
+    from spl_sage import rotary as R
+
+    i, far = torch.zeros(2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32, device="meta")
+    assert R._device_of("all", i, i) == -1
+    with pytest.raises(SageError, match="the cache's index are on different devices"):
+        R._device_of("the cache's index", i, far)
+    assert K.CacheIndex(i, i, i)._device == -1
+
+
 def test_oracle_quantiser():
     """Known answers, ties to the even code, the scale's edge at 1.5 * 2^k, NaN blocks, and no level nearer."""
     x = np.zeros((6, 32))

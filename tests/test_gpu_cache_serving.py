@@ -244,6 +244,13 @@ def test_refused_on_the_gpu(torch_gpu):
         sa.cache_attend(ws, p.cache, p.index, S.Tensor(q), S.TensorMut(out[:, :1].clone()))
     with pytest.raises(S.SageError, match="bf16 or fp16"):
         sa.cache_attend(ws, p.cache, p.index, S.Tensor(q.float()), S.TensorMut(out))
+    from spl_sage import cache as C
+
+    host = C.CacheIndex(p.index.starts.cpu(), p.index.lengths.cpu(), p.index.page_table.cpu())
+    with pytest.raises(S.SageError, match="in host memory"):
+        sa.cache_attend(ws, p.cache, host, S.Tensor(q), S.TensorMut(out))
+    with pytest.raises(S.SageError, match="in host memory"):
+        sa.cache_attend(ws, p.cache, p.index, S.Tensor(q.cpu()), S.TensorMut(out))
     torch.cuda.synchronize()
     assert (out == 3.0).all()
     sa.cache_attend(ws, p.cache, p.index, S.Tensor(q), S.TensorMut(out))
