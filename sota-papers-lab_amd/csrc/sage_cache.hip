@@ -163,8 +163,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
 // rows; fill: workgroups that are enough. 1024 for the rotation (the 5003 rows
 // above, before the hint: 30.8 us, 32 with 2048, 45 with 8192), 1536 for the
 // append (6000 rows of 40 KV heads of 128, with the read: 70 us, 76 with 1024,
-// 73 with 2048), 4096 for the read, whose loads are a quarter as wide (46875 rows of 8 KV heads of 128: 51.6 us, 53.5 with 2048 and
-// with 8192).
+// 73 with 2048), 4096 for the read, whose loads are a quarter as wide (46875 rows
+// of 8 KV heads of 128: 51.6 us, 53.5 with 2048 and with 8192).
 unsigned share_heads(long long blocks, long long parts, long long fill) {
     return (unsigned)std::min(parts, std::max(1ll, (fill + blocks - 1) / blocks));
 }

@@ -71,11 +71,11 @@ hipError_t launch_rotary(int head_dim, const RotaryArgs& a, hipStream_t s);
 hipError_t launch_cache_append(int head_dim, const AppendArgs& a, hipStream_t s);
 hipError_t launch_cache_read(int head_dim, const ReadArgs& a, hipStream_t s);
 // How an attention call of these sizes runs: the chunk kernel, its keys split
-// over wgs workgroups at most, or the one for few rows, in whole units or on
-// wgs workgroups; and the partial outputs that the workspace holds. max_tokens: most tokens that
-// the page table holds.
+// over wgs workgroups at most, or the one for few rows, in whole units (wide:
+// of eight waves) or on wgs workgroups; and the partial outputs that the
+// workspace holds. max_tokens: most tokens that the page table holds.
 struct CachePlan {
-    bool chunks, whole;
+    bool chunks, whole, wide;
     int wgs;
     uint64_t part_rows;
 };

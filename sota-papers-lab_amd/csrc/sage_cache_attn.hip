@@ -280,16 +280,17 @@ struct Line {
 // Steps of a share; at least two, so that a share is more than a unit's first step.
 __device__ __forceinline__ long long share_of(long long total, int wgs) { return max(2ll, (total + wgs - 1) / wgs); }
 
-// QP, PP: bf16 parts of a query and of a probability.
-template <int D, int QP, int PP>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void cache_attn(CacheAttnArgs a) {
+// QP, PP: bf16 parts of a query and of a probability. W: waves, four, or eight
+// for whole units that do not fill the chip (cache_plan).
+template <int D, int QP, int PP, int W>
+__global__ __launch_bounds__(64 * W, D == 64 && W == 4 ? 3 : 2) void cache_attn(CacheAttnArgs a) {
     constexpr int G = D / 32;        // scale blocks of a row
     constexpr int VT = 64 / G;       // tokens of one V load
     constexpr int UNITS = D / 16;    // 32-byte units of a V row in LDS
     constexpr int KS = D / 32;       // MFMA steps over the channels
     constexpr int PAD = D + 4;       // floats of a column where the waves' parts meet
     constexpr int HALF = TOKENS / 2; // tokens of V in LDS at a time, per wave
-    constexpr int LDS = 4 * (HALF * D * 2 > COLS * PAD * 4 ? HALF * D * 2 : COLS * PAD * 4);
+    constexpr int LDS = W * (HALF * D * 2 > COLS * PAD * 4 ? HALF * D * 2 : COLS * PAD * 4);
     __shared__ __align__(16) uint8_t lds[LDS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
@@ -521,7 +522,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void cache_attn(CacheAttnArgs
                     if (hit >> (u / 2) & 1) o[u] = f4{1, 1, 1, 1} * __builtin_nanf("");
             }
         };
-        constexpr int STRIDE = 4 * TOKENS;
+        constexpr int STRIDE = W * TOKENS;
         if (t_first < end) load(t_first, one);
         for (int t = t_first; t < end; t += 2 * STRIDE) {
             if (t + STRIDE < end) load(t + STRIDE, two);
@@ -532,9 +533,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void cache_attn(CacheAttnArgs
         }
         l = col_sum(l);
 
-        // The four waves' parts meet in LDS.
-        __shared__ float wm[4][COLS], wl[4][COLS];
-        float* ol = reinterpret_cast<float*>(lds);  // [4][COLS][PAD]
+        // The waves' parts meet in LDS.
+        __shared__ float wm[W][COLS], wl[W][COLS];
+        float* ol = reinterpret_cast<float*>(lds);  // [W][COLS][PAD]
         __syncthreads();
 #pragma unroll
         for (int u = 0; u < UNITS; u++) *reinterpret_cast<f4*>(ol + (wave * COLS + col) * PAD + 16 * u + 4 * g) = o[u];
@@ -547,10 +548,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void cache_attn(CacheAttnArgs
             const long long orow = now.start + oj;
             float top = NEG_INF, sum = 0.0f, f[8] = {};
 #pragma unroll
-            for (int w = 0; w < 4; w++) top = fmaxf(top, wm[w][oc]);
+            for (int w = 0; w < W; w++) top = fmaxf(top, wm[w][oc]);
             const float base = top == NEG_INF ? 0.0f : top;
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
+            for (int w = 0; w < W; w++) {
                 const float s = __builtin_amdgcn_exp2f(wm[w][oc] - base);
                 sum += wl[w][oc] * s;
                 const float* p = ol + (w * COLS + oc) * PAD + ch;
@@ -920,10 +921,14 @@ CachePlan cache_plan(int head_dim, int batch, int rows, int heads, int kv_heads,
         // Units of a few steps that fill the chip run whole, a workgroup each
         // (a decoder's 448 rows of 16 heads over 1500 states, six sequences: 34 us
         // against 43 in shares); so do units of four steps at most, which a second
-        // kernel would not shorten (16 heads over 778 tokens: 10.6 us against 14),
+        // kernel would not shorten (16 heads over 778 tokens, four waves: 10.6 us against 14),
         // and more sequences than the shares are cheap to find among, which fill
         // the chip whatever their lengths.
         p.whole = max_tokens <= 4 * STEP || batch > 512 || (max_tokens <= 8 * STEP && units >= p.wgs);
+        // Whole units that leave CUs free have eight waves, so half as many turns
+        // (16 heads over 778 tokens 8.3 us against 9.1, 32/8 heads of 128 over 901
+        // tokens 9.7 against 10.8, 32 sequences of them 11.5 against 12.9).
+        p.wide = p.whole && units <= 256 && max_tokens > STEP;
         p.part_rows = p.whole ? 0 : 2ull * p.wgs * COLS;
     }
     return p;
@@ -939,8 +944,9 @@ static hipError_t launch(const CacheAttnArgs& a, const CachePlan& plan, hipStrea
         if (plan.chunks)
             hipLaunchKernelGGL((cache_attn_chunk<D, QP, PP>), dim3(tiles * a.splits, heads, batch), block, 0, s, a);
         else
-            hipLaunchKernelGGL((cache_attn<D, QP, PP>), a.whole ? dim3(tiles, heads, batch) : dim3(plan.wgs), block, 0,
-                               s, a);
+            hipLaunchKernelGGL((plan.wide ? cache_attn<D, QP, PP, 8> : cache_attn<D, QP, PP, 4>),
+                               a.whole ? dim3(tiles, heads, batch) : dim3(plan.wgs), dim3(plan.wide ? 512 : 256), 0, s,
+                               a);
     };
     constexpr std::integral_constant<int, 1> one;
     constexpr std::integral_constant<int, 2> two;

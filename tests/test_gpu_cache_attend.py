@@ -97,6 +97,19 @@ def test_many_sequences(torch_gpu, d, batch):
 
 
 @pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("batch", [128, 130])
+def test_short_sequences(torch_gpu, d, t, batch):
+    """Up to 1000 tokens, a workgroup a unit: 256 units, and a few more than the chip has CUs."""
+    rng = np.random.default_rng(batch)
+    lengths = rng.integers(1, 1000, batch)
+    lengths[:6] = [1000, 256, 257, 512, 513, 0]
+    p = Pool(torch_gpu, d, list(range(batch + 1)), lengths.tolist(), 2, 16, 6, extra_cols=0, seed=batch)
+    q, qv = draw16(torch_gpu, rng, (1, batch, 6, d), t)
+    check(torch_gpu, p, q, qv, t)
+
+
+@pytest.mark.parametrize("d", [64, 128])
 def test_a_long_prefix_under_a_few_rows(torch_gpu, d):
     """Chunks whose keys are split over workgroups, and more rows than a workgroup's columns."""
     rng = np.random.default_rng(d)
