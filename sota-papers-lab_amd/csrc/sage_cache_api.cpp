@@ -120,13 +120,16 @@ sage_status shape_checked(const sage_cache_shape& h) {
                          (u64)h.max_pages, (u64)h.page_tokens);
     if (h.rows >= ROWS)
         return set_error(SAGE_ERR_INVALID, "cache: %llu rows exceed the launch grid", (u64)h.rows);
-    // Launch grids: the KV heads (append: K, V and query heads) in y, the batch in z.
+    // Launch grids: x below 2^24 workgroups, append's K, V and query heads and the
+    // joins' KV heads in y, the batch in z.
     if (h.batch > 65535 || h.heads > 65535 || 2 * h.kv_heads + h.heads > 65535)
         return set_error(SAGE_ERR_INVALID, "cache: %llu sequences of %llu and %llu heads exceed the launch grid",
                          (u64)h.batch, (u64)h.heads, (u64)h.kv_heads);
-    if (h.max_new > I32 / 64 / (h.heads / h.kv_heads))
+    // A tile is 16 columns or more; 128 where there are many.
+    const uint64_t group = h.heads / h.kv_heads;
+    if (h.max_new > I32 / 64 / group || (h.max_new * group + 127) / 128 * h.kv_heads >= 1ull << 24)
         return set_error(SAGE_ERR_INVALID, "cache: %llu new rows of %llu heads a KV head exceed the launch grid",
-                         (u64)h.max_new, (u64)(h.heads / h.kv_heads));
+                         (u64)h.max_new, (u64)group);
     return SAGE_OK;
 }
 

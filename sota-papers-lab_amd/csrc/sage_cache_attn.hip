@@ -305,8 +305,9 @@ __global__ __launch_bounds__(64 * W, D == 64 && W == 4 ? 3 : 2) void cache_attn(
         b = blockIdx.z, base_b = 0;
         seq = sequence_index(c, b, a.max_new);
         const Units units(a, seq);
-        if ((int)blockIdx.x >= units.tiles) return;
-        pos = ((long long)blockIdx.y * units.tiles + blockIdx.x) * (units.steps + 1);
+        const int kvh = blockIdx.x % c.kv_heads, tile = blockIdx.x / c.kv_heads;
+        if (tile >= units.tiles) return;
+        pos = ((long long)kvh * units.tiles + tile) * (units.steps + 1);
         stop = pos + units.steps + 1;
     } else {
         const Line line(a, lane);
@@ -579,7 +580,7 @@ __global__ __launch_bounds__(64 * W, D == 64 && W == 4 ? 3 : 2) void cache_attn(
 // K would double what the waves read from LDS, which is then what bounds the
 // kernel, while the conversion (one instruction for two codes) runs beside the
 // MFMAs of the logits. Chunks of 2048 rows behind 8190 tokens, 32/8 heads of 128
-// (425 GFLOP): 482 us, 0.88 PFLOP/s; the chip's clock falls to 1.9 GHz under
+// (425 GFLOP): 445 us, 0.96 PFLOP/s; the chip's clock falls to 1.9 GHz under
 // it, with the MFMA pipe busy 44% of the time.
 constexpr int CCOLS = 128;
 typedef float f16v __attribute__((ext_vector_type(16)));
@@ -600,9 +601,9 @@ __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
     __shared__ __align__(16) ChunkLds<D> lds;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
-    const int split = blockIdx.x % a.splits, kvh = blockIdx.y, b = blockIdx.z;
-    const int tile = gridDim.x / a.splits - 1 - blockIdx.x / a.splits;  // the last rows see most: first
     const CacheDev& c = a.c;
+    const int b = blockIdx.z, kvh = blockIdx.x % c.kv_heads, at = blockIdx.x / c.kv_heads, split = at % a.splits;
+    const int tile = gridDim.x / c.kv_heads / a.splits - 1 - at / a.splits;  // the last rows see most: first
     const SequenceIndex seq = sequence_index(c, b, a.max_new);
     const int first = tile * CCOLS, cols = seq.n * a.group;
     if (first >= cols) return;
@@ -939,13 +940,19 @@ static hipError_t launch(const CacheAttnArgs& a, const CachePlan& plan, hipStrea
     const dim3 block(256);
     const unsigned per = plan.chunks ? CCOLS : COLS, heads = a.c.kv_heads, batch = a.c.batch;
     const unsigned tiles = (unsigned)(((long long)a.max_new * a.group + per - 1) / per);
+    // KV heads run fastest: the workgroups that read one head's keys are eight or
+    // a multiple of it apart where there are as many heads, so on one XCD, whose
+    // L2 holds that head's pages and not a part of all (chunks of 2048 rows behind 8190
+    // tokens, 32/8 heads of 128: 445 us, 481 with the tiles fastest, fp16 336
+    // and 384; 1327 rows over 1500 states, 16 heads of 64: 30.7 and 33.5).
     const auto go = [&](auto qp, auto pp) {
         constexpr int QP = decltype(qp)::value, PP = decltype(pp)::value;
         if (plan.chunks)
-            hipLaunchKernelGGL((cache_attn_chunk<D, QP, PP>), dim3(tiles * a.splits, heads, batch), block, 0, s, a);
+            hipLaunchKernelGGL((cache_attn_chunk<D, QP, PP>), dim3(heads * tiles * a.splits, 1, batch), block, 0, s,
+                               a);
         else
             hipLaunchKernelGGL((plan.wide ? cache_attn<D, QP, PP, 8> : cache_attn<D, QP, PP, 4>),
-                               a.whole ? dim3(tiles, heads, batch) : dim3(plan.wgs), dim3(plan.wide ? 512 : 256), 0, s,
+                               a.whole ? dim3(heads * tiles, 1, batch) : dim3(plan.wgs), dim3(plan.wide ? 512 : 256), 0, s,
                                a);
     };
     constexpr std::integral_constant<int, 1> one;

@@ -222,6 +222,7 @@ static void refusals() {
     all([](H h, C, I) { h.heads = 65536, h.kv_heads = 1; }, "exceed the launch grid");
     all([](H h, C, I) { h.heads = h.kv_heads = 30000; }, "exceed the launch grid");
     all([](H h, C, I) { h.max_new = 1ull << 31; }, "exceed the launch grid");
+    all([](H h, C, I) { h.heads = h.kv_heads = 64, h.max_new = (1ull << 25) - 1; }, "exceed the launch grid");
     all([](H h, C, I) { h.pages = 6; }, "cache K codes: buffer holds 10240 elements, needs 12288");
     all([](H, C c, I) { c.scales_len--; }, "cache K scales: buffer holds 639 elements, needs 640");
     all([](H, C c, I) { c.k_codes = nullptr; }, "cache K codes: buffer holds 0");
