@@ -730,7 +730,7 @@ __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
     __syncthreads();
     int buf = 0;
     for (int t = t0; t < end; t += TOKENS, buf ^= 1) {
-        const int4 fl = *reinterpret_cast<const int4*>(lds.flags[buf]);
+        int4 fl = *reinterpret_cast<const int4*>(lds.flags[buf]);
         if (t + TOKENS < end) {
             store_k(buf ^ 1);
             store_v(buf ^ 1);
@@ -739,6 +739,9 @@ __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
         f16v x[2];
         scores(buf, 0, x[0]);
         scores(buf, 1, x[1]);
+        // The flags are waited for here, not where they are read (head dim 64, 2 x 1500
+        // rows behind 3000 tokens, 16 heads: 79.1 us against 81.4).
+        asm volatile("" : "+v"(fl.x), "+v"(fl.y), "+v"(fl.z), "+v"(fl.w));
         const int flags = __builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w);
         uint32_t hit = 0;
         if (flags || t + TOKENS > least) {
