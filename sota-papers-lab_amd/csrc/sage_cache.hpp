@@ -75,9 +75,10 @@ hipError_t launch_cache_read(int head_dim, const ReadArgs& a, hipStream_t s);
 // of eight waves) or on wgs workgroups; and the partial outputs that the
 // workspace holds. max_tokens: most tokens that the page table holds.
 struct CachePlan {
-    bool chunks, whole, wide;
+    bool chunks, whole;
     int wgs;
     uint64_t part_rows;
+    bool wide;
 };
 CachePlan cache_plan(int head_dim, int batch, int rows, int heads, int kv_heads, int max_new, int max_tokens);
 hipError_t launch_cache_attend(int head_dim, const CacheAttnArgs& a, const CachePlan& plan, hipStream_t s);
