@@ -548,9 +548,11 @@ typedef struct sage_cache_options {
  * own type; out may be q itself (one address and strides, the same 16-bit
  * size) where no two rows of it share an element, else the two share none.
  * A row that sees nothing becomes zeros. The shape is the workspace's.
- * Logits, softmax statistics and sums are fp32; cached values are exact, and
- * the probabilities are rounded to bf16 for the second product, for an fp16
- * out to two bf16 parts. The sums are of weights up to 2^8, so values of V
+ * Logits, softmax statistics and sums are fp32; cached values are exact. For the
+ * second product the probabilities are rounded to two bf16 parts (2^-16 of
+ * each); in chunks of rows with a bf16 out, where V's scales are 2^-13 to 2^13,
+ * to fp16: 2^-11 of each, and 2^-32 of the row's greatest of those below 2^-21
+ * of it. The sums are of weights up to 2^8, so values of V
  * past 2^100 can overflow them; V blocks of scale 2^126 and up (bytes 253 and
  * 254), which hold infinities, count as NaN. The same call gives the same bits;
  * the order of a row's sums, and so its last bits, depend on the shape and on

@@ -7,12 +7,16 @@
 // E2M1 codes and an E8M0 scale are exact in bf16, and gfx950 converts two codes
 // and their scale in one instruction (v_cvt_scalef32_pk_bf16_fp4), so both
 // products run on the bf16 MFMA with fp32 sums: K and V enter exactly, bf16
-// queries too, fp16 ones as two bf16 parts; the probabilities are rounded to
-// bf16 (half a step: 2^-8 of each), or, where the output is fp16, to two bf16
-// parts. The scaled FP8 x FP4 MFMA would take K's
-// codes as they are, but it drops the terms of a dot product that lie some
+// queries too, fp16 ones as two bf16 parts. The scaled FP8 x FP4 MFMA would take
+// K's codes as they are, but it drops the terms of a dot product that lie some
 // 2^-12 below its largest: under a channel of K with a large offset, which the
 // softmax cancels, that is more than the differences between the keys.
+//
+// The probabilities enter the second product as two bf16 parts (half a step of
+// half a step: 2^-16 of each); one part, 2^-8 of each, would be an error of the
+// size of a bf16 output's own rounding (0.0023 against 64 bits where the output
+// alone has 0.0017). Decoding has the room: 63 sequences of up to 16384 tokens 125
+// us, 123.5 with one part. Chunks do not (cache_attn_chunk).
 //
 // A tile's "columns" are (row, head of the group) pairs of one KV head: S^T =
 // K Q^T gives each lane one column and four tokens of each 16-token tile, and
@@ -29,10 +33,13 @@ namespace {
 
 typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef short s8 __attribute__((ext_vector_type(8)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
 
 constexpr int COLS = 16;    // columns of a workgroup
 constexpr int TOKENS = 64;  // tokens of a wave's step
@@ -46,7 +53,19 @@ constexpr float NEG_INF = -__builtin_inff();
 // rows that do not see it as 0 * inf.
 constexpr uint32_t V_NAN = 253;
 
+// Codes 2 which and 2 which + 1 of a dword times s, as bf16 or fp16 (H16).
+template <bool H16>
 __device__ __forceinline__ uint32_t cvt2(uint32_t codes, float s, int which) {
+    if constexpr (H16) {
+        h2 r;
+        switch (which) {
+            case 0: r = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, s, 0); break;
+            case 1: r = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, s, 1); break;
+            case 2: r = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, s, 2); break;
+            default: r = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, s, 3);
+        }
+        return __builtin_bit_cast(uint32_t, r);
+    }
     bf2 r;
     switch (which) {
         case 0: r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, s, 0); break;
@@ -58,8 +77,10 @@ __device__ __forceinline__ uint32_t cvt2(uint32_t codes, float s, int which) {
 }
 
 // Eight channels of one code dword.
+template <bool H16 = false>
 __device__ __forceinline__ uint4 decode8(uint32_t codes, float s) {
-    return make_uint4(cvt2(codes, s, 0), cvt2(codes, s, 1), cvt2(codes, s, 2), cvt2(codes, s, 3));
+    return make_uint4(cvt2<H16>(codes, s, 0), cvt2<H16>(codes, s, 1), cvt2<H16>(codes, s, 2),
+                      cvt2<H16>(codes, s, 3));
 }
 
 // Eight values as bf16, or as two bf16 parts: the nearest and the rest's.
@@ -280,9 +301,9 @@ struct Line {
 // Steps of a share; at least two, so that a share is more than a unit's first step.
 __device__ __forceinline__ long long share_of(long long total, int wgs) { return max(2ll, (total + wgs - 1) / wgs); }
 
-// QP, PP: bf16 parts of a query and of a probability. W: waves, four, or eight
-// for whole units that do not fill the chip (cache_plan).
-template <int D, int QP, int PP, int W>
+// QP: bf16 parts of a query. W: waves, four, or eight for whole units that do
+// not fill the chip (cache_plan).
+template <int D, int QP, int W>
 __global__ __launch_bounds__(64 * W, D == 64 && W == 4 ? 3 : 2) void cache_attn(CacheAttnArgs a) {
     constexpr int G = D / 32;        // scale blocks of a row
     constexpr int VT = 64 / G;       // tokens of one V load
@@ -505,14 +526,14 @@ __global__ __launch_bounds__(64 * W, D == 64 && W == 4 ? 3 : 2) void cache_attn(
                 float e[8];
 #pragma unroll
                 for (int r = 0; r < 8; r++) e[r] = x[i + r / 4][r % 4];
-                bf8 p[PP];
-                parts_of<PP>(e, p);
+                bf8 p[2];
+                parts_of<2>(e, p);
 #pragma unroll
                 for (int u = 0; u < UNITS; u++) {
                     const uint8_t* at = vl + unit_at<D>(4 * g + (col >> 2), u, col >> 1 & 1) + (col & 1) * 8;
                     const bf8 vv = read_v(at, 16 * (D * 2));
 #pragma unroll
-                    for (int k = 0; k < PP; k++)
+                    for (int k = 0; k < 2; k++)
                         o[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, p[k], o[u], 0, 0, 0);
                 }
             }
@@ -582,8 +603,26 @@ __global__ __launch_bounds__(64 * W, D == 64 && W == 4 ? 3 : 2) void cache_attn(
 // MFMAs of the logits. Chunks of 2048 rows behind 8190 tokens, 32/8 heads of 128
 // (425 GFLOP): 445 us, 0.96 PFLOP/s; the chip's clock falls to 1.9 GHz under
 // it, with the MFMA pipe busy 44% of the time.
+//
+// For a bf16 output the weights are fp16 (2^-11 of each) and V goes through the
+// fp16 MFMA, while its scales are within HALF_LEAST .. HALF_MOST, where codes times
+// scale are exact normal fp16 values as well; from the first tile with a block
+// that fp16 does not hold on, a second loop, entered once, takes two bf16 parts.
+// Two parts everywhere took the chunks above from 427 us to 565, fp16 from 448 to
+// 460 (another box).
 constexpr int CCOLS = 128;
-typedef float f16v __attribute__((ext_vector_type(16)));
+// V's scale bytes whose values, 0.5 to 6 times the scale, are normal fp16
+// numbers: 2^-13 to 2^13.
+constexpr uint32_t HALF_LEAST = 114, HALF_MOST = 140;
+// Weights of fp16 are 2^LIFT times those of bf16, from 2^-21 on normal numbers and
+// 2^15 at most; the reference that goes with their sums is as much lower.
+constexpr float LIFT = 7.0f;
+// Whether a scale byte is past HALF_LEAST .. HALF_MOST, and whether its block is
+// more than fp16 holds: NaN, or codes (its dwords or'ed) other than zeros.
+__device__ __forceinline__ bool past_half(uint32_t scale) { return scale - HALF_LEAST > HALF_MOST - HALF_LEAST; }
+__device__ __forceinline__ bool past_half(uint32_t scale, uint32_t codes) {
+    return past_half(scale) && (scale >= V_NAN || (codes & 0x77777777u));
+}
 
 template <int D>
 struct ChunkLds {
@@ -591,11 +630,11 @@ struct ChunkLds {
     uint8_t k[2][TOKENS * D / 2];
     uint32_t ks[2][TOKENS];      // the token's scale bytes
     uint64_t bad[2][4];          // V blocks that are NaN, bit (token % 16) * 4 + block, by 16 tokens
-    int flags[2][4];             // by 16 tokens: 1 bad blocks, 2 no page
+    int flags[2][4];             // by 16 tokens: 1 bad blocks, 2 no page, 4 past fp16
 };
 
-// QP, PP: bf16 parts of a query and of a probability.
-template <int D, int QP, int PP>
+// QP: bf16 parts of a query. OUT16: the output is fp16.
+template <int D, int QP, bool OUT16>
 __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
     constexpr int G = D / 32, KS = D / 16, CT = D / 32, WORDS = D / 32;  // WORDS: code dwords a thread loads
     __shared__ __align__(16) ChunkLds<D> lds;
@@ -676,16 +715,29 @@ __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
             *reinterpret_cast<uint2*>(lds.k[buf] + k_at) = make_uint2(kr.w[0], kr.w[1]);
         lds.ks[buf][tok] = kr.sc;  // (four threads, one value)
     };
-    auto store_v = [&](int buf) {
-        const bool nan = vr.sc >= V_NAN;
-        const uint64_t bad = __ballot(D == 128 ? nan : nan && !(part & 1));
-        if (bad) lds.bad[buf][wave] = bad;
-        lds.flags[buf][wave] = (bad != 0) | (v_there ? 0 : 2);
-        const float s = __uint_as_float(nan ? 0 : vr.sc << 23);
+    auto store_v = [&](int buf, auto fp16) {
+        constexpr bool H16 = decltype(fp16)::value;
+        uint32_t sc = vr.sc;
+        int flag = v_there ? 0 : 2;
+        if (H16) {
+            if (__any(past_half(sc))) {
+                uint32_t codes = 0;
+#pragma unroll
+                for (int w = 0; w < WORDS; w++) codes |= vr.w[w];
+                if (__any(past_half(sc, codes))) flag |= 4;
+            }
+        } else {
+            const bool nan = sc >= V_NAN;
+            const uint64_t bad = __ballot(D == 128 ? nan : nan && !(part & 1));
+            if (bad) lds.bad[buf][wave] = bad, flag |= 1;
+            if (nan) sc = 0;
+        }
+        lds.flags[buf][wave] = flag;
+        const float s = __uint_as_float(sc << 23);
 #pragma unroll
         for (int w = 0; w < WORDS; w++) {
             const int ch = part * (D / 4) + 8 * w;
-            *reinterpret_cast<uint4*>(lds.v[buf] + unit_at<D>(tok, ch / 16, ch >> 3 & 1)) = decode8(vr.w[w], s);
+            *reinterpret_cast<uint4*>(lds.v[buf] + unit_at<D>(tok, ch / 16, ch >> 3 & 1)) = decode8<H16>(vr.w[w], s);
         }
     };
 
@@ -694,7 +746,7 @@ __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
     for (int u = 0; u < CT; u++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[u][i] = 0.0f;
-    float m = NEG_INF, l = 0.0f;
+    float m = NEG_INF, l = 0.0f, lift = OUT16 ? 0.0f : LIFT;
     // Where a lane reads K's codes, and the place of a transposing read of V:
     // lanes 0-15 and 32-47 the first 16 of 32 channels, tokens 4 * half +
     // (lane % 16) / 4.
@@ -721,96 +773,126 @@ __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
         }
     };
 
-    if (t0 < end) {
-        load(t0);
-        store_k(0);
-        store_v(0);
-        load(t0 + TOKENS);
-    }
-    __syncthreads();
-    int buf = 0;
-    for (int t = t0; t < end; t += TOKENS, buf ^= 1) {
-        int4 fl = *reinterpret_cast<const int4*>(lds.flags[buf]);
-        if (t + TOKENS < end) {
-            store_k(buf ^ 1);
-            store_v(buf ^ 1);
-            load(t + 2 * TOKENS);
+    // The tiles from t on, with fp16 weights (H16) until a scale of V is past
+    // them; returns where they stopped, in every wave alike.
+    auto walk = [&](int t, auto fp16) __attribute__((always_inline)) {
+        constexpr bool H16 = decltype(fp16)::value;
+        if (t < end) {
+            load(t);
+            store_k(0);
+            store_v(0, fp16);
+            load(t + TOKENS);
         }
-        f16v x[2];
-        scores(buf, 0, x[0]);
-        scores(buf, 1, x[1]);
-        // The flags are waited for here, not where they are read (head dim 64, 2 x 1500
-        // rows behind 3000 tokens, 16 heads: 79.1 us against 81.4).
-        asm volatile("" : "+v"(fl.x), "+v"(fl.y), "+v"(fl.z), "+v"(fl.w));
-        const int flags = __builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w);
-        uint32_t hit = 0;
-        if (flags || t + TOKENS > least) {
-            const int fi[4] = {fl.x, fl.y, fl.z, fl.w};
+        __syncthreads();
+        int buf = 0;
+        for (; t < end; t += TOKENS, buf ^= 1) {
+            int4 fl = *reinterpret_cast<const int4*>(lds.flags[buf]);
+            if (t + TOKENS < end) {
+                store_k(buf ^ 1);
+                store_v(buf ^ 1, fp16);
+                load(t + 2 * TOKENS);
+            }
+            f16v x[2];
+            scores(buf, 0, x[0]);
+            scores(buf, 1, x[1]);
+            // The flags are waited for here, not where they are read (head dim 64, 2 x 1500
+            // rows behind 3000 tokens, 16 heads: 79.1 us against 81.4).
+            asm volatile("" : "+v"(fl.x), "+v"(fl.y), "+v"(fl.z), "+v"(fl.w));
+            const int flags = __builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w);
+            if (H16 && flags & 4) return t;
+            uint32_t hit = 0;
+            if (flags || t + TOKENS > least) {
+                const int fi[4] = {fl.x, fl.y, fl.z, fl.w};
+#pragma unroll
+                for (int sub = 0; sub < 2; sub++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const int k = 32 * sub + 8 * (i / 4) + 4 * half + i % 4, six = 2 * sub + i / 8;
+                        const bool seen = t + k < limit && !(fi[six] & 2);
+                        if (!seen) x[sub][i] = NEG_INF;
+                        if (!H16 && flags & 1) {
+                            const uint32_t blocks = (uint32_t)(lds.bad[buf][six] >> ((k & 15) * 4)) & 15;
+                            if (seen && (fi[six] & 1)) hit |= blocks;
+                        }
+                    }
+                if (!H16 && flags & 1) {
+                    auto r = __builtin_amdgcn_permlane32_swap(hit, hit, false, false);
+                    hit = r[0] | r[1];
+                }
+            }
+            float mx = NEG_INF;
 #pragma unroll
             for (int sub = 0; sub < 2; sub++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int k = 32 * sub + 8 * (i / 4) + 4 * half + i % 4, six = 2 * sub + i / 8;
-                    const bool seen = t + k < limit && !(fi[six] & 2);
-                    if (!seen) x[sub][i] = NEG_INF;
-                    if (flags & 1) {
-                        const uint32_t blocks = (uint32_t)(lds.bad[buf][six] >> ((k & 15) * 4)) & 15;
-                        if (seen && (fi[six] & 1)) hit |= blocks;
+                for (int i = 0; i < 16; i++) mx = fmaxf(mx, x[sub][i]);
+            {
+                auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+                mx = fmaxf(m, fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+            }
+            if (__any((mx - m) * a.qk_mul > SLACK)) {
+                const float scale = __builtin_amdgcn_exp2f((m - (mx == NEG_INF ? 0.0f : mx)) * a.qk_mul);
+                m = mx;
+                l *= scale;
+#pragma unroll
+                for (int u = 0; u < CT; u++) o[u] *= scale;
+            }
+            const float base = (m == NEG_INF ? 0.0f : m * a.qk_mul) - (H16 ? LIFT : 0.0f);
+#pragma unroll
+            for (int sub = 0; sub < 2; sub++)
+#pragma unroll
+                for (int st = 0; st < 2; st++) {
+                    float e[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[sub][8 * st + i], a.qk_mul, -base));
+                        l += e[i];
+                    }
+                    bf8 p[2];
+                    if constexpr (H16)
+                        p[0] = __builtin_bit_cast(bf8, make_uint4(pack_f16x2(e[0], e[1]), pack_f16x2(e[2], e[3]),
+                                                                  pack_f16x2(e[4], e[5]), pack_f16x2(e[6], e[7])));
+                    else
+                        parts_of<2>(e, p);
+#pragma unroll
+                    for (int u = 0; u < CT; u++) {
+                        const uint8_t* at = lds.v[buf] + (32 * sub + 16 * st) * (D * 2) +
+                                            unit_at<D>(vtok, 2 * u + vunit, lane >> 1 & 1) + (lane & 1) * 8;
+                        const bf8 vv = read_v(at, 8 * (D * 2));
+                        if constexpr (H16) {
+                            o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, vv),
+                                                                          __builtin_bit_cast(h8, p[0]), o[u], 0, 0, 0);
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 2; k++)
+                                o[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv, p[k], o[u], 0, 0, 0);
+                        }
                     }
                 }
-            if (flags & 1) {
-                auto r = __builtin_amdgcn_permlane32_swap(hit, hit, false, false);
-                hit = r[0] | r[1];
+            if (!H16 && flags & 1) {
+                asm volatile("" : "+v"(hit));  // a branch, not a select of every sum in every step
+#pragma unroll
+                for (int u = 0; u < CT; u++)
+                    if (hit >> (D == 128 ? u : 2 * u) & 1)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) o[u][i] = __builtin_nanf("");
             }
+            __syncthreads();
         }
-        float mx = NEG_INF;
+        return t;
+    };
+    if constexpr (OUT16) {
+        walk(t0, std::false_type{});
+    } else {
+        const int t = walk(t0, std::true_type{});
+        if (t < end) {
+            lift = 0.0f;
+            l *= __builtin_amdgcn_exp2f(-LIFT);
 #pragma unroll
-        for (int sub = 0; sub < 2; sub++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) mx = fmaxf(mx, x[sub][i]);
-        {
-            auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-            mx = fmaxf(m, fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+            for (int u = 0; u < CT; u++) o[u] *= __builtin_amdgcn_exp2f(-LIFT);
+            __syncthreads();  // every wave has read the tile's flags
+            pages.fill((t + 16 * wave) >> c.page_shift);
+            walk(t, std::false_type{});
         }
-        if (__any((mx - m) * a.qk_mul > SLACK)) {
-            const float scale = __builtin_amdgcn_exp2f((m - (mx == NEG_INF ? 0.0f : mx)) * a.qk_mul);
-            m = mx;
-            l *= scale;
-#pragma unroll
-            for (int u = 0; u < CT; u++) o[u] *= scale;
-        }
-        const float base = m == NEG_INF ? 0.0f : m * a.qk_mul;
-#pragma unroll
-        for (int sub = 0; sub < 2; sub++)
-#pragma unroll
-            for (int st = 0; st < 2; st++) {
-                float e[8];
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[sub][8 * st + i], a.qk_mul, -base));
-                    l += e[i];
-                }
-                bf8 p[PP];
-                parts_of<PP>(e, p);
-#pragma unroll
-                for (int u = 0; u < CT; u++) {
-                    const uint8_t* at = lds.v[buf] + (32 * sub + 16 * st) * (D * 2) +
-                                        unit_at<D>(vtok, 2 * u + vunit, lane >> 1 & 1) + (lane & 1) * 8;
-                    const bf8 vv = read_v(at, 8 * (D * 2));
-#pragma unroll
-                    for (int k = 0; k < PP; k++)
-                        o[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv, p[k], o[u], 0, 0, 0);
-                }
-            }
-        if (flags & 1) {
-            asm volatile("" : "+v"(hit));  // a branch, not a select of every sum in every step
-#pragma unroll
-            for (int u = 0; u < CT; u++)
-                if (hit >> (D == 128 ? u : 2 * u) & 1)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) o[u][i] = __builtin_nanf("");
-        }
-        __syncthreads();
     }
     {
         auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
@@ -839,7 +921,7 @@ __global__ __launch_bounds__(256, 2) void cache_attn_chunk(CacheAttnArgs a) {
                 *reinterpret_cast<f4*>(a.part_o + at * D + 32 * u + 2 * i + 4 * half) =
                     f4{o[u][i], o[u][i + 1], o[u][i + 2], o[u][i + 3]};
         if (half == 0) {
-            a.part_ml[at * 2] = m * a.qk_mul;
+            a.part_ml[at * 2] = m * a.qk_mul - lift;
             a.part_ml[at * 2 + 1] = l;
         }
     }
@@ -948,22 +1030,23 @@ static hipError_t launch(const CacheAttnArgs& a, const CachePlan& plan, hipStrea
     // L2 holds that head's pages and not a part of all (chunks of 2048 rows behind 8190
     // tokens, 32/8 heads of 128: 445 us, 481 with the tiles fastest, fp16 336
     // and 384; 1327 rows over 1500 states, 16 heads of 64: 30.7 and 33.5).
-    const auto go = [&](auto qp, auto pp) {
-        constexpr int QP = decltype(qp)::value, PP = decltype(pp)::value;
-        if (plan.chunks)
-            hipLaunchKernelGGL((cache_attn_chunk<D, QP, PP>), dim3(heads * tiles * a.splits, 1, batch), block, 0, s,
-                               a);
-        else
-            hipLaunchKernelGGL((plan.wide ? cache_attn<D, QP, PP, 8> : cache_attn<D, QP, PP, 4>),
-                               a.whole ? dim3(heads * tiles, 1, batch) : dim3(plan.wgs), dim3(plan.wide ? 512 : 256), 0, s,
-                               a);
+    const auto few = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, a.whole ? dim3(heads * tiles, 1, batch) : dim3(plan.wgs),
+                           dim3(plan.wide ? 512 : 256), 0, s, a);
     };
-    constexpr std::integral_constant<int, 1> one;
-    constexpr std::integral_constant<int, 2> two;
-    if (a.q_f16)
-        a.out_f16 ? go(two, two) : go(two, one);
-    else
-        a.out_f16 ? go(one, two) : go(one, one);
+    const auto chunk = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(heads * tiles * a.splits, 1, batch), block, 0, s, a);
+    };
+    if (plan.chunks) {
+        if (a.q_f16)
+            chunk(a.out_f16 ? cache_attn_chunk<D, 2, true> : cache_attn_chunk<D, 2, false>);
+        else
+            chunk(a.out_f16 ? cache_attn_chunk<D, 1, true> : cache_attn_chunk<D, 1, false>);
+    } else if (a.q_f16) {
+        few(plan.wide ? cache_attn<D, 2, 8> : cache_attn<D, 2, 4>);
+    } else {
+        few(plan.wide ? cache_attn<D, 1, 8> : cache_attn<D, 1, 4>);
+    }
     // Many parts of few columns are joined by a workgroup a column (20000 tokens,
     // 32/8 heads of 128: one row each of 2 sequences 21.5 us against 24, of 8 47.7
     // against 46.8; chunks of 32 rows 37.4 against 39.3, of 128 76 against 70).
