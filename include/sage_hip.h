@@ -547,7 +547,9 @@ typedef struct sage_cache_options {
  * of [row][head][head_dim] (strides.batch is not read), bf16 or fp16, each its
  * own type; out may be q itself (one address and strides, the same 16-bit
  * size) where no two rows of it share an element, else the two share none.
- * A row that sees nothing becomes zeros. The shape is the workspace's.
+ * A row that sees nothing becomes zeros. The shape is the workspace's: the
+ * pool's pages, page_tokens and kv_heads have to be the same, of which the
+ * buffers' lengths tell only so much.
  * Logits, softmax statistics and sums are fp32; cached values are exact. For the
  * second product the probabilities are rounded to two bf16 parts (2^-16 of
  * each); in chunks of rows with a bf16 out, where V's scales are 2^-13 to 2^13,

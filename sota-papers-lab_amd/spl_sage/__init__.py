@@ -438,6 +438,10 @@ def _current_device() -> int:
     return torch.cuda.current_device()
 
 
+def _layouts_differ(what: str, a: tuple, b: tuple) -> SageError:
+    return SageError(1, f"{what} differ: {a[0]} pages of {a[2]} tokens and {a[1]} KV heads, {b[0]} of {b[2]} and {b[1]}")
+
+
 class SageAttention:
     """Kernels for one head dim and Config on one stream (mod.rs:509-901).
     Every call enqueues work and returns without synchronising."""
@@ -449,6 +453,7 @@ class SageAttention:
         self._h = h.value
         self._stream = stream
         self._device = _current_device()
+        self._head_dim = head_dim
         self._destroy = lib().sage_destroy
 
     @classmethod
@@ -561,6 +566,16 @@ class SageAttention:
             st = (s.batch, s.token, s.head)
         return C.byref(cls(t.data_ptr(), _elems_from(t), st, _dtype_code(t)))
 
+    # A pool or a page table of another layout than the call's is long enough as
+    # often as not, and its rows are elsewhere.
+    def _fits(self, cache, index, shape) -> None:
+        if cache._head_dim not in (None, self._head_dim):
+            raise SageError(1, f"the cache is made for head dim {cache._head_dim}, the context for {self._head_dim}")
+        if cache.shape._layout != shape._layout:
+            raise _layouts_differ("the workspace and the cache", shape._layout, cache.shape._layout)
+        if index._cols not in (None, shape.max_pages) and shape.batch > 1:
+            raise SageError(1, f"the page table has {index._cols} columns, the shape {shape.max_pages}")
+
     def _out_of_reach(self, device: int) -> SageError:
         where = "in host memory" if device < 0 else f"on device {device}"
         return SageError(1, f"a tensor is {where}, the context on device {self._device}")
@@ -581,25 +596,29 @@ class SageAttention:
                      q_out: Optional[TensorMut] = None) -> None:
         """The step's keys (rotated) and values written to their slots of the
         cache, and its queries rotated into q_out in the same launch."""
-        _check(lib().sage_cache_append(self._h, C.byref(cache.shape._c()), self._handle(cache), self._handle(index),
-                                       self._view(_abi.sage_tensor, k), self._view(_abi.sage_tensor, v),
-                                       None if rotary is None else self._handle(rotary),
-                                       None if q is None else self._view(_abi.sage_tensor, q),
-                                       None if q_out is None else self._view(_abi.sage_tensor_mut, q_out)))
+        args = (C.byref(cache.shape._c()), self._handle(cache), self._handle(index), self._view(_abi.sage_tensor, k),
+                self._view(_abi.sage_tensor, v), None if rotary is None else self._handle(rotary),
+                None if q is None else self._view(_abi.sage_tensor, q),
+                None if q_out is None else self._view(_abi.sage_tensor_mut, q_out))
+        self._fits(cache, index, cache.shape)
+        _check(lib().sage_cache_append(self._h, *args))
 
     def cache_read(self, cache, index, k: TensorMut, v: TensorMut) -> None:
         """Cached rows back as 16-bit keys and values."""
-        _check(lib().sage_cache_read(self._h, C.byref(cache.shape._c()), self._handle(cache), self._handle(index),
-                                     self._view(_abi.sage_tensor_mut, k), self._view(_abi.sage_tensor_mut, v)))
+        args = (C.byref(cache.shape._c()), self._handle(cache), self._handle(index),
+                self._view(_abi.sage_tensor_mut, k), self._view(_abi.sage_tensor_mut, v))
+        self._fits(cache, index, cache.shape)
+        _check(lib().sage_cache_read(self._h, *args))
 
     def cache_attend(self, ws, cache, index, q: Tensor, out: TensorMut, softmax_scale: Optional[float] = None,
                      causal: bool = True) -> None:
         """Attention of the rows' queries over the cached keys of their sequences."""
         o = _abi.sage_cache_options(0.0 if softmax_scale is None else float(softmax_scale),
                                     0 if softmax_scale is None else 1, int(causal))
-        _check(lib().sage_cache_attend(self._h, ws._h, self._handle(cache), self._handle(index),
-                                       self._view(_abi.sage_tensor, q), self._view(_abi.sage_tensor_mut, out),
-                                       C.byref(o)))
+        args = (self._handle(cache), self._handle(index), self._view(_abi.sage_tensor, q),
+                self._view(_abi.sage_tensor_mut, out), C.byref(o))
+        self._fits(cache, index, ws.shape)
+        _check(lib().sage_cache_attend(self._h, ws._h, *args))
 
     def peak(self, which: int, iters: int = 2048) -> float:
         """Measured dense TOPS of one MFMA shape (0 INT8, 1 FP8, 2 BF16)."""

@@ -11,7 +11,7 @@ from __future__ import annotations
 import ctypes as C
 from dataclasses import dataclass
 
-from . import SageError, _abi, _check
+from . import SageError, _abi, _check, _layouts_differ
 from ._abi import lib
 from .rotary import _device_of, _ints
 
@@ -36,6 +36,7 @@ class CacheShape:
         c = _abi.sage_cache_shape(self.batch, self.rows, self.max_new, self.heads, self.kv_heads, self.pages,
                                   self.page_tokens, self.max_pages)
         object.__setattr__(self, "_struct", c)
+        object.__setattr__(self, "_layout", (self.pages, self.kv_heads, self.page_tokens))
 
     def _c(self) -> _abi.sage_cache_shape:
         return self._struct
@@ -60,7 +61,7 @@ class PagedCache:
     """The pool: uint8 device tensors [pages][kv_heads][page_tokens][head_dim/2]
     (codes) and [..][head_dim/32] (scales). Made once for its tensors; one pool
     serves steps of any shape with its pages, page_tokens and kv_heads
-    (with_shape)."""
+    (with_shape); another shape's rows lie elsewhere in it, and is refused."""
 
     shape: CacheShape
     k_codes: object
@@ -84,6 +85,17 @@ class PagedCache:
     def __post_init__(self):
         kc, ks = _bytes(self.k_codes, "cache K codes"), _bytes(self.k_scales, "cache K scales")
         vc, vs = _bytes(self.v_codes, "cache V codes"), _bytes(self.v_scales, "cache V scales")
+        dims = None  # of a row's codes and scales, where the tensors say them
+        for pair in ((self.k_codes, self.k_scales), (self.v_codes, self.v_scales)):
+            for t, channels in zip(pair, (2, BLOCK)):
+                if t.dim() != 4:
+                    continue
+                if tuple(t.shape[:3]) != self.shape._layout:
+                    raise _layouts_differ("the cache's tensors and shape", tuple(t.shape[:3]), self.shape._layout)
+                if dims not in (None, t.shape[3] * channels):
+                    raise SageError(1, f"the cache's tensors are of head dims {dims} and {t.shape[3] * channels}")
+                dims = t.shape[3] * channels
+        object.__setattr__(self, "_head_dim", dims)
         c = _abi.sage_cache(kc[0], ks[0], vc[0], vs[0], min(kc[1], vc[1]), min(ks[1], vs[1]))
         object.__setattr__(self, "_struct", c)
         object.__setattr__(self, "_device", _device_of("the cache's buffers", self.k_codes, self.k_scales, self.v_codes,
@@ -104,6 +116,7 @@ class CacheIndex:
         c = _abi.sage_cache_index(*_ints(self.starts, "cache starts"), *_ints(self.lengths, "cache lengths"),
                                   *_ints(self.page_table, "cache page table"))
         object.__setattr__(self, "_struct", c)
+        object.__setattr__(self, "_cols", self.page_table.shape[1] if self.page_table.dim() == 2 else None)
         object.__setattr__(self, "_device", _device_of("the cache's index", self.starts, self.lengths, self.page_table))
 
 

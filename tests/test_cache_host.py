@@ -197,3 +197,49 @@ def test_oracle_attention_is_the_softmax():
         x[np.arange(n)[None] > np.arange(n - 5, n)[:, None]] = -np.inf
         p = np.exp(x) / np.exp(x).sum(1, keepdims=True)
         assert np.allclose(got[:, h], p @ v[:, h // 2], rtol=1e-12, atol=1e-12)
+
+
+def test_layouts_that_differ_are_refused():
+    """A pool, workspace or page table of another layout, whose buffers are long enough: refused before the library is
+    called."""
+    import torch
+
+    import spl_sage as S
+    from spl_sage import cache as K
+
+    sa = object.__new__(S.SageAttention)  # no GPU here: the checks come before the handle's use
+    sa._h, sa._device, sa._head_dim = None, -1, 64
+    shape = K.CacheShape(2, 4, 2, 4, 2, 8, 32, 3)
+    pool = K.PagedCache.new(shape, 64, device="cpu")
+    ints = lambda *n: torch.zeros(*n, dtype=torch.int32)  # noqa: E731
+    index = K.CacheIndex(ints(3), ints(2), ints(2, 3))
+    x = torch.zeros(1, 4, 4, 64, dtype=torch.bfloat16)
+    t, m = S.Tensor(x), S.TensorMut(x)
+    ws = lambda h: type("", (), {"_h": None, "shape": h})  # noqa: E731
+
+    # A step of any size over the same pool passes the checks, up to the library's own.
+    for h in (shape, K.CacheShape(1, 1, 1, 2, 2, 8, 32, 3)):
+        with pytest.raises(S.SageError, match="null argument"):
+            sa.cache_attend(ws(h), pool.with_shape(h), index, t, m)
+    for h in (K.CacheShape(2, 4, 2, 4, 2, 16, 16, 6), K.CacheShape(2, 4, 2, 4, 4, 4, 32, 3), K.CacheShape(2, 4, 2, 4, 2, 7, 32, 3)):
+        with pytest.raises(S.SageError, match="KV heads"):
+            pool.with_shape(h)
+        with pytest.raises(S.SageError, match="the workspace and the cache differ"):
+            sa.cache_attend(ws(h), pool, index, t, m)
+    wide = K.CacheIndex(ints(3), ints(2), ints(2, 4))
+    calls = [lambda p, i: sa.cache_attend(ws(shape), p, i, t, m), lambda p, i: sa.cache_append(p, i, t, t),
+             lambda p, i: sa.cache_read(p, i, m, m)]
+    for call in calls:
+        with pytest.raises(S.SageError, match="4 columns, the shape 3"):
+            call(pool, wide)
+        with pytest.raises(S.SageError, match="made for head dim 128, the context for 64"):
+            call(K.PagedCache.new(shape, 128, device="cpu"), index)
+        with pytest.raises(S.SageError, match="null argument"):
+            call(pool, index)
+    big = K.PagedCache.new(shape, 128, device="cpu")
+    with pytest.raises(S.SageError, match="head dims 128 and 64"):
+        K.PagedCache(shape, big.k_codes, big.k_scales, pool.v_codes, pool.v_scales)
+    # Tensors that say no layout are the caller's word.
+    flat = K.PagedCache(shape, *(getattr(pool, n).flatten() for n in ("k_codes", "k_scales", "v_codes", "v_scales")))
+    with pytest.raises(S.SageError, match="null argument"):
+        sa.cache_read(flat, K.CacheIndex(ints(3), ints(2), ints(6)), m, m)
