@@ -435,10 +435,11 @@ typedef struct sage_rotary {
 } sage_rotary;
 
 /* x rotated into out, [batch][token][head][head_dim] views of shape's batch,
- * tokens and heads (kv_heads is not read), fewer than 2^26 rows (batch *
+ * tokens and heads (kv_heads is not read), at most 2^26 - 4 rows (batch *
  * tokens), both of one type; positions holds an entry a row. Each product and
- * sum is rounded in fp32, the result once to the type. transpose != 0 turns the other way: the gradient of the
- * rotation (its transpose, any attention factor included). out may be x itself
+ * sum is rounded in fp32, the result once to the type. transpose != 0 turns
+ * the other way: the gradient of the rotation (its transpose, any attention
+ * factor included). out may be x itself
  * (one address and strides) where no two rows of it share an element, else the
  * two share no element. An empty shape is a no-op. */
 sage_status sage_rotary_apply(const sage_attention* s, const sage_shape* shape, const sage_rotary* rotary,

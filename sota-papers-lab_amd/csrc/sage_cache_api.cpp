@@ -24,7 +24,8 @@ namespace {
 
 using u64 = unsigned long long;
 constexpr uint64_t I32 = 2147483647ull;
-// Rows below it: at most 64 threads a row in a grid's x, of which a launch takes less than 2^32.
+// Rows below it: at most 64 threads a row in a grid's x, of which a launch takes
+// less than 2^32. The rotation's workgroups take four rows each: 2^26 - 4 at most.
 constexpr uint64_t ROWS = 1ull << 26;
 
 sage_status hip_failed(hipError_t e, const char* what) {
@@ -218,7 +219,7 @@ sage_status sage_rotary_apply(const sage_attention* s, const sage_shape* shape, 
     if (__builtin_mul_overflow(shape->batch, shape->tokens, &rows) || rows > I32 || shape->heads > I32)
         return set_error(SAGE_ERR_INVALID, "rotary: %llu x %llu rows of %llu heads do not fit in i32",
                          (u64)shape->batch, (u64)shape->tokens, (u64)shape->heads);
-    if (rows >= ROWS || shape->heads > 1ull << 30)
+    if (rows > ROWS - 4 || shape->heads > 1ull << 30)
         return set_error(SAGE_ERR_INVALID, "rotary: %llu rows of %llu heads exceed the launch grid", (u64)rows,
                          (u64)shape->heads);
     const uint64_t d = s->head_dim;

@@ -242,9 +242,26 @@ static void refusals() {
     CHECK(passed(sage_cache_read(&ctx, &zero, &cache, &index, &eo, &eo)));
 }
 
+// The most rows that a rotation takes: four to a workgroup of 256, so 2^26 - 4
+// of them are the last below a launch's 2^32 threads.
+static void row_limit() {
+    sage_attention ctx{nullptr, -2, 128, sage_config_for_head_dim(128)};
+    alignas(256) static char mem[256];
+    const sage_strides st{0, 128, 128};
+    const sage_tensor x{mem, 1ull << 40, st, SAGE_BF16};
+    const sage_tensor_mut o{mem, 1ull << 40, st, SAGE_BF16};
+    const sage_rotary r{reinterpret_cast<float*>(mem), 64, 64, SAGE_ROTARY_HALF, nullptr, 0};
+    for (uint64_t more = 0; more <= 5; more++) {
+        const sage_shape shape{1, 1, (1ull << 26) - 5 + more, 0};
+        const sage_status s = sage_rotary_apply(&ctx, &shape, &r, &x, &o, 0);
+        CHECK(more < 2 ? passed(s) : refused(s, "exceed the launch grid"));
+    }
+}
+
 int main() {
     index_lookups();
     refusals();
+    row_limit();
     if (failed) return std::printf("%d checks failed\n", failed), 1;
     std::printf("cache host tests passed\n");
     return 0;
