@@ -62,15 +62,16 @@ def tolerance(want, size, reach, count, top, d, out_type, fp16_weights):
     return err + O.HALF_STEP[out_type] * (np.abs(want) + err) + least + 1e-37
 
 
-def spread(p, rng, v_shift=None):
-    """The pool's keys and values from normal draws: values of the tokens and channels have sizes of their own, and a
-    mean, so that sums do not cancel. v_shift: their exponents' shift, [.. dims of the pool .. or fewer]."""
-    shape = p.host["k_codes"].shape[:3] + (p.d,)
-    p.host["k_codes"], p.host["k_scales"], _ = O.quantise(rng.standard_normal(shape))
-    v = (rng.standard_normal(shape) + 0.5) * np.exp(0.5 * rng.standard_normal(shape[:3] + (1,)))
-    if v_shift is not None:
-        v = v * np.exp2(np.broadcast_to(v_shift, v.shape))
-    p.host["v_codes"], p.host["v_scales"], _ = O.quantise(v)
+def spread(p, rng, v_shift=0, positive=False):
+    """Keys whose logits are of the queries' size, and values whose tokens have sizes of their own and a mean, so that
+    sums do not cancel (positive: none does). v_shift: more of V's exponents, an integer a block of a row."""
+    dims = p.host["k_codes"].shape[:3]
+    codes = lambda: rng.integers(0, 256, dims + (p.d // 2,)).astype(np.uint8)  # noqa: E731
+    blocks = dims + (p.d // O.BLOCK,)
+    p.host["k_codes"] = codes()
+    p.host["k_scales"] = rng.integers(125, 127, blocks).astype(np.uint8)
+    p.host["v_codes"] = codes() & (0x77 if positive else codes() | 0x77)  # half of the negative ones turned
+    p.host["v_scales"] = (rng.integers(124, 128, dims + (1,)) + np.broadcast_to(v_shift, blocks)).astype(np.uint8)
     p.upload()
 
 

@@ -263,3 +263,58 @@ def test_cpp_calls(torch_gpu):
     assert exe.exists(), f"{exe} is not built; run `python __graft_entry__.py` (build)"
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0 and "0 failure(s)" in r.stdout, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("d,heads,kv", [(64, 6, 6), (128, 8, 2)])
+def test_an_encoder_s_states_beside_a_decoder_s_steps(torch_gpu, d, heads, kv):
+    """A decoder whose layer attends to its own cached tokens and to an encoder's cached states, in one pool: a prompt of
+    more rows than a tile (the chunk kernel, under a wide page table), then single tokens."""
+    import spl_sage as S
+    from cache_plans import plan
+    from spl_sage import cache as C
+    from spl_sage import rotary as R
+
+    torch, t, page, cols = torch_gpu, "bf16", 64, 40
+    rng = np.random.default_rng(4)
+    states, prompts = [301, 64, 7], [130, 20, 77]
+    m = Model(torch, d, heads, kv, [n + 3 for n in prompts], t, seed=4)
+    sa = S.SageAttention(torch.cuda.current_stream(), d)
+    pages = 6 * cols
+    tables = np.random.default_rng(5).permutation(pages).reshape(2, 3, cols)
+    own, other = ints(torch, tables[0]), ints(torch, tables[1])
+    # The encoder's states, once: no positions.
+    x, xv = draw16(torch, rng, (sum(states), 2 * kv, d), t)
+    at = np.concatenate([[0], np.cumsum(states)]).tolist()
+    pool = C.PagedCache.new(C.CacheShape(3, at[-1], max(states), heads, kv, pages, page, cols), d)
+    sa.cache_append(pool, C.CacheIndex(ints(torch, at), ints(torch, states), other), S.Tensor(x[None, :, :kv]),
+                    S.Tensor(x[None, :, kv:]))
+    keys, values = O.quantise(xv[:, :kv])[2], O.quantise(xv[:, kv:])[2]
+    kinds, begin = set(), [0, 0, 0]
+    for step in range(4):
+        end = [n + step for n in prompts]
+        fused, starts = step_rows(m, begin, end)
+        rows = starts[-1]
+        shape = C.CacheShape(3, rows, max(e - b for b, e in zip(begin, end)), heads, kv, pages, page, cols)
+        kinds.add(plan(shape, d).chunks)
+        cache, index, f = pool.with_shape(shape), C.CacheIndex(ints(torch, starts), ints(torch, end), own), fused[None]
+        q, k, v = f[:, :, :heads], f[:, :, heads:heads + kv], f[:, :, heads + kv:]
+        qr, out, cross = (torch.empty(1, rows, heads, d, dtype=f.dtype, device="cuda") for _ in range(3))
+        sa.cache_append(cache, index, S.Tensor(k), S.Tensor(v), R.Rotary(m.device_table, m.rot), S.Tensor(q), S.TensorMut(qr))
+        ws = sa.cache_workspace(shape)
+        sa.cache_attend(ws, cache, index, S.Tensor(qr), S.TensorMut(out))
+        sa.cache_attend(ws, cache, C.CacheIndex(ints(torch, starts), ints(torch, states), other), S.Tensor(q),
+                        S.TensorMut(cross), causal=False)
+        got, got_cross, qv = (y[0].double().cpu().numpy() for y in (out, cross, q))
+        for b in range(3):
+            want, size, reach = m.want[b]
+            s = slice(starts[b], starts[b + 1])
+            w, z = want[begin[b]:end[b]], size[begin[b]:end[b]]
+            assert (np.abs(got[s] - w) <= O.attend_tolerance(w, z, reach, d, t)).all(), (step, b)
+            pad = -states[b] % 16
+            one = lambda y: np.concatenate([y[at[b]:at[b + 1]], np.zeros((pad, kv, d))]).reshape(-1, 16, kv, d).transpose(0, 2, 1, 3)  # noqa: E731
+            n = starts[b + 1] - starts[b]
+            w, z, reach = O.attend(qv[s], one(keys), one(values), [0, n], [states[b]], np.arange((states[b] + pad) // 16)[None],
+                                   16, False, 1 / math.sqrt(d), np.zeros((n, heads, d)))
+            assert (np.abs(got_cross[s] - w) <= O.attend_tolerance(w, z, reach, d, t)).all(), (step, b)
+        begin = end
+    assert kinds == {True, False}
