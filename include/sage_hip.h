@@ -398,7 +398,10 @@ typedef enum sage_rotary_layout { SAGE_ROTARY_HALF = 0, SAGE_ROTARY_PAIRS = 1 } 
  *   NTK     base * factor^(rot / (rot - 2)) for the base (rot > 2)
  *   YARN    g_i w_i + (1 - g_i) w_i / factor, where g_i rises from 0 at
  *           beta_slow turns of the pair over `original` positions to 1 at
- *           beta_fast turns (0 for either: 1 and 32).
+ *           beta_fast turns (0 for either: 1 and 32), in proportion to the
+ *           turns. A model tuned with a ramp in proportion to i, between the
+ *           rounded indexes of those two pairs, has other angles in between:
+ *           it needs a table of its own, which the calls take as well.
  * attention multiplies cos and sin; 0: 0.1 ln(factor) + 1 under YARN, else 1. */
 typedef enum sage_rotary_scaling_kind {
     SAGE_ROTARY_NONE = 0,

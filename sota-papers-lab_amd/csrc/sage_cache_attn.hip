@@ -15,8 +15,9 @@
 // The probabilities enter the second product as two bf16 parts (half a step of
 // half a step: 2^-16 of each); one part, 2^-8 of each, would be an error of the
 // size of a bf16 output's own rounding (0.0023 against 64 bits where the output
-// alone has 0.0017). Decoding has the room: 63 sequences of up to 16384 tokens 125
-// us, 123.5 with one part. Chunks do not (cache_attn_chunk).
+// alone has 0.0017). Decoding has the room (2% of 63 sequences of up to 16384
+// tokens, 7% of 8 rows of 8 sequences behind 20000), chunks do not
+// (cache_attn_chunk).
 //
 // A tile's "columns" are (row, head of the group) pairs of one KV head: S^T =
 // K Q^T gives each lane one column and four tokens of each 16-token tile, and
@@ -253,10 +254,10 @@ __device__ __forceinline__ float join_parts(const CacheAttnArgs& a, int parts, i
 // lengths end together, and only the units that a cut goes through leave
 // partial outputs, two a workgroup at most.
 // The cache is read once, at one pass's worth of MFMA and conversions beside
-// it: the memory bounds it. 63 sequences of up to 16384 tokens (532542 in all),
-// 32/8 heads of 128, one row each: 564 MB in 119 us, 4.7 TB/s. (Cut into
-// equal parts of each sequence instead: 137 us at the best number of parts; in
-// twice as many shares as the chip holds: 132.)
+// it: the memory bounds it. 63 sequences of up to 16384 tokens (517438 in all),
+// 32/8 heads of 128, one row each: 564 MB in 121 us, 4.7 TB/s. (When it took
+// 119, cut into equal parts of each sequence instead: 137 us at the best number
+// of parts; in twice as many shares as the chip holds: 132.)
 constexpr int STEP = 4 * TOKENS;
 
 struct Units {
@@ -597,19 +598,20 @@ __global__ __launch_bounds__(64 * W, D == 64 && W == 4 ? 3 : 2) void cache_attn(
 //
 // 128 columns a workgroup, 32 a wave, over tiles of 64 tokens. Each thread
 // loads 16 (D = 64: 8) bytes of K's and V's codes two tiles ahead; V goes into
-// LDS as bf16, K as the codes, which every wave converts for itself: as bf16,
-// K would double what the waves read from LDS, which is then what bounds the
-// kernel, while the conversion (one instruction for two codes) runs beside the
-// MFMAs of the logits. Chunks of 2048 rows behind 8190 tokens, 32/8 heads of 128
-// (425 GFLOP): 445 us, 0.96 PFLOP/s; the chip's clock falls to 1.9 GHz under
-// it, with the MFMA pipe busy 44% of the time.
+// LDS as 16-bit values, K as the codes, which every wave converts for itself
+// (one instruction for two codes, beside the MFMAs of the logits): 16-bit keys
+// would take a wave's reads of a tile from 20 KB to 32 and the workgroup's
+// writes as well, where LDS is active 39% of the time now; which of the two is
+// faster was not measured. Chunks of 2048 rows behind 8190 tokens, 32/8 heads of
+// 128 (425 GFLOP): 466 us, 0.91 PFLOP/s; the chip's clock falls to 1.9 GHz
+// under it, with the MFMA pipe busy 47% of the time.
 //
 // For a bf16 output the weights are fp16 (2^-11 of each) and V goes through the
 // fp16 MFMA, while its scales are within HALF_LEAST .. HALF_MOST, where codes times
 // scale are exact normal fp16 values as well; from the first tile with a block
 // that fp16 does not hold on, a second loop, entered once, takes two bf16 parts.
-// Two parts everywhere took the chunks above from 427 us to 565, fp16 from 448 to
-// 460 (another box).
+// Two parts everywhere took the chunks above from 427 us to 565, fp16 from 448
+// to 460 (another box).
 constexpr int CCOLS = 128;
 // V's scale bytes whose values, 0.5 to 6 times the scale, are normal fp16
 // numbers: 2^-13 to 2^13.
@@ -975,12 +977,20 @@ __global__ __launch_bounds__(256) void cache_attn_join(CacheAttnArgs a, int wgs)
 }  // namespace
 
 // Whether a call runs the chunk kernel: above 64 columns, over which the other
-// kernel would read a tile's keys more than four times, and with keys to split
-// or tiles that fill the chip. Behind 20000 tokens, 32/8 heads of 128, chunk
-// kernel and the other: 12 rows (48 columns) 50 and 62 us, 24 rows 78 and 95,
-// 64 rows 55 and 80 (8 sequences: 139 and 256); 448 rows of 16 heads over 1500
-// states, 6 sequences: head dim 64 36 and 32, fp16 48 and 35, head dim 128 52
-// and 52; 100 rows of them 28 and 22.
+// kernel would read and convert a tile's keys more than four times, and with
+// keys to split or tiles that fill the chip. The other kernel and the chunk
+// kernel, us, behind 20000 tokens, 32/8 heads of 128 (4 columns a row):
+//              1 sequence   2           4            8
+//   12 rows    26  30       38   37     57   58      102  104
+//   16 rows    27  31       40   40     67   60      130  105
+//   17 rows    35  32       51   40     82   60      155  107
+//   64 rows    65  51       113  66     205  114     425  206
+// 16 heads of 64 (a column a row), 8 sequences: 48 rows 114 and 126 (fp16 120 and
+// 178), 64 rows 146 and 127 (fp16 151 and 178), 66 rows 177 and 128 (183 and
+// 179). Of 49 to 64 columns the chunk kernel would be the faster one for bf16
+// and the slower one for fp16, and a shape does not say which it is. Over 1500
+// states, 6 sequences, 16 heads: 448 rows of 64 28 and 32 (fp16 30 and 45), of
+// 128 45 and 45 (47 and 64); 100 rows of 64 20 and 21.
 static bool in_chunks(int batch, int kv_heads, int group, int max_new, int max_tokens) {
     const long long cols = (long long)max_new * group;
     return cols > 64 && (max_tokens > 2048 || (cols + CCOLS - 1) / CCOLS * kv_heads * batch >= 512);

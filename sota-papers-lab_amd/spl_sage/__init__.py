@@ -569,11 +569,11 @@ class SageAttention:
     # A pool or a page table of another layout than the call's is long enough as
     # often as not, and its rows are elsewhere.
     def _fits(self, cache, index, shape) -> None:
-        if cache._head_dim not in (None, self._head_dim):
+        if cache._head_dim != self._head_dim and cache._head_dim is not None:
             raise SageError(1, f"the cache is made for head dim {cache._head_dim}, the context for {self._head_dim}")
-        if cache.shape._layout != shape._layout:
+        if cache.shape is not shape and cache.shape._layout != shape._layout:
             raise _layouts_differ("the workspace and the cache", shape._layout, cache.shape._layout)
-        if index._cols not in (None, shape.max_pages) and shape.batch > 1:
+        if index._cols != shape.max_pages and index._cols is not None and shape.batch > 1:
             raise SageError(1, f"the page table has {index._cols} columns, the shape {shape.max_pages}")
 
     def _out_of_reach(self, device: int) -> SageError:
