@@ -59,9 +59,10 @@ def _bytes(t, what: str) -> tuple:
 @dataclass(frozen=True)
 class PagedCache:
     """The pool: uint8 device tensors [pages][kv_heads][page_tokens][head_dim/2]
-    (codes) and [..][head_dim/32] (scales). Made once for its tensors; one pool
-    serves steps of any shape with its pages, page_tokens and kv_heads
-    (with_shape); another shape's rows lie elsewhere in it, and is refused."""
+    (codes) and [..][head_dim/32] (scales), of the shape's pages or more. Made
+    once for its tensors; one pool serves steps of any shape with its
+    page_tokens and kv_heads (with_shape): another's rows lie elsewhere in it,
+    and tensors of four dimensions refuse it."""
 
     shape: CacheShape
     k_codes: object
@@ -71,7 +72,7 @@ class PagedCache:
 
     @staticmethod
     def new(shape: CacheShape, head_dim: int, device="cuda") -> "PagedCache":
-        """A pool of zeros."""
+        """A pool of zeros, which torch's current stream fills."""
         import torch
 
         shape.sizes(head_dim)  # its refusals
@@ -90,7 +91,7 @@ class PagedCache:
             for t, channels in zip(pair, (2, BLOCK)):
                 if t.dim() != 4:
                     continue
-                if tuple(t.shape[:3]) != self.shape._layout:
+                if t.shape[0] < self.shape.pages or tuple(t.shape[1:3]) != self.shape._layout[1:]:
                     raise _layouts_differ("the cache's tensors and shape", tuple(t.shape[:3]), self.shape._layout)
                 if dims not in (None, t.shape[3] * channels):
                     raise SageError(1, f"the cache's tensors are of head dims {dims} and {t.shape[3] * channels}")

@@ -336,3 +336,34 @@ def test_many_sequences(torch_gpu):
         for row, pg, tok, _ in p.cells():
             p.host["k_codes"][pg, :, tok], p.host["k_scales"][pg, :, tok] = codes[row], scales[row]
         assert (p.device("k_codes") == p.host["k_codes"]).all() and (p.device("k_scales") == p.host["k_scales"]).all()
+
+
+def test_rotary_of_the_most_rows(torch_gpu):
+    """2^26 - 4 rows, the last count whose launch is allowed, over themselves: every 2^20th row and the ends turn, and the
+    rest is what was there (zeros); one row more is refused."""
+    import spl_sage as S
+    from spl_sage import rotary as R
+
+    torch, d, rows = torch_gpu, 64, 2 ** 26 - 4
+    rng = np.random.default_rng(0)
+    at = sorted({0, 1, 2, 3, *range(5, rows, 2 ** 20), rows - 4, rows - 3, rows - 2, rows - 1})
+    x = torch.zeros(1, rows + 1, 1, d, dtype=torch.bfloat16, device="cuda")
+    some, sv = draw16(torch, rng, (len(at), 1, d), "bf16")
+    index = torch.tensor(at, device="cuda")
+    x[0, index] = some
+    x[0, rows] = 7.0
+    table = R.RotaryTable.new(d, 100)
+    pos = torch.zeros(rows + 1, dtype=torch.int32, device="cuda")
+    want_pos = rng.integers(0, 100, len(at))
+    pos[index] = ints(torch, want_pos)
+    sa = S.SageAttention(torch.cuda.current_stream(), d)
+    r = R.Rotary(table.upload(), d, R.RotaryLayout.Half, pos)
+    with pytest.raises(S.SageError, match="exceed the launch grid"):
+        sa.rotary(S.Shape(1, 1, rows + 1), r, S.Tensor(x), S.TensorMut(x))
+    sa.rotary(S.Shape(1, 1, rows), r, S.Tensor(x), S.TensorMut(x))
+    want = O.rotate(sv, table.cos_sin, want_pos, d, False)
+    terms = O.rotate(np.abs(sv), np.abs(table.cos_sin) * [1, -1], want_pos, d, False)  # |a c| + |b s|
+    got = x[0, index].double().cpu().numpy()
+    assert (np.abs(got - want) <= O.HALF_STEP["bf16"] * (np.abs(want) + 2.0 ** -20) + np.abs(terms).max() * 2.0 ** -22).all()
+    x[0, index] = 0
+    assert (x[0, rows] == 7.0).all() and not x[0, :rows].any()
