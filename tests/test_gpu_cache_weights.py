@@ -76,3 +76,20 @@ def test_many_small_weights(torch_gpu, d, new, most, kind, first):
     q = torch_gpu.zeros(1, new, 1, d, dtype=torch_gpu.bfloat16, device="cuda")
     q[..., 0] = 3.8125  # a logit of 15.25, e^-15.25 = 2^-22.0
     R.check(torch_gpu, p, q, q.double().cpu().numpy(), "bf16", scale=1.0)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("at", [900, 960, 1000, 1023, 1024, 1087, 1100, 1152, 2048, 2899])
+@pytest.mark.parametrize("most,kind", [(40, "splits"), (9000, "chunk"), (4, "shares")])
+def test_a_value_past_fp16_around_a_window_of_pages(torch_gpu, d, at, most, kind):
+    """The tokens' pages are looked up 64 at a time, ahead of the tile at work: the loop that goes on from a tile with
+    such a value may have to go back to pages before them."""
+    rng = np.random.default_rng(at)
+    new = min(most, 40)
+    p = Pool(torch_gpu, d, [0, new], [2900], 1, 16, 4, seed=at, max_new=most, extra_cols=60)
+    assert plan(p.shape, d).kind == kind
+    R.spread(p, rng)
+    p.host["v_scales"][p.table[0, at // 16], 0, at % 16, 1] = 60
+    p.upload()
+    q, qv = R.queries(torch_gpu, rng, p, "bf16")
+    R.check(torch_gpu, p, q, qv, "bf16")
