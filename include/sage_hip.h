@@ -448,6 +448,51 @@ typedef struct sage_rotary {
 sage_status sage_rotary_apply(const sage_attention* s, const sage_shape* shape, const sage_rotary* rotary,
                               const sage_tensor* x, const sage_tensor_mut* out, int32_t transpose);
 
+/* Rotary positions with several axes (time, height, width of an image's or a
+ * video's tokens): every row has a position on each of 1 to SAGE_ROTARY_AXES
+ * axes, and each pair turns by the one of its own axis.
+ *   sections   pairs of each axis (1 or more; what is behind axes is not read);
+ *              rot is twice their sum, an even number up to the head dim
+ *   dealt      0: the axes' pairs are runs, one behind the other; else the
+ *              pairs are dealt to the axes in turn, passing over those that
+ *              have all of theirs
+ *   layout     HALF pairs channels (i, i + rot / 2), PAIRS (2 i, 2 i + 1), AXIS_HALF
+ *              (dealt == 0) the halves within the channels of each axis:
+ *              with n pairs before the axis's own, (2 n + j, 2 n + j + section) */
+#define SAGE_ROTARY_AXES 4
+typedef enum sage_rotary_axes_layout {
+    SAGE_ROTARY_AXES_HALF = 0,
+    SAGE_ROTARY_AXES_PAIRS = 1,
+    SAGE_ROTARY_AXES_AXIS_HALF = 2
+} sage_rotary_axes_layout;
+
+/* Host only: sage_rotary_table for several axes, [positions][rot / 2][2] floats, with the angle
+ * position * w_i in each pair's column. per_axis == 0: pair i has the w_i of sage_rotary_table over
+ * the whole of rot; else the j-th of an axis's n pairs has the w_j of a table of
+ * rot = 2 n (NTK scaling needs n > 1). */
+sage_status sage_rotary_axes_table(const uint64_t* sections, uint64_t axes, int32_t dealt, int32_t per_axis,
+                                   uint64_t positions, double base, const sage_rotary_scaling* scaling, float* out,
+                                   uint64_t out_len);
+
+/* table: as sage_rotary's, for the greatest position of any axis. positions: device
+ * int32, axis a's of row r at a * positions_stride + r (positions_stride >= rows). The
+ * channels of an axis whose position the table does not hold become NaN. */
+typedef struct sage_rotary_axes {
+    const float* table;
+    uint64_t table_len;
+    uint64_t sections[SAGE_ROTARY_AXES];
+    uint64_t axes;
+    int32_t layout; /* sage_rotary_axes_layout */
+    int32_t dealt;
+    const int32_t* positions;
+    uint64_t positions_len;
+    uint64_t positions_stride;
+} sage_rotary_axes;
+
+/* sage_rotary_apply with several axes: its roundings, views, refusals and transpose. */
+sage_status sage_rotary_axes_apply(const sage_attention* s, const sage_shape* shape, const sage_rotary_axes* rotary,
+                                   const sage_tensor* x, const sage_tensor_mut* out, int32_t transpose);
+
 /* A batch of sequences over a pool of pages.
  *   batch        sequences (at most 65535)
  *   rows         rows of the packed q, k, v and out (below 2^26): the new tokens
@@ -521,6 +566,11 @@ sage_status sage_cache_append(const sage_attention* s, const sage_cache_shape* s
                               const sage_cache_index* index, const sage_tensor* k, const sage_tensor* v,
                               const sage_rotary* rotary, const sage_tensor* q, const sage_tensor_mut* q_out);
 
+/* sage_cache_append with rotary positions of several axes (rotary is not NULL). */
+sage_status sage_cache_append_axes(const sage_attention* s, const sage_cache_shape* shape, const sage_cache* cache,
+                                   const sage_cache_index* index, const sage_tensor* k, const sage_tensor* v,
+                                   const sage_rotary_axes* rotary, const sage_tensor* q, const sage_tensor_mut* q_out);
+
 /* The rows' keys and values back from their slots as 16-bit values (rounded
  * once; fp16 overflows to infinity), zeros where a slot holds nothing: starts
  * and lengths that cover whole sequences give the K and V that sage_forward
@@ -566,6 +616,138 @@ typedef struct sage_cache_options {
 sage_status sage_cache_attend(const sage_attention* s, const sage_cache_workspace* ws, const sage_cache* cache,
                               const sage_cache_index* index, const sage_tensor* q, const sage_tensor_mut* out,
                               const sage_cache_options* opts);
+
+/* ---- A step's index from the requests' lengths ----
+ *
+ * news [batch]: the rows that each request has in this step, below 0 for a request
+ * that has ended; past [batch]: its tokens that are cached already (below 0: 0). */
+typedef struct sage_cache_requests {
+    const int32_t* news;
+    uint64_t news_len;
+    const int32_t* past;
+    uint64_t past_len;
+} sage_cache_requests;
+
+/* The free pages: a ring of page ids, of which state [0] is the place of the
+ * first and state [1] their number. A ring of as many places as the pool has pages
+ * holds whatever is given back. */
+typedef struct sage_cache_free {
+    int32_t* pages;
+    uint64_t pages_len;
+    const int32_t* state;
+    uint64_t state_len; /* 2 or more */
+} sage_cache_free;
+
+/* What a step's calls take, device memory. starts, lengths and page_table are
+ * sage_cache_index's. positions, slots and sequences (each may be NULL, 16-byte
+ * aligned) hold an entry a row of the shape: the row's position in its sequence
+ * (0), page * page_tokens + its token in the page (-1) and its sequence (-1), in
+ * brackets that of a row behind the last sequence. state [4]: the ring's first
+ * place and number after the step, the pages that were missing, the rows past
+ * the shape's. scratch: int32 [2 * batch]. */
+typedef struct sage_cache_step {
+    int32_t* starts;
+    uint64_t starts_len;
+    int32_t* lengths;
+    uint64_t lengths_len;
+    int32_t* page_table;
+    uint64_t page_table_len;
+    int32_t* positions;
+    uint64_t positions_len;
+    int64_t* slots;
+    uint64_t slots_len;
+    int32_t* sequences;
+    uint64_t sequences_len;
+    int32_t* state;
+    uint64_t state_len;
+    int32_t* scratch;
+    uint64_t scratch_len;
+} sage_cache_step;
+
+/* Builds a step's index on the device: the requests' rows one behind the other
+ * (starts), their lengths with them, and pages from the front of the ring, in the
+ * requests' and then the columns' order, in the new columns of the page table (the
+ * others stay). An ended request has no row and length 0; its pages go behind the
+ * ring's last, for later steps, as far as the ring has room (the columns stay, and are
+ * nobody's). The step is void where the ring has too few pages or a request's
+ * tokens pass the page table (state [2], the pages missing), or the rows pass
+ * the shape's (state [3]): no request has a row then and lengths are past's, but what
+ * ended is given back. past may be lengths and free's state the step's, so that a captured step
+ * serves one after the other; otherwise the inputs stay as they are but for
+ * the ring's places behind its last. The shape's max_new is not read. */
+sage_status sage_cache_tables(const sage_attention* s, const sage_cache_shape* shape,
+                              const sage_cache_requests* requests, const sage_cache_free* free,
+                              const sage_cache_step* step);
+
+/* ---- Attention over picked pages ----
+ *
+ * For contexts of which a row needs only a part: bounds of each page's keys, a
+ * pick of pages by them, and attention over those. Page tables of at most
+ * SAGE_PICK_PAGES columns, picks of at most SAGE_PICK_TOP. */
+#define SAGE_PICK_PAGES 32768
+#define SAGE_PICK_TOP 256
+
+/* Bounds of a pool's keys, in the caller's device memory (16-byte aligned):
+ *   codes   [pages][kv_heads][2][D]: with E the greatest scale byte (of those
+ *           that are not NaN) of the page's keys, the least whole number that no
+ *           key of the channel times 16 / 2^(E - 127) is above, and the greatest
+ *           that none is below, within +-96; a channel in a block that is
+ *           NaN: 127 and -127
+ *   scales  [pages][kv_heads]: E */
+typedef struct sage_cache_bounds {
+    int8_t* codes;
+    uint8_t* scales;
+    uint64_t codes_len;
+    uint64_t scales_len;
+} sage_cache_bounds;
+
+/* The bounds of the pages that hold a row of the step, over their slots below the
+ * sequence's length: what a step calls behind sage_cache_append. The pages of rows
+ * past max_new of a sequence stay as they are. The values are not read. Two
+ * sequences that share a page that the step writes race. */
+sage_status sage_cache_bounds_update(const sage_attention* s, const sage_cache_shape* shape, const sage_cache* cache,
+                                     const sage_cache_index* index, const sage_cache_bounds* bounds);
+
+/* What sage_cache_pick and sage_cache_attend_picked keep between their kernels,
+ * for picks of `top` pages. One call at a time may use it. */
+typedef struct sage_pick_workspace sage_pick_workspace;
+sage_status sage_pick_workspace_new(const sage_attention* s, const sage_cache_shape* shape, uint64_t top,
+                                    sage_pick_workspace** out);
+void sage_pick_workspace_destroy(sage_pick_workspace* ws);
+uint64_t sage_pick_workspace_bytes(const sage_pick_workspace* ws);
+
+/* first, last: pages that are always picked, of those that a row sees (last >= 1:
+ * under a causal mask the row's own page holds later keys too; first + last <= top). */
+typedef struct sage_pick_options {
+    uint64_t first;
+    uint64_t last;
+    int32_t causal;
+} sage_pick_options;
+
+/* picked [rows][kv_heads][top], device int32: for each row and KV head the columns
+ * of the page table that the row's queries of that head's group attend to,
+ * ascending, -1 behind them: every page that the row sees (a slot of) where
+ * those are top or fewer, else the first and the last ones and, of the others,
+ * those of the greatest scores, the lower column first where scores are equal.
+ * With u the group's queries times the greatest power of two (2^-126 to 2^126) that keeps
+ * them within 127, rounded to whole numbers (all 0 where one is not finite), a
+ * page's score is 2^E times the greatest, over the heads, of the sum of u_c hi_c
+ * where u_c > 0 and u_c lo_c elsewhere: what the group's greatest logit (of a
+ * positive softmax scale) could be there. It is computed in whole numbers, exactly
+ * (of E past 228 as of 228). A page that the pool does not have comes behind all
+ * others. Rows of no sequence or past max_new keep what they have. q as in
+ * sage_cache_attend. */
+sage_status sage_cache_pick(const sage_attention* s, const sage_pick_workspace* ws, const sage_cache_bounds* bounds,
+                            const sage_cache_index* index, const sage_tensor* q, int32_t* picked, uint64_t picked_len,
+                            const sage_pick_options* opts);
+
+/* sage_cache_attend over the slots of each row's picked columns alone, with its
+ * masks, numerics and aliasing. picked [rows][kv_heads][top] may be a pick or the
+ * caller's own, in any order; a column given twice counts once, one that the row does
+ * not see, or outside the page table, not at all. */
+sage_status sage_cache_attend_picked(const sage_attention* s, const sage_pick_workspace* ws, const sage_cache* cache,
+                                     const sage_cache_index* index, const int32_t* picked, uint64_t picked_len,
+                                     const sage_tensor* q, const sage_tensor_mut* out, const sage_cache_options* opts);
 
 /* Byte position of key k (0..63) of a 64-key block inside each channel row
  * of the v8 layout (the CDNA4 counterpart of sg_vpos, sage_common.cu:151-155):

@@ -52,8 +52,11 @@ UNITS = [
     ("sage_noalloc.hip", "sage_noalloc.hip.o", []),
     ("sage_cache.hip", "sage_cache.hip.o", ["-ffp-contract=off"]),
     ("sage_cache_attn.hip", "sage_cache_attn.hip.o", []),
+    ("sage_cache_step.hip", "sage_cache_step.hip.o", []),
+    ("sage_cache_pick.hip", "sage_cache_pick.hip.o", []),
     ("sage_api.cpp", "sage_api.cpp.o", []),
     ("sage_cache_api.cpp", "sage_cache_api.cpp.o", []),
+    ("sage_cache_pick_api.cpp", "sage_cache_pick_api.cpp.o", []),
 ]
 
 

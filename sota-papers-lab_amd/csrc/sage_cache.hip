@@ -5,6 +5,7 @@
 // sage_cache_append's keys are those of sage_rotary_apply bit for bit.
 #include <algorithm>
 
+#include "../../include/sage_hip.h"
 #include "sage_cache.hpp"
 
 namespace sage {
@@ -34,24 +35,38 @@ __device__ __forceinline__ float load1(const uint16_t* p, bool f16) {
 }
 
 // The turns of a lane's eight channels c0 .. c0 + 7.
-// VEC: rot is a multiple of 16, so that the lane's pairs are whole vectors of
-// the table and its partners (HALF) those that one lane of the head holds. Other
-// rots go channel by channel and load the partners one by one (5003 rows of
+// VEC: the lane's pairs are whole vectors of the table and its partners (halves)
+// those that one lane of the head holds: rot is a multiple of 16, or each axis's
+// channels are where the halves are an axis's. Other rots go channel by channel
+// and load the partners one by one (5003 rows of
 // 96 heads of 64, HALF: rot 64 26 us, 62 57 us; pairs of neighbours: 26 us both).
-template <bool VEC>
+// AXES: every pair turns by its own axis's position, so that its table entry is
+// loaded by itself.
+template <bool VEC, bool AXES>
 struct Turns {
     f2 cs[8];   // channel c0 + k's pair
-    int from;   // HALF: the lane of the wave that holds the lane's partners
+    int from;   // halves: the lane of the wave that holds the lane's partners
+    int part[VEC ? 1 : 8];  // halves: how far channel c0 + k's partner is (VEC: all of them)
     bool on;    // whether any of its channels turns
 
-    // At position pos; NaN where the table has no such position.
-    __device__ __forceinline__ void load(const RotaryDev& r, int pos, int c0) {
-        const bool in = (unsigned)pos < (unsigned)r.table_rows;
-        const f2* row = reinterpret_cast<const f2*>(r.table) + (long long)(in ? pos : 0) * (r.rot >> 1);
-        const int half = r.rot >> 1;
+    // Of row `row` at position pos (one axis); NaN where the table has no such position.
+    __device__ __forceinline__ void load(const RotaryDev& r, int pos, long long row, int c0) {
         on = c0 < r.rot;
-        from = (threadIdx.x & 63) + (c0 < half ? half : -half) / 8;
-        if (!on) return;
+        from = threadIdx.x & 63;
+#pragma unroll
+        for (int k = 0; k < (VEC ? 1 : 8); k++) part[k] = c0 + k < r.rot >> 1 ? r.rot >> 1 : -(r.rot >> 1);
+        if (AXES) {
+            load_axes(r, row, c0);
+        } else {
+            const bool in = (unsigned)pos < (unsigned)r.table_rows;
+            const f2* at = reinterpret_cast<const f2*>(r.table) + (long long)(in ? pos : 0) * (r.rot >> 1);
+            if (on) load_one(r, at, in, c0);
+        }
+        from += part[0] / 8;
+    }
+
+    __device__ __forceinline__ void load_one(const RotaryDev& r, const f2* row, bool in, int c0) {
+        const int half = r.rot >> 1;
         if (VEC) {
             const int i = r.layout ? c0 >> 1 : c0 < half ? c0 : c0 - half;
             const float4* v = reinterpret_cast<const float4*>(row + i);
@@ -81,13 +96,57 @@ struct Turns {
         }
     }
 
+    __device__ __forceinline__ void load_axes(const RotaryDev& r, long long row, int c0) {
+        int pos[4];
+#pragma unroll
+        for (int a = 0; a < 4; a++) pos[a] = a < r.axes ? r.positions[a * r.positions_stride + row] : 0;
+        const int half = r.rot >> 1;
+        // Channel c's pair i and axis a; where the halves are an axis's, its partner too.
+        const f2* at[8];
+        bool in[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int c = c0 + k < r.rot ? c0 + k : 0;
+            int i, a;
+            if (r.layout == SAGE_ROTARY_AXES_AXIS_HALF) {
+                int before = 0, n = r.sections[0];  // pairs of the axes before, pairs of the axis
+                a = 0;
+#pragma unroll
+                for (int x = 1; x < 4; x++)
+                    if (x < r.axes && c >= 2 * (before + n)) before += n, n = r.sections[x], a = x;
+                const bool low = c - 2 * before < n;
+                i = c - before - (low ? 0 : n);
+                if (!VEC || k == 0) part[VEC ? 0 : k] = low ? n : -n;
+            } else {
+                i = r.layout == SAGE_ROTARY_AXES_PAIRS ? c >> 1 : c < half ? c : c - half;
+                const uint32_t w = i < 32 ? (i < 16 ? r.axis_of[0] : r.axis_of[1]) : (i < 48 ? r.axis_of[2] : r.axis_of[3]);
+                a = w >> (i % 16 * 2) & 3;
+            }
+            const int p = a < 2 ? (a ? pos[1] : pos[0]) : (a == 2 ? pos[2] : pos[3]);
+            in[k] = (unsigned)p < (unsigned)r.table_rows;
+            at[k] = reinterpret_cast<const f2*>(r.table) + (long long)(in[k] ? p : 0) * half + i;
+        }
+        if (!on) return;
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (k % 2 == 0 || r.layout != SAGE_ROTARY_AXES_PAIRS) cs[k] = *at[k];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            if (k % 2 && r.layout == SAGE_ROTARY_AXES_PAIRS) cs[k] = cs[k - 1];
+            else {
+                if (!in[k]) cs[k] = f2{__builtin_nanf(""), __builtin_nanf("")};
+                if (r.transpose) cs[k].y = -cs[k].y;
+            }
+        }
+    }
+
     // The lane's channels raw of the row at p, turned, in x. All lanes of the
     // head call together: they exchange their channels.
     __device__ __forceinline__ void apply(const RotaryDev& r, const uint16_t* p, int c0, bool f16, uint4 raw,
                                           float (&x)[8]) const {
         unpack8(raw, x, f16);
         if (!on) return;
-        if (r.layout) {
+        if (r.layout == SAGE_ROTARY_PAIRS) {
 #pragma unroll
             for (int k = 0; k < 8; k += 2)
                 if (VEC || c0 + k < r.rot) {
@@ -97,7 +156,6 @@ struct Turns {
                 }
             return;
         }
-        const int half = r.rot >> 1;
         float z[8];
         if (VEC) {
             unpack8(make_uint4(__shfl(raw.x, from), __shfl(raw.y, from), __shfl(raw.z, from), __shfl(raw.w, from)), z,
@@ -105,16 +163,24 @@ struct Turns {
         } else {
 #pragma unroll
             for (int k = 0; k < 8; k++)
-                if (c0 + k < r.rot) z[k] = load1(p + (c0 + k < half ? c0 + k + half : c0 + k - half), f16);
+                if (c0 + k < r.rot) z[k] = load1(p + (c0 + k + part[VEC ? 0 : k]), f16);
         }
 #pragma unroll
         for (int k = 0; k < 8; k++)
             if (VEC || c0 + k < r.rot) {
                 const float t = z[k] * cs[k].y;
-                x[k] = (VEC ? c0 : c0 + k) < half ? x[k] * cs[k].x - t : x[k] * cs[k].x + t;
+                x[k] = part[VEC ? 0 : k] > 0 ? x[k] * cs[k].x - t : x[k] * cs[k].x + t;
             }
     }
 };
+
+// Whether Turns's VEC serves the channels.
+bool in_vectors(const RotaryDev& r) {
+    if (r.axes == 0 || r.layout != SAGE_ROTARY_AXES_AXIS_HALF) return r.rot % 16 == 0;  // (no rotation: 0)
+    bool vec = true;
+    for (int a = 0; a < r.axes; a++) vec = vec && r.sections[a] % 8 == 0;
+    return vec;
+}
 
 // A workgroup's run of `parts` parts, gridDim.y of which there are (share_heads).
 __device__ __forceinline__ int run_of(int parts) { return (parts + gridDim.y - 1) / gridDim.y; }
@@ -128,7 +194,7 @@ __device__ __forceinline__ int run_of(int parts) { return (parts + gridDim.y - 1
 // so the turns of a lane's channels are loaded once and serve every head.
 // A head's loads come before its stores, all in one wave: out may be x.
 // Two heads' loads are in flight together.
-template <int D, bool VEC>
+template <int D, bool VEC, bool AXES>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
     constexpr int CH = D / 8, SLOTS = 64 / CH, AHEAD = VEC ? 2 : 1;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -136,8 +202,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
     if (row >= (long long)a.batch * a.tokens) return;
     const int b = (int)(row / a.tokens), t = (int)(row - (long long)b * a.tokens);
     const int c0 = (lane % CH) * 8;
-    Turns<VEC> turns;
-    turns.load(a.r, a.r.positions ? a.r.positions[row] : t, c0);
+    Turns<VEC, AXES> turns;
+    turns.load(a.r, !AXES && a.r.positions ? a.r.positions[row] : t, row, c0);
     const uint16_t* px = a.x.p + b * a.x.sb + t * a.x.st;
     uint16_t* po = a.out.p + b * a.out.sb + t * a.out.st;
     const int run = run_of((a.heads + SLOTS - 1) / SLOTS) * SLOTS, end = min(a.heads, (int)(blockIdx.y + 1) * run);
@@ -229,7 +295,7 @@ __device__ __forceinline__ Place place_of(CacheDev c, int row, int* starts) {
 // consecutive and of one head at a time: their code rows are consecutive
 // too, so the stores fill whole lines. Two parts' loads are ahead of the two at
 // work, the first two ahead of the lookups.
-template <int D, bool VEC>
+template <int D, bool VEC, bool AXES>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     constexpr int CH = D / 8, ROWS = 256 / CH, AHEAD = VEC ? 2 : 1;
     __shared__ int starts[STARTS];
@@ -250,9 +316,9 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     load(blockIdx.y * run);
     const Place place = place_of(a.c, row, starts);
     if (place.b < 0) return;
-    Turns<VEC> turns;
+    Turns<VEC, AXES> turns;
     turns.on = false;
-    if (a.r.table) turns.load(a.r, a.r.positions ? a.r.positions[row] : place.slot, c0);
+    if (AXES || a.r.table) turns.load(a.r, !AXES && a.r.positions ? a.r.positions[row] : place.slot, row, c0);
     for (int first = blockIdx.y * run; first < end; first += AHEAD) {
         uint4 raw[AHEAD];
 #pragma unroll
@@ -333,11 +399,16 @@ hipError_t launch_rotary(int head_dim, const RotaryArgs& a, hipStream_t s) {
     const long long blocks = ((long long)a.batch * a.tokens + 3) / 4;
     const int slots = 64 / (head_dim / 8);
     const dim3 grid((unsigned)blocks, share_heads(blocks, std::min(65535, (a.heads + slots - 1) / slots), 1024));
-    const bool vec = a.r.rot % 16 == 0;
-    if (head_dim == 64)
-        hipLaunchKernelGGL((vec ? rotary_kernel<64, true> : rotary_kernel<64, false>), grid, dim3(256), 0, s, a);
+    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a); };
+    const bool vec = in_vectors(a.r);
+    if (a.r.axes && head_dim == 64)
+        go(vec ? rotary_kernel<64, true, true> : rotary_kernel<64, false, true>);
+    else if (a.r.axes)
+        go(vec ? rotary_kernel<128, true, true> : rotary_kernel<128, false, true>);
+    else if (head_dim == 64)
+        go(vec ? rotary_kernel<64, true, false> : rotary_kernel<64, false, false>);
     else
-        hipLaunchKernelGGL((vec ? rotary_kernel<128, true> : rotary_kernel<128, false>), grid, dim3(256), 0, s, a);
+        go(vec ? rotary_kernel<128, true, false> : rotary_kernel<128, false, false>);
     return hipGetLastError();
 }
 
@@ -345,11 +416,16 @@ hipError_t launch_cache_append(int head_dim, const AppendArgs& a, hipStream_t s)
     const int rows = 256 / (head_dim / 8);
     const long long blocks = ((long long)a.c.rows + rows - 1) / rows;
     const dim3 grid((unsigned)blocks, share_heads(blocks, 2 * a.c.kv_heads + (a.q.p ? a.heads : 0), 1536));
-    const bool vec = a.r.rot % 16 == 0;  // (no rotation: 0)
-    if (head_dim == 64)
-        hipLaunchKernelGGL((vec ? append_kernel<64, true> : append_kernel<64, false>), grid, dim3(256), 0, s, a);
+    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a); };
+    const bool vec = in_vectors(a.r);
+    if (a.r.axes && head_dim == 64)
+        go(vec ? append_kernel<64, true, true> : append_kernel<64, false, true>);
+    else if (a.r.axes)
+        go(vec ? append_kernel<128, true, true> : append_kernel<128, false, true>);
+    else if (head_dim == 64)
+        go(vec ? append_kernel<64, true, false> : append_kernel<64, false, false>);
     else
-        hipLaunchKernelGGL((vec ? append_kernel<128, true> : append_kernel<128, false>), grid, dim3(256), 0, s, a);
+        go(vec ? append_kernel<128, true, false> : append_kernel<128, false, false>);
     return hipGetLastError();
 }
 

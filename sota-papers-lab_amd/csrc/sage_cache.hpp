@@ -25,6 +25,12 @@ struct RotaryDev {
     const float* table;  // [table_rows][rot / 2][2]
     const int* positions;
     int table_rows, rot, layout, transpose;
+    // Several axes (0: one): the position of axis a and row r at a * positions_stride + r,
+    // the pairs of each axis, and the axis of each pair, two bits each.
+    int axes;
+    long long positions_stride;
+    int sections[4];
+    uint32_t axis_of[4];
 };
 
 // Device view of sage_cache, sage_cache_index and sage_cache_shape.
@@ -63,9 +69,50 @@ struct CacheAttnArgs {
     float qk_mul;     // |softmax scale| * log2(e), over 0
     uint32_t q_sign;  // 0x80008000 under a negative scale: the queries' signs
     int heads, group, max_new, causal, q_f16, out_f16;
-    int splits;  // chunks: workgroups that a sequence's keys are split over, at most
+    int splits;  // chunks: workgroups that a sequence's keys are split over, at most; picked pages: that a unit's are
     int whole;   // few rows: a workgroup a unit
+    const int* picked;  // [rows][kv_heads][top], or null
+    int top;
 };
+
+// A step's index from the requests' lengths (sage_cache_tables).
+struct StepArgs {
+    const int *news, *past, *state_in;
+    int* ring;
+    int *starts, *lengths, *page_table, *state, *scratch;
+    int *positions, *sequences;  // null: not asked for
+    long long* slots;
+    int batch, rows, page_shift, max_pages, pages, cap;
+};
+hipError_t launch_cache_step(const StepArgs& a, hipStream_t s);
+
+// Device view of sage_cache_bounds, and its update for the pages of a step.
+struct BoundsDev {
+    int8_t* codes;    // [pages][kv_heads][2][D]
+    uint8_t* scales;  // [pages][kv_heads]
+};
+struct BoundsArgs {
+    CacheDev c;
+    BoundsDev bounds;
+    int max_new;
+};
+hipError_t launch_cache_bounds(int head_dim, const BoundsArgs& a, hipStream_t s);
+
+// One pick. keys: an ordered score for each of `window` packed rows from row0 on, KV head
+// and column (key_cols of them).
+struct PickArgs {
+    RowView q;
+    CacheDev c;
+    BoundsDev bounds;
+    uint32_t* keys;
+    int* picked;  // [rows][kv_heads][top]
+    int heads, group, max_new, causal, q_f16;
+    int top, first, last;
+    int row0, window, key_cols;
+};
+// Rows of a call that the scores are kept for at a time.
+int pick_window(int rows, int kv_heads, int max_pages);
+hipError_t launch_cache_pick(int head_dim, const PickArgs& a, hipStream_t s);
 
 hipError_t launch_rotary(int head_dim, const RotaryArgs& a, hipStream_t s);
 hipError_t launch_cache_append(int head_dim, const AppendArgs& a, hipStream_t s);
@@ -82,6 +129,17 @@ struct CachePlan {
 };
 CachePlan cache_plan(int head_dim, int batch, int rows, int heads, int kv_heads, int max_new, int max_tokens);
 hipError_t launch_cache_attend(int head_dim, const CacheAttnArgs& a, const CachePlan& plan, hipStream_t s);
+
+// How a call over picked pages runs: workgroups that a unit's pages are split over, the
+// partial outputs that the workspace holds, and the bytes of LDS of its lists.
+struct PickedPlan {
+    int splits;
+    uint64_t part_rows;
+    unsigned lds;
+};
+PickedPlan picked_plan(int head_dim, int batch, int rows, int heads, int kv_heads, int max_new, int max_pages,
+                       int page_tokens, int top);
+hipError_t launch_cache_attend_picked(int head_dim, const CacheAttnArgs& a, const PickedPlan& plan, hipStream_t s);
 
 // The index lookups, host and device: tests/cpp/cache_host.cpp runs them on bad
 // indexes on the CPU.

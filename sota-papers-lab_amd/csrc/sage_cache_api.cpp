@@ -6,9 +6,9 @@
 #include <cmath>
 #include <new>
 
-#include "sage_cache.hpp"
-#include "sage_internal.hpp"
+#include "sage_cache_checks.hpp"
 
+using namespace sage::checks;
 using sage::set_error;
 using sage::succeeded;
 
@@ -22,73 +22,94 @@ struct sage_cache_workspace {
 
 namespace {
 
-using u64 = unsigned long long;
-constexpr uint64_t I32 = 2147483647ull;
-// Rows below it: at most 64 threads a row in a grid's x, of which a launch takes
-// less than 2^32. The rotation's workgroups take four rows each: 2^26 - 4 at most.
-constexpr uint64_t ROWS = 1ull << 26;
+// The angles' speeds under a scaling: w_i of a table of rot channels.
+struct Speeds {
+    int kind = SAGE_ROTARY_NONE;
+    double base = 0, f = 1, original = 0, fast = 0, slow = 0, attention = 1;
 
-sage_status hip_failed(hipError_t e, const char* what) {
-    return set_error(SAGE_ERR_DEVICE, "%s: %s (%s)", what, hipGetErrorName(e), hipGetErrorString(e));
+    sage_status checked(double base_, const sage_rotary_scaling* scaling, uint64_t least_rot) {
+        base = base_;
+        kind = scaling ? scaling->kind : SAGE_ROTARY_NONE;
+        if (kind < SAGE_ROTARY_NONE || kind > SAGE_ROTARY_YARN)
+            return set_error(SAGE_ERR_INVALID, "rotary: unknown scaling %d", kind);
+        f = kind == SAGE_ROTARY_NONE ? 1.0 : scaling->factor;
+        if (!(f >= 1.0) || !std::isfinite(f))
+            return set_error(SAGE_ERR_INVALID, "rotary: scaling factor %g is not 1 or more", f);
+        attention = scaling && scaling->attention != 0.0 ? scaling->attention : 1.0;
+        if (!std::isfinite(attention)) return set_error(SAGE_ERR_INVALID, "rotary: attention factor %g", attention);
+        if (kind == SAGE_ROTARY_NTK && least_rot < 4)
+            return set_error(SAGE_ERR_INVALID, "rotary: NTK scaling needs 4 rotated channels or more");
+        if (kind == SAGE_ROTARY_YARN) {
+            original = scaling->original;
+            fast = scaling->beta_fast != 0.0 ? scaling->beta_fast : 32.0;
+            slow = scaling->beta_slow != 0.0 ? scaling->beta_slow : 1.0;
+            if (!(original > 0.0) || !std::isfinite(original) || !(slow < fast) || !std::isfinite(fast))
+                return set_error(SAGE_ERR_INVALID, "rotary: YaRN scaling of %g positions between %g and %g turns",
+                                 original, slow, fast);
+            if (scaling->attention == 0.0) attention = 0.1 * std::log(f) + 1.0;
+        }
+        return SAGE_OK;
+    }
+
+    double of(uint64_t i, uint64_t rot) const {
+        const double b = kind == SAGE_ROTARY_NTK ? base * std::pow(f, (double)rot / (double)(rot - 2)) : base;
+        double w = std::pow(b, -2.0 * (double)i / (double)rot);
+        if (kind == SAGE_ROTARY_LINEAR) w /= f;
+        if (kind == SAGE_ROTARY_YARN) {
+            // Peng et al., "YaRN: Efficient Context Window Extension of Large Language
+            // Models", 2023: pairs that turn often keep their angle, slow ones are interpolated.
+            const double turns = original * w / (2.0 * 3.14159265358979323846);
+            const double g = std::min(1.0, std::max(0.0, (turns - slow) / (fast - slow)));
+            w = g * w + (1.0 - g) * w / f;
+        }
+        return w;
+    }
+
+    // One pair's column of a table of `pairs` pairs.
+    void column(float* out, uint64_t pairs, uint64_t pair, uint64_t positions, double w) const {
+        for (uint64_t p = 0; p < positions; p++) {
+            const double a = (double)p * w;
+            out[(p * pairs + pair) * 2] = (float)(attention * std::cos(a));
+            out[(p * pairs + pair) * 2 + 1] = (float)(attention * std::sin(a));
+        }
+    }
+};
+
+sage_status table_room(uint64_t positions, uint64_t rot, uint64_t out_len) {
+    const sage_status st = in_i32(positions, "rotary positions");
+    if (st != SAGE_OK || out_len >= positions * rot) return st;
+    return set_error(SAGE_ERR_INVALID, "rotary table: buffer holds %llu elements, needs %llu", (u64)out_len,
+                     (u64)(positions * rot));
 }
 
-sage_status done(hipError_t e, const char* what) {
-    if (e != hipSuccess) return hip_failed(e, what);
-    return succeeded();
-}
-
-// The kernels run on the current device; the context's stream and the memory
-// it was made for are its own device's.
-sage_status on_device(const sage_attention* s) {
-    int dev = -1;
-    const hipError_t e = hipGetDevice(&dev);
-    if (e != hipSuccess) return hip_failed(e, "current device");
-    if (dev != s->device)
-        return set_error(SAGE_ERR_INVALID, "the context is of device %d, the current device is %d", s->device, dev);
+// The pairs of all axes together, at most `most`.
+sage_status sections_checked(const uint64_t* sections, uint64_t axes, uint64_t most, uint64_t* pairs) {
+    if (axes < 1 || axes > SAGE_ROTARY_AXES)
+        return set_error(SAGE_ERR_INVALID, "rotary: %llu axes (1 to %d are supported)", (u64)axes, SAGE_ROTARY_AXES);
+    *pairs = 0;
+    for (uint64_t a = 0; a < axes; a++) {
+        if (sections[a] < 1 || sections[a] > most)
+            return set_error(SAGE_ERR_INVALID, "rotary: axis %llu of %llu pairs (1 to %llu)", (u64)a, (u64)sections[a],
+                             (u64)most);
+        *pairs += sections[a];
+    }
+    if (*pairs > most)
+        return set_error(SAGE_ERR_INVALID, "rotary: %llu rotated channels of head dim %llu: an even number from 2 to it",
+                         (u64)(2 * *pairs), (u64)(2 * most));
     return SAGE_OK;
 }
-
-sage_status in_i32(uint64_t v, const char* what) {
-    return v <= I32 ? SAGE_OK : set_error(SAGE_ERR_INVALID, "%s = %llu does not fit in i32", what, (u64)v);
+// each(i, a, j): pair i is the j-th of axis a.
+template <class Each>
+void deal(const uint64_t* sections, uint64_t axes, uint64_t pairs, bool dealt, Each each) {
+    uint64_t got[SAGE_ROTARY_AXES] = {}, a = 0;
+    for (uint64_t i = 0; i < pairs; i++) {
+        while (got[a] == sections[a]) a = (a + 1) % axes;
+        each(i, a, got[a]++);
+        if (dealt) a = (a + 1) % axes;
+    }
 }
 
-sage_status buffer(const void* p, uint64_t have, uint64_t need, uintptr_t align, const char* what) {
-    if (need == 0) return SAGE_OK;
-    if (!p || have < need)
-        return set_error(SAGE_ERR_INVALID, "%s: buffer holds %llu elements, needs %llu", what, (u64)(p ? have : 0),
-                         (u64)need);
-    if (reinterpret_cast<uintptr_t>(p) % align)
-        return set_error(SAGE_ERR_INVALID, "%s must start at a %u-byte aligned device address", what, (unsigned)align);
-    return SAGE_OK;
-}
-
-// A 16-bit view of batch x tokens rows of heads.
-sage_status view(const void* data, uint64_t len, const sage_strides& st, int32_t dtype, uint64_t batch, uint64_t tokens,
-                 uint64_t heads, uint64_t d, const char* what) {
-    sage_status r = sage_strides_check(&st, what);
-    if (r != SAGE_OK) return r;
-    if (dtype != SAGE_BF16 && dtype != SAGE_F16)
-        return set_error(SAGE_ERR_INVALID, "%s: unknown dtype %d", what, dtype);
-    if (st.token >= 1ull << 62 || st.head >= 1ull << 62 || (batch > 1 && st.batch >= 1ull << 62))
-        return set_error(SAGE_ERR_INVALID, "%s: strides exceed 2^62 elements", what);
-    return buffer(data, len, sage_strides_extent(&st, batch, tokens, heads, d), 16, what);
-}
-sage_status view(const sage_tensor* t, uint64_t rows, uint64_t heads, uint64_t d, const char* what) {
-    const sage_strides st{0, t->strides.token, t->strides.head};
-    return view(t->data, t->len, st, t->dtype, 1, rows, heads, d, what);
-}
-sage_status view(const sage_tensor_mut* t, uint64_t rows, uint64_t heads, uint64_t d, const char* what) {
-    const sage_strides st{0, t->strides.token, t->strides.head};
-    return view(t->data, t->len, st, t->dtype, 1, rows, heads, d, what);
-}
-
-template <class T>
-sage::RowView rows_of(const T* t) {
-    return {static_cast<uint16_t*>(const_cast<void*>(static_cast<const void*>(t->data))), (long long)t->strides.batch,
-            (long long)t->strides.token, (long long)t->strides.head};
-}
-
-sage_status rotary_checked(const sage_rotary* r, uint64_t d, uint64_t rows, int transpose, sage::RotaryDev* out) {
+sage_status checked(const sage_rotary* r, uint64_t d, uint64_t rows, int transpose, sage::RotaryDev* out) {
     if (r->layout != SAGE_ROTARY_HALF && r->layout != SAGE_ROTARY_PAIRS)
         return set_error(SAGE_ERR_INVALID, "rotary: unknown layout %d", r->layout);
     if (r->rot < 2 || r->rot % 2 || r->rot > d)
@@ -103,116 +124,34 @@ sage_status rotary_checked(const sage_rotary* r, uint64_t d, uint64_t rows, int 
     return SAGE_OK;
 }
 
-sage_status shape_checked(const sage_cache_shape& h) {
-    if (h.kv_heads == 0 || h.heads == 0 || h.heads % h.kv_heads)
-        return set_error(SAGE_ERR_INVALID, "%llu query heads are not a multiple of %llu KV heads", (u64)h.heads,
-                         (u64)h.kv_heads);
-    if (h.page_tokens < 16 || h.page_tokens > 256 || (h.page_tokens & (h.page_tokens - 1)))
-        return set_error(SAGE_ERR_INVALID, "cache: pages of %llu tokens (16, 32, 64, 128 or 256 are supported)",
-                         (u64)h.page_tokens);
-    if (h.pages == 0 || h.max_pages == 0)
-        return set_error(SAGE_ERR_INVALID, "cache: %llu pages in the pool, %llu columns in the page table",
-                         (u64)h.pages, (u64)h.max_pages);
-    sage_status st = in_i32(h.pages, "cache pages");
-    if (st == SAGE_OK) st = in_i32(h.rows, "cache rows");
+sage_status checked(const sage_rotary_axes* r, uint64_t d, uint64_t rows, int transpose, sage::RotaryDev* out) {
+    if (r->layout < SAGE_ROTARY_AXES_HALF || r->layout > SAGE_ROTARY_AXES_AXIS_HALF)
+        return set_error(SAGE_ERR_INVALID, "rotary: unknown layout %d", r->layout);
+    uint64_t pairs = 0;
+    sage_status st = sections_checked(r->sections, r->axes, d / 2, &pairs);
     if (st != SAGE_OK) return st;
-    if (h.max_pages > (1ull << 30) / h.page_tokens)
-        return set_error(SAGE_ERR_INVALID, "cache: %llu pages of %llu tokens exceed 2^30 tokens a sequence",
-                         (u64)h.max_pages, (u64)h.page_tokens);
-    if (h.rows >= ROWS)
-        return set_error(SAGE_ERR_INVALID, "cache: %llu rows exceed the launch grid", (u64)h.rows);
-    // Launch grids: x below 2^24 workgroups, append's K, V and query heads and the
-    // joins' KV heads in y, the batch in z.
-    if (h.batch > 65535 || h.heads > 65535 || 2 * h.kv_heads + h.heads > 65535)
-        return set_error(SAGE_ERR_INVALID, "cache: %llu sequences of %llu and %llu heads exceed the launch grid",
-                         (u64)h.batch, (u64)h.heads, (u64)h.kv_heads);
-    // A tile is 16 columns or more; 128 where there are many.
-    const uint64_t group = h.heads / h.kv_heads;
-    if (h.max_new > I32 / 64 / group || (h.max_new * group + 127) / 128 * h.kv_heads >= 1ull << 24)
-        return set_error(SAGE_ERR_INVALID, "cache: %llu new rows of %llu heads a KV head exceed the launch grid",
-                         (u64)h.max_new, (u64)group);
+    if (r->dealt && r->layout == SAGE_ROTARY_AXES_AXIS_HALF)
+        return set_error(SAGE_ERR_INVALID, "rotary: the halves of an axis's channels need its pairs in one run");
+    st = buffer(r->table, r->table_len, 2 * pairs, 16, "rotary table");
+    if (st == SAGE_OK) st = in_i32(r->table_len / (2 * pairs), "rotary positions");
+    if (st == SAGE_OK && (r->positions_stride < rows || r->positions_stride >= 1ull << 60))
+        st = set_error(SAGE_ERR_INVALID, "rotary positions: %llu entries from axis to axis, %llu rows",
+                       (u64)r->positions_stride, (u64)rows);
+    if (st == SAGE_OK)
+        st = buffer(r->positions, r->positions_len, (r->axes - 1) * r->positions_stride + rows, 4, "rotary positions");
+    if (st != SAGE_OK) return st;
+    *out = {r->table, r->positions, (int)(r->table_len / (2 * pairs)), (int)(2 * pairs), r->layout, transpose != 0};
+    out->axes = (int)r->axes;
+    out->positions_stride = (long long)r->positions_stride;
+    deal(r->sections, r->axes, pairs, r->dealt != 0,
+         [&](uint64_t i, uint64_t a, uint64_t) { out->axis_of[i / 16] |= (uint32_t)a << (i % 16 * 2); });
+    for (uint64_t a = 0; a < r->axes; a++) out->sections[a] = (int)r->sections[a];
     return SAGE_OK;
 }
 
-// Code rows of a pool, at most 2^31 pages x 65535 heads x 256 tokens: no wrap.
-uint64_t code_rows(const sage_cache_shape& h) { return h.pages * h.kv_heads * h.page_tokens; }
-
-sage_status cache_checked(const sage_cache_shape& h, uint64_t d, const sage_cache& c, const sage_cache_index& i,
-                          sage::CacheDev* out) {
-    sage_status st = shape_checked(h);
-    const uint64_t codes = st == SAGE_OK ? code_rows(h) * (d / 2) : 0, scales = codes / (sage::CACHE_BLOCK / 2);
-    if (st == SAGE_OK) st = buffer(c.k_codes, c.codes_len, codes, 16, "cache K codes");
-    if (st == SAGE_OK) st = buffer(c.k_scales, c.scales_len, scales, 16, "cache K scales");
-    if (st == SAGE_OK) st = buffer(c.v_codes, c.codes_len, codes, 16, "cache V codes");
-    if (st == SAGE_OK) st = buffer(c.v_scales, c.scales_len, scales, 16, "cache V scales");
-    if (st == SAGE_OK) st = buffer(i.starts, i.starts_len, h.batch + 1, 4, "cache starts");
-    if (st == SAGE_OK) st = buffer(i.lengths, i.lengths_len, h.batch, 4, "cache lengths");
-    if (st == SAGE_OK) st = buffer(i.page_table, i.page_table_len, h.batch * h.max_pages, 4, "cache page table");
-    if (st != SAGE_OK) return st;
-    int shift = 4;
-    while ((1ull << shift) < h.page_tokens) shift++;
-    *out = {c.k_codes, c.k_scales, c.v_codes, c.v_scales, i.starts, i.lengths, i.page_table, (int)h.batch,
-            (int)h.rows, (int)h.kv_heads, (int)h.pages, shift, (int)h.max_pages};
-    return SAGE_OK;
-}
-
-}  // namespace
-
-extern "C" {
-
-sage_status sage_rotary_table(uint64_t rot, uint64_t positions, double base, const sage_rotary_scaling* scaling,
-                              float* out, uint64_t out_len) {
-    if (!out) return set_error(SAGE_ERR_INVALID, "null argument");
-    if (rot < 2 || rot % 2 || rot > 1u << 16)
-        return set_error(SAGE_ERR_INVALID, "rotary: %llu rotated channels: an even number from 2", (u64)rot);
-    if (!(base > 1.0) || !std::isfinite(base))
-        return set_error(SAGE_ERR_INVALID, "rotary: base %g is not over 1", base);
-    sage_status st = in_i32(positions, "rotary positions");
-    if (st == SAGE_OK && out_len < positions * rot)
-        st = set_error(SAGE_ERR_INVALID, "rotary table: buffer holds %llu elements, needs %llu", (u64)out_len,
-                       (u64)(positions * rot));
-    if (st != SAGE_OK) return st;
-    const int kind = scaling ? scaling->kind : SAGE_ROTARY_NONE;
-    const double f = kind == SAGE_ROTARY_NONE ? 1.0 : scaling->factor, pi = 3.14159265358979323846;
-    if (kind < SAGE_ROTARY_NONE || kind > SAGE_ROTARY_YARN)
-        return set_error(SAGE_ERR_INVALID, "rotary: unknown scaling %d", kind);
-    if (!(f >= 1.0) || !std::isfinite(f))
-        return set_error(SAGE_ERR_INVALID, "rotary: scaling factor %g is not 1 or more", f);
-    double attention = scaling && scaling->attention != 0.0 ? scaling->attention : 1.0, fast = 0, slow = 0;
-    if (!std::isfinite(attention)) return set_error(SAGE_ERR_INVALID, "rotary: attention factor %g", attention);
-    if (kind == SAGE_ROTARY_NTK) {
-        if (rot < 4) return set_error(SAGE_ERR_INVALID, "rotary: NTK scaling needs 4 rotated channels or more");
-        base *= std::pow(f, (double)rot / (double)(rot - 2));
-    }
-    if (kind == SAGE_ROTARY_YARN) {
-        fast = scaling->beta_fast != 0.0 ? scaling->beta_fast : 32.0;
-        slow = scaling->beta_slow != 0.0 ? scaling->beta_slow : 1.0;
-        if (!(scaling->original > 0.0) || !std::isfinite(scaling->original) || !(slow < fast) || !std::isfinite(fast))
-            return set_error(SAGE_ERR_INVALID, "rotary: YaRN scaling of %g positions between %g and %g turns",
-                             scaling->original, slow, fast);
-        if (scaling->attention == 0.0) attention = 0.1 * std::log(f) + 1.0;
-    }
-    for (uint64_t i = 0; i < rot / 2; i++) {
-        double w = std::pow(base, -2.0 * (double)i / (double)rot);
-        if (kind == SAGE_ROTARY_LINEAR) w /= f;
-        if (kind == SAGE_ROTARY_YARN) {
-            // Peng et al., "YaRN: Efficient Context Window Extension of Large Language
-            // Models", 2023: pairs that turn often keep their angle, slow ones are interpolated.
-            const double turns = scaling->original * w / (2.0 * pi);
-            const double g = std::min(1.0, std::max(0.0, (turns - slow) / (fast - slow)));
-            w = g * w + (1.0 - g) * w / f;
-        }
-        for (uint64_t p = 0; p < positions; p++) {
-            const double a = (double)p * w;
-            out[(p * (rot / 2) + i) * 2] = (float)(attention * std::cos(a));
-            out[(p * (rot / 2) + i) * 2 + 1] = (float)(attention * std::sin(a));
-        }
-    }
-    return succeeded();
-}
-
-sage_status sage_rotary_apply(const sage_attention* s, const sage_shape* shape, const sage_rotary* rotary,
-                              const sage_tensor* x, const sage_tensor_mut* out, int32_t transpose) {
+template <class R>
+sage_status apply(const sage_attention* s, const sage_shape* shape, const R* rotary, const sage_tensor* x,
+                  const sage_tensor_mut* out, int32_t transpose) {
     if (!s || !shape || !rotary || !x || !out) return set_error(SAGE_ERR_INVALID, "null argument");
     if (shape->batch == 0 || shape->tokens == 0 || shape->heads == 0) return succeeded();
     uint64_t rows;
@@ -230,7 +169,7 @@ sage_status sage_rotary_apply(const sage_attention* s, const sage_shape* shape, 
     if (st == SAGE_OK && x->dtype != out->dtype)
         st = set_error(SAGE_ERR_INVALID, "rotary input and output must share one element type");
     sage::RotaryArgs a{};
-    if (st == SAGE_OK) st = rotary_checked(rotary, d, rows, transpose, &a.r);
+    if (st == SAGE_OK) st = checked(rotary, d, rows, transpose, &a.r);
     if (st == SAGE_OK) st = on_device(s);
     if (st != SAGE_OK) return st;
     a.x = rows_of(x);
@@ -240,6 +179,86 @@ sage_status sage_rotary_apply(const sage_attention* s, const sage_shape* shape, 
     a.heads = (int)shape->heads;
     a.f16 = x->dtype == SAGE_F16;
     return done(sage::launch_rotary((int)d, a, s->stream), "launch rotary");
+}
+
+template <class R>
+sage_status append(const sage_attention* s, const sage_cache_shape* shape, const sage_cache* cache,
+                   const sage_cache_index* index, const sage_tensor* k, const sage_tensor* v, const R* rotary,
+                   const sage_tensor* q, const sage_tensor_mut* q_out) {
+    if (!s || !shape || !cache || !index || !k || !v) return set_error(SAGE_ERR_INVALID, "null argument");
+    if (!q != !q_out || (q && !rotary))
+        return set_error(SAGE_ERR_INVALID, "cache append: queries need an output and a rotary");
+    const uint64_t d = s->head_dim;
+    sage::AppendArgs a{};
+    sage_status st = cache_checked(*shape, d, *cache, *index, &a.c);
+    if (st == SAGE_OK) st = view(k, shape->rows, shape->kv_heads, d, "cache append K");
+    if (st == SAGE_OK) st = view(v, shape->rows, shape->kv_heads, d, "cache append V");
+    if (st == SAGE_OK && q) st = view(q, shape->rows, shape->heads, d, "cache append Q");
+    if (st == SAGE_OK && q) st = view(q_out, shape->rows, shape->heads, d, "cache append Q output");
+    if (st == SAGE_OK && (k->dtype != v->dtype || (q && (q->dtype != k->dtype || q_out->dtype != k->dtype))))
+        st = set_error(SAGE_ERR_INVALID, "Q, K and V must share one element type");
+    if (st == SAGE_OK && rotary) st = checked(rotary, d, shape->rows, 0, &a.r);
+    if (st == SAGE_OK) st = on_device(s);
+    if (st != SAGE_OK) return st;
+    if (shape->rows == 0 || shape->batch == 0) return succeeded();
+    a.k = rows_of(k);
+    a.v = rows_of(v);
+    if (q) {
+        a.q = rows_of(q);
+        a.q_out = rows_of(q_out);
+    }
+    a.heads = (int)shape->heads;
+    a.f16 = k->dtype == SAGE_F16;
+    return done(sage::launch_cache_append((int)d, a, s->stream), "launch cache append");
+}
+
+}  // namespace
+
+extern "C" {
+
+sage_status sage_rotary_table(uint64_t rot, uint64_t positions, double base, const sage_rotary_scaling* scaling,
+                              float* out, uint64_t out_len) {
+    if (!out) return set_error(SAGE_ERR_INVALID, "null argument");
+    if (rot < 2 || rot % 2 || rot > 1u << 16)
+        return set_error(SAGE_ERR_INVALID, "rotary: %llu rotated channels: an even number from 2", (u64)rot);
+    if (!(base > 1.0) || !std::isfinite(base))
+        return set_error(SAGE_ERR_INVALID, "rotary: base %g is not over 1", base);
+    sage_status st = table_room(positions, rot, out_len);
+    Speeds speeds;
+    if (st == SAGE_OK) st = speeds.checked(base, scaling, rot);
+    if (st != SAGE_OK) return st;
+    for (uint64_t i = 0; i < rot / 2; i++) speeds.column(out, rot / 2, i, positions, speeds.of(i, rot));
+    return succeeded();
+}
+
+sage_status sage_rotary_axes_table(const uint64_t* sections, uint64_t axes, int32_t dealt, int32_t per_axis,
+                                   uint64_t positions, double base, const sage_rotary_scaling* scaling, float* out,
+                                   uint64_t out_len) {
+    if (!sections || !out) return set_error(SAGE_ERR_INVALID, "null argument");
+    uint64_t pairs = 0, least = 1u << 15;
+    sage_status st = sections_checked(sections, axes, 1u << 15, &pairs);
+    if (st != SAGE_OK) return st;
+    if (!(base > 1.0) || !std::isfinite(base))
+        return set_error(SAGE_ERR_INVALID, "rotary: base %g is not over 1", base);
+    for (uint64_t a = 0; a < axes; a++) least = std::min(least, sections[a]);
+    st = table_room(positions, 2 * pairs, out_len);
+    Speeds speeds;
+    if (st == SAGE_OK) st = speeds.checked(base, scaling, 2 * (per_axis ? least : pairs));
+    if (st != SAGE_OK) return st;
+    deal(sections, axes, pairs, dealt != 0, [&](uint64_t i, uint64_t a, uint64_t j) {
+        speeds.column(out, pairs, i, positions, per_axis ? speeds.of(j, 2 * sections[a]) : speeds.of(i, 2 * pairs));
+    });
+    return succeeded();
+}
+
+sage_status sage_rotary_apply(const sage_attention* s, const sage_shape* shape, const sage_rotary* rotary,
+                              const sage_tensor* x, const sage_tensor_mut* out, int32_t transpose) {
+    return apply(s, shape, rotary, x, out, transpose);
+}
+
+sage_status sage_rotary_axes_apply(const sage_attention* s, const sage_shape* shape, const sage_rotary_axes* rotary,
+                                   const sage_tensor* x, const sage_tensor_mut* out, int32_t transpose) {
+    return apply(s, shape, rotary, x, out, transpose);
 }
 
 sage_status sage_cache_sizes(const sage_cache_shape* shape, uint64_t head_dim, uint64_t* codes, uint64_t* scales) {
@@ -256,31 +275,14 @@ sage_status sage_cache_sizes(const sage_cache_shape* shape, uint64_t head_dim, u
 sage_status sage_cache_append(const sage_attention* s, const sage_cache_shape* shape, const sage_cache* cache,
                               const sage_cache_index* index, const sage_tensor* k, const sage_tensor* v,
                               const sage_rotary* rotary, const sage_tensor* q, const sage_tensor_mut* q_out) {
-    if (!s || !shape || !cache || !index || !k || !v) return set_error(SAGE_ERR_INVALID, "null argument");
-    if (!q != !q_out || (q && !rotary))
-        return set_error(SAGE_ERR_INVALID, "cache append: queries need an output and a rotary");
-    const uint64_t d = s->head_dim;
-    sage::AppendArgs a{};
-    sage_status st = cache_checked(*shape, d, *cache, *index, &a.c);
-    if (st == SAGE_OK) st = view(k, shape->rows, shape->kv_heads, d, "cache append K");
-    if (st == SAGE_OK) st = view(v, shape->rows, shape->kv_heads, d, "cache append V");
-    if (st == SAGE_OK && q) st = view(q, shape->rows, shape->heads, d, "cache append Q");
-    if (st == SAGE_OK && q) st = view(q_out, shape->rows, shape->heads, d, "cache append Q output");
-    if (st == SAGE_OK && (k->dtype != v->dtype || (q && (q->dtype != k->dtype || q_out->dtype != k->dtype))))
-        st = set_error(SAGE_ERR_INVALID, "Q, K and V must share one element type");
-    if (st == SAGE_OK && rotary) st = rotary_checked(rotary, d, shape->rows, 0, &a.r);
-    if (st == SAGE_OK) st = on_device(s);
-    if (st != SAGE_OK) return st;
-    if (shape->rows == 0 || shape->batch == 0) return succeeded();
-    a.k = rows_of(k);
-    a.v = rows_of(v);
-    if (q) {
-        a.q = rows_of(q);
-        a.q_out = rows_of(q_out);
-    }
-    a.heads = (int)shape->heads;
-    a.f16 = k->dtype == SAGE_F16;
-    return done(sage::launch_cache_append((int)d, a, s->stream), "launch cache append");
+    return append(s, shape, cache, index, k, v, rotary, q, q_out);
+}
+
+sage_status sage_cache_append_axes(const sage_attention* s, const sage_cache_shape* shape, const sage_cache* cache,
+                                   const sage_cache_index* index, const sage_tensor* k, const sage_tensor* v,
+                                   const sage_rotary_axes* rotary, const sage_tensor* q, const sage_tensor_mut* q_out) {
+    if (!rotary) return set_error(SAGE_ERR_INVALID, "null argument");
+    return append(s, shape, cache, index, k, v, rotary, q, q_out);
 }
 
 sage_status sage_cache_read(const sage_attention* s, const sage_cache_shape* shape, const sage_cache* cache,
@@ -350,25 +352,10 @@ sage_status sage_cache_attend(const sage_attention* s, const sage_cache_workspac
     const uint64_t d = s->head_dim;
     sage::CacheAttnArgs a{};
     sage_status st = cache_checked(h, d, *cache, *index, &a.c);
-    if (st == SAGE_OK) st = view(q, h.rows, h.heads, d, "Q");
-    if (st == SAGE_OK) st = view(out, h.rows, h.heads, d, "output");
+    if (st == SAGE_OK) st = attend_checked(h, d, q, out, *opts, &a);
     if (st == SAGE_OK) st = on_device(s);
     if (st != SAGE_OK) return st;
     if (h.rows == 0 || h.batch == 0 || h.max_new == 0) return succeeded();
-    a.q = rows_of(q);
-    a.out = rows_of(out);
-    a.heads = (int)h.heads;
-    a.group = (int)(h.heads / h.kv_heads);
-    a.max_new = (int)h.max_new;
-    a.causal = opts->causal != 0;
-    a.q_f16 = q->dtype == SAGE_F16;
-    a.out_f16 = out->dtype == SAGE_F16;
-    const float scale = opts->has_softmax_scale ? opts->softmax_scale : (float)(1.0 / std::sqrt((double)d));
-    // A scale of 0 becomes the least normal float: every weight is 1 still, and
-    // the -infinity of a masked logit stays what it is.
-    a.qk_mul = std::max(std::fabs(scale) * 1.44269504088896340736f, 1.17549435e-38f);
-    if (scale != scale) a.qk_mul = scale;
-    a.q_sign = std::signbit(scale) ? 0x80008000u : 0u;
     a.splits = ws->plan.chunks ? ws->plan.wgs : 1;
     a.whole = ws->plan.whole;
     a.part_o = static_cast<float*>(ws->buf);

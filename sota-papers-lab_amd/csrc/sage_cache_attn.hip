@@ -299,12 +299,152 @@ struct Line {
         total = uniform(upto, (c.batch - 1) / run);
     }
 };
+// ---- Picked pages ----
+//
+// The pages that a unit's rows have picked (sage_cache_attend_picked), one behind
+// the other, in place of a sequence's own: the tokens of a unit are those of the
+// pages that any of its rows picked, ascending, and each page carries the rows that
+// did. 16 columns of a group of four heads are four rows, whose picks share much: a
+// page is read and converted once for all of them, and never costs more than the
+// rows' own would, whose columns would fill a tile as wide.
+struct Entries {
+    uint32_t* entry;  // column << 16 | rows of the unit, a bit each
+    int* page;        // the pool's page, or -1
+    int count;
+};
+
+// LDS of a unit: the columns' bits, how many are set before each word, and the entries.
+// rows: of a unit, at most.
+__host__ __device__ __forceinline__ int unit_rows(int group, int max_new) {
+    const int rows = (COLS + group - 2) / group + 1;
+    return rows < max_new ? rows : max_new;
+}
+__host__ __device__ __forceinline__ int pick_words(int max_pages) { return (max_pages + 31) / 32; }
+__host__ __device__ __forceinline__ int pick_entries(int top, int group, int max_new, int max_pages) {
+    const int most = unit_rows(group, max_new) * top;
+    return most < max_pages ? most : max_pages;
+}
+
+// The entries of rows j0 .. j0 + rows - 1 of sequence b, whose columns are below `pages`.
+// All threads of the workgroup together.
+template <int W>
+__device__ __forceinline__ Entries entries_of(const CacheAttnArgs& a, const SequenceIndex& seq, int b, int kvh, int j0,
+                                              int rows, int pages, uint32_t* lds) {
+    const CacheDev& c = a.c;
+    const int words = pick_words(pages), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t *bits = lds, *before = bits + pick_words(c.max_pages);
+    Entries e{before + pick_words(c.max_pages), nullptr, 0};
+    e.page = reinterpret_cast<int*>(e.entry) + pick_entries(a.top, a.group, a.max_new, c.max_pages);
+    __shared__ int found[W], odd[W];
+    const int* table = c.page_table + (long long)b * c.max_pages;
+    auto page_at = [&](int col) {
+        const int id = table[col];
+        return (unsigned)id < (unsigned)c.pages ? id : -1;
+    };
+    // Row r's i-th column, or -1.
+    auto picked = [&](int r, int i) {
+        const long long row = seq.start + j0 + r;
+        if (row < 0 || row >= c.rows) return -1;
+        const int col = a.picked[(row * c.kv_heads + kvh) * a.top + i];
+        return (unsigned)col < (unsigned)pages ? col : -1;
+    };
+    if (rows == 1) {
+        // One row's list as it is, if it ascends, with nothing behind a -1.
+        int n = 0;
+        bool out_of_order = false;
+        for (int i0 = 0; i0 < a.top; i0 += 64 * W) {
+            const int i = i0 + (int)threadIdx.x, col = i < a.top ? picked(0, i) : -1;
+            const int last = i > 0 && i < a.top ? picked(0, i - 1) : -1;
+            if (col >= 0) {
+                out_of_order |= i > 0 && last >= col;
+                out_of_order |= i > 0 && last < 0;
+                e.entry[min(i, pages - 1)] = (uint32_t)col << 16 | 1;
+                e.page[min(i, pages - 1)] = page_at(col);
+            }
+            n += __builtin_popcountll(__ballot(col >= 0));
+        }
+        const bool wrong = __any(out_of_order);
+        if (lane == 0) found[wave] = n, odd[wave] = wrong;
+        __syncthreads();
+        bool any = false;
+#pragma unroll
+        for (int w = 0; w < W; w++) e.count += found[w], any = any || odd[w];
+        if (!any) return e;
+        __syncthreads();
+        e.count = 0;
+    }
+    for (int i = threadIdx.x; i < words; i += 64 * W) bits[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * a.top; i += 64 * W) {
+        const int col = picked(i / a.top, i % a.top);
+        if (col >= 0) atomicOr(&bits[col >> 5], 1u << (col & 31));
+    }
+    __syncthreads();
+    // A run of words a thread.
+    const int run = (words + 64 * W - 1) / (64 * W), w0 = min(words, (int)threadIdx.x * run), w1 = min(words, w0 + run);
+    int mine = 0;
+    for (int w = w0; w < w1; w++) mine += __builtin_popcount(bits[w]);
+    int upto = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int x = __shfl_up(upto, d);
+        if (lane >= d) upto += x;
+    }
+    if (lane == 63) found[wave] = upto;
+    __syncthreads();
+    int at = upto - mine;
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+        if (w < wave) at += found[w];
+        e.count += found[w];
+    }
+    for (int w = w0; w < w1; w++) {
+        before[w] = at;
+        for (uint32_t x = bits[w]; x; x &= x - 1) e.entry[at++] = (uint32_t)(w * 32 + __builtin_ctz(x)) << 16;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < e.count; i += 64 * W) e.page[i] = page_at((int)(e.entry[i] >> 16));
+    for (int i = threadIdx.x; i < rows * a.top; i += 64 * W) {
+        const int r = i / a.top, col = picked(r, i - r * a.top);
+        if (col < 0) continue;
+        const int place = before[col >> 5] + __builtin_popcount(bits[col >> 5] & ((1u << (col & 31)) - 1));
+        atomicOr(&e.entry[place], 1u << r);
+    }
+    __syncthreads();
+    return e;
+}
+
+// The entries as a wave walks them, 64 at a time, as Pages does a table's columns.
+struct Walk {
+    Entries e;
+    int shift, lane, base, ids;
+    uint32_t entries;
+    __device__ __forceinline__ Walk(const Entries& e_, int shift_, int lane_, int t) : e(e_), shift(shift_), lane(lane_) {
+        fill(t >> shift);
+    }
+    __device__ __forceinline__ void fill(int i) {
+        base = i;
+        const int at = i + lane;
+        ids = at < e.count ? e.page[at] : -1;
+        entries = at < e.count ? e.entry[at] : 0;
+        asm volatile("" : "+v"(ids), "+v"(entries));  // waited for here, once a window
+    }
+    // The page of token t of the list, or -1, and its entry.
+    __device__ __forceinline__ int of(int t, uint32_t& entry) {
+        const int i = t >> shift;
+        if (i - base >= 64) fill(i);
+        entry = __builtin_amdgcn_readlane(entries, i - base);
+        return __builtin_amdgcn_readlane(ids, i - base);
+    }
+};
+
 // Steps of a share; at least two, so that a share is more than a unit's first step.
 __device__ __forceinline__ long long share_of(long long total, int wgs) { return max(2ll, (total + wgs - 1) / wgs); }
 
 // QP: bf16 parts of a query. W: waves, four, or eight for whole units that do
-// not fill the chip (cache_plan).
-template <int D, int QP, int W>
+// not fill the chip (cache_plan). PICKED: the units' tokens are those of picked
+// pages, in a.splits equal parts a unit, a workgroup each.
+template <int D, int QP, int W, bool PICKED>
 __global__ __launch_bounds__(64 * W, D == 64 && W == 4 ? 3 : 2) void cache_attn(CacheAttnArgs a) {
     constexpr int G = D / 32;        // scale blocks of a row
     constexpr int VT = 64 / G;       // tokens of one V load
@@ -314,6 +454,7 @@ __global__ __launch_bounds__(64 * W, D == 64 && W == 4 ? 3 : 2) void cache_attn(
     constexpr int HALF = TOKENS / 2; // tokens of V in LDS at a time, per wave
     constexpr int LDS = W * (HALF * D * 2 > COLS * PAD * 4 ? HALF * D * 2 : COLS * PAD * 4);
     __shared__ __align__(16) uint8_t lds[LDS];
+    extern __shared__ uint32_t pick_lds[];  // PICKED: entries_of's
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
     const CacheDev& c = a.c;
@@ -323,7 +464,10 @@ __global__ __launch_bounds__(64 * W, D == 64 && W == 4 ? 3 : 2) void cache_attn(
     int b;
     long long pos, stop, base_b;
     SequenceIndex seq;
-    if (a.whole) {
+    if constexpr (PICKED) {
+        b = blockIdx.z, base_b = 0, pos = 0, stop = 1;
+        seq = sequence_index(c, b, a.max_new);
+    } else if (a.whole) {
         b = blockIdx.z, base_b = 0;
         seq = sequence_index(c, b, a.max_new);
         const Units units(a, seq);
@@ -352,30 +496,50 @@ __global__ __launch_bounds__(64 * W, D == 64 && W == 4 ? 3 : 2) void cache_attn(
     while (pos < stop) {
         const Units units(a, seq);
         if (units.tiles == 0) return;
-        const long long idx = (pos - base_b) / (units.steps + 1), begin = base_b + idx * (units.steps + 1);
-        const long long next = begin + units.steps + 1;
-        const int kvh = (int)(idx / units.tiles), tile = (int)(idx - (long long)kvh * units.tiles);
-        const int s0 = (int)max(0ll, pos - begin - 1), s1 = (int)(min(stop, next) - begin - 1);
         const SequenceIndex now = seq;
         const int b_now = b;
-        pos = next;
-        if (next >= base_b + units.cost(c)) {  // on to the next sequence that has rows
-            base_b = next;
-            while (pos < stop && b < c.batch - 1) {
-                seq = sequence_index(c, ++b, a.max_new);
-                if (seq.n) break;
+        int kvh, tile, s0, s1, split = 0;
+        bool whole;
+        if constexpr (PICKED) {
+            kvh = blockIdx.x % c.kv_heads, split = blockIdx.x / c.kv_heads % a.splits;
+            tile = blockIdx.x / c.kv_heads / a.splits;
+            if (tile >= units.tiles) return;
+            pos = stop;
+            whole = a.splits == 1;
+        } else {
+            const long long idx = (pos - base_b) / (units.steps + 1), begin = base_b + idx * (units.steps + 1);
+            const long long next = begin + units.steps + 1;
+            kvh = (int)(idx / units.tiles), tile = (int)(idx - (long long)kvh * units.tiles);
+            s0 = (int)max(0ll, pos - begin - 1), s1 = (int)(min(stop, next) - begin - 1);
+            pos = next;
+            if (next >= base_b + units.cost(c)) {  // on to the next sequence that has rows
+                base_b = next;
+                while (pos < stop && b < c.batch - 1) {
+                    seq = sequence_index(c, ++b, a.max_new);
+                    if (seq.n) break;
+                }
             }
+            if (s1 <= s0) continue;  // no more than the unit's beginning
+            whole = s0 == 0 && s1 == units.steps;
         }
-        if (s1 <= s0) continue;  // no more than the unit's beginning
-        const bool whole = s0 == 0 && s1 == units.steps;
+        const int c0 = tile * COLS, cols = now.n * a.group;
+        const int j0 = c0 / a.group, j1 = (min(c0 + COLS, cols) - 1) / a.group;  // its rows
+        Entries entries{};
+        if constexpr (PICKED) {
+            const int pages = (now.limit(j1, a.causal) + (1 << c.page_shift) - 1) >> c.page_shift;
+            entries = entries_of<W>(a, now, b_now, kvh, j0, j1 - j0 + 1, pages, pick_lds);
+            const int steps = ((entries.count << c.page_shift) + STEP - 1) / STEP;
+            s0 = (int)((long long)steps * split / a.splits), s1 = (int)((long long)steps * (split + 1) / a.splits);
+        }
         const long long part = 2ll * blockIdx.x + (s0 == 0);
-        const int c0 = tile * COLS, cols = now.n * a.group, t0 = s0 * STEP;
+        const int t0 = s0 * STEP;
         const int j = (c0 + col) / a.group, head = kvh * a.group + (c0 + col) - j * a.group;
         const long long row = now.start + j;
         const bool have = c0 + col < cols && row >= 0 && row < c.rows;
         const int limit = now.limit(j, a.causal);              // this column sees slots below it
-        const int least = now.limit(c0 / a.group, a.causal);   // every column sees these
-        const int end = min(s1 * STEP, now.limit((min(c0 + COLS, cols) - 1) / a.group, a.causal));
+        const int least = now.limit(j0, a.causal);             // every column sees these
+        // (a picked unit's tokens are its entries')
+        const int end = min(s1 * STEP, PICKED ? entries.count << c.page_shift : now.limit(j1, a.causal));
 
         // Q^T, the second operand: column lane % 16, channels in K's order.
         bf8 q[QP][KS];
@@ -398,7 +562,15 @@ __global__ __launch_bounds__(64 * W, D == 64 && W == 4 ? 3 : 2) void cache_attn(
         }
 
         const int t_first = t0 + wave * TOKENS;
-        Pages pages(c, b_now, lane, t_first);
+        using Source = std::conditional_t<PICKED, Walk, Pages>;
+        auto source = [&] {
+            if constexpr (PICKED)
+                return Source(entries, c.page_shift, lane, t_first);
+            else
+                return Source(c, b_now, lane, t_first);
+        };
+        Source pages = source();
+        const uint32_t every = (2u << (j1 - j0)) - 1;  // picked by all rows
         // One step's codes and scales: K's token lane % 16 of each 16-token tile,
         // channels (lane / 16) * D / 4 on; V's token lane / G + i * VT, block lane % G.
         struct Step {
@@ -406,6 +578,19 @@ __global__ __launch_bounds__(64 * W, D == 64 && W == 4 ? 3 : 2) void cache_attn(
             uint4 v[G];
             uint32_t vs[G];
             int valid;  // bit i: the page of 16-token tile i is one of the pool's
+            uint32_t entry[PICKED ? 4 : 1];
+        };
+        // Slot of the first token of 16-token tile i at t, and whether the lane's column
+        // sees token k of the tile.
+        auto slot_at = [&](int t, int i, const Step& st) {
+            if constexpr (PICKED)
+                return (int)(st.entry[i] >> 16 << c.page_shift) + ((t + 16 * i) & ((1 << c.page_shift) - 1));
+            else
+                return t + 16 * i;
+        };
+        auto sees = [&](int t, int i, int k, const Step& st) {
+            return slot_at(t, i, st) + k < limit && (st.valid >> i & 1) &&
+                   (!PICKED || (st.entry[PICKED ? i : 0] >> (j - j0) & 1));
         };
         auto row_of = [&](int t, int page) {
             return cache_row(c, max(page, 0), kvh, t & ((1 << c.page_shift) - 1));
@@ -415,7 +600,11 @@ __global__ __launch_bounds__(64 * W, D == 64 && W == 4 ? 3 : 2) void cache_attn(
             long long rows[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int page = pages.of(t + 16 * i);
+                int page;
+                if constexpr (PICKED)
+                    page = pages.of(t + 16 * i, st.entry[i]);
+                else
+                    page = pages.of(t + 16 * i);
                 st.valid |= (page >= 0) << i;
                 rows[i] = row_of(t + 16 * i, page);
             }
@@ -471,13 +660,20 @@ __global__ __launch_bounds__(64 * W, D == 64 && W == 4 ? 3 : 2) void cache_attn(
 #pragma unroll
             for (int i = 0; i < G; i++) bad[i] = __ballot(st.vs[i] >= V_NAN);
             // The softmax's step.
-            const bool masked = t + TOKENS > least || there != 15;
+            bool masked = there != 15;
+            if constexpr (PICKED) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    masked = masked || slot_at(t, i, st) + 16 > least || (st.entry[i] & 0xffff) != every;
+            } else {
+                masked = masked || t + TOKENS > least;
+            }
             float mx = NEG_INF;
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    if (masked && (t + 16 * i + 4 * g + r >= limit || !(there >> i & 1))) x[i][r] = NEG_INF;
+                    if (masked && !sees(t, i, 4 * g + r, st)) x[i][r] = NEG_INF;
                     mx = fmaxf(mx, x[i][r]);
                 }
             mx = fmaxf(m, col_max(mx));
@@ -500,7 +696,7 @@ __global__ __launch_bounds__(64 * W, D == 64 && W == 4 ? 3 : 2) void cache_attn(
                     for (int r = 0; r < 4; r++) {
                         const int tok = 16 * i + 4 * g + r;
                         const uint32_t blocks = (uint32_t)(bad[16 * i / VT] >> (tok % VT * G)) & ((1u << G) - 1);
-                        if (t + tok < limit && (there >> i & 1)) hit |= blocks;
+                        if (sees(t, i, 4 * g + r, st)) hit |= blocks;
                     }
                 hit = col_or(hit);
             }
@@ -582,14 +778,17 @@ __global__ __launch_bounds__(64 * W, D == 64 && W == 4 ? 3 : 2) void cache_attn(
                 for (int i = 0; i < 8; i++) f[i] += p[i] * s;
             }
             if (!whole) {
-                float* p = a.part_o + (part * COLS + oc) * D + ch;
+                if (PICKED && (orow < 0 || orow >= c.rows)) return;
+                const long long at = PICKED ? ((long long)split * c.rows + orow) * a.heads + oh : part * COLS + oc;
+                float* p = a.part_o + at * D + ch;
                 *reinterpret_cast<f4*>(p) = f4{f[0], f[1], f[2], f[3]};
                 *reinterpret_cast<f4*>(p + 4) = f4{f[4], f[5], f[6], f[7]};
-                if (ch == 0) reinterpret_cast<f2*>(a.part_ml)[part * COLS + oc] = f2{top, sum};
+                if (ch == 0) reinterpret_cast<f2*>(a.part_ml)[at] = f2{top, sum};
             } else if (orow >= 0 && orow < c.rows) {
                 store_row(a, orow, oh, ch, f, sum);
             }
         }
+        if (PICKED) return;
         __syncthreads();  // LDS is the next unit's
     }
 }
@@ -939,7 +1138,8 @@ __global__ __launch_bounds__(256) void cache_chunk_join(CacheAttnArgs a) {
     const SequenceIndex seq = sequence_index(c, b, a.max_new);
     const long long row = seq.start + j;
     if (j >= seq.n || row < 0 || row >= c.rows) return;  // (SHARE: all threads or none)
-    const int chunk = split_tokens(seq.len, a.splits), parts = seq.len ? (seq.len + chunk - 1) / chunk : 1;
+    const int chunk = split_tokens(seq.len, a.splits);
+    const int parts = a.picked ? a.splits : seq.len ? (seq.len + chunk - 1) / chunk : 1;
     const long long first = row * a.heads + h, step = (long long)c.rows * a.heads;
     float f[8];
     const float l = join_parts<D, SHARE>(a, parts, ch, [&](int p) { return first + p * step; }, f);
@@ -1030,6 +1230,20 @@ CachePlan cache_plan(int head_dim, int batch, int rows, int heads, int kv_heads,
     return p;
 }
 
+// Many parts of few columns are joined by a workgroup a column (20000 tokens,
+// 32/8 heads of 128: one row each of 2 sequences 21.5 us against 24, of 8 47.7
+// against 46.8; chunks of 32 rows 37.4 against 39.3, of 128 76 against 70).
+template <int D>
+static void join_splits(const CacheAttnArgs& a, hipStream_t s) {
+    const long long pairs = (long long)a.max_new * a.heads;
+    constexpr int PER = 256 / (D / 8);
+    if (a.splits > 8 && pairs * a.c.batch <= 2048)
+        hipLaunchKernelGGL((cache_chunk_join<D, true>), dim3((unsigned)pairs, 1, a.c.batch), dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((cache_chunk_join<D, false>), dim3((unsigned)((pairs + PER - 1) / PER), 1, a.c.batch),
+                           dim3(256), 0, s, a);
+}
+
 template <int D>
 static hipError_t launch(const CacheAttnArgs& a, const CachePlan& plan, hipStream_t s) {
     const dim3 block(256);
@@ -1053,22 +1267,13 @@ static hipError_t launch(const CacheAttnArgs& a, const CachePlan& plan, hipStrea
         else
             chunk(a.out_f16 ? cache_attn_chunk<D, 1, true> : cache_attn_chunk<D, 1, false>);
     } else if (a.q_f16) {
-        few(plan.wide ? cache_attn<D, 2, 8> : cache_attn<D, 2, 4>);
+        few(plan.wide ? cache_attn<D, 2, 8, false> : cache_attn<D, 2, 4, false>);
     } else {
-        few(plan.wide ? cache_attn<D, 1, 8> : cache_attn<D, 1, 4>);
+        few(plan.wide ? cache_attn<D, 1, 8, false> : cache_attn<D, 1, 4, false>);
     }
-    // Many parts of few columns are joined by a workgroup a column (20000 tokens,
-    // 32/8 heads of 128: one row each of 2 sequences 21.5 us against 24, of 8 47.7
-    // against 46.8; chunks of 32 rows 37.4 against 39.3, of 128 76 against 70).
-    if (plan.chunks && a.splits > 1) {
-        const long long pairs = (long long)a.max_new * a.heads;
-        constexpr int PER = 256 / (D / 8);
-        if (a.splits > 8 && pairs * batch <= 2048)
-            hipLaunchKernelGGL((cache_chunk_join<D, true>), dim3((unsigned)pairs, 1, batch), block, 0, s, a);
-        else
-            hipLaunchKernelGGL((cache_chunk_join<D, false>), dim3((unsigned)((pairs + PER - 1) / PER), 1, batch), block,
-                               0, s, a);
-    } else if (!plan.chunks && !a.whole) {
+    if (plan.chunks) {
+        if (a.splits > 1) join_splits<D>(a, s);
+    } else if (!a.whole) {
         if ((long long)tiles * heads * batch <= 32)
             hipLaunchKernelGGL((cache_attn_join<D, true>), dim3(tiles * COLS, heads, batch), block, 0, s, a, plan.wgs);
         else
@@ -1079,6 +1284,34 @@ static hipError_t launch(const CacheAttnArgs& a, const CachePlan& plan, hipStrea
 
 hipError_t launch_cache_attend(int head_dim, const CacheAttnArgs& a, const CachePlan& plan, hipStream_t s) {
     return head_dim == 64 ? launch<64>(a, plan, s) : launch<128>(a, plan, s);
+}
+
+PickedPlan picked_plan(int head_dim, int batch, int rows, int heads, int kv_heads, int max_new, int max_pages,
+                       int page_tokens, int top) {
+    const int group = heads / kv_heads;
+    PickedPlan p{};
+    p.lds = 4u * (2 * pick_words(max_pages) + 2 * pick_entries(top, group, max_new, max_pages));
+    const long long units = ((long long)max_new * group + COLS - 1) / COLS * kv_heads * batch;
+    const long long steps = ((long long)pick_entries(top, group, max_new, max_pages) * page_tokens + STEP - 1) / STEP;
+    const long long fill = head_dim == 64 ? 768 : 512;
+    p.splits = (int)std::max(1ll, std::min({fill / std::max(units, 1ll), (steps + 1) / 2, (long long)MAX_SPLITS}));
+    p.part_rows = p.splits > 1 ? (uint64_t)p.splits * rows * heads : 0;
+    return p;
+}
+
+template <int D>
+static hipError_t launch_picked(const CacheAttnArgs& a, const PickedPlan& plan, hipStream_t s) {
+    const unsigned tiles = (unsigned)(((long long)a.max_new * a.group + COLS - 1) / COLS);
+    const auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(tiles * a.splits * a.c.kv_heads, 1, a.c.batch), dim3(256), plan.lds, s, a);
+    };
+    a.q_f16 ? go(cache_attn<D, 2, 4, true>) : go(cache_attn<D, 1, 4, true>);
+    if (a.splits > 1) join_splits<D>(a, s);
+    return hipGetLastError();
+}
+
+hipError_t launch_cache_attend_picked(int head_dim, const CacheAttnArgs& a, const PickedPlan& plan, hipStream_t s) {
+    return head_dim == 64 ? launch_picked<64>(a, plan, s) : launch_picked<128>(a, plan, s);
 }
 
 }  // namespace sage

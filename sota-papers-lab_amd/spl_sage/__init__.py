@@ -573,6 +573,9 @@ class SageAttention:
             raise SageError(1, f"the cache is made for head dim {cache._head_dim}, the context for {self._head_dim}")
         if cache.shape is not shape and cache.shape._layout != shape._layout:
             raise _layouts_differ("the workspace and the cache", shape._layout, cache.shape._layout)
+        self._fits_index(index, shape)
+
+    def _fits_index(self, index, shape) -> None:
         if index._cols != shape.max_pages and index._cols is not None and shape.batch > 1:
             raise SageError(1, f"the page table has {index._cols} columns, the shape {shape.max_pages}")
 
@@ -581,10 +584,10 @@ class SageAttention:
         return SageError(1, f"a tensor is {where}, the context on device {self._device}")
 
     def rotary(self, shape: Shape, rotary, x: Tensor, out: TensorMut, transpose: bool = False) -> None:
-        """x's heads turned by their rows' positions into out (spl_sage.rotary)."""
-        _check(lib().sage_rotary_apply(self._h, C.byref(shape._c()), self._handle(rotary),
-                                       self._view(_abi.sage_tensor, x), self._view(_abi.sage_tensor_mut, out),
-                                       int(transpose)))
+        """x's heads turned by their rows' positions into out (spl_sage.rotary: a
+        Rotary, or an AxesRotary)."""
+        args = (self._handle(rotary), self._view(_abi.sage_tensor, x), self._view(_abi.sage_tensor_mut, out))
+        _check(getattr(lib(), rotary.APPLY)(self._h, C.byref(shape._c()), *args, int(transpose)))
 
     def cache_workspace(self, shape):
         """The workspace of cache_attend for one CacheShape (spl_sage.cache)."""
@@ -601,7 +604,7 @@ class SageAttention:
                 None if q is None else self._view(_abi.sage_tensor, q),
                 None if q_out is None else self._view(_abi.sage_tensor_mut, q_out))
         self._fits(cache, index, cache.shape)
-        _check(lib().sage_cache_append(self._h, *args))
+        _check(getattr(lib(), "sage_cache_append" if rotary is None else rotary.APPEND)(self._h, *args))
 
     def cache_read(self, cache, index, k: TensorMut, v: TensorMut) -> None:
         """Cached rows back as 16-bit keys and values."""
@@ -619,6 +622,67 @@ class SageAttention:
                 self._view(_abi.sage_tensor_mut, out), C.byref(o))
         self._fits(cache, index, ws.shape)
         _check(lib().sage_cache_attend(self._h, ws._h, *args))
+
+    def cache_tables(self, tables, news, past, free) -> None:
+        """A step's index (spl_sage.cache.CacheTables) from its requests' new rows
+        (int32 [batch]; below 0: ended) and cached tokens, with pages of the ring
+        `free`. past may be tables.lengths, and free's state tables.state."""
+        from .rotary import _ints
+
+        r = _abi.sage_cache_requests(*_ints(news, "request rows"), *_ints(past, "request lengths"))
+        for t in (news, past):
+            if t.get_device() != self._device:
+                raise self._out_of_reach(t.get_device())
+        _check(lib().sage_cache_tables(self._h, C.byref(tables.shape._c()), C.byref(r), self._handle(free),
+                                       self._handle(tables)))
+
+    def cache_bounds(self, cache, index, bounds) -> None:
+        """The bounds of the pages that the step wrote to (spl_sage.cache.PageBounds)."""
+        args = (C.byref(cache.shape._c()), self._handle(cache), self._handle(index), self._handle(bounds))
+        self._fits(cache, index, cache.shape)
+        self._fits_bounds(bounds, cache.shape)
+        _check(lib().sage_cache_bounds_update(self._h, *args))
+
+    def _fits_bounds(self, bounds, shape) -> None:
+        if bounds._head_dim != self._head_dim and bounds._head_dim is not None:
+            raise SageError(1, f"the bounds are made for head dim {bounds._head_dim}, the context for {self._head_dim}")
+        if (bounds.shape.pages, bounds.shape.kv_heads) != (shape.pages, shape.kv_heads):
+            raise SageError(1, f"the bounds are of {bounds.shape.pages} pages and {bounds.shape.kv_heads} KV heads, the "
+                               f"shape of {shape.pages} and {shape.kv_heads}")
+
+    def cache_pick_workspace(self, shape, top: int):
+        """The workspace of cache_pick and cache_attend_picked for one CacheShape
+        and number of pages a row (spl_sage.cache)."""
+        from . import cache
+
+        return cache.PickWorkspace(self, shape, top)
+
+    def cache_pick(self, ws, bounds, index, q: Tensor, picked, first: int = 1, last: int = 1, causal: bool = True) -> None:
+        """For each row and KV head the pages that its queries attend to: the first
+        and last ones and those whose bounds allow the greatest logits, into `picked`."""
+        o = _abi.sage_pick_options(max(first, 0), max(last, 0), int(causal))
+        args = (self._handle(bounds), self._handle(index), self._view(_abi.sage_tensor, q), *self._picked(ws, picked))
+        self._fits_bounds(bounds, ws.shape)
+        self._fits_index(index, ws.shape)
+        _check(lib().sage_cache_pick(self._h, ws._h, *args, C.byref(o)))
+
+    def cache_attend_picked(self, ws, cache, index, picked, q: Tensor, out: TensorMut,
+                            softmax_scale: Optional[float] = None, causal: bool = True) -> None:
+        """Attention of the rows' queries over the cached keys of the pages that each picked."""
+        o = _abi.sage_cache_options(0.0 if softmax_scale is None else float(softmax_scale),
+                                    0 if softmax_scale is None else 1, int(causal))
+        args = (self._handle(cache), self._handle(index), *self._picked(ws, picked), self._view(_abi.sage_tensor, q),
+                self._view(_abi.sage_tensor_mut, out), C.byref(o))
+        self._fits(cache, index, ws.shape)
+        _check(lib().sage_cache_attend_picked(self._h, ws._h, *args))
+
+    def _picked(self, ws, picked) -> tuple:
+        if picked._device != self._device:
+            raise self._out_of_reach(picked._device)
+        t = picked.columns
+        if t.dim() == 3 and tuple(t.shape[1:]) != (ws.shape.kv_heads, ws.top):
+            raise SageError(1, f"picked pages of {tuple(t.shape)}: {ws.top} of {ws.shape.kv_heads} KV heads a row are expected")
+        return picked._struct
 
     def peak(self, which: int, iters: int = 2048) -> float:
         """Measured dense TOPS of one MFMA shape (0 INT8, 1 FP8, 2 BF16)."""

@@ -113,6 +113,13 @@ class sage_rotary(C.Structure):
     ]
 
 
+class sage_rotary_axes(C.Structure):
+    _fields_ = [
+        ("table", C.c_void_p), ("table_len", u64), ("sections", u64 * 4), ("axes", u64), ("layout", i32),
+        ("dealt", i32), ("positions", C.c_void_p), ("positions_len", u64), ("positions_stride", u64),
+    ]
+
+
 class sage_cache_shape(C.Structure):
     _fields_ = [
         ("batch", u64), ("rows", u64), ("max_new", u64), ("heads", u64), ("kv_heads", u64), ("pages", u64),
@@ -136,6 +143,30 @@ class sage_cache_index(C.Structure):
 
 class sage_cache_options(C.Structure):
     _fields_ = [("softmax_scale", C.c_float), ("has_softmax_scale", i32), ("causal", i32)]
+
+
+class sage_cache_requests(C.Structure):
+    _fields_ = [("news", C.c_void_p), ("news_len", u64), ("past", C.c_void_p), ("past_len", u64)]
+
+
+class sage_cache_free(C.Structure):
+    _fields_ = [("pages", C.c_void_p), ("pages_len", u64), ("state", C.c_void_p), ("state_len", u64)]
+
+
+class sage_cache_step(C.Structure):
+    _fields_ = [
+        (name, kind)
+        for what in ("starts", "lengths", "page_table", "positions", "slots", "sequences", "state", "scratch")
+        for name, kind in ((what, C.c_void_p), (what + "_len", u64))
+    ]
+
+
+class sage_cache_bounds(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("codes_len", u64), ("scales_len", u64)]
+
+
+class sage_pick_options(C.Structure):
+    _fields_ = [("first", u64), ("last", u64), ("causal", i32)]
 
 
 P = C.POINTER
@@ -207,6 +238,36 @@ SIGNATURES = {
         i32,
         [C.c_void_p, C.c_void_p, P(sage_cache), P(sage_cache_index), P(sage_tensor), P(sage_tensor_mut),
          P(sage_cache_options)],
+    ),
+    "sage_rotary_axes_table": (
+        i32, [P(u64), u64, i32, i32, u64, C.c_double, P(sage_rotary_scaling), C.c_void_p, u64],
+    ),
+    "sage_rotary_axes_apply": (
+        i32, [C.c_void_p, P(sage_shape), P(sage_rotary_axes), P(sage_tensor), P(sage_tensor_mut), i32],
+    ),
+    "sage_cache_append_axes": (
+        i32,
+        [C.c_void_p, P(sage_cache_shape), P(sage_cache), P(sage_cache_index), P(sage_tensor), P(sage_tensor),
+         P(sage_rotary_axes), P(sage_tensor), P(sage_tensor_mut)],
+    ),
+    "sage_cache_tables": (
+        i32, [C.c_void_p, P(sage_cache_shape), P(sage_cache_requests), P(sage_cache_free), P(sage_cache_step)],
+    ),
+    "sage_cache_bounds_update": (
+        i32, [C.c_void_p, P(sage_cache_shape), P(sage_cache), P(sage_cache_index), P(sage_cache_bounds)],
+    ),
+    "sage_pick_workspace_new": (i32, [C.c_void_p, P(sage_cache_shape), u64, P(C.c_void_p)]),
+    "sage_pick_workspace_destroy": (None, [C.c_void_p]),
+    "sage_pick_workspace_bytes": (u64, [C.c_void_p]),
+    "sage_cache_pick": (
+        i32,
+        [C.c_void_p, C.c_void_p, P(sage_cache_bounds), P(sage_cache_index), P(sage_tensor), C.c_void_p, u64,
+         P(sage_pick_options)],
+    ),
+    "sage_cache_attend_picked": (
+        i32,
+        [C.c_void_p, C.c_void_p, P(sage_cache), P(sage_cache_index), C.c_void_p, u64, P(sage_tensor),
+         P(sage_tensor_mut), P(sage_cache_options)],
     ),
     "sage_v8_position": (i32, [i32]),
     "sage_peak": (i32, [C.c_void_p, i32, i32, P(C.c_double)]),

@@ -1,7 +1,9 @@
 """spl_sage.cache -- a paged 4-bit key/value cache and the attention over it.
 
 The types of SageAttention.cache_append, cache_read, cache_workspace and
-cache_attend (sage_cache_* in include/sage_hip.h; no counterpart in the
+cache_attend, of cache_tables (a step's index from its requests' lengths), and of
+cache_bounds, cache_pick and cache_attend_picked (attention over the pages that
+each row picks; sage_cache_* in include/sage_hip.h; no counterpart in the
 reference). Q, K, V and outputs are [1][row][head][head_dim] views (Tensor,
 TensorMut): the sequences' rows packed one behind the other. Device buffers are
 torch tensors.
@@ -142,4 +144,164 @@ class CacheWorkspace:
         return lib().sage_cache_workspace_bytes(self._h)
 
 
-__all__ = ["BLOCK", "CacheShape", "PagedCache", "CacheIndex", "CacheWorkspace"]
+@dataclass(frozen=True)
+class FreePages:
+    """The free pages: an int32 ring of page ids and its state (the place of the
+    first, their number, and whatever follows: a CacheTables's state serves).
+    Made once for its tensors, whose contents change."""
+
+    pages: object
+    state: object
+
+    @staticmethod
+    def new(pages: int, device="cuda") -> "FreePages":
+        """All of a pool's pages, free."""
+        import torch
+
+        i = dict(dtype=torch.int32, device=device)
+        return FreePages(torch.arange(pages, **i), torch.tensor([0, pages, 0, 0], **i))
+
+    def __post_init__(self):
+        c = _abi.sage_cache_free(*_ints(self.pages, "free pages"), *_ints(self.state, "free pages' state"))
+        object.__setattr__(self, "_struct", c)
+        object.__setattr__(self, "_device", _device_of("the free pages", self.pages, self.state))
+
+
+@dataclass(frozen=True)
+class CacheTables:
+    """What cache_tables writes: int32 starts [batch + 1], lengths [batch],
+    page_table [batch][max_pages], positions and sequences [rows], state [4] (the
+    ring's first place and number, the pages missing, the rows too many), int64
+    slots [rows], and scratch [2 batch]. positions, slots and sequences may be
+    None. Made once for its tensors, whose contents change."""
+
+    shape: CacheShape
+    starts: object
+    lengths: object
+    page_table: object
+    positions: object
+    slots: object
+    sequences: object
+    state: object
+    scratch: object
+
+    @staticmethod
+    def new(shape: CacheShape, device="cuda", page_table=None, state=None) -> "CacheTables":
+        """Tensors of zeros, which torch's current stream fills; page_table and
+        state (a ring's, which then goes on from step to step) may be the caller's."""
+        import torch
+
+        def z(*n, dtype=torch.int32):
+            return torch.zeros(*n, dtype=dtype, device=device)
+
+        table = z(shape.batch, shape.max_pages) if page_table is None else page_table
+        return CacheTables(shape, z(shape.batch + 1), z(shape.batch), table, z(shape.rows),
+                           z(shape.rows, dtype=torch.int64), z(shape.rows), z(4) if state is None else state,
+                           z(2 * shape.batch))
+
+    def index(self) -> CacheIndex:
+        """The index of the step's other calls."""
+        return CacheIndex(self.starts, self.lengths, self.page_table)
+
+    def __post_init__(self):
+        import torch
+
+        def ints(t, what):
+            return (None, 0) if t is None else _ints(t, what)
+
+        slots = (None, 0)
+        if self.slots is not None:
+            if self.slots.dtype != torch.int64 or not self.slots.is_contiguous():
+                raise SageError(1, f"step slots must be a contiguous int64 device tensor, got {self.slots.dtype}")
+            slots = self.slots.data_ptr(), self.slots.numel()
+        t = self.page_table
+        if t.dim() == 2 and t.shape[1] != self.shape.max_pages and self.shape.batch > 1:
+            raise SageError(1, f"the page table has {t.shape[1]} columns, the shape {self.shape.max_pages}")
+        c = _abi.sage_cache_step(*_ints(self.starts, "cache starts"), *_ints(self.lengths, "cache lengths"),
+                                 *_ints(t, "cache page table"), *ints(self.positions, "step positions"), *slots,
+                                 *ints(self.sequences, "step sequences"), *_ints(self.state, "step state"),
+                                 *_ints(self.scratch, "step scratch"))
+        object.__setattr__(self, "_struct", c)
+        some = [x for x in (self.positions, self.slots, self.sequences) if x is not None]
+        object.__setattr__(self, "_device", _device_of("the step's tensors", self.starts, self.lengths, t, self.state,
+                                                       self.scratch, *some))
+
+
+@dataclass(frozen=True)
+class PageBounds:
+    """Bounds of a pool's keys: codes int8 [pages][kv_heads][2][head_dim] (greatest,
+    least) and scales uint8 [pages][kv_heads] on the device, of the shape's pages or
+    more. Made once for its tensors; as a PagedCache, it serves steps of any shape."""
+
+    shape: CacheShape
+    codes: object
+    scales: object
+
+    @staticmethod
+    def new(shape: CacheShape, head_dim: int, device="cuda") -> "PageBounds":
+        """Bounds of zeros, which torch's current stream fills."""
+        import torch
+
+        shape.sizes(head_dim)  # its refusals
+        dims = (shape.pages, shape.kv_heads)
+        return PageBounds(shape, torch.zeros(*dims, 2, head_dim, dtype=torch.int8, device=device),
+                          torch.zeros(*dims, dtype=torch.uint8, device=device))
+
+    def with_shape(self, shape: CacheShape) -> "PageBounds":
+        return PageBounds(shape, self.codes, self.scales)
+
+    def __post_init__(self):
+        import torch
+
+        if self.codes.dtype != torch.int8 or not self.codes.is_contiguous():
+            raise SageError(1, f"bounds codes must be a contiguous int8 device tensor, got {self.codes.dtype}")
+        scales = _bytes(self.scales, "bounds scales")
+        have, want = tuple(self.codes.shape), (self.shape.pages, self.shape.kv_heads, 2)
+        if self.codes.dim() == 4 and (have[0] < want[0] or have[1:3] != want[1:]):
+            raise SageError(1, f"bounds codes of {have} do not fit {want[0]} pages and {want[1]} KV heads")
+        c = _abi.sage_cache_bounds(self.codes.data_ptr(), scales[0], self.codes.numel(), scales[1])
+        object.__setattr__(self, "_struct", c)
+        object.__setattr__(self, "_head_dim", have[3] if self.codes.dim() == 4 else None)
+        object.__setattr__(self, "_device", _device_of("the bounds", self.codes, self.scales))
+
+
+@dataclass(frozen=True)
+class Picked:
+    """The picked columns, int32 [rows][kv_heads][top] on the device. Made once for
+    its tensor, whose contents change."""
+
+    columns: object
+
+    def __post_init__(self):
+        p, n = _ints(self.columns, "picked pages")
+        object.__setattr__(self, "_struct", (p, n))
+        object.__setattr__(self, "_device", self.columns.get_device())
+
+
+class PickWorkspace:
+    """What cache_pick and cache_attend_picked keep between their kernels, for one
+    shape and number of pages a row; one call at a time uses it."""
+
+    def __init__(self, sa, shape: CacheShape, top: int):
+        h = C.c_void_p()
+        _check(lib().sage_pick_workspace_new(sa._h, C.byref(shape._c()), max(top, 0), C.byref(h)))
+        self._h = h.value
+        self.shape = shape
+        self.top = top
+        # Bound now: at interpreter exit the module's globals may be gone before __del__ runs.
+        self._destroy = lib().sage_pick_workspace_destroy
+
+    def __del__(self):
+        h, self._h = getattr(self, "_h", None), None
+        destroy = getattr(self, "_destroy", None)
+        if h and destroy is not None:
+            destroy(h)
+
+    def bytes(self) -> int:
+        return lib().sage_pick_workspace_bytes(self._h)
+
+
+__all__ = [
+    "BLOCK", "CacheShape", "PagedCache", "CacheIndex", "CacheWorkspace", "FreePages", "CacheTables", "PageBounds",
+    "Picked", "PickWorkspace",
+]

@@ -1,9 +1,9 @@
-"""spl_sage.rotary -- rotary positions along a sequence.
+"""spl_sage.rotary -- rotary positions along a sequence, or on several axes.
 
 The tables and options of SageAttention.rotary and SageAttention.cache_append
-(sage_rotary_table, sage_rotary_apply in include/sage_hip.h; no counterpart in
-the reference, whose 2D tables are spl_sage.qkv's). Device buffers are torch
-tensors.
+(sage_rotary_table, sage_rotary_apply and their forms for several axes in
+include/sage_hip.h; no counterpart in the reference, whose 2D tables are
+spl_sage.qkv's). Device buffers are torch tensors.
 """
 from __future__ import annotations
 
@@ -64,6 +64,19 @@ class RotaryTable:
         _check(lib().sage_rotary_table(rot, positions, float(base), sc, out.ctypes.data, out.size))
         return RotaryTable(rot, positions, out)
 
+    @staticmethod
+    def axes(sections, positions: int, base: float = 10000.0, scaling: Optional[RotaryScaling] = None,
+             dealt: bool = False, per_axis: bool = False) -> "RotaryTable":
+        """The table of AxesRotary: sections pairs of each axis, whose frequencies
+        are the whole head's, or each axis's own (per_axis)."""
+        c = (C.c_uint64 * max(len(sections), 1))(*(max(n, 0) for n in sections))
+        rot = 2 * sum(c)
+        out = np.empty((max(positions, 0), rot // 2, 2), np.float32)
+        sc = None if scaling is None else C.byref(scaling._c())
+        _check(lib().sage_rotary_axes_table(c, len(sections), int(dealt), int(per_axis), positions, float(base), sc,
+                                            out.ctypes.data, out.size))
+        return RotaryTable(rot, positions, out)
+
     def upload(self, device="cuda"):
         import torch
 
@@ -86,6 +99,14 @@ def _device_of(what: str, *tensors) -> int:
     return tensors[0].get_device()
 
 
+def _floats(t, what: str) -> tuple:
+    import torch
+
+    if t.dtype != torch.float32 or not t.is_contiguous():
+        raise SageError(1, f"{what} must be a contiguous float32 device tensor, got {t.dtype}")
+    return t.data_ptr(), t.numel()
+
+
 @dataclass(frozen=True)
 class Rotary:
     """An uploaded RotaryTable with its layout, and the rows' positions (int32
@@ -97,16 +118,58 @@ class Rotary:
     layout: RotaryLayout = RotaryLayout.Half
     positions: object = None
 
-    def __post_init__(self):
-        import torch
+    APPLY, APPEND = "sage_rotary_apply", "sage_cache_append"  # the calls that take it
 
-        if self.table.dtype != torch.float32 or not self.table.is_contiguous():
-            raise SageError(1, f"the rotary table must be a contiguous float32 device tensor, got {self.table.dtype}")
+    def __post_init__(self):
+        t, m = _floats(self.table, "the rotary table")
         p, n = (None, 0) if self.positions is None else _ints(self.positions, "rotary positions")
-        c = _abi.sage_rotary(self.table.data_ptr(), self.table.numel(), self.rot, int(self.layout), p, n)
+        c = _abi.sage_rotary(t, m, self.rot, int(self.layout), p, n)
         object.__setattr__(self, "_struct", c)
         at = (self.table,) if self.positions is None else (self.table, self.positions)
         object.__setattr__(self, "_device", _device_of("the rotary table and positions", *at))
 
 
-__all__ = ["RotaryLayout", "ScalingKind", "RotaryScaling", "RotaryTable", "Rotary"]
+class AxisLayout(enum.IntEnum):
+    """Half rotates channels (i, i + rot / 2), Pairs (2 i, 2 i + 1), AxisHalf the
+    halves within each axis's channels."""
+
+    Half = 0
+    Pairs = 1
+    AxisHalf = 2
+
+
+@dataclass(frozen=True)
+class AxesRotary:
+    """Rotary positions with one to four axes, wherever a Rotary is taken: an
+    uploaded RotaryTable.axes, the pairs of each axis, and the rows' positions,
+    int32 [axes][rows] on the device (rows of it may be apart). dealt: the pairs
+    go to the axes in turn, else in runs. Made once for its tensors, whose contents may change."""
+
+    table: object
+    sections: tuple
+    positions: object
+    layout: AxisLayout = AxisLayout.Half
+    dealt: bool = False
+
+    APPLY, APPEND = "sage_rotary_axes_apply", "sage_cache_append_axes"  # the calls that take it
+
+    def __post_init__(self):
+        import torch
+
+        t, m = _floats(self.table, "the rotary table")
+        x = self.positions
+        if x.dtype != torch.int32 or x.dim() != 2 or x.shape[0] != len(self.sections) or (x.shape[1] > 1 and x.stride(1) != 1):
+            raise SageError(1, "rotary positions must be an int32 device tensor [axes][rows] with contiguous rows, got "
+                               f"{x.dtype} {tuple(x.shape)}")
+        if not 1 <= len(self.sections) <= 4:
+            raise SageError(1, f"rotary: {len(self.sections)} axes (1 to 4 are supported)")
+        rows, stride = x.shape[1], x.shape[1] if x.shape[0] == 1 else x.stride(0)
+        if x.shape[0] > 1 and stride < rows:
+            raise SageError(1, "the axes' rotary positions overlap")
+        c = _abi.sage_rotary_axes(t, m, (C.c_uint64 * 4)(*(max(n, 0) for n in self.sections)), len(self.sections),
+                                  int(self.layout), int(self.dealt), x.data_ptr(), (x.shape[0] - 1) * stride + rows, stride)
+        object.__setattr__(self, "_struct", c)
+        object.__setattr__(self, "_device", _device_of("the rotary table and positions", self.table, x))
+
+
+__all__ = ["RotaryLayout", "ScalingKind", "RotaryScaling", "RotaryTable", "Rotary", "AxisLayout", "AxesRotary"]
