@@ -17,6 +17,7 @@ namespace {
 typedef int i4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 
+constexpr int CHUNK_TILES = 4;  // of a wave's columns, in chunks of rows
 constexpr uint32_t SCALE_NAN = 255;
 constexpr uint32_t SCALE_MOST = 228;  // 2^21 * 2^(228 - 127) is an fp32 number
 
@@ -100,27 +101,32 @@ __global__ __launch_bounds__(256) void bounds_kernel(BoundsArgs a) {
 // ---- Scores ----
 //
 // A tile is 16 (row, head of the group) columns of one KV head; a row's heads
-// fill a power of two of them, `slots`, the last head again where the group is smaller
+// fill a power of two of them, 2^slots, the last head again where the group is smaller
 // (a maximum does not mind), so that a row's maximum over its heads stays in a lane's
 // four results or between lanes 16 and 32 apart. Groups over 16 take several
-// tiles of one row. Pages run along the lanes, 16 a step.
+// turns of one row. Pages run along the lanes, 16 a step.
 
-// Eight channels' codes, u = rint(x * up): max(u, 0) or, under `neg`, min(u, 0), a byte each.
-__device__ __forceinline__ uint2 codes_of(uint4 raw, bool f16, float up, bool neg) {
+// Eight channels' codes, a byte each: rint(x * up) of x kept within lo .. hi. The sum
+// with 1.5 * 2^23 has units of 1, so its low byte is the nearest whole number, ties to even.
+__device__ __forceinline__ uint2 codes_of(uint4 raw, bool f16, float up, float lo, float hi) {
     float f[8];
     unpack8(raw, f, f16);
-    uint32_t w[2] = {0, 0};
+    uint32_t w[2];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int u = (int)__builtin_rintf(f[i] * up), v = neg ? min(u, 0) : max(u, 0);
-        w[i / 4] |= (uint32_t)(v & 255) << (i % 4 * 8);
+    for (int i = 0; i < 2; i++) {
+        uint32_t u[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            u[k] = __float_as_uint(__builtin_fmaf(__builtin_amdgcn_fmed3f(f[4 * i + k], lo, hi), up, 12582912.0f));
+        w[i] = __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400) | __builtin_amdgcn_perm(u[3], u[2], 0x04000c0c);
     }
-    return make_uint2(w[0], w[1]);
+    return up == 0.0f ? make_uint2(0, 0) : make_uint2(w[0], w[1]);
 }
 
-// The greatest power of two 2^e, |e| <= 126, with top * 2^e <= 127 (top: fp32 bits, 0 or finite).
+// The greatest power of two 2^e, |e| <= 126, with top * 2^e <= 127 (top: fp32 bits); 0
+// where top is 0 or not finite.
 __device__ __forceinline__ float power_for(uint32_t top) {
-    if (top == 0) return 0.0f;
+    if (top == 0 || top >= 0x7f800000u) return 0.0f;
     int e;
     const float m = __builtin_frexpf(__uint_as_float(top), &e);
     e = m <= 127.0f / 128 ? 7 - e : 6 - e;
@@ -142,101 +148,314 @@ __device__ __forceinline__ uint32_t key_of(float score) {
     return (int)u < 0 ? ~u : u | 0x80000000u;
 }
 
-// TILES: column tiles of a wave, over which a page's bounds are loaded once.
-// Grid: x = KV heads, `parts` parts of the pages, row tiles; z = sequences.
-template <int D, int TILES>
-__global__ __launch_bounds__(256, 2) void score_kernel(PickArgs a, int slots, int parts) {
-    constexpr int KS = 2 * D / 64, RAW = D / 16;  // MFMA steps; loads of 8 channels a lane, D / 2 channels in all
-    const CacheDev& c = a.c;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int g = lane >> 4, n = lane & 15;
-    const int b = blockIdx.z, kvh = blockIdx.x % c.kv_heads, rest = blockIdx.x / c.kv_heads;
-    const int part = rest % parts, tile = rest / parts, tile_rows = 16 / slots * TILES, j0 = tile * tile_rows;
-    const SequenceIndex seq = sequence_index(c, b, a.max_new);
-    const int count = min(seq.n - j0, tile_rows);
-    if (count <= 0 || seq.start + j0 >= (long long)a.row0 + a.window || seq.start + j0 + count <= a.row0) return;
-    const int page_tokens = 1 << c.page_shift;
-    const int pages = (seq.limit(j0 + count - 1, a.causal) + page_tokens - 1) >> c.page_shift;
-    if (pages <= a.top) return;  // every page is picked
+constexpr float INF = __builtin_inff();
 
-    // Where this lane's results belong: rows j0 + ... of tile t, see below.
-    const int heads_tiles = (a.group + 15) / 16;
-    i4 q[TILES][KS];
-    auto load = [&](int t, int ht, auto each) {
-        const int j = j0 + t * (16 / slots) + n / slots;
-        const int head = kvh * a.group + min(ht * 16 + n % slots, a.group - 1);
-        const long long row = seq.start + j;
-        const bool have = j < seq.n && row >= 0 && row < c.rows;
-        const uint16_t* p = a.q.p + row * a.q.st + head * a.q.sh + (g & 1) * (D / 2);
+// What a wave holds of 16 pages: lane (page, quarter of its bounds' bytes).
+template <int D>
+struct PageStep {
+    i4 w[2 * D / 64];
+    uint32_t scale;
+    bool there;
+    __device__ __forceinline__ void load(const PickArgs& a, int kvh, int id) {
+        there = (unsigned)id < (unsigned)a.c.pages;
+        const long long cell = (long long)(there ? id : 0) * a.c.kv_heads + kvh;
+        const int8_t* at = a.bounds.codes + cell * (2 * D) + (threadIdx.x >> 4 & 3) * (D / 2);
 #pragma unroll
-        for (int i = 0; i < RAW; i++)
-            each(i, have ? *reinterpret_cast<const uint4*>(p + 8 * i) : make_uint4(0, 0, 0, 0));
-    };
-    float up[TILES];
-#pragma unroll
-    for (int t = 0; t < TILES; t++) {
-        uint32_t top = 0;
-        for (int ht = 0; ht < heads_tiles; ht++) load(t, ht, [&](int, uint4 x) { top = max(top, greatest(x, a.q_f16)); });
-        top = max(top, (uint32_t)__shfl_xor((int)top, 16));
-        for (int d = 1; d < slots; d *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d));
-        up[t] = top < 0x7f800000u ? power_for(top) : 0.0f;
+        for (int s = 0; s < 2 * D / 64; s++) w[s] = *reinterpret_cast<const i4*>(at + 16 * s);
+        scale = a.bounds.scales[cell];
     }
-    auto encode = [&](int t, int ht) {
-        load(t, ht, [&](int i, uint4 x) {
-            const uint2 w = up[t] == 0.0f ? make_uint2(0, 0) : codes_of(x, a.q_f16, up[t], g >= 2);
-            q[t][i / 2][i % 2 * 2] = (int)w.x;
-            q[t][i / 2][i % 2 * 2 + 1] = (int)w.y;
-        });
-    };
-    if (heads_tiles == 1)
-#pragma unroll
-        for (int t = 0; t < TILES; t++) encode(t, 0);
+};
 
-    for (int p0 = (part * 4 + wave) * 16; p0 < pages; p0 += parts * 64) {
-        const int col = p0 + n, id = col < pages ? c.page_table[(long long)b * c.max_pages + col] : -1;
-        const bool there = (unsigned)id < (unsigned)c.pages;
-        const long long cell = (long long)(there ? id : 0) * c.kv_heads + kvh;
-        const int8_t* at = a.bounds.codes + cell * (2 * D) + g * (D / 2);
-        i4 w[KS];
+// Pages first, first + step, ... (16 at a time) below `pages`, each step's on their
+// way while the one before is at work: the first are asked for when this is made.
+template <int D>
+struct PageWalk {
+    const int* table;
+    int first, step, pages, id;
+    PageStep<D> next;
+    __device__ __forceinline__ PageWalk(const PickArgs& a, int b, int kvh, int first_, int step_, int pages_)
+        : table(a.c.page_table + (long long)b * a.c.max_pages), first(first_), step(step_), pages(pages_) {
+        next.load(a, kvh, id_at(first));
+        id = id_at(first + step);
+    }
+    __device__ __forceinline__ int id_at(int p0) const {
+        const int col = p0 + (threadIdx.x & 15);
+        return col < pages ? table[col] : -1;
+    }
+    // The queries' codes against the pages: store(t, r, col, key) has the key of row t << (4 - slots) |
+    // (4 (lane / 16) + r) >> slots, where that is the row's first result.
+    template <int TILES, class Store>
+    __device__ __forceinline__ void run(const PickArgs& a, int kvh, int slots, const i4 (&q)[TILES][2 * D / 64],
+                                        Store store) {
+        const int g = threadIdx.x >> 4 & 3, n = threadIdx.x & 15;
+        for (int p0 = first; p0 < pages; p0 += step) {
+            const PageStep<D> now = next;
+            next.load(a, kvh, id);
+            id = id_at(p0 + 2 * step);
+            const int col = p0 + n;
+            const float unit = __uint_as_float(max(min(now.scale, SCALE_MOST), 1u) << 23);
 #pragma unroll
-        for (int s = 0; s < KS; s++) w[s] = *reinterpret_cast<const i4*>(at + 16 * s);
-        const uint32_t sc = min((uint32_t)a.bounds.scales[cell], SCALE_MOST);
-        const float unit = __uint_as_float(max(sc, 1u) << 23);
+            for (int t = 0; t < TILES; t++) {
+                i4 x{};
 #pragma unroll
-        for (int t = 0; t < TILES; t++) {
-            i4 x{};
-            for (int ht = 0; ht < heads_tiles; ht++) {
-                if (heads_tiles > 1) encode(t, ht);
-                i4 y{};
-#pragma unroll
-                for (int s = 0; s < KS; s++) y = __builtin_amdgcn_mfma_i32_16x16x64_i8(q[t][s], w[s], y, 0, 0, 0);
-#pragma unroll
-                for (int r = 0; r < 4; r++) x[r] = ht ? max(x[r], y[r]) : y[r];
-            }
-            // Result r is column 4 g + r: row (4 g + r) / slots of the tile.
-            if (slots >= 2) x[0] = max(x[0], x[1]), x[2] = max(x[2], x[3]);
-            if (slots >= 4) x[0] = max(x[0], x[2]);
-            if (slots >= 8) x[0] = max(x[0], __shfl_xor(x[0], 16));
-            if (slots >= 16) x[0] = max(x[0], __shfl_xor(x[0], 32));
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int j = j0 + t * (16 / slots) + (4 * g + r) / slots;
-                const long long row = seq.start + j;
-                if ((4 * g + r) % slots || j >= seq.n || col >= pages || row < a.row0 ||
-                    row >= (long long)a.row0 + a.window)
-                    continue;
-                a.keys[((row - a.row0) * c.kv_heads + kvh) * a.key_cols + col] = there ? key_of((float)x[r] * unit) : 1;
+                for (int s = 0; s < 2 * D / 64; s++)
+                    x = __builtin_amdgcn_mfma_i32_16x16x64_i8(q[t][s], now.w[s], x, 0, 0, 0);
+                // Result r is column 4 g + r.
+                if (slots >= 1) x[0] = max(x[0], x[1]), x[2] = max(x[2], x[3]);
+                if (slots >= 2) x[0] = max(x[0], x[2]);
+                if (slots >= 3) x[0] = max(x[0], __shfl_xor(x[0], 16));
+                if (slots >= 4) x[0] = max(x[0], __shfl_xor(x[0], 32));
+                if (col < pages) {
+                    auto key = [&](int r) { return now.there ? key_of((float)x[r] * unit) : 1u; };
+                    if (slots < 3 || (g & ((1 << slots) / 4 - 1)) == 0) store(t, 0, col, key(0));
+                    if (slots < 2) store(t, 2, col, key(2));
+                    if (slots < 1) store(t, 1, col, key(1)), store(t, 3, col, key(3));
+                }
             }
         }
+    }
+};
+
+// Where a tile's column n finds its query: the row's head of that place (from 16 * turn on).
+__device__ __forceinline__ const uint16_t* query_of(const PickArgs& a, const SequenceIndex& seq, int kvh, int j0, int n,
+                                                    int slots, int turn) {
+    const int j = j0 + (n >> slots), head = kvh * a.group + min(turn * 16 + (n & ((1 << slots) - 1)), a.group - 1);
+    const long long row = seq.start + j;
+    return j < seq.n && row >= 0 && row < a.c.rows ? a.q.p + row * a.q.st + head * a.q.sh : nullptr;
+}
+
+// A tile's codes in LDS, column by column: those of the channels above 0, which meet
+// the greatest keys, then those below.
+template <int D>
+struct TileLds {
+    static constexpr int STRIDE = 2 * D + 16;
+    uint32_t top[16];
+    alignas(16) uint8_t codes[16 * STRIDE];
+    __device__ __forceinline__ void put(int n, int part, uint4 raw, bool f16, float up) {
+        uint8_t* at = codes + n * STRIDE + 8 * part;
+        *reinterpret_cast<uint2*>(at) = codes_of(raw, f16, up, 0.0f, INF);
+        *reinterpret_cast<uint2*>(at + D) = codes_of(raw, f16, up, -INF, 0.0f);
+    }
+    __device__ __forceinline__ void get(i4 (&q)[2 * D / 64]) const {
+        const uint8_t* at = codes + (threadIdx.x & 15) * STRIDE + (threadIdx.x >> 4 & 3) * (D / 2);
+#pragma unroll
+        for (int s = 0; s < 2 * D / 64; s++) q[s] = *reinterpret_cast<const i4*>(at + 16 * s);
+    }
+};
+
+// By a wave for itself, eight channels a lane, a few columns at a time.
+template <int D>
+__device__ __forceinline__ void encode_tile(const PickArgs& a, const SequenceIndex& seq, int kvh, int j0, int slots,
+                                            TileLds<D>& lds, i4 (&q)[2 * D / 64]) {
+    constexpr int PARTS = D / 8, COLS = 64 / PARTS, TURNS = 16 / COLS;  // columns at a time
+    const int lane = threadIdx.x & 63, n = lane / PARTS, part = lane % PARTS;
+    uint4 raw[TURNS];
+    uint32_t top[TURNS];
+#pragma unroll
+    for (int i = 0; i < TURNS; i++) {
+        const uint16_t* p = query_of(a, seq, kvh, j0, i * COLS + n, slots, 0);
+        raw[i] = p ? *reinterpret_cast<const uint4*>(p + 8 * part) : make_uint4(0, 0, 0, 0);
+    }
+    // Over a column's channels and a row's columns.
+#pragma unroll
+    for (int i = 0; i < TURNS; i++) {
+        top[i] = greatest(raw[i], a.q_f16);
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2)
+            if (d < PARTS << slots) top[i] = max(top[i], (uint32_t)__shfl_xor((int)top[i], d));
+    }
+#pragma unroll
+    for (int d = 1; d < TURNS; d *= 2) {
+        if (1 << slots <= COLS * d) continue;
+        uint32_t other[TURNS];
+#pragma unroll
+        for (int i = 0; i < TURNS; i++) other[i] = top[i ^ d];
+#pragma unroll
+        for (int i = 0; i < TURNS; i++) top[i] = max(top[i], other[i]);
+    }
+    __builtin_amdgcn_wave_barrier();  // the tile before is read
+#pragma unroll
+    for (int i = 0; i < TURNS; i++) lds.put(i * COLS + n, part, raw[i], a.q_f16, power_for(top[i]));
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    lds.get(q);
+}
+
+// By a workgroup for all its waves, eight channels a thread.
+template <int D>
+__device__ __forceinline__ void encode_shared(const PickArgs& a, const SequenceIndex& seq, int kvh, int j0, int slots,
+                                              int turn, TileLds<D>& lds, i4 (&q)[2 * D / 64]) {
+    constexpr int PARTS = D / 8;
+    const int n = threadIdx.x / PARTS, part = threadIdx.x % PARTS, turns = (a.group + 15) / 16;
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (n < 16) {  // (whole waves)
+        uint32_t top = 0;
+        for (int i = 0; i < turns; i++) {
+            const uint16_t* p = query_of(a, seq, kvh, j0, n, slots, i);
+            const uint4 x = p ? *reinterpret_cast<const uint4*>(p + 8 * part) : make_uint4(0, 0, 0, 0);
+            if (i == turn) raw = x;
+            top = max(top, greatest(x, a.q_f16));
+        }
+#pragma unroll
+        for (int d = 1; d < PARTS; d *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+        if (part == 0) lds.top[n] = top;
+    }
+    __syncthreads();
+    if (n < 16) {
+        const int first = n >> slots << slots;
+        uint32_t top = 0;
+        for (int i = 0; i < 1 << slots; i++) top = max(top, lds.top[first + i]);
+        lds.put(n, part, raw, a.q_f16, power_for(top));
+    }
+    __syncthreads();
+    lds.get(q);
+}
+
+// Chunks of rows: TILES tiles of columns a wave, all waves of a workgroup over the
+// same pages. Grid: x = KV heads, `parts` parts of the pages, row tiles; z = sequences.
+template <int D, int TILES>
+__global__ __launch_bounds__(256, 2) void score_kernel(PickArgs a, int slots, int parts) {
+    const CacheDev& c = a.c;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = threadIdx.x >> 4 & 3;
+    const int b = blockIdx.z, kvh = blockIdx.x % c.kv_heads, rest = blockIdx.x / c.kv_heads;
+    const int part = rest % parts, tile = rest / parts, rows = TILES << (4 - slots), j0 = (tile * 4 + wave) * rows;
+    const SequenceIndex seq = sequence_index(c, b, a.max_new);
+    const int count = min(seq.n - j0, rows);
+    const long long row0 = seq.start + j0 - a.row0;  // within the window
+    if (count <= 0 || row0 >= a.window || row0 + count <= 0) return;
+    const int pages = (seq.limit(j0 + count - 1, a.causal) + (1 << c.page_shift) - 1) >> c.page_shift;
+    if (pages <= a.top) return;  // every page is picked
+    PageWalk<D> walk(a, b, kvh, part * 16, parts * 16, pages);
+    __shared__ TileLds<D> lds[4];
+    i4 q[TILES][2 * D / 64];
+#pragma unroll
+    for (int t = 0; t < TILES; t++)
+        encode_tile<D>(a, seq, kvh, j0 + (t << (4 - slots)), slots, lds[wave], q[t]);
+    walk.template run<TILES>(a, kvh, slots, q, [&](int t, int r, int col, uint32_t key) {
+        const int j = (t << (4 - slots)) + ((4 * g + r) >> slots);
+        const long long row = row0 + j;
+        if (j < count && row >= 0 && row < a.window) a.keys[(row * c.kv_heads + kvh) * a.key_cols + col] = key;
+    });
+}
+
+// One tile a workgroup, its waves over pages of their own; groups over 16 heads in
+// turns, of which each keeps the greater key.
+template <int D>
+__global__ __launch_bounds__(256, 2) void score_tile_kernel(PickArgs a, int slots, int parts) {
+    __shared__ TileLds<D> lds;
+    const CacheDev& c = a.c;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = threadIdx.x >> 4 & 3;
+    const int b = blockIdx.z, kvh = blockIdx.x % c.kv_heads, rest = blockIdx.x / c.kv_heads;
+    const int part = rest % parts, tile = rest / parts, rows = 16 >> slots, j0 = tile * rows;
+    const SequenceIndex seq = sequence_index(c, b, a.max_new);
+    const int count = min(seq.n - j0, rows);
+    const long long row0 = seq.start + j0 - a.row0;  // within the window
+    if (count <= 0 || row0 >= a.window || row0 + count <= 0) return;
+    const int pages = (seq.limit(j0 + count - 1, a.causal) + (1 << c.page_shift) - 1) >> c.page_shift;
+    if (pages <= a.top) return;  // every page is picked
+    for (int turn = 0; turn < (a.group + 15) / 16; turn++) {
+        PageWalk<D> walk(a, b, kvh, (part * 4 + wave) * 16, parts * 64, pages);
+        i4 q[1][2 * D / 64];
+        encode_shared<D>(a, seq, kvh, j0, slots, turn, lds, q[0]);
+        walk.template run<1>(a, kvh, slots, q, [&](int, int r, int col, uint32_t key) {
+            const int j = (4 * g + r) >> slots;
+            const long long row = row0 + j;
+            if (j >= count || row < 0 || row >= a.window) return;
+            uint32_t& at = a.keys[(row * c.kv_heads + kvh) * a.key_cols + col];
+            at = turn ? max(at, key) : key;
+        });
     }
 }
 
 // ---- The greatest ----
 //
-// The least key that is picked is found bit by bit: 32 counts at most of how many
-// of a row's keys, which stay in registers, reach it, over WAVES waves together;
-// then the keys above it, and of those equal to it the first ones, go out in the
-// columns' order. Grid: x = rows and KV heads, z = sequences.
+// The least key that is picked is found bit by bit: a count for each bit of how many
+// of a row's keys, which stay in registers, reach it, over WAVES waves together. Then the keys above it, and of those equal to it the
+// first ones, go out in the columns' order.
+struct Counts {
+    int* lds;  // [2][WAVES]
+    int turn;
+    // Sum over the waves, and over those before this one.
+    template <int WAVES>
+    __device__ __forceinline__ int total(int mine, int wave, int& before) {
+        before = 0;
+        if (WAVES == 1) return mine;
+        int* at = lds + turn * WAVES;
+        if ((threadIdx.x & 63) == 0) at[wave] = mine;
+        __syncthreads();
+        int sum = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+            const int x = at[w];
+            if (w < wave) before += x;
+            sum += x;
+        }
+        turn ^= 1;
+        return sum;
+    }
+};
+
+// Bits set in any of the wave's values.
+__device__ __forceinline__ uint32_t any_bits(uint32_t v) {
+#pragma unroll
+    for (int d = 32; d; d /= 2) v |= (uint32_t)__shfl_xor((int)v, d);
+    return __builtin_amdgcn_readfirstlane(v);
+}
+
+// key[i]: of column (wave * KEYS + i) * 64 + lane, more than top of them over 0.
+template <int WAVES, int KEYS>
+__device__ __forceinline__ void write_greatest(const uint32_t (&key)[KEYS], int top, int wave, int* out, int* lds) {
+    const int lane = threadIdx.x & 63;
+    Counts counts{lds, 0};
+    int before;
+    uint32_t least = 0;
+    int bit = 31, end = 0;
+    if (WAVES == 1) {
+        // Below the lowest bit that any key has, none is worth a count.
+        uint32_t any = 0;
+#pragma unroll
+        for (int i = 0; i < KEYS; i++)
+            if (key[i] != 0xffffffffu) any |= key[i];
+        any = any_bits(any);
+        end = any ? __builtin_ctz(any) : 0;
+    }
+    for (; bit >= end; bit--) {
+        const uint32_t t = least | 1u << bit;
+        int mine = 0;
+#pragma unroll
+        for (int i = 0; i < KEYS; i++) mine += __builtin_popcountll(__ballot(key[i] >= t));
+        const int sum = counts.total<WAVES>(mine, wave, before);
+        if (sum >= top) least = t;
+        if (sum == top) break;
+    }
+    int above = 0, equal = 0, above_before, equal_before;
+#pragma unroll
+    for (int i = 0; i < KEYS; i++) {
+        above += __builtin_popcountll(__ballot(key[i] > least));
+        equal += __builtin_popcountll(__ballot(key[i] == least));
+    }
+    const int room = top - counts.total<WAVES>(above, wave, above_before);  // of the keys equal to the least
+    counts.total<WAVES>(equal, wave, equal_before);
+    const uint64_t lower = (1ull << lane) - 1;
+    int seen = equal_before, place = above_before + min(equal_before, room);
+#pragma unroll
+    for (int i = 0; i < KEYS; i++) {
+        const uint64_t eq = __ballot(key[i] == least);
+        const bool in = key[i] > least || (key[i] == least && seen + __builtin_popcountll(eq & lower) < room);
+        const uint64_t ins = __ballot(in);
+        if (in) out[place + __builtin_popcountll(ins & lower)] = (wave * KEYS + i) * 64 + lane;
+        place += __builtin_popcountll(ins);
+        seen += __builtin_popcountll(eq);
+    }
+}
+
+// A row's list where all its pages are picked.
+__device__ __forceinline__ void write_all(int* out, int pages, int top, int first, int step) {
+    for (int i = first; i < top; i += step) out[i] = i < pages ? i : -1;
+}
+
+// From the keys in memory. Grid: x = rows and KV heads, z = sequences.
 template <int WAVES, int KEYS>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void pick_kernel(PickArgs a) {
     const CacheDev& c = a.c;
@@ -249,10 +468,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void pick_kernel(Pic
     if (j >= seq.n || row < a.row0 || row >= (long long)a.row0 + a.window) return;
     const int pages = (seq.limit(j, a.causal) + (1 << c.page_shift) - 1) >> c.page_shift;
     int* out = a.picked + (row * c.kv_heads + kvh) * a.top;
-    if (pages <= a.top) {
-        for (int i = WAVES == 1 ? lane : (int)threadIdx.x; i < a.top; i += WAVES * 64) out[i] = i < pages ? i : -1;
-        return;
-    }
+    if (pages <= a.top) return write_all(out, pages, a.top, WAVES == 1 ? lane : (int)threadIdx.x, WAVES * 64);
     const uint32_t* keys = a.keys + ((row - a.row0) * c.kv_heads + kvh) * a.key_cols;
     uint32_t key[KEYS];
 #pragma unroll
@@ -260,53 +476,49 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void pick_kernel(Pic
         const int col = (wave * KEYS + i) * 64 + lane;
         key[i] = col >= pages ? 0 : col < a.first || col >= pages - a.last ? 0xffffffffu : keys[col];
     }
-    __shared__ int counts[2][WAVES];
-    int turn = 0;
-    // Sum over the waves, and over those before this one.
-    auto total = [&](int mine, int& before) {
-        before = 0;
-        if (WAVES == 1) return mine;
-        if (lane == 0) counts[turn][wave] = mine;
-        __syncthreads();
-        int sum = 0;
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) {
-            const int x = counts[turn][w];
-            if (w < wave) before += x;
-            sum += x;
+    __shared__ int lds[2 * WAVES];
+    write_greatest<WAVES, KEYS>(key, a.top, wave, out, lds);
+}
+
+// Steps whose rows fit one tile, and whose keys LDS: both in one launch, a workgroup of
+// eight waves a (sequence, KV head), a wave a row in the end.
+template <int D, int KEYS>
+__global__ __launch_bounds__(512, 2) void step_pick_kernel(PickArgs a, int slots) {
+    extern __shared__ uint32_t step_keys[];  // [rows][KEYS * 64]
+    const CacheDev& c = a.c;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
+    const int b = blockIdx.z, kvh = blockIdx.x;
+    const SequenceIndex seq = sequence_index(c, b, a.max_new);
+    if (seq.n == 0) return;
+    auto pages_of = [&](int j) { return (seq.limit(j, a.causal) + (1 << c.page_shift) - 1) >> c.page_shift; };
+    const int pages = pages_of(seq.n - 1);
+    if (pages > a.top) {
+        __shared__ TileLds<D> lds;
+        PageWalk<D> walk(a, b, kvh, wave * 16, 128, pages);
+        i4 q[1][2 * D / 64];
+        encode_shared<D>(a, seq, kvh, 0, slots, 0, lds, q[0]);
+        walk.template run<1>(a, kvh, slots, q, [&](int, int r, int col, uint32_t key) {
+            const int j = (4 * g + r) >> slots;
+            if (j < seq.n) step_keys[j * (KEYS * 64) + col] = key;
+        });
+    }
+    __syncthreads();
+    for (int j = wave; j < seq.n; j += 8) {
+        const long long row = seq.start + j;
+        if (row < 0 || row >= c.rows) continue;
+        const int mine = pages_of(j);
+        int* out = a.picked + (row * c.kv_heads + kvh) * a.top;
+        if (mine <= a.top) {
+            write_all(out, mine, a.top, lane, 64);
+            continue;
         }
-        turn ^= 1;
-        return sum;
-    };
-    int before;
-    uint32_t least = 0;
-    for (int bit = 31; bit >= 0; bit--) {
-        const uint32_t t = least | 1u << bit;
-        int mine = 0;
+        uint32_t key[KEYS];
 #pragma unroll
-        for (int i = 0; i < KEYS; i++) mine += __builtin_popcountll(__ballot(key[i] >= t));
-        const int sum = total(mine, before);
-        if (sum >= a.top) least = t;
-        if (sum == a.top) break;
-    }
-    int above = 0, equal = 0, above_before, equal_before;
-#pragma unroll
-    for (int i = 0; i < KEYS; i++) {
-        above += __builtin_popcountll(__ballot(key[i] > least));
-        equal += __builtin_popcountll(__ballot(key[i] == least));
-    }
-    const int room = a.top - total(above, above_before);  // of the keys equal to the least
-    total(equal, equal_before);
-    const uint64_t lower = (1ull << lane) - 1;
-    int seen = equal_before, place = above_before + min(equal_before, room);
-#pragma unroll
-    for (int i = 0; i < KEYS; i++) {
-        const uint64_t eq = __ballot(key[i] == least);
-        const bool in = key[i] > least || (key[i] == least && seen + __builtin_popcountll(eq & lower) < room);
-        const uint64_t ins = __ballot(in);
-        if (in) out[place + __builtin_popcountll(ins & lower)] = (wave * KEYS + i) * 64 + lane;
-        place += __builtin_popcountll(ins);
-        seen += __builtin_popcountll(eq);
+        for (int i = 0; i < KEYS; i++) {
+            const int col = i * 64 + lane;
+            key[i] = col >= mine ? 0 : col < a.first || col >= mine - a.last ? 0xffffffffu : step_keys[j * (KEYS * 64) + col];
+        }
+        write_greatest<1, KEYS>(key, a.top, 0, out, nullptr);
     }
 }
 
@@ -327,25 +539,53 @@ int pick_window(int rows, int kv_heads, int max_pages) {
     return (int)std::min<long long>(rows, std::max(1ll, most / ((long long)kv_heads * max_pages)));
 }
 
+// Columns of a tile that a row takes, as a power of two.
+static int slots_of(int group) {
+    int slots = 0;
+    while (slots < 4 && 1 << slots < group) slots++;
+    return slots;
+}
+
 template <int D>
 static void score(const PickArgs& a, hipStream_t s) {
-    int slots = 1;
-    while (slots < 16 && slots < a.group) slots *= 2;
-    const auto go = [&](auto kernel, int tiles) {
-        const long long rows = 16 / slots * tiles, row_tiles = (a.max_new + rows - 1) / rows;
-        const long long units = row_tiles * a.c.kv_heads * a.c.batch;
-        const long long parts = std::max(1ll, std::min<long long>(1024 / units, (a.c.max_pages + 63) / 64));
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(row_tiles * parts * a.c.kv_heads), 1, a.c.batch), dim3(256), 0, s, a,
-                           slots, (int)parts);
+    const int slots = slots_of(a.group);
+    const bool chunks = a.group <= 16 && (long long)a.max_new << slots > 16;
+    const long long rows = (chunks ? 4 * CHUNK_TILES : 1) << (4 - slots), row_tiles = (a.max_new + rows - 1) / rows;
+    const long long units = row_tiles * a.c.kv_heads * a.c.batch, most = chunks ? 512 : 1024, each = chunks ? 64 : 64;
+    const int parts = (int)std::max(1ll, std::min(most / units, (a.c.max_pages + each - 1) / each));
+    hipLaunchKernelGGL((chunks ? score_kernel<D, CHUNK_TILES> : score_tile_kernel<D>),
+                       dim3((unsigned)(row_tiles * parts * a.c.kv_heads), 1, a.c.batch), dim3(256), 0, s, a, slots, parts);
+}
+
+// Whether one launch serves the call.
+static bool in_one_step(const PickArgs& a) {
+    const long long rows = a.max_new, units = (long long)a.c.kv_heads * a.c.batch;
+    return a.group <= 16 && rows << slots_of(a.group) <= 16 && a.c.max_pages <= 2048 && (units >= 128 || a.c.max_pages <= 512) &&
+           rows * ((a.c.max_pages + 63) / 64) <= 128;
+}
+
+template <int D>
+static void step_pick(const PickArgs& a, hipStream_t s) {
+    const auto go = [&](auto kernel, int keys) {
+        hipLaunchKernelGGL(kernel, dim3(a.c.kv_heads, 1, a.c.batch), dim3(512), a.max_new * keys * 256, s, a,
+                           slots_of(a.group));
     };
-    if (a.max_new * slots <= 16 || a.group > 16)
-        go(score_kernel<D, 1>, 1);
+    if (a.c.max_pages <= 256)
+        go(step_pick_kernel<D, 4>, 4);
+    else if (a.c.max_pages <= 512)
+        go(step_pick_kernel<D, 8>, 8);
+    else if (a.c.max_pages <= 1024)
+        go(step_pick_kernel<D, 16>, 16);
     else
-        go(score_kernel<D, 4>, 4);
+        go(step_pick_kernel<D, 32>, 32);
 }
 
 hipError_t launch_cache_pick(int head_dim, const PickArgs& a_, hipStream_t s) {
     PickArgs a = a_;
+    if (in_one_step(a)) {
+        head_dim == 64 ? step_pick<64>(a, s) : step_pick<128>(a, s);
+        return hipGetLastError();
+    }
     const int window = a.window;
     for (a.row0 = 0; a.row0 < a.c.rows; a.row0 += window) {
         a.window = std::min(window, a.c.rows - a.row0);
@@ -357,6 +597,8 @@ hipError_t launch_cache_pick(int head_dim, const PickArgs& a_, hipStream_t s) {
         };
         if (a.c.max_pages <= 256)
             pick(pick_kernel<1, 4>, 1);
+        else if (a.c.max_pages <= 512)
+            pick(pick_kernel<1, 8>, 1);
         else if (a.c.max_pages <= 1024)
             pick(pick_kernel<1, 16>, 1);
         else if (a.c.max_pages <= 4096)
