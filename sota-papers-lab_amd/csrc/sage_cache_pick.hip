@@ -396,31 +396,15 @@ struct Counts {
     }
 };
 
-// Bits set in any of the wave's values.
-__device__ __forceinline__ uint32_t any_bits(uint32_t v) {
-#pragma unroll
-    for (int d = 32; d; d /= 2) v |= (uint32_t)__shfl_xor((int)v, d);
-    return __builtin_amdgcn_readfirstlane(v);
-}
-
-// key[i]: of column (wave * KEYS + i) * 64 + lane, more than top of them over 0.
-template <int WAVES, int KEYS>
-__device__ __forceinline__ void write_greatest(const uint32_t (&key)[KEYS], int top, int wave, int* out, int* lds) {
+// The list from a row's keys, all more than 0 of which are more than top: key[i] is of
+// the i-th of the wave's columns that col(i) gives, in their order.
+template <int WAVES, int KEYS, class Col>
+__device__ __forceinline__ void write_greatest(const uint32_t (&key)[KEYS], int top, int wave, int* out, int* lds, Col col) {
     const int lane = threadIdx.x & 63;
     Counts counts{lds, 0};
     int before;
     uint32_t least = 0;
-    int bit = 31, end = 0;
-    if (WAVES == 1) {
-        // Below the lowest bit that any key has, none is worth a count.
-        uint32_t any = 0;
-#pragma unroll
-        for (int i = 0; i < KEYS; i++)
-            if (key[i] != 0xffffffffu) any |= key[i];
-        any = any_bits(any);
-        end = any ? __builtin_ctz(any) : 0;
-    }
-    for (; bit >= end; bit--) {
+    for (int bit = 31; bit >= 0; bit--) {
         const uint32_t t = least | 1u << bit;
         int mine = 0;
 #pragma unroll
@@ -444,10 +428,58 @@ __device__ __forceinline__ void write_greatest(const uint32_t (&key)[KEYS], int 
         const uint64_t eq = __ballot(key[i] == least);
         const bool in = key[i] > least || (key[i] == least && seen + __builtin_popcountll(eq & lower) < room);
         const uint64_t ins = __ballot(in);
-        if (in) out[place + __builtin_popcountll(ins & lower)] = (wave * KEYS + i) * 64 + lane;
+        if (in) out[place + __builtin_popcountll(ins & lower)] = col(i);
         place += __builtin_popcountll(ins);
         seen += __builtin_popcountll(eq);
     }
+}
+
+// A wave's writes to LDS before its reads behind this.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// A row's list by one wave; key[i]: of column i * 64 + lane. For lists of at most
+// 64, the top-th greatest of the lanes' greatest keys is no more than the list's least, and
+// few keys reach it: the counts go over those, two a lane (954 columns, a list of 32:
+// PICKED_FEW). `few`: LDS of the wave.
+struct Few {
+    uint32_t key[128];
+    int col[128];
+};
+template <int KEYS>
+__device__ __forceinline__ void write_greatest_of_wave(const uint32_t (&key)[KEYS], int top, int* out, Few& few) {
+    const int lane = threadIdx.x & 63;
+    auto plain = [&] { write_greatest<1, KEYS>(key, top, 0, out, nullptr, [&](int i) { return i * 64 + lane; }); };
+    if (KEYS <= 2 || top > 64) return plain();
+    uint32_t most = 0, bound = 0;
+#pragma unroll
+    for (int i = 0; i < KEYS; i++) most = max(most, key[i]);
+    for (int bit = 31; bit >= 0; bit--) {
+        const uint32_t t = bound | 1u << bit;
+        const int sum = __builtin_popcountll(__ballot(most >= t));
+        if (sum >= top) bound = t;
+        if (sum == top) break;
+    }
+    const uint64_t lower = (1ull << lane) - 1;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < KEYS; i++) n += __builtin_popcountll(__ballot(key[i] >= bound));
+    if (n > 128) return plain();
+    wave_sync();  // the row before is read
+    n = 0;
+#pragma unroll
+    for (int i = 0; i < KEYS; i++) {
+        const uint64_t in = __ballot(key[i] >= bound);
+        const int at = n + __builtin_popcountll(in & lower);
+        if (key[i] >= bound) few.key[at] = key[i], few.col[at] = i * 64 + lane;
+        n += __builtin_popcountll(in);
+    }
+    wave_sync();
+    const uint32_t two[2] = {lane < n ? few.key[lane] : 0, 64 + lane < n ? few.key[64 + lane] : 0};
+    write_greatest<1, 2>(two, top, 0, out, nullptr, [&](int i) { return few.col[i * 64 + lane]; });
 }
 
 // A row's list where all its pages are picked.
@@ -476,35 +508,52 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void pick_kernel(Pic
         const int col = (wave * KEYS + i) * 64 + lane;
         key[i] = col >= pages ? 0 : col < a.first || col >= pages - a.last ? 0xffffffffu : keys[col];
     }
-    __shared__ int lds[2 * WAVES];
-    write_greatest<WAVES, KEYS>(key, a.top, wave, out, lds);
+    if constexpr (WAVES == 1) {
+        __shared__ Few few[4];
+        write_greatest_of_wave<KEYS>(key, a.top, out, few[wave_id]);
+    } else {
+        __shared__ int lds[2 * WAVES];
+        write_greatest<WAVES, KEYS>(key, a.top, wave, out, lds, [&](int i) { return (wave * KEYS + i) * 64 + lane; });
+    }
 }
 
-// Steps whose rows fit one tile, and whose keys LDS: both in one launch, a workgroup of
-// eight waves a (sequence, KV head), a wave a row in the end.
-template <int D, int KEYS>
-__global__ __launch_bounds__(512, 2) void step_pick_kernel(PickArgs a, int slots) {
-    extern __shared__ uint32_t step_keys[];  // [rows][KEYS * 64]
+// Rows whose keys fit LDS: both in one launch, eight waves over the pages of TILES
+// tiles of rows, then over the rows. Grid: x = KV heads, row tiles; z = sequences.
+template <int D, int TILES, int KEYS>
+__global__ __launch_bounds__(512, TILES == 1 ? 2 : 4) void row_pick_kernel(PickArgs a, int slots) {
+    extern __shared__ uint32_t row_keys[];  // [rows][key_cols]
+    __shared__ union {
+        TileLds<D> tile[TILES];
+        Few few[8];
+    } lds;
     const CacheDev& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
-    const int b = blockIdx.z, kvh = blockIdx.x;
+    const int b = blockIdx.z, kvh = blockIdx.x % c.kv_heads, rows = TILES << (4 - slots);
+    const int j0 = blockIdx.x / c.kv_heads * rows;
     const SequenceIndex seq = sequence_index(c, b, a.max_new);
-    if (seq.n == 0) return;
-    auto pages_of = [&](int j) { return (seq.limit(j, a.causal) + (1 << c.page_shift) - 1) >> c.page_shift; };
-    const int pages = pages_of(seq.n - 1);
+    const int count = min(seq.n - j0, rows);
+    if (count <= 0) return;
+    auto pages_of = [&](int j) { return (seq.limit(j0 + j, a.causal) + (1 << c.page_shift) - 1) >> c.page_shift; };
+    const int pages = pages_of(count - 1);
     if (pages > a.top) {
-        __shared__ TileLds<D> lds;
         PageWalk<D> walk(a, b, kvh, wave * 16, 128, pages);
-        i4 q[1][2 * D / 64];
-        encode_shared<D>(a, seq, kvh, 0, slots, 0, lds, q[0]);
-        walk.template run<1>(a, kvh, slots, q, [&](int, int r, int col, uint32_t key) {
-            const int j = (4 * g + r) >> slots;
-            if (j < seq.n) step_keys[j * (KEYS * 64) + col] = key;
+        i4 q[TILES][2 * D / 64];
+        if constexpr (TILES == 1) {
+            encode_shared<D>(a, seq, kvh, j0, slots, 0, lds.tile[0], q[0]);
+        } else {
+            if (wave < TILES) encode_tile<D>(a, seq, kvh, j0 + (wave << (4 - slots)), slots, lds.tile[wave], q[0]);
+            __syncthreads();
+#pragma unroll
+            for (int t = 0; t < TILES; t++) lds.tile[t].get(q[t]);
+        }
+        walk.template run<TILES>(a, kvh, slots, q, [&](int t, int r, int col, uint32_t key) {
+            const int j = (t << (4 - slots)) + ((4 * g + r) >> slots);
+            if (j < count) row_keys[j * a.key_cols + col] = key;
         });
     }
-    __syncthreads();
-    for (int j = wave; j < seq.n; j += 8) {
-        const long long row = seq.start + j;
+    __syncthreads();  // (the tiles are read, too)
+    for (int j = wave; j < count; j += 8) {
+        const long long row = seq.start + j0 + j;
         if (row < 0 || row >= c.rows) continue;
         const int mine = pages_of(j);
         int* out = a.picked + (row * c.kv_heads + kvh) * a.top;
@@ -516,9 +565,9 @@ __global__ __launch_bounds__(512, 2) void step_pick_kernel(PickArgs a, int slots
 #pragma unroll
         for (int i = 0; i < KEYS; i++) {
             const int col = i * 64 + lane;
-            key[i] = col >= mine ? 0 : col < a.first || col >= mine - a.last ? 0xffffffffu : step_keys[j * (KEYS * 64) + col];
+            key[i] = col >= mine ? 0 : col < a.first || col >= mine - a.last ? 0xffffffffu : row_keys[j * a.key_cols + col];
         }
-        write_greatest<1, KEYS>(key, a.top, 0, out, nullptr);
+        write_greatest_of_wave<KEYS>(key, a.top, out, lds.few[wave]);
     }
 }
 
@@ -557,35 +606,49 @@ static void score(const PickArgs& a, hipStream_t s) {
                        dim3((unsigned)(row_tiles * parts * a.c.kv_heads), 1, a.c.batch), dim3(256), 0, s, a, slots, parts);
 }
 
-// Whether one launch serves the call.
-static bool in_one_step(const PickArgs& a) {
-    const long long rows = a.max_new, units = (long long)a.c.kv_heads * a.c.batch;
-    return a.group <= 16 && rows << slots_of(a.group) <= 16 && a.c.max_pages <= 2048 && (units >= 128 || a.c.max_pages <= 512) &&
-           rows * ((a.c.max_pages + 63) / 64) <= 128;
+// One launch, where the keys of a workgroup's rows fit 64 KB of LDS and there are
+// workgroups enough, or few pages; the tiles of a workgroup, or 0.
+static int tiles_in_one(const PickArgs& a, int keys) {
+    const int slots = slots_of(a.group);
+    if (a.group > 16 || a.c.max_pages > keys * 64) return 0;
+    for (int tiles = 4; tiles; tiles /= 2) {
+        const int rows = tiles << (4 - slots);
+        if (tiles > 1 && rows / 2 >= a.max_new) continue;  // half the tiles hold them
+        if (std::min(rows, a.max_new) * a.c.max_pages > 1 << 14) continue;
+        const long long units = ((long long)a.max_new + rows - 1) / rows * a.c.kv_heads * a.c.batch;
+        return units >= 128 || a.c.max_pages <= 512 ? tiles : 0;
+    }
+    return 0;
+}
+
+template <int D, int KEYS>
+static bool row_pick(const PickArgs& a, hipStream_t s) {
+    const int tiles = tiles_in_one(a, KEYS), slots = slots_of(a.group), rows = tiles << (4 - slots);
+    if (!tiles) return false;
+    const auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((a.max_new + rows - 1) / rows * a.c.kv_heads), 1, a.c.batch), dim3(512),
+                           std::min(rows, a.max_new) * a.c.max_pages * 4, s, a, slots);
+    };
+    if (tiles == 4)
+        go(row_pick_kernel<D, 4, KEYS>);
+    else if (tiles == 2)
+        go(row_pick_kernel<D, 2, KEYS>);
+    else
+        go(row_pick_kernel<D, 1, KEYS>);
+    return true;
 }
 
 template <int D>
-static void step_pick(const PickArgs& a, hipStream_t s) {
-    const auto go = [&](auto kernel, int keys) {
-        hipLaunchKernelGGL(kernel, dim3(a.c.kv_heads, 1, a.c.batch), dim3(512), a.max_new * keys * 256, s, a,
-                           slots_of(a.group));
-    };
-    if (a.c.max_pages <= 256)
-        go(step_pick_kernel<D, 4>, 4);
-    else if (a.c.max_pages <= 512)
-        go(step_pick_kernel<D, 8>, 8);
-    else if (a.c.max_pages <= 1024)
-        go(step_pick_kernel<D, 16>, 16);
-    else
-        go(step_pick_kernel<D, 32>, 32);
+static bool rows_in_one(const PickArgs& a, hipStream_t s) {
+    if (a.c.max_pages <= 256) return row_pick<D, 4>(a, s);
+    if (a.c.max_pages <= 512) return row_pick<D, 8>(a, s);
+    if (a.c.max_pages <= 1024) return row_pick<D, 16>(a, s);
+    return row_pick<D, 32>(a, s);
 }
 
 hipError_t launch_cache_pick(int head_dim, const PickArgs& a_, hipStream_t s) {
     PickArgs a = a_;
-    if (in_one_step(a)) {
-        head_dim == 64 ? step_pick<64>(a, s) : step_pick<128>(a, s);
-        return hipGetLastError();
-    }
+    if (head_dim == 64 ? rows_in_one<64>(a, s) : rows_in_one<128>(a, s)) return hipGetLastError();
     const int window = a.window;
     for (a.row0 = 0; a.row0 < a.c.rows; a.row0 += window) {
         a.window = std::min(window, a.c.rows - a.row0);
