@@ -21,81 +21,182 @@ constexpr int CHUNK_TILES = 4;  // of a wave's columns, in chunks of rows
 constexpr uint32_t SCALE_NAN = 255;
 constexpr uint32_t SCALE_MOST = 228;  // 2^21 * 2^(228 - 127) is an fp32 number
 
+// The greatest of a wave's values.
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false));   // lane ^ 1
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false));   // lane ^ 2
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, false));  // the other quad of 8
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, false));  // the other 8 of 16
+    auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(r[0], r[1]);
+    r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return __builtin_amdgcn_readfirstlane(max(r[0], r[1]));
+}
+
 // ---- Bounds ----
 //
-// A wave a (page, KV head): the greatest scale byte first, then the codes as fp16
+// A wave takes a page's KV heads one by one, `heads` of them, each head's bytes on
+// their way while the one before is at work: a lane has 16 channels of every
+// TOK-th token. With the greatest scale byte known, the codes become fp16
 // sixteenths of that scale (exact: 96 at most, what is under 2^-20 of the scale
-// counts as if it were that much), of which two take part in one maximum or minimum.
+// counts as if it were that much), of which two take part in one maximum or
+// minimum. The VALU bounds it, so the lanes' meet by halves: of two registers, each
+// half of the lanes goes on with one.
 // Reads 17/32 of a byte a key's channel and writes two a page's.
+constexpr int BOUNDS_LOADS = 8;  // of a lane at a time: pages of 64 tokens (head dim 64: 128) at once
+
+constexpr uint32_t H2_INF = 0x7c007c00u, H2_SIGNS = 0x80008000u;
+__device__ __forceinline__ uint32_t pk_max(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(h2, a), __builtin_bit_cast(h2, b)));
+}
+__device__ __forceinline__ uint32_t pk_min(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(h2, a), __builtin_bit_cast(h2, b)));
+}
+
 template <int D>
-__global__ __launch_bounds__(256) void bounds_kernel(BoundsArgs a) {
-    constexpr int G = D / CACHE_BLOCK, LANES = D / 16, TOK = 64 / LANES;  // lanes a token (16 channels each), tokens a load
+struct BoundsPart {
+    static constexpr int G = D / CACHE_BLOCK, LANES = D / 16, TOK = 64 / LANES;  // lanes a token, tokens a load
+    uint2 w[BOUNDS_LOADS];
+    uint32_t sc[BOUNDS_LOADS];
+    // Tokens t0 .. of a page and head of code row `row`, `held` of which hold something;
+    // the others count as the last of them.
+    __device__ __forceinline__ void load(const CacheDev& c, long long row, int t0, int held) {
+        const int lane = threadIdx.x & 63, part = lane % LANES;
+        const uint8_t* codes = c.k_codes + row * (D / 2);
+        const uint8_t* scales = c.k_scales + row * G;
+#pragma unroll
+        for (int i = 0; i < BOUNDS_LOADS; i++) {
+            if (t0 + i * TOK >= held) break;
+            const uint32_t t = min(t0 + i * TOK + lane / LANES, held - 1);
+            w[i] = *reinterpret_cast<const uint2*>(codes + t * (uint32_t)(D / 2) + part * 8);
+            sc[i] = scales[t * (uint32_t)G + part / 2];
+        }
+    }
+    // The greatest scale byte, and whether any block is NaN.
+    __device__ __forceinline__ uint32_t top(int t0, int held, bool& nan) const {
+        uint32_t top = 1, most = 0;
+#pragma unroll
+        for (int i = 0; i < BOUNDS_LOADS; i++) {
+            if (t0 + i * TOK >= held) break;
+            most = max(most, sc[i]);
+            top = max(top, sc[i] == SCALE_NAN ? 0u : sc[i]);
+        }
+        nan = nan || __any(most == SCALE_NAN);
+        return top;
+    }
+    __device__ __forceinline__ void take(int t0, int held, uint32_t top, bool nan, uint32_t (&hi)[8], uint32_t (&lo)[8]) const {
+#pragma unroll
+        for (int i = 0; i < BOUNDS_LOADS; i++) {
+            if (t0 + i * TOK >= held) break;
+            const float s = __uint_as_float((uint32_t)(127 + max((int)sc[i] - (int)top + 4, -20)) << 23);
+            const uint2 c = w[i];
+            const h2 x[8] = {
+                __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.x, s, 0), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.x, s, 1),
+                __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.x, s, 2), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.x, s, 3),
+                __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.y, s, 0), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.y, s, 1),
+                __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.y, s, 2), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.y, s, 3)};
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const uint32_t u = __builtin_bit_cast(uint32_t, x[k]);
+                hi[k] = pk_max(hi[k], u), lo[k] = pk_min(lo[k], u);
+            }
+            if (nan && sc[i] == SCALE_NAN)
+#pragma unroll
+                for (int k = 0; k < 8; k++) hi[k] = H2_INF, lo[k] = H2_INF | H2_SIGNS;
+        }
+    }
+};
+
+// The maxima over all the lanes that have the same channels of 16 registers hi, -lo (8 each): the
+// lanes above 32 go on with lo, those of odd rows of 16 with registers 4 .. 7, those above 8 of
+// a row with two of four, and where four lanes have a token, those above 4 of 8 with
+// one of two. out: the lane's registers, D / 64 of them.
+template <int D>
+__device__ __forceinline__ void over_tokens(uint32_t (&hi)[8], uint32_t (&lo)[8], uint32_t (&out)[D / 64]) {
+    const int lane = threadIdx.x & 63;
+    uint32_t four[4];
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        const auto r = __builtin_amdgcn_permlane32_swap(hi[k], lo[k] ^ H2_SIGNS, false, false);
+        hi[k] = pk_max(r[0], r[1]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const auto r = __builtin_amdgcn_permlane16_swap(hi[k], hi[k + 4], false, false);
+        four[k] = pk_max(r[0], r[1]);
+    }
+    uint32_t two[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        uint32_t y = __builtin_amdgcn_update_dpp(0, four[k], 0x128, 0xf, 0x3, false);  // row_ror:8
+        y = __builtin_amdgcn_update_dpp(y, four[k + 2], 0x128, 0xf, 0xc, false);
+        two[k] = pk_max(lane & 8 ? four[k + 2] : four[k], y);
+    }
+    if constexpr (D == 64) {
+        uint32_t y = __builtin_amdgcn_update_dpp(0, two[0], 0x104, 0xf, 0x5, false);  // row_shl:4
+        y = __builtin_amdgcn_update_dpp(y, two[1], 0x114, 0xf, 0xa, false);           // row_shr:4
+        out[0] = pk_max(lane & 4 ? two[1] : two[0], y);
+    } else {
+        out[0] = two[0], out[1] = two[1];
+    }
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void bounds_kernel(BoundsArgs a, int heads) {
+    using Part = BoundsPart<D>;
+    constexpr int SPAN = BOUNDS_LOADS * Part::TOK;
     const CacheDev& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int b = blockIdx.y;
+    const int b = blockIdx.y, runs = (c.kv_heads + heads - 1) / heads;
     const long long unit = (long long)blockIdx.x * 4 + wave;
-    const int kvh = (int)(unit % c.kv_heads), at = (int)(unit / c.kv_heads);
+    const int h0 = (int)(unit % runs) * heads, h1 = min(h0 + heads, c.kv_heads);
     const SequenceIndex seq = sequence_index(c, b, a.max_new);
     if (seq.n == 0 || seq.diff + seq.n <= 0) return;
-    const int page_tokens = 1 << c.page_shift;
-    const long long col = (max(seq.diff, 0ll) >> c.page_shift) + at;
+    const long long col = (max(seq.diff, 0ll) >> c.page_shift) + unit / runs;
     if (col > (seq.diff + seq.n - 1) >> c.page_shift || col >= c.max_pages) return;
-    const int page = cache_page(c, b, (int)col << c.page_shift);
-    const int held = min(seq.len - ((int)col << c.page_shift), page_tokens);
+    const int page = __builtin_amdgcn_readfirstlane(cache_page(c, b, (int)col << c.page_shift));
+    const int held = min(seq.len - ((int)col << c.page_shift), 1 << c.page_shift);
     if (page < 0 || held <= 0) return;
-    const long long row = cache_row(c, page, kvh, 0);
-    const uint8_t* scales = c.k_scales + row * G;
-    uint32_t top = 1;
-    for (int t = lane; t < held; t += 64)
-#pragma unroll
-        for (int g = 0; g < G; g++) {
-            const uint32_t s = scales[t * G + g];
-            if (s != SCALE_NAN) top = max(top, s);
+    Part next;
+    next.load(c, cache_row(c, page, h0, 0), 0, held);
+    for (int h = h0; h < h1; h++) {
+        const long long row = cache_row(c, page, h, 0);
+        Part now = next;
+        if (h + 1 < h1) next.load(c, cache_row(c, page, h + 1, 0), 0, held);
+        bool nan = false;
+        uint32_t top = now.top(0, held, nan);
+        for (int t0 = SPAN; t0 < held; t0 += SPAN) {
+            Part more;
+            more.load(c, row, t0, held);
+            top = max(top, more.top(t0, held, nan));
         }
+        top = wave_max(top);
+        uint32_t hi[8], lo[8], best[D / 64];
 #pragma unroll
-    for (int d = 32; d; d /= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d));
-    const uint8_t* codes = c.k_codes + row * (D / 2);
-    const _Float16 inf = (_Float16)__builtin_inff();
-    h2 hi[8], lo[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) hi[i] = h2{-inf, -inf}, lo[i] = h2{inf, inf};
-    const int part = lane % LANES;
-#pragma unroll 4
-    for (int t = lane / LANES; t < held; t += TOK) {
-        const uint2 w = *reinterpret_cast<const uint2*>(codes + t * (D / 2) + part * 8);
-        const uint32_t sc = scales[t * G + part / 2];
-        const float s = __uint_as_float((uint32_t)(127 + max((int)sc - (int)top + 4, -20)) << 23);
-        h2 x[8] = {__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w.x, s, 0), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w.x, s, 1),
-                   __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w.x, s, 2), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w.x, s, 3),
-                   __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w.y, s, 0), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w.y, s, 1),
-                   __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w.y, s, 2), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w.y, s, 3)};
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            hi[i] = __builtin_elementwise_max(hi[i], sc == SCALE_NAN ? h2{inf, inf} : x[i]);
-            lo[i] = __builtin_elementwise_min(lo[i], sc == SCALE_NAN ? h2{-inf, -inf} : x[i]);
+        for (int i = 0; i < 8; i++) hi[i] = H2_INF | H2_SIGNS, lo[i] = H2_INF;
+        now.take(0, held, top, nan, hi, lo);
+        for (int t0 = SPAN; t0 < held; t0 += SPAN) {
+            now.load(c, row, t0, held);
+            now.take(t0, held, top, nan, hi, lo);
         }
+        over_tokens<D>(hi, lo, best);
+        const bool low = lane >= 32;
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) {
+            const h2 x = __builtin_bit_cast(h2, best[i / 2]);
+            const int y = (int)fminf(__builtin_ceilf((float)x[i % 2]), 127.0f);
+            w |= (uint32_t)((low ? -y : y) & 255) << (8 * i);
+        }
+        const long long cell = (long long)page * c.kv_heads + h;
+        const int part = lane % Part::LANES, first = part * 16 + (lane >> 4 & 1) * 8 + (lane >> 3 & 1) * 4;
+        int8_t* out = a.bounds.codes + cell * (2 * D) + low * D;
+        if constexpr (D == 64)
+            *reinterpret_cast<uint16_t*>(out + first + (lane >> 2 & 1) * 2) = (uint16_t)w;
+        else
+            *reinterpret_cast<uint32_t*>(out + first) = w;
+        if (lane == 0) a.bounds.scales[cell] = (uint8_t)top;
     }
-#pragma unroll
-    for (int d = LANES; d < 64; d *= 2)
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            hi[i] = __builtin_elementwise_max(hi[i], __builtin_bit_cast(h2, __shfl_xor(__builtin_bit_cast(int, hi[i]), d)));
-            lo[i] = __builtin_elementwise_min(lo[i], __builtin_bit_cast(h2, __shfl_xor(__builtin_bit_cast(int, lo[i]), d)));
-        }
-    if (lane >= LANES) return;
-    uint32_t w[2][4];
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const float up = __builtin_ceilf((float)hi[i / 2][i % 2]), down = __builtin_floorf((float)lo[i / 2][i % 2]);
-        const uint32_t u = (uint32_t)(int)fminf(up, 127.0f) & 255, v = (uint32_t)(int)fmaxf(down, -127.0f) & 255;
-        w[0][i / 4] = i % 4 ? w[0][i / 4] | u << (i % 4 * 8) : u;
-        w[1][i / 4] = i % 4 ? w[1][i / 4] | v << (i % 4 * 8) : v;
-    }
-    const long long cell = (long long)page * c.kv_heads + kvh;
-    int8_t* out = a.bounds.codes + cell * (2 * D) + part * 16;
-    *reinterpret_cast<uint4*>(out) = make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]);
-    *reinterpret_cast<uint4*>(out + D) = make_uint4(w[1][0], w[1][1], w[1][2], w[1][3]);
-    if (lane == 0) a.bounds.scales[cell] = (uint8_t)top;
 }
 
 // ---- Scores ----
@@ -123,23 +224,23 @@ __device__ __forceinline__ uint2 codes_of(uint4 raw, bool f16, float up, float l
     return up == 0.0f ? make_uint2(0, 0) : make_uint2(w[0], w[1]);
 }
 
-// The greatest power of two 2^e, |e| <= 126, with top * 2^e <= 127 (top: fp32 bits); 0
-// where top is 0 or not finite.
-__device__ __forceinline__ float power_for(uint32_t top) {
-    if (top == 0 || top >= 0x7f800000u) return 0.0f;
-    int e;
-    const float m = __builtin_frexpf(__uint_as_float(top), &e);
-    e = m <= 127.0f / 128 ? 7 - e : 6 - e;
-    return __uint_as_float((uint32_t)(127 + min(max(e, -126), 126)) << 23);
+// The greatest magnitude of eight channels, as its 16 bits.
+__device__ __forceinline__ uint32_t greatest(uint4 raw) {
+    typedef uint16_t u2 __attribute__((ext_vector_type(2)));
+    const auto mag = [](uint32_t w) { return __builtin_bit_cast(u2, w & 0x7fff7fffu); };
+    const u2 m = __builtin_elementwise_max(__builtin_elementwise_max(mag(raw.x), mag(raw.y)),
+                                           __builtin_elementwise_max(mag(raw.z), mag(raw.w)));
+    return max((uint32_t)m.x, (uint32_t)m.y);
 }
 
-__device__ __forceinline__ uint32_t greatest(uint4 raw, bool f16) {
-    float f[8];
-    unpack8(raw, f, f16);
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-    return top;
+// The greatest power of two 2^e, |e| <= 126, with top * 2^e <= 127, of a magnitude's
+// bits; 0 where it is 0 or not finite.
+__device__ __forceinline__ float power_for(uint32_t top, bool f16) {
+    if (top == 0 || top >= (f16 ? 0x7c00u : 0x7f80u)) return 0.0f;
+    int e;
+    const float m = __builtin_frexpf(f16 ? f16_to_f32((uint16_t)top) : __uint_as_float(top << 16), &e);
+    e = m <= 127.0f / 128 ? 7 - e : 6 - e;
+    return __uint_as_float((uint32_t)(127 + min(max(e, -126), 126)) << 23);
 }
 
 // Ascending with the score; 0 is no page's and 1 a page's that is not there.
@@ -150,7 +251,7 @@ __device__ __forceinline__ uint32_t key_of(float score) {
 
 constexpr float INF = __builtin_inff();
 
-// What a wave holds of 16 pages: lane (page, quarter of its bounds' bytes).
+// What a wave holds of 16 pages: lane (page, quarter of each 64 bytes of its bounds).
 template <int D>
 struct PageStep {
     i4 w[2 * D / 64];
@@ -259,7 +360,7 @@ __device__ __forceinline__ void encode_tile(const PickArgs& a, const SequenceInd
     // Over a column's channels and a row's columns.
 #pragma unroll
     for (int i = 0; i < TURNS; i++) {
-        top[i] = greatest(raw[i], a.q_f16);
+        top[i] = greatest(raw[i]);
 #pragma unroll
         for (int d = 1; d < 64; d *= 2)
             if (d < PARTS << slots) top[i] = max(top[i], (uint32_t)__shfl_xor((int)top[i], d));
@@ -275,28 +376,31 @@ __device__ __forceinline__ void encode_tile(const PickArgs& a, const SequenceInd
     }
     __builtin_amdgcn_wave_barrier();  // the tile before is read
 #pragma unroll
-    for (int i = 0; i < TURNS; i++) lds.put(i * COLS + n, part, raw[i], a.q_f16, power_for(top[i]));
+    for (int i = 0; i < TURNS; i++) lds.put(i * COLS + n, part, raw[i], a.q_f16, power_for(top[i], a.q_f16));
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     lds.get(q);
 }
 
-// By a workgroup for all its waves, eight channels a thread.
+// By a workgroup for all its waves, eight channels a thread; raw: those of this
+// turn's head (raw_part), asked for before the pages.
+template <int D>
+__device__ __forceinline__ uint4 raw_part(const PickArgs& a, const SequenceIndex& seq, int kvh, int j0, int slots, int turn) {
+    constexpr int PARTS = D / 8;
+    const int n = threadIdx.x / PARTS, part = threadIdx.x % PARTS;
+    const uint16_t* p = n < 16 ? query_of(a, seq, kvh, j0, n, slots, turn) : nullptr;
+    return p ? *reinterpret_cast<const uint4*>(p + 8 * part) : make_uint4(0, 0, 0, 0);
+}
 template <int D>
 __device__ __forceinline__ void encode_shared(const PickArgs& a, const SequenceIndex& seq, int kvh, int j0, int slots,
-                                              int turn, TileLds<D>& lds, i4 (&q)[2 * D / 64]) {
+                                              int turn, uint4 raw, TileLds<D>& lds, i4 (&q)[2 * D / 64]) {
     constexpr int PARTS = D / 8;
     const int n = threadIdx.x / PARTS, part = threadIdx.x % PARTS, turns = (a.group + 15) / 16;
-    uint4 raw = make_uint4(0, 0, 0, 0);
     if (n < 16) {  // (whole waves)
-        uint32_t top = 0;
-        for (int i = 0; i < turns; i++) {
-            const uint16_t* p = query_of(a, seq, kvh, j0, n, slots, i);
-            const uint4 x = p ? *reinterpret_cast<const uint4*>(p + 8 * part) : make_uint4(0, 0, 0, 0);
-            if (i == turn) raw = x;
-            top = max(top, greatest(x, a.q_f16));
-        }
+        uint32_t top = greatest(raw);
+        for (int i = 0; i < turns; i++)
+            if (i != turn) top = max(top, greatest(raw_part<D>(a, seq, kvh, j0, slots, i)));
 #pragma unroll
         for (int d = 1; d < PARTS; d *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d));
         if (part == 0) lds.top[n] = top;
@@ -306,7 +410,7 @@ __device__ __forceinline__ void encode_shared(const PickArgs& a, const SequenceI
         const int first = n >> slots << slots;
         uint32_t top = 0;
         for (int i = 0; i < 1 << slots; i++) top = max(top, lds.top[first + i]);
-        lds.put(n, part, raw, a.q_f16, power_for(top));
+        lds.put(n, part, raw, a.q_f16, power_for(top, a.q_f16));
     }
     __syncthreads();
     lds.get(q);
@@ -355,9 +459,10 @@ __global__ __launch_bounds__(256, 2) void score_tile_kernel(PickArgs a, int slot
     const int pages = (seq.limit(j0 + count - 1, a.causal) + (1 << c.page_shift) - 1) >> c.page_shift;
     if (pages <= a.top) return;  // every page is picked
     for (int turn = 0; turn < (a.group + 15) / 16; turn++) {
+        const uint4 raw = raw_part<D>(a, seq, kvh, j0, slots, turn);
         PageWalk<D> walk(a, b, kvh, (part * 4 + wave) * 16, parts * 64, pages);
         i4 q[1][2 * D / 64];
-        encode_shared<D>(a, seq, kvh, j0, slots, turn, lds, q[0]);
+        encode_shared<D>(a, seq, kvh, j0, slots, turn, raw, lds, q[0]);
         walk.template run<1>(a, kvh, slots, q, [&](int, int r, int col, uint32_t key) {
             const int j = (4 * g + r) >> slots;
             const long long row = row0 + j;
@@ -396,15 +501,28 @@ struct Counts {
     }
 };
 
+// Where a search for the top-th greatest key begins: the bits from `bit` on, on `least`,
+// which top keys reach.
+struct Search {
+    uint32_t least = 0;
+    int bit = 31;
+    // The top-th greatest is within lo .. hi, or any key over hi is.
+    static __device__ __forceinline__ Search between(uint32_t lo, uint32_t hi) {
+        const int n = lo == hi ? 0 : 32 - __builtin_clz(lo ^ hi);  // bits in which they differ
+        return {n == 32 ? 0 : lo >> n << n, n - 1};
+    }
+};
+
 // The list from a row's keys, all more than 0 of which are more than top: key[i] is of
 // the i-th of the wave's columns that col(i) gives, in their order.
 template <int WAVES, int KEYS, class Col>
-__device__ __forceinline__ void write_greatest(const uint32_t (&key)[KEYS], int top, int wave, int* out, int* lds, Col col) {
+__device__ __forceinline__ void write_greatest(const uint32_t (&key)[KEYS], int top, int wave, int* out, int* lds, Col col,
+                                               Search from = Search{}) {
     const int lane = threadIdx.x & 63;
     Counts counts{lds, 0};
     int before;
-    uint32_t least = 0;
-    for (int bit = 31; bit >= 0; bit--) {
+    uint32_t least = from.least;
+    for (int bit = from.bit; bit >= 0; bit--) {
         const uint32_t t = least | 1u << bit;
         int mine = 0;
 #pragma unroll
@@ -452,12 +570,19 @@ struct Few {
 template <int KEYS>
 __device__ __forceinline__ void write_greatest_of_wave(const uint32_t (&key)[KEYS], int top, int* out, Few& few) {
     const int lane = threadIdx.x & 63;
-    auto plain = [&] { write_greatest<1, KEYS>(key, top, 0, out, nullptr, [&](int i) { return i * 64 + lane; }); };
-    if (KEYS <= 2 || top > 64) return plain();
-    uint32_t most = 0, bound = 0;
+    uint32_t most = 0, highest = 0;
 #pragma unroll
-    for (int i = 0; i < KEYS; i++) most = max(most, key[i]);
-    for (int bit = 31; bit >= 0; bit--) {
+    for (int i = 0; i < KEYS; i++) {
+        most = max(most, key[i]);
+        highest = max(highest, key[i] + 1 ? key[i] : 0);  // of those that are not always picked
+    }
+    highest = wave_max(highest);
+    // (top is at most the lanes that have a key: the least of their greatest bounds the list's.)
+    const Search from = top > 64 ? Search{} : Search::between(min(~wave_max(~most), highest), highest);
+    auto plain = [&] { write_greatest<1, KEYS>(key, top, 0, out, nullptr, [&](int i) { return i * 64 + lane; }, from); };
+    if (KEYS <= 4 || top > 64) return plain();
+    uint32_t bound = from.least;
+    for (int bit = from.bit; bit >= 0; bit--) {
         const uint32_t t = bound | 1u << bit;
         const int sum = __builtin_popcountll(__ballot(most >= t));
         if (sum >= top) bound = t;
@@ -479,7 +604,8 @@ __device__ __forceinline__ void write_greatest_of_wave(const uint32_t (&key)[KEY
     }
     wave_sync();
     const uint32_t two[2] = {lane < n ? few.key[lane] : 0, 64 + lane < n ? few.key[64 + lane] : 0};
-    write_greatest<1, 2>(two, top, 0, out, nullptr, [&](int i) { return few.col[i * 64 + lane]; });
+    write_greatest<1, 2>(two, top, 0, out, nullptr, [&](int i) { return few.col[i * 64 + lane]; },
+                         Search::between(min(bound, highest), highest));
 }
 
 // A row's list where all its pages are picked.
@@ -536,10 +662,12 @@ __global__ __launch_bounds__(512, TILES == 1 ? 2 : 4) void row_pick_kernel(PickA
     auto pages_of = [&](int j) { return (seq.limit(j0 + j, a.causal) + (1 << c.page_shift) - 1) >> c.page_shift; };
     const int pages = pages_of(count - 1);
     if (pages > a.top) {
+        uint4 raw;
+        if (TILES == 1) raw = raw_part<D>(a, seq, kvh, j0, slots, 0);
         PageWalk<D> walk(a, b, kvh, wave * 16, 128, pages);
         i4 q[TILES][2 * D / 64];
         if constexpr (TILES == 1) {
-            encode_shared<D>(a, seq, kvh, j0, slots, 0, lds.tile[0], q[0]);
+            encode_shared<D>(a, seq, kvh, j0, slots, 0, raw, lds.tile[0], q[0]);
         } else {
             if (wave < TILES) encode_tile<D>(a, seq, kvh, j0 + (wave << (4 - slots)), slots, lds.tile[wave], q[0]);
             __syncthreads();
@@ -575,11 +703,14 @@ __global__ __launch_bounds__(512, TILES == 1 ? 2 : 4) void row_pick_kernel(PickA
 
 hipError_t launch_cache_bounds(int head_dim, const BoundsArgs& a, hipStream_t s) {
     const long long pages = std::min<long long>(((long long)a.max_new + (1 << a.c.page_shift) - 1) >> a.c.page_shift, a.c.max_pages) + 1;
-    const dim3 grid((unsigned)((pages * a.c.kv_heads + 3) / 4), a.c.batch);
+    // Heads of a page by one wave, where that leaves waves enough to fill the chip.
+    const int heads = (int)std::max(1ll, std::min<long long>({4, a.c.kv_heads, pages * a.c.batch * a.c.kv_heads / 4096}));
+    const long long units = pages * ((a.c.kv_heads + heads - 1) / heads);
+    const dim3 grid((unsigned)((units + 3) / 4), a.c.batch);
     if (head_dim == 64)
-        hipLaunchKernelGGL(bounds_kernel<64>, grid, dim3(256), 0, s, a);
+        hipLaunchKernelGGL(bounds_kernel<64>, grid, dim3(256), 0, s, a, heads);
     else
-        hipLaunchKernelGGL(bounds_kernel<128>, grid, dim3(256), 0, s, a);
+        hipLaunchKernelGGL(bounds_kernel<128>, grid, dim3(256), 0, s, a, heads);
     return hipGetLastError();
 }
 
