@@ -20,36 +20,57 @@ namespace {
 typedef long long ll;
 typedef ll ll2 __attribute__((ext_vector_type(2)));
 
-constexpr int THREADS = 1024;
+constexpr int THREADS = 1024;  // at most, of the workgroup that makes the sums
 
-__device__ __forceinline__ ll pages_of(ll tokens, int shift) { return (tokens + (1 << shift) - 1) >> shift; }
+__device__ __forceinline__ uint32_t pages_of(uint32_t tokens, int shift) {
+    return (tokens >> shift) + ((tokens & ((1u << shift) - 1)) != 0);
+}
 
 // What a request asks for: rows, new pages (held: those it has), columns past
-// the table, pages that it gives back.
+// the table, pages that it gives back. Below 2^32 all of them, and sums of them stop
+// there: what a step can be served with is below 2^31.
+struct Sums {
+    uint32_t rows, fresh, back, over;
+    __device__ __forceinline__ void operator+=(const Sums& o) {
+        rows = __builtin_elementwise_add_sat(rows, o.rows), fresh = __builtin_elementwise_add_sat(fresh, o.fresh);
+        back = __builtin_elementwise_add_sat(back, o.back), over = __builtin_elementwise_add_sat(over, o.over);
+    }
+};
 struct Request {
-    ll rows, fresh, over, back, past, held;
+    Sums s;
+    uint32_t past, held;
     bool ended;
     __device__ __forceinline__ Request(const StepArgs& a, int news, int past_) {
         past = max(past_, 0);
         ended = news < 0;
-        rows = max(news, 0);
         held = pages_of(past, a.page_shift);
-        const ll want = pages_of(past + rows, a.page_shift);
-        fresh = ended ? 0 : want - held;
-        over = ended ? 0 : max(0ll, want - a.max_pages);
-        back = ended ? min(held, (ll)a.max_pages) : 0;
+        const uint32_t rows = max(news, 0), want = pages_of(past + rows, a.page_shift), most = a.max_pages;
+        s = Sums{rows, ended ? 0 : want - held, ended ? min(held, most) : 0, !ended && want > most ? want - most : 0};
     }
 };
 
-struct Sums {
-    ll rows, fresh, back, over;
-    __device__ __forceinline__ void operator+=(const Sums& o) {
-        rows += o.rows, fresh += o.fresh, back += o.back, over += o.over;
-    }
-};
-
-__device__ __forceinline__ Sums shfl_up(const Sums& s, int d) {
-    return {__shfl_up(s.rows, d), __shfl_up(s.fresh, d), __shfl_up(s.back, d), __shfl_up(s.over, d)};
+// v of the lanes of CTRL's place, 0 where there is none: a step of a sum over the lanes before.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ Sums moved(const Sums& s) {
+    return {moved<CTRL, ROWS>(s.rows), moved<CTRL, ROWS>(s.fresh), moved<CTRL, ROWS>(s.back), moved<CTRL, ROWS>(s.over)};
+}
+// Of the lanes up to each.
+__device__ __forceinline__ Sums upto_lane(Sums s) {
+    s += moved<0x111, 0xf>(s);  // row_shr:1, 2, 4, 8
+    s += moved<0x112, 0xf>(s);
+    s += moved<0x114, 0xf>(s);
+    s += moved<0x118, 0xf>(s);
+    s += moved<0x142, 0xa>(s);  // row_bcast:15 into rows 1 and 3
+    s += moved<0x143, 0xc>(s);  // row_bcast:31 into rows 2 and 3
+    return s;
+}
+__device__ __forceinline__ Sums of_lane(const Sums& s, int lane) {
+    auto get = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); };
+    return {get(s.rows), get(s.fresh), get(s.back), get(s.over)};
 }
 
 // The ring as the step finds it; numbers that make no sense are brought into range.
@@ -59,7 +80,8 @@ struct Ring {
         head = (int)((uint32_t)a.state_in[0] % (uint32_t)cap);
         count = min(max(a.state_in[1], 0), cap);
     }
-    __device__ __forceinline__ int at(ll i) const { return (int)((head + i) % cap); }
+    // The place i behind the first; i < 2^31.
+    __device__ __forceinline__ int at(uint32_t i) const { return (int)(((uint32_t)head + i) % (uint32_t)cap); }
 };
 
 // One row: its page from the ring where its column is new, else from the table.
@@ -116,65 +138,57 @@ __device__ __forceinline__ int request_of(const Starts& starts, int batch, int r
 // The sums, and with ROWS (a request a thread at most) everything else too.
 // scratch [batch] gets the ring's place of each request's first page, taken or given back,
 // and behind them [batch] the pages it gives back.
-template <bool ROWS>
-__global__ __launch_bounds__(THREADS) void step_kernel(StepArgs a) {
-    __shared__ Sums waves[THREADS / 64];
-    __shared__ int starts[ROWS ? THREADS + 1 : 1], past_of[ROWS ? THREADS : 1], first_of[ROWS ? THREADS : 1],
-        back_of[ROWS ? THREADS : 1];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+template <int N, bool ROWS>
+__global__ __launch_bounds__(N) void step_kernel(StepArgs a) {
+    __shared__ Sums waves[16];
+    __shared__ int starts[ROWS ? N + 1 : 1], past_of[ROWS ? N : 1], first_of[ROWS ? N : 1], back_of[ROWS ? N : 1];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Ring ring(a);
-    const int run = (a.batch + THREADS - 1) / THREADS;
+    const int run = ROWS ? 1 : (a.batch + N - 1) / N;
     const int b0 = min(a.batch, (int)threadIdx.x * run), b1 = min(a.batch, b0 + run);
     Sums mine{0, 0, 0, 0};
-    for (int b = b0; b < b1; b++) {
-        const Request q(a, a.news[b], a.past[b]);
-        mine += Sums{q.rows, q.fresh, q.back, q.over};
-    }
-    Sums upto = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const Sums o = shfl_up(upto, d);
-        if (lane >= d) upto += o;
-    }
-    if (lane == 63) waves[wave] = upto;
+    for (int b = b0; b < b1; b++) mine += Request(a, a.news[b], a.past[b]).s;
+    Sums at = upto_lane(mine);
+    if (lane == 63) waves[wave] = at;
     __syncthreads();  // (the inputs that may be outputs too are read)
-    Sums all{0, 0, 0, 0}, at{0, 0, 0, 0};
-    for (int w = 0; w < THREADS / 64; w++) {
-        if (w == wave) at = all;
-        all += waves[w];
-    }
-    at += upto;
+    Sums all = upto_lane(lane < N / 64 ? waves[lane] : Sums{0, 0, 0, 0});
+    // The sums before the thread's; exact where the step is good, and `back` up to the ring's room.
     at.rows -= mine.rows, at.fresh -= mine.fresh, at.back -= mine.back;
-    const ll missing = max(0ll, all.fresh - ring.count) + all.over, more = max(0ll, all.rows - a.rows);
+    if (wave) at += of_lane(all, wave - 1);
+    all = of_lane(all, 15);
+    const uint32_t count = ring.count, room = ring.cap - ring.count;
+    uint32_t missing = all.fresh > count ? all.fresh - count : 0;
+    missing = __builtin_elementwise_add_sat(missing, all.over);
+    const uint32_t more = all.rows > (uint32_t)a.rows ? all.rows - a.rows : 0;
     const bool good = missing == 0 && more == 0;
-    const ll room = ring.cap - ring.count;
     for (int b = b0; b < b1; b++) {
         const Request q(a, a.news[b], a.past[b]);
         const int start = good ? (int)at.rows : 0;
-        const int first = q.ended ? ring.at((ring.count + min(at.back, room))) : ring.at(good ? at.fresh : 0);
-        const int back = (int)max(0ll, min(q.back, room - at.back));
+        const int first = q.ended ? ring.at(count + min(at.back, room)) : ring.at(good ? at.fresh : 0);
+        const int back = at.back < room ? (int)min(q.s.back, room - at.back) : 0;
         a.starts[b] = start;
-        a.lengths[b] = q.ended ? 0 : (int)(q.past + (good ? q.rows : 0));
+        a.lengths[b] = q.ended ? 0 : (int)(q.past + (good ? q.s.rows : 0));
         if (ROWS) {
             starts[b] = start, past_of[b] = (int)q.past, first_of[b] = first, back_of[b] = back;
         } else {
             a.scratch[b] = first;
             a.scratch[a.batch + b] = back;
         }
-        at.rows += q.rows, at.fresh += q.fresh, at.back += q.back;
+        at += q.s;
     }
     const int rows = good ? (int)all.rows : 0;
     if (threadIdx.x == 0) {
         a.starts[a.batch] = rows;
         if (ROWS) starts[a.batch] = rows;
-        a.state[0] = ring.at(good ? all.fresh : 0);
-        a.state[1] = (int)(ring.count - (good ? all.fresh : 0) + min(all.back, room));
-        a.state[2] = (int)min(missing, 2147483647ll);
-        a.state[3] = (int)min(more, 2147483647ll);
+        const uint32_t taken = good ? all.fresh : 0;
+        a.state[0] = ring.at(taken);
+        a.state[1] = (int)(count - taken + min(all.back, room));
+        a.state[2] = (int)min(missing, 2147483647u);
+        a.state[3] = (int)min(more, 2147483647u);
     }
     if (!ROWS) return;
     __syncthreads();
-    for (int row = threadIdx.x; row < a.rows; row += THREADS) {
+    for (int row = threadIdx.x; row < a.rows; row += N) {
         RowPlace p{0, -1, -1};
         if (row < rows) {
             const int b = request_of(starts, a.batch, row);
@@ -183,12 +197,27 @@ __global__ __launch_bounds__(THREADS) void step_kernel(StepArgs a) {
         write_row(a, row, p);
     }
     if (all.back == 0) return;
-    for (int b = wave; b < a.batch; b += THREADS / 64)
+    for (int b = wave; b < a.batch; b += N / 64)
         if (back_of[b]) give_back(a, b, back_of[b], first_of[b]);
 }
 
+// The request of a row below starts[batch] (another one's number for any other row), by
+// a wave: 64 starts at a time, so two loads in a row up to 4096 requests.
+__device__ __forceinline__ int request_of_wave(const int* starts, int batch, int row) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = batch;  // starts[lo] <= row < starts[lo + n]
+    while (n > 1) {
+        const int run = (n + 63) / 64, at = lo + lane * run;
+        const int from = max(__builtin_popcountll(__ballot(at < lo + n && starts[at] <= row)) - 1, 0);
+        n = min(run, n - from * run);
+        lo += from * run;
+    }
+    return lo;
+}
+
 // The rows of a large step, four a thread, and behind their workgroups a
-// wave for each request that may have ended.
+// wave for each request that may have ended. A workgroup whose rows are all one
+// request's looks it up once; others look through the starts in LDS, row by row.
 constexpr int ROWS_WG = 1024, STARTS = 2048;
 __global__ __launch_bounds__(256) void step_rows_kernel(StepArgs a, int row_wgs) {
     if ((int)blockIdx.x >= row_wgs) {
@@ -196,28 +225,51 @@ __global__ __launch_bounds__(256) void step_rows_kernel(StepArgs a, int row_wgs)
         if (b < a.batch && a.scratch[a.batch + b]) give_back(a, b, a.scratch[a.batch + b], a.scratch[b]);
         return;
     }
-    __shared__ int lds[STARTS];
-    const int* starts = a.starts;
-    if (a.batch < STARTS) {
-        for (int i = threadIdx.x; i <= a.batch; i += 256) lds[i] = a.starts[i];
-        __syncthreads();
-        starts = lds;
-    }
-    const int total = starts[a.batch], row0 = blockIdx.x * ROWS_WG + threadIdx.x * 4;
-    if (row0 >= a.rows) return;
-    int b = -1, start = 0, end = 0, past = 0, held = 0, first = 0;
+    const int total = a.starts[a.batch], wg0 = blockIdx.x * ROWS_WG, row0 = wg0 + threadIdx.x * 4;
     RowPlace p[4];
+    const int one = __builtin_amdgcn_readfirstlane(request_of_wave(a.starts, a.batch, wg0));
+    if (a.batch && wg0 + ROWS_WG <= a.starts[one + 1]) {
+        const int start = a.starts[one], past = a.lengths[one] - (a.starts[one + 1] - start);
+        const int held = (int)pages_of(past, a.page_shift), first = a.scratch[one];
+        // Four tokens are of two pages at most: the first one's and the last one's.
+        const int t = past + row0 - start, in_page = (1 << a.page_shift) - 1, turn = (t | in_page) + 1;
+        const int* table = a.page_table + (ll)one * a.max_pages;
+        auto page_of = [&](int col) {
+            const uint32_t at = (uint32_t)first + (uint32_t)(col - held);
+            return col < held ? table[col] : a.ring[at < (uint32_t)a.cap ? at : at - a.cap];
+        };
+        const int c0 = t >> a.page_shift, c1 = (t + 3) >> a.page_shift;
+        const int p0 = page_of(c0), p1 = c1 == c0 ? p0 : page_of(c1);
+        // The row that begins a new column writes it.
+        if (c0 >= held && (t & in_page) == 0) a.page_table[(ll)one * a.max_pages + c0] = p0;
+        if (c1 > c0 && c1 >= held) a.page_table[(ll)one * a.max_pages + c1] = p1;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int row = row0 + i;
-        p[i] = RowPlace{0, -1, -1};
-        if (row >= total) continue;
-        if (row >= end) {
-            b = request_of(starts, a.batch, row);
-            start = starts[b], end = starts[b + 1];
-            past = a.lengths[b] - (end - start), held = (int)pages_of(past, a.page_shift), first = a.scratch[b];
+        for (int i = 0; i < 4; i++) {
+            const int page = t + i < turn ? p0 : p1;
+            p[i] = RowPlace{t + i, one, -1};
+            if ((unsigned)page < (unsigned)a.pages) p[i].slot = ((ll)page << a.page_shift) + ((t + i) & in_page);
         }
-        p[i] = place_row(a, b, past + row - start, held, first);
+    } else {
+        __shared__ int lds[STARTS];
+        const int* starts = a.starts;
+        if (a.batch < STARTS) {
+            for (int i = threadIdx.x; i <= a.batch; i += 256) lds[i] = a.starts[i];
+            __syncthreads();
+            starts = lds;
+        }
+        int b = -1, start = 0, end = 0, past = 0, held = 0, first = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int row = row0 + i;
+            p[i] = RowPlace{0, -1, -1};
+            if (row >= total) continue;
+            if (row >= end) {
+                b = request_of(starts, a.batch, row);
+                start = starts[b], end = starts[b + 1];
+                past = a.lengths[b] - (end - start), held = (int)pages_of(past, a.page_shift), first = a.scratch[b];
+            }
+            p[i] = place_row(a, b, past + row - start, held, first);
+        }
     }
     if (row0 + 3 < a.rows) {
         if (a.positions)
@@ -238,12 +290,22 @@ __global__ __launch_bounds__(256) void step_rows_kernel(StepArgs a, int row_wgs)
 }  // namespace
 
 // One launch where a workgroup has the requests in its threads and few rows and
-// pages to see to; its rounds of 1024 rows are cheaper than a second launch up to 8.
+// pages to see to. Replayed from a graph, us, 64 requests:
+//   rows                            64    512   1024  2048  4096  8192
+//   one launch of 256 threads       2.9   3.9   5.5   8.7   15.3  28.0
+//   one launch of 1024              3.4   3.7   3.9   4.8   6.7   10.3
+//   two launches                    7.2   5.9   6.0   6.6   6.6   6.7
+// (the eager call pays the host another 2 us for the second). A call that fills the
+// chip, 512 requests of 1380301 rows together: 13.0 us for 23 MB, of which the second
+// launch's chain start -> request -> page -> rows takes most; without the slots' 11 MB 11.1.
 hipError_t launch_cache_step(const StepArgs& a, hipStream_t s) {
-    if (a.batch <= THREADS && a.rows <= 8 * THREADS && (ll)a.batch * a.max_pages <= 1 << 18) {
-        hipLaunchKernelGGL(step_kernel<true>, dim3(1), dim3(THREADS), 0, s, a);
+    const bool one = a.batch <= THREADS && a.rows <= 4 * THREADS && (ll)a.batch * a.max_pages <= 1 << 18;
+    if (one && a.batch <= 256 && a.rows <= 256) {
+        hipLaunchKernelGGL((step_kernel<256, true>), dim3(1), dim3(256), 0, s, a);
+    } else if (one) {
+        hipLaunchKernelGGL((step_kernel<THREADS, true>), dim3(1), dim3(THREADS), 0, s, a);
     } else {
-        hipLaunchKernelGGL(step_kernel<false>, dim3(1), dim3(THREADS), 0, s, a);
+        hipLaunchKernelGGL((step_kernel<THREADS, false>), dim3(1), dim3(THREADS), 0, s, a);
         const int row_wgs = (int)(((ll)a.rows + ROWS_WG - 1) / ROWS_WG);
         hipLaunchKernelGGL(step_rows_kernel, dim3(row_wgs + (a.batch + 3) / 4), dim3(256), 0, s, a, row_wgs);
     }
