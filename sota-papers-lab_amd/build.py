@@ -53,6 +53,7 @@ UNITS = [
     ("sage_cache.hip", "sage_cache.hip.o", ["-ffp-contract=off"]),
     ("sage_cache_attn.hip", "sage_cache_attn.hip.o", []),
     ("sage_cache_step.hip", "sage_cache_step.hip.o", []),
+    ("sage_cache_picked.hip", "sage_cache_picked.hip.o", []),
     ("sage_cache_pick.hip", "sage_cache_pick.hip.o", ["-fno-honor-nans"]),
     ("sage_api.cpp", "sage_api.cpp.o", []),
     ("sage_cache_api.cpp", "sage_cache_api.cpp.o", []),

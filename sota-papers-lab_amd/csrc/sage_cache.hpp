@@ -130,15 +130,19 @@ struct CachePlan {
 CachePlan cache_plan(int head_dim, int batch, int rows, int heads, int kv_heads, int max_new, int max_tokens);
 hipError_t launch_cache_attend(int head_dim, const CacheAttnArgs& a, const CachePlan& plan, hipStream_t s);
 
-// How a call over picked pages runs: workgroups that a unit's pages are split over, the
-// partial outputs that the workspace holds, and the bytes of LDS of its lists.
+// How a call over picked pages runs: in units of 32 columns (chunks) or of 16,
+// workgroups that a unit's pages are split over, the partial outputs that the workspace
+// holds, and the bytes of LDS of its lists.
 struct PickedPlan {
     int splits;
     uint64_t part_rows;
     unsigned lds;
+    bool chunks;
 };
 PickedPlan picked_plan(int head_dim, int batch, int rows, int heads, int kv_heads, int max_new, int max_pages,
                        int page_tokens, int top);
+hipError_t launch_cache_attend_few_picked(int head_dim, const CacheAttnArgs& a, unsigned lds, hipStream_t s);
+hipError_t launch_cache_join_splits(int head_dim, const CacheAttnArgs& a, hipStream_t s);
 hipError_t launch_cache_attend_picked(int head_dim, const CacheAttnArgs& a, const PickedPlan& plan, hipStream_t s);
 
 // The index lookups, host and device: tests/cpp/cache_host.cpp runs them on bad

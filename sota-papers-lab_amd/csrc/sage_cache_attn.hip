@@ -24,226 +24,12 @@
 // those four are the order in which O^T = V^T P^T takes its tokens, so P goes
 // from one MFMA to the next without leaving the lane's registers.
 #include <algorithm>
-#include <type_traits>
 
-#include "sage_cache.hpp"
+#include "sage_cache_attn.hpp"
 
 namespace sage {
 
 namespace {
-
-typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef short s4 __attribute__((ext_vector_type(4)));
-typedef short s8 __attribute__((ext_vector_type(8)));
-typedef float f2 __attribute__((ext_vector_type(2)));
-typedef float f4 __attribute__((ext_vector_type(4)));
-typedef float f16v __attribute__((ext_vector_type(16)));
-
-constexpr int COLS = 16;    // columns of a workgroup
-constexpr int TOKENS = 64;  // tokens of a wave's step
-constexpr int MAX_SPLITS = 256;
-// The reference m of the softmax follows the maximum only where that is 2^8
-// past it: the fp32 sums have room for that, and rescaling them becomes rare.
-constexpr float SLACK = 8.0f;
-constexpr float NEG_INF = -__builtin_inff();
-// V's blocks from this scale on (2^126: a code of 4 is past every 16- and 32-bit
-// type) are NaN as 255 is: an infinity of a masked token would reach the
-// rows that do not see it as 0 * inf.
-constexpr uint32_t V_NAN = 253;
-
-// Codes 2 which and 2 which + 1 of a dword times s, as bf16 or fp16 (H16).
-template <bool H16>
-__device__ __forceinline__ uint32_t cvt2(uint32_t codes, float s, int which) {
-    if constexpr (H16) {
-        h2 r;
-        switch (which) {
-            case 0: r = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, s, 0); break;
-            case 1: r = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, s, 1); break;
-            case 2: r = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, s, 2); break;
-            default: r = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, s, 3);
-        }
-        return __builtin_bit_cast(uint32_t, r);
-    }
-    bf2 r;
-    switch (which) {
-        case 0: r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, s, 0); break;
-        case 1: r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, s, 1); break;
-        case 2: r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, s, 2); break;
-        default: r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, s, 3);
-    }
-    return __builtin_bit_cast(uint32_t, r);
-}
-
-// Eight channels of one code dword.
-template <bool H16 = false>
-__device__ __forceinline__ uint4 decode8(uint32_t codes, float s) {
-    return make_uint4(cvt2<H16>(codes, s, 0), cvt2<H16>(codes, s, 1), cvt2<H16>(codes, s, 2),
-                      cvt2<H16>(codes, s, 3));
-}
-
-// Eight values as bf16, or as two bf16 parts: the nearest and the rest's.
-template <int PARTS>
-__device__ __forceinline__ void parts_of(const float* f, bf8 (&p)[PARTS]) {
-    uint32_t w[PARTS][4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        w[0][i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
-        if (PARTS == 2)
-            w[PARTS - 1][i] = pack_bf16x2(f[2 * i] - __uint_as_float(w[0][i] << 16),
-                                          f[2 * i + 1] - __uint_as_float(w[0][i] & 0xffff0000u));
-    }
-#pragma unroll
-    for (int k = 0; k < PARTS; k++) p[k] = __builtin_bit_cast(bf8, make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]));
-}
-
-// Eight channels of a query, negated under a negative softmax scale (so that
-// the greatest logit is the greatest product).
-__device__ __forceinline__ uint4 load_q(const uint16_t* p, uint32_t sign) {
-    const uint4 x = *reinterpret_cast<const uint4*>(p);
-    return make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign);
-}
-
-// Maximum and sum over the four lanes of a column (lanes 16 apart).
-__device__ __forceinline__ float col_max(float v) {
-    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float col_sum(float v) {
-    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-// Maximum over the aligned LANES (8 or 16) lanes of a row, in each of them.
-template <int LANES>
-__device__ __forceinline__ float row_max(float v) {
-    v = fmaxf(v, dpp<0xB1>(v));
-    v = fmaxf(v, dpp<0x4E>(v));
-    v = fmaxf(v, dpp<0x141>(v));
-    return LANES > 8 ? fmaxf(v, dpp<0x140>(v)) : v;
-}
-__device__ __forceinline__ uint32_t col_or(uint32_t v) {
-    auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    v = r[0] | r[1];
-    r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    return r[0] | r[1];
-}
-
-// A sequence's pages as a wave walks it: 64 columns of the page table, one a
-// lane, loaded at once and read by lane index. Looked up one by one, each id is
-// a load in front of the loads that need it, and waiting for it waits for
-// all that are in flight (64 ragged sequences of up to 16384 tokens, 32/8 heads
-// of 128: 173 us, with the window 152).
-struct Pages {
-    const int* table;  // the sequence's row
-    int cols, pages, shift, lane;
-    int base, ids;
-    __device__ __forceinline__ Pages(const CacheDev& c, int b, int lane_, int t)
-        : table(c.page_table + (long long)b * c.max_pages), cols(c.max_pages), pages(c.pages), shift(c.page_shift),
-          lane(lane_) {
-        fill(t >> shift);
-    }
-    __device__ __forceinline__ void fill(int col) {
-        base = col;
-        const int at = col + lane;
-        const int id = at < cols ? table[at] : -1;
-        ids = (unsigned)id < (unsigned)pages ? id : -1;
-        asm volatile("" : "+v"(ids));  // waited for here, once a window, not at every use
-    }
-    // The page of slot t (of the window's first column or behind it), or -1.
-    __device__ __forceinline__ int of(int t) {
-        const int col = t >> shift;
-        if (col - base >= 64) fill(col);
-        return __builtin_amdgcn_readlane(ids, col - base);
-    }
-};
-
-// Tokens of one of the chunk kernel's splits of a sequence of len tokens: whole tiles.
-__device__ __forceinline__ int split_tokens(int len, int splits) {
-    return ((len + splits - 1) / splits + TOKENS - 1) / TOKENS * TOKENS;
-}
-
-// Byte of half h (eight channels) of 16-channel unit u of a token's bf16 V row
-// in LDS. LDS serves 128 bytes a clock: the units of a row are permuted by the
-// token, so that the four tokens that 16 lanes of a transposing read take meet
-// all of them, and the halves of some are swapped, so that what eight lanes
-// write at once does too.
-template <int D>
-__device__ __forceinline__ int unit_at(int tok, int u, int h) {
-    const int f = D == 128 ? tok & 7 : tok & 3, s = D == 128 ? u >> 2 & 1 : (tok ^ tok >> 1) & 1;
-    return tok * (D * 2) + ((u ^ f) << 5) + ((h ^ s) << 4);
-}
-
-// Eight tokens of a lane's channel from two transposing reads, of four tokens
-// each, at v and `on` bytes behind it.
-__device__ __forceinline__ bf8 read_v(const uint8_t* v, int on) {
-    typedef __attribute__((address_space(3))) s4* lds_ptr;
-    const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(v));
-    const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(v + on));
-    return __builtin_bit_cast(bf8, (s8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-}
-
-// Eight channels of an output row: the sums over the softmax's.
-__device__ __forceinline__ void store_row(const CacheAttnArgs& a, long long row, int head, int ch, const float* f,
-                                          float sum) {
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float x = f[2 * i] * inv, y = f[2 * i + 1] * inv;
-        w[i] = a.out_f16 ? pack_f16x2(x, y) : pack_bf16x2(x, y);
-    }
-    *reinterpret_cast<uint4*>(a.out.p + row * a.out.st + head * a.out.sh + ch) = make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-// Parts first .. first + parts - 1 of one column joined by a group of D / 8
-// lanes, eight channels a lane (ch); or, with SHARE, by all the groups of a
-// workgroup together (the first has the result): each sums the parts that fall
-// to it in their order and the groups' sums are added in theirs, so the same
-// call gives the same bits. at(p): part p's place. Returns the softmax's sum.
-template <int D, bool SHARE, class At>
-__device__ __forceinline__ float join_parts(const CacheAttnArgs& a, int parts, int ch, At at, float (&out)[8]) {
-    constexpr int LANES = D / 8, GROUPS = 256 / LANES;
-    __shared__ float sums[SHARE ? GROUPS : 1][D + 4], ls[GROUPS];
-    const f2* ml = reinterpret_cast<const f2*>(a.part_ml);
-    const int grp = threadIdx.x / LANES;
-    // The maximum over all parts, then this group's share of the sums.
-    float m = NEG_INF, l = 0.0f;
-    for (int p = threadIdx.x % LANES; p < parts; p += LANES) m = fmaxf(m, ml[at(p)].x);
-    m = row_max<LANES>(m);
-    const float base = m == NEG_INF ? 0.0f : m;
-    f4 f[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
-#pragma unroll 4
-    for (int p = SHARE ? grp : 0; p < parts; p += SHARE ? GROUPS : 1) {
-        const f2 s = ml[at(p)];
-        const f4* o = reinterpret_cast<const f4*>(a.part_o + at(p) * D + ch);
-        const float w = __builtin_amdgcn_exp2f(s.x - base);
-        l += w * s.y;
-        f[0] += o[0] * w;
-        f[1] += o[1] * w;
-    }
-    if (SHARE) {
-        *reinterpret_cast<f4*>(&sums[SHARE ? grp : 0][ch]) = f[0];
-        *reinterpret_cast<f4*>(&sums[SHARE ? grp : 0][ch + 4]) = f[1];
-        ls[grp] = l;
-        __syncthreads();
-        l = 0.0f, f[0] = f[1] = f4{0, 0, 0, 0};
-#pragma unroll
-        for (int g = 0; g < GROUPS; g++) {
-            l += ls[g];
-            f[0] += *reinterpret_cast<const f4*>(&sums[SHARE ? g : 0][ch]);
-            f[1] += *reinterpret_cast<const f4*>(&sums[SHARE ? g : 0][ch + 4]);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 8; i++) out[i] = f[i / 4][i % 4];
-    return l;
-}
 
 // ---- Few rows ----
 //
@@ -258,6 +44,7 @@ __device__ __forceinline__ float join_parts(const CacheAttnArgs& a, int parts, i
 // 32/8 heads of 128, one row each: 564 MB in 121 us, 4.7 TB/s. (When it took
 // 119, cut into equal parts of each sequence instead: 137 us at the best number
 // of parts; in twice as many shares as the chip holds: 132.)
+constexpr int COLS = 16;  // columns of a workgroup
 constexpr int STEP = 4 * TOKENS;
 
 struct Units {
@@ -297,144 +84,6 @@ struct Line {
         }
         before = upto - sum;
         total = uniform(upto, (c.batch - 1) / run);
-    }
-};
-// ---- Picked pages ----
-//
-// The pages that a unit's rows have picked (sage_cache_attend_picked), one behind
-// the other, in place of a sequence's own: the tokens of a unit are those of the
-// pages that any of its rows picked, ascending, and each page carries the rows that
-// did. 16 columns of a group of four heads are four rows, whose picks share much: a
-// page is read and converted once for all of them, and never costs more than the
-// rows' own would, whose columns would fill a tile as wide.
-struct Entries {
-    uint32_t* entry;  // column << 16 | rows of the unit, a bit each
-    int* page;        // the pool's page, or -1
-    int count;
-};
-
-// LDS of a unit: the columns' bits, how many are set before each word, and the entries.
-// rows: of a unit, at most.
-__host__ __device__ __forceinline__ int unit_rows(int group, int max_new) {
-    const int rows = (COLS + group - 2) / group + 1;
-    return rows < max_new ? rows : max_new;
-}
-__host__ __device__ __forceinline__ int pick_words(int max_pages) { return (max_pages + 31) / 32; }
-__host__ __device__ __forceinline__ int pick_entries(int top, int group, int max_new, int max_pages) {
-    const int most = unit_rows(group, max_new) * top;
-    return most < max_pages ? most : max_pages;
-}
-
-// The entries of rows j0 .. j0 + rows - 1 of sequence b, whose columns are below `pages`.
-// All threads of the workgroup together.
-template <int W>
-__device__ __forceinline__ Entries entries_of(const CacheAttnArgs& a, const SequenceIndex& seq, int b, int kvh, int j0,
-                                              int rows, int pages, uint32_t* lds) {
-    const CacheDev& c = a.c;
-    const int words = pick_words(pages), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint32_t *bits = lds, *before = bits + pick_words(c.max_pages);
-    Entries e{before + pick_words(c.max_pages), nullptr, 0};
-    e.page = reinterpret_cast<int*>(e.entry) + pick_entries(a.top, a.group, a.max_new, c.max_pages);
-    __shared__ int found[W], odd[W];
-    const int* table = c.page_table + (long long)b * c.max_pages;
-    auto page_at = [&](int col) {
-        const int id = table[col];
-        return (unsigned)id < (unsigned)c.pages ? id : -1;
-    };
-    // Row r's i-th column, or -1.
-    auto picked = [&](int r, int i) {
-        const long long row = seq.start + j0 + r;
-        if (row < 0 || row >= c.rows) return -1;
-        const int col = a.picked[(row * c.kv_heads + kvh) * a.top + i];
-        return (unsigned)col < (unsigned)pages ? col : -1;
-    };
-    if (rows == 1) {
-        // One row's list as it is, if it ascends, with nothing behind a -1.
-        int n = 0;
-        bool out_of_order = false;
-        for (int i0 = 0; i0 < a.top; i0 += 64 * W) {
-            const int i = i0 + (int)threadIdx.x, col = i < a.top ? picked(0, i) : -1;
-            const int last = i > 0 && i < a.top ? picked(0, i - 1) : -1;
-            if (col >= 0) {
-                out_of_order |= i > 0 && last >= col;
-                out_of_order |= i > 0 && last < 0;
-                e.entry[min(i, pages - 1)] = (uint32_t)col << 16 | 1;
-                e.page[min(i, pages - 1)] = page_at(col);
-            }
-            n += __builtin_popcountll(__ballot(col >= 0));
-        }
-        const bool wrong = __any(out_of_order);
-        if (lane == 0) found[wave] = n, odd[wave] = wrong;
-        __syncthreads();
-        bool any = false;
-#pragma unroll
-        for (int w = 0; w < W; w++) e.count += found[w], any = any || odd[w];
-        if (!any) return e;
-        __syncthreads();
-        e.count = 0;
-    }
-    for (int i = threadIdx.x; i < words; i += 64 * W) bits[i] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < rows * a.top; i += 64 * W) {
-        const int col = picked(i / a.top, i % a.top);
-        if (col >= 0) atomicOr(&bits[col >> 5], 1u << (col & 31));
-    }
-    __syncthreads();
-    // A run of words a thread.
-    const int run = (words + 64 * W - 1) / (64 * W), w0 = min(words, (int)threadIdx.x * run), w1 = min(words, w0 + run);
-    int mine = 0;
-    for (int w = w0; w < w1; w++) mine += __builtin_popcount(bits[w]);
-    int upto = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const int x = __shfl_up(upto, d);
-        if (lane >= d) upto += x;
-    }
-    if (lane == 63) found[wave] = upto;
-    __syncthreads();
-    int at = upto - mine;
-#pragma unroll
-    for (int w = 0; w < W; w++) {
-        if (w < wave) at += found[w];
-        e.count += found[w];
-    }
-    for (int w = w0; w < w1; w++) {
-        before[w] = at;
-        for (uint32_t x = bits[w]; x; x &= x - 1) e.entry[at++] = (uint32_t)(w * 32 + __builtin_ctz(x)) << 16;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < e.count; i += 64 * W) e.page[i] = page_at((int)(e.entry[i] >> 16));
-    for (int i = threadIdx.x; i < rows * a.top; i += 64 * W) {
-        const int r = i / a.top, col = picked(r, i - r * a.top);
-        if (col < 0) continue;
-        const int place = before[col >> 5] + __builtin_popcount(bits[col >> 5] & ((1u << (col & 31)) - 1));
-        atomicOr(&e.entry[place], 1u << r);
-    }
-    __syncthreads();
-    return e;
-}
-
-// The entries as a wave walks them, 64 at a time, as Pages does a table's columns.
-struct Walk {
-    Entries e;
-    int shift, lane, base, ids;
-    uint32_t entries;
-    __device__ __forceinline__ Walk(const Entries& e_, int shift_, int lane_, int t) : e(e_), shift(shift_), lane(lane_) {
-        fill(t >> shift);
-    }
-    __device__ __forceinline__ void fill(int i) {
-        base = i;
-        const int at = i + lane;
-        ids = at < e.count ? e.page[at] : -1;
-        entries = at < e.count ? e.entry[at] : 0;
-        asm volatile("" : "+v"(ids), "+v"(entries));  // waited for here, once a window
-    }
-    // The page of token t of the list, or -1, and its entry.
-    __device__ __forceinline__ int of(int t, uint32_t& entry) {
-        const int i = t >> shift;
-        if (i - base >= 64) fill(i);
-        entry = __builtin_amdgcn_readlane(entries, i - base);
-        return __builtin_amdgcn_readlane(ids, i - base);
     }
 };
 
@@ -527,7 +176,7 @@ __global__ __launch_bounds__(64 * W, D == 64 && W == 4 ? 3 : 2) void cache_attn(
         Entries entries{};
         if constexpr (PICKED) {
             const int pages = (now.limit(j1, a.causal) + (1 << c.page_shift) - 1) >> c.page_shift;
-            entries = entries_of<W>(a, now, b_now, kvh, j0, j1 - j0 + 1, pages, pick_lds);
+            entries = entries_of<W, COLS>(a, now, b_now, kvh, j0, j1 - j0 + 1, pages, pick_lds);
             const int steps = ((entries.count << c.page_shift) + STEP - 1) / STEP;
             s0 = (int)((long long)steps * split / a.splits), s1 = (int)((long long)steps * (split + 1) / a.splits);
         }
@@ -578,19 +227,17 @@ __global__ __launch_bounds__(64 * W, D == 64 && W == 4 ? 3 : 2) void cache_attn(
             uint4 v[G];
             uint32_t vs[G];
             int valid;  // bit i: the page of 16-token tile i is one of the pool's
-            uint32_t entry[PICKED ? 4 : 1];
+            int slot[PICKED ? 4 : 1];  // of its first token
+            uint32_t rows[PICKED ? 4 : 1];
         };
         // Slot of the first token of 16-token tile i at t, and whether the lane's column
         // sees token k of the tile.
         auto slot_at = [&](int t, int i, const Step& st) {
-            if constexpr (PICKED)
-                return (int)(st.entry[i] >> 16 << c.page_shift) + ((t + 16 * i) & ((1 << c.page_shift) - 1));
-            else
-                return t + 16 * i;
+            return PICKED ? st.slot[PICKED ? i : 0] : t + 16 * i;
         };
         auto sees = [&](int t, int i, int k, const Step& st) {
             return slot_at(t, i, st) + k < limit && (st.valid >> i & 1) &&
-                   (!PICKED || (st.entry[PICKED ? i : 0] >> (j - j0) & 1));
+                   (!PICKED || (st.rows[PICKED ? i : 0] >> (j - j0) & 1));
         };
         auto row_of = [&](int t, int page) {
             return cache_row(c, max(page, 0), kvh, t & ((1 << c.page_shift) - 1));
@@ -602,7 +249,7 @@ __global__ __launch_bounds__(64 * W, D == 64 && W == 4 ? 3 : 2) void cache_attn(
             for (int i = 0; i < 4; i++) {
                 int page;
                 if constexpr (PICKED)
-                    page = pages.of(t + 16 * i, st.entry[i]);
+                    page = pages.of(t + 16 * i, st.slot[i], st.rows[i]);
                 else
                     page = pages.of(t + 16 * i);
                 st.valid |= (page >= 0) << i;
@@ -664,7 +311,7 @@ __global__ __launch_bounds__(64 * W, D == 64 && W == 4 ? 3 : 2) void cache_attn(
             if constexpr (PICKED) {
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    masked = masked || slot_at(t, i, st) + 16 > least || (st.entry[i] & 0xffff) != every;
+                    masked = masked || st.slot[i] + 16 > least || st.rows[i] != every;
             } else {
                 masked = masked || t + TOKENS > least;
             }
@@ -812,19 +459,6 @@ __global__ __launch_bounds__(64 * W, D == 64 && W == 4 ? 3 : 2) void cache_attn(
 // Two parts everywhere took the chunks above from 427 us to 565, fp16 from 448
 // to 460 (another box).
 constexpr int CCOLS = 128;
-// V's scale bytes whose values, 0.5 to 6 times the scale, are normal fp16
-// numbers: 2^-13 to 2^13.
-constexpr uint32_t HALF_LEAST = 114, HALF_MOST = 140;
-// Weights of fp16 are 2^LIFT times those of bf16, from 2^-21 on normal numbers and
-// 2^15 at most; the reference that goes with their sums is as much lower.
-constexpr float LIFT = 7.0f;
-// Whether a scale byte is past HALF_LEAST .. HALF_MOST, and whether its block is
-// more than fp16 holds: NaN, or codes (its dwords or'ed) other than zeros.
-__device__ __forceinline__ bool past_half(uint32_t scale) { return scale - HALF_LEAST > HALF_MOST - HALF_LEAST; }
-__device__ __forceinline__ bool past_half(uint32_t scale, uint32_t codes) {
-    return past_half(scale) && (scale >= V_NAN || (codes & 0x77777777u));
-}
-
 template <int D>
 struct ChunkLds {
     uint8_t v[2][TOKENS * D * 2];
@@ -1286,32 +920,21 @@ hipError_t launch_cache_attend(int head_dim, const CacheAttnArgs& a, const Cache
     return head_dim == 64 ? launch<64>(a, plan, s) : launch<128>(a, plan, s);
 }
 
-PickedPlan picked_plan(int head_dim, int batch, int rows, int heads, int kv_heads, int max_new, int max_pages,
-                       int page_tokens, int top) {
-    const int group = heads / kv_heads;
-    PickedPlan p{};
-    p.lds = 4u * (2 * pick_words(max_pages) + 2 * pick_entries(top, group, max_new, max_pages));
-    const long long units = ((long long)max_new * group + COLS - 1) / COLS * kv_heads * batch;
-    const long long steps = ((long long)pick_entries(top, group, max_new, max_pages) * page_tokens + STEP - 1) / STEP;
-    const long long fill = head_dim == 64 ? 768 : 512;
-    p.splits = (int)std::max(1ll, std::min({fill / std::max(units, 1ll), (steps + 1) / 2, (long long)MAX_SPLITS}));
-    p.part_rows = p.splits > 1 ? (uint64_t)p.splits * rows * heads : 0;
-    return p;
-}
-
-template <int D>
-static hipError_t launch_picked(const CacheAttnArgs& a, const PickedPlan& plan, hipStream_t s) {
+hipError_t launch_cache_attend_few_picked(int head_dim, const CacheAttnArgs& a, unsigned lds, hipStream_t s) {
     const unsigned tiles = (unsigned)(((long long)a.max_new * a.group + COLS - 1) / COLS);
     const auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(tiles * a.splits * a.c.kv_heads, 1, a.c.batch), dim3(256), plan.lds, s, a);
+        hipLaunchKernelGGL(kernel, dim3(tiles * a.splits * a.c.kv_heads, 1, a.c.batch), dim3(256), lds, s, a);
     };
-    a.q_f16 ? go(cache_attn<D, 2, 4, true>) : go(cache_attn<D, 1, 4, true>);
-    if (a.splits > 1) join_splits<D>(a, s);
+    if (head_dim == 64)
+        go(a.q_f16 ? cache_attn<64, 2, 4, true> : cache_attn<64, 1, 4, true>);
+    else
+        go(a.q_f16 ? cache_attn<128, 2, 4, true> : cache_attn<128, 1, 4, true>);
     return hipGetLastError();
 }
 
-hipError_t launch_cache_attend_picked(int head_dim, const CacheAttnArgs& a, const PickedPlan& plan, hipStream_t s) {
-    return head_dim == 64 ? launch_picked<64>(a, plan, s) : launch_picked<128>(a, plan, s);
+hipError_t launch_cache_join_splits(int head_dim, const CacheAttnArgs& a, hipStream_t s) {
+    head_dim == 64 ? join_splits<64>(a, s) : join_splits<128>(a, s);
+    return hipGetLastError();
 }
 
 }  // namespace sage

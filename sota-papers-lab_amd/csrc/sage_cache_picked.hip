@@ -1,0 +1,383 @@
+// Attention over picked pages (gfx950): chunks of rows, and how a call runs.
+//
+// Steps and other few rows run the few-rows kernel over their lists
+// (sage_cache_attn.hip). Chunks take 32 columns a unit: a page that any of the unit's
+// rows picked is read and converted once for all of them, so that wider units convert less
+// and multiply more for rows that have not picked it. 32 is the width of the larger
+// MFMA, whose operands a wave's registers hold beside the outputs of its own tokens.
+#include <algorithm>
+
+#include "sage_cache_attn.hpp"
+
+namespace sage {
+
+namespace {
+
+constexpr int UCOLS = 32;        // columns of a unit
+constexpr int USTEP = 4 * TOKENS;
+
+// Four waves take 64 tokens of the list each in turn; their outputs meet in LDS in the
+// end. K's codes go from memory to the MFMA's rows (a lane: a token, half of its channels)
+// and are converted there; V's through the wave's own part of LDS, 32 tokens at a time,
+// for the transposing read. A step's keys are asked for once the one before has its
+// logits, its values once the one before has its sums.
+// QP: bf16 parts of a query. OUT16: the output is fp16. For a bf16 one the weights
+// are fp16 while V's scales are within HALF_LEAST .. HALF_MOST, from the wave's first
+// step past them on two bf16 parts.
+template <int D, int QP, bool OUT16>
+__global__ __launch_bounds__(256, 2) void picked_chunk(CacheAttnArgs a) {
+    constexpr int G = D / 32, KS = D / 16, CT = D / 32;  // scale blocks, MFMA steps over the channels, channel tiles
+    constexpr int VT = 64 / G, HALF = TOKENS / 2;        // tokens of a V load; of V in LDS at a time
+    constexpr int PAD = D / 2 + 4;                       // floats of a column where half the outputs meet
+    constexpr int PART = HALF * D * 2 > UCOLS * PAD * 4 ? HALF * D * 2 : UCOLS * PAD * 4;
+    __shared__ __align__(16) uint8_t lds[4 * PART];
+    __shared__ float wm[4][UCOLS], wl[4][UCOLS];
+    extern __shared__ uint32_t pick_lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, half = lane >> 5;
+    const CacheDev& c = a.c;
+    const int b = blockIdx.z, kvh = blockIdx.x % c.kv_heads, split = blockIdx.x / c.kv_heads % a.splits;
+    const int c0 = blockIdx.x / c.kv_heads / a.splits * UCOLS;
+    const SequenceIndex seq = sequence_index(c, b, a.max_new);
+    const int cols = seq.n * a.group;
+    if (c0 >= cols) return;
+    const int j0 = c0 / a.group, j1 = (min(c0 + UCOLS, cols) - 1) / a.group;
+    const int j = (c0 + col) / a.group, head = kvh * a.group + (c0 + col) - j * a.group;
+    const long long row = seq.start + j;
+    const bool have = c0 + col < cols && row >= 0 && row < c.rows;
+    const int limit = seq.limit(j, a.causal), least = seq.limit(j0, a.causal);
+    bf8 q[QP][KS];
+    {
+        const uint16_t* p = a.q.p + row * a.q.st + head * a.q.sh + half * (D / 2);
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (have) x = load_q(p + 8 * s, a.q_sign);
+            if (QP == 2) {
+                float f[8];
+                unpack8(x, f, true);
+                bf8 two[2];
+                parts_of<2>(f, two);
+                q[0][s] = two[0], q[QP - 1][s] = two[1];
+            } else {
+                q[0][s] = __builtin_bit_cast(bf8, x);
+            }
+        }
+    }
+    const int in_page = (1 << c.page_shift) - 1;
+    const int pages = (seq.limit(j1, a.causal) + in_page) >> c.page_shift;
+    const Entries entries = entries_of<4, UCOLS>(a, seq, b, kvh, j0, j1 - j0 + 1, pages, pick_lds);
+    const int tokens = entries.count << c.page_shift, steps = (tokens + USTEP - 1) / USTEP;
+    const int s0 = (int)((long long)steps * split / a.splits), s1 = (int)((long long)steps * (split + 1) / a.splits);
+    const int t_first = s0 * USTEP + wave * TOKENS, end = min(s1 * USTEP, tokens);
+
+    // A step's 16-token tiles: code row, slot of the first token, the rows that see it.
+    struct Tiles {
+        long long at[4];
+        int slot[4];
+        uint32_t rows[4];
+    };
+    Walk walk(entries, c.page_shift, lane, t_first);
+    auto look_up = [&](int t, Tiles& x) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int page = walk.of(t + 16 * i, x.slot[i], x.rows[i]);
+            if (page < 0) x.rows[i] = 0;
+            x.at[i] = cache_row(c, max(page, 0), kvh, (t + 16 * i) & in_page);
+        }
+    };
+    uint32_t kw[2][KS], ks[2];
+    auto load_k = [&](const Tiles& x) {
+#pragma unroll
+        for (int sub = 0; sub < 2; sub++) {
+            const long long r = x.at[2 * sub] + ((x.at[2 * sub + 1] - x.at[2 * sub]) & -(long long)(col >> 4)) + (col & 15);
+            const uint8_t* p = c.k_codes + r * (D / 2) + half * (D / 4);
+#pragma unroll
+            for (int n = 0; n < KS / 4; n++) {
+                const uint4 z = *reinterpret_cast<const uint4*>(p + 16 * n);
+                kw[sub][4 * n] = z.x, kw[sub][4 * n + 1] = z.y, kw[sub][4 * n + 2] = z.z, kw[sub][4 * n + 3] = z.w;
+            }
+            const uint8_t* z = c.k_scales + r * G + half * (G / 2);
+            ks[sub] = D == 128 ? *reinterpret_cast<const uint16_t*>(z) : *z;
+        }
+    };
+    uint4 v[G];
+    uint32_t vs[G];
+    auto load_v = [&](const Tiles& x) {
+#pragma unroll
+        for (int i = 0; i < G; i++) {
+            long long r = x.at[i * VT / 16];
+            if (VT == 32 && lane >= 32) r = x.at[i * VT / 16 + 1];
+            r += lane / G & 15;
+            v[i] = *reinterpret_cast<const uint4*>(c.v_codes + r * (D / 2) + (lane % G) * 16);
+            vs[i] = c.v_scales[r * G + lane % G];
+        }
+    };
+
+    f16v o[CT];
+#pragma unroll
+    for (int u = 0; u < CT; u++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[u][i] = 0.0f;
+    float m = NEG_INF, l = 0.0f, lift = OUT16 ? 0.0f : LIFT;
+    uint8_t* vl = lds + wave * PART;
+    const int vtok = 4 * half + (lane >> 2 & 3), vunit = lane >> 4 & 1;
+    // The wave's steps from t on, with fp16 weights (H16) until a scale of V is past
+    // them; returns where they stopped.
+    auto pass = [&](int t, auto fp16) __attribute__((always_inline)) {
+        constexpr bool H16 = decltype(fp16)::value;
+        Tiles next;
+        if (t < end) {
+            look_up(t, next);
+            load_k(next);
+            load_v(next);
+        }
+        for (; t < end; t += USTEP) {
+            const Tiles now = next;
+            const bool more = t + USTEP < end;
+            f16v x[2];
+#pragma unroll
+            for (int sub = 0; sub < 2; sub++) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) x[sub][i] = 0.0f;
+                const float sf[2] = {__uint_as_float((ks[sub] & 255) << 23), __uint_as_float((ks[sub] >> 8) << 23)};
+#pragma unroll
+                for (int s = 0; s < KS; s++) {
+                    const bf8 kk = __builtin_bit_cast(bf8, decode8(kw[sub][s], sf[s / 4]));
+#pragma unroll
+                    for (int p = 0; p < QP; p++) x[sub] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kk, q[p][s], x[sub], 0, 0, 0);
+                }
+            }
+            if (more) {
+                look_up(t + USTEP, next);
+                load_k(next);
+            }
+            // Register i of sub is token 8 (i / 4) + 4 half + i % 4 of its 32: of 16-token tile 2 sub + i / 8.
+            auto sees = [&](int sub, int i) {
+                const int tile = 2 * sub + i / 8, k = (8 * (i / 4) + i % 4) & 15;
+                return (now.rows[tile] >> (j - j0) & 1) && now.slot[tile] + k + 4 * half < limit;
+            };
+            float mx = NEG_INF;
+#pragma unroll
+            for (int tile = 0; tile < 4; tile++) {
+                if (now.slot[tile] + 16 > least) {
+#pragma unroll
+                    for (int i = 8 * (tile & 1); i < 8 * (tile & 1) + 8; i++)
+                        if (!sees(tile / 2, i)) x[tile / 2][i] = NEG_INF;
+                } else {
+                    const bool in = now.rows[tile] >> (j - j0) & 1;
+#pragma unroll
+                    for (int i = 8 * (tile & 1); i < 8 * (tile & 1) + 8; i++) x[tile / 2][i] = in ? x[tile / 2][i] : NEG_INF;
+                }
+#pragma unroll
+                for (int i = 8 * (tile & 1); i < 8 * (tile & 1) + 8; i++) mx = fmaxf(mx, x[tile / 2][i]);
+            }
+            {
+                auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+                mx = fmaxf(m, fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+            }
+            if constexpr (H16) {
+                bool past = false;
+#pragma unroll
+                for (int i = 0; i < G; i++) past = past || past_half(vs[i]);
+                if (__any(past)) {
+                    past = false;
+#pragma unroll
+                    for (int i = 0; i < G; i++) past = past || past_half(vs[i], v[i].x | v[i].y | v[i].z | v[i].w);
+                    if (__any(past)) return t;
+                }
+            }
+            if (__any((mx - m) * a.qk_mul > SLACK)) {
+                const float scale = __builtin_amdgcn_exp2f((m - (mx == NEG_INF ? 0.0f : mx)) * a.qk_mul);
+                m = mx;
+                l *= scale;
+#pragma unroll
+                for (int u = 0; u < CT; u++) o[u] *= scale;
+            }
+            const float base = (m == NEG_INF ? 0.0f : m * a.qk_mul) - (H16 ? LIFT : 0.0f);
+#pragma unroll
+            for (int sub = 0; sub < 2; sub++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    x[sub][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[sub][i], a.qk_mul, -base));
+                    l += x[sub][i];
+                }
+            // 32 tokens of V into LDS as 16-bit values, then O^T += V^T P^T.
+#pragma unroll
+            for (int sub = 0; sub < 2; sub++) {
+#pragma unroll
+                for (int n = sub * G / 2; n < (sub + 1) * G / 2; n++) {
+                    const float s = __uint_as_float(!H16 && vs[n] >= V_NAN ? 0 : vs[n] << 23);
+                    const uint32_t w[4] = {v[n].x, v[n].y, v[n].z, v[n].w};
+#pragma unroll
+                    for (int d = 0; d < 4; d++)
+                        *reinterpret_cast<uint4*>(vl + unit_at<D>((lane / G + n * VT) % HALF, (lane % G) * 2 + d / 2, d & 1)) =
+                            decode8<H16>(w[d], s);
+                }
+#pragma unroll
+                for (int st = 0; st < 2; st++) {
+                    float e[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) e[i] = x[sub][8 * st + i];
+                    bf8 p[2];
+                    if constexpr (H16)
+                        p[0] = __builtin_bit_cast(bf8, make_uint4(pack_f16x2(e[0], e[1]), pack_f16x2(e[2], e[3]),
+                                                                  pack_f16x2(e[4], e[5]), pack_f16x2(e[6], e[7])));
+                    else
+                        parts_of<2>(e, p);
+#pragma unroll
+                    for (int u = 0; u < CT; u++) {
+                        const uint8_t* at = vl + 16 * st * (D * 2) + unit_at<D>(vtok, 2 * u + vunit, lane >> 1 & 1) + (lane & 1) * 8;
+                        const bf8 vv = read_v(at, 8 * (D * 2));
+                        if constexpr (H16) {
+                            o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, vv),
+                                                                          __builtin_bit_cast(h8, p[0]), o[u], 0, 0, 0);
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 2; k++)
+                                o[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv, p[k], o[u], 0, 0, 0);
+                        }
+                    }
+                }
+            }
+            if constexpr (!H16) {
+                // Blocks of NaN, bit (token % VT) * G + block of each load.
+                uint64_t bad[G], any_bad = 0;
+#pragma unroll
+                for (int i = 0; i < G; i++) bad[i] = __ballot(vs[i] >= V_NAN), any_bad |= bad[i];
+                if (any_bad) {
+                    uint32_t hit = 0;  // blocks of NaN that this lane's tokens bring to its column
+#pragma unroll
+                    for (int sub = 0; sub < 2; sub++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const int tok = 32 * sub + 8 * (i / 4) + 4 * half + i % 4;
+                            const uint32_t blocks = (uint32_t)(bad[(32 * sub + 8 * (i / 4)) / VT] >> (tok % VT * G)) & ((1u << G) - 1);
+                            if (sees(sub, i)) hit |= blocks;
+                        }
+                    auto r = __builtin_amdgcn_permlane32_swap(hit, hit, false, false);
+                    hit = r[0] | r[1];
+#pragma unroll
+                    for (int u = 0; u < CT; u++)
+                        if (hit >> u & 1)
+#pragma unroll
+                            for (int i = 0; i < 16; i++) o[u][i] = __builtin_nanf("");
+                }
+            }
+            if (more) load_v(next);
+        }
+        return t;
+    };
+    if constexpr (OUT16) {
+        pass(t_first, std::false_type{});
+    } else {
+        const int t = pass(t_first, std::true_type{});
+        if (t < end) {
+            lift = 0.0f;
+            l *= __builtin_amdgcn_exp2f(-LIFT);
+#pragma unroll
+            for (int u = 0; u < CT; u++) o[u] *= __builtin_amdgcn_exp2f(-LIFT);
+            walk.fill(t >> c.page_shift);
+            pass(t, std::false_type{});
+        }
+    }
+    {
+        auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+        l = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+
+    // The waves' parts meet in LDS, half of the channels at a time: a thread sums N of a column.
+    constexpr int N = D / 16;
+    float* ol = reinterpret_cast<float*>(lds);  // [4][UCOLS][PAD]
+    const int oc = threadIdx.x / 8, ch = threadIdx.x % 8 * N;
+    const int oj = (c0 + oc) / a.group, oh = kvh * a.group + (c0 + oc) - oj * a.group;
+    const long long orow = seq.start + oj;
+    const bool out = c0 + oc < cols && orow >= 0 && orow < c.rows;
+    if (half == 0) wm[wave][col] = m * a.qk_mul - lift, wl[wave][col] = l;
+#pragma unroll
+    for (int pass = 0; pass < 2; pass++) {
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < CT / 2; u++)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const f16v& x = o[pass * (CT / 2) + u];
+                *reinterpret_cast<f4*>(ol + (wave * UCOLS + col) * PAD + 32 * u + 2 * i + 4 * half) =
+                    f4{x[i], x[i + 1], x[i + 2], x[i + 3]};
+            }
+        __syncthreads();
+        if (!out) continue;
+        float top = NEG_INF, sum = 0.0f, f[N] = {};
+#pragma unroll
+        for (int w = 0; w < 4; w++) top = fmaxf(top, wm[w][oc]);
+        const float base = top == NEG_INF ? 0.0f : top;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float s = __builtin_amdgcn_exp2f(wm[w][oc] - base);
+            sum += wl[w][oc] * s;
+            const float* p = ol + (w * UCOLS + oc) * PAD + ch;
+#pragma unroll
+            for (int i = 0; i < N; i++) f[i] += p[i] * s;
+        }
+        const int channel = pass * (D / 2) + ch;
+        if (a.splits > 1) {
+            const long long at = ((long long)split * c.rows + orow) * a.heads + oh;
+#pragma unroll
+            for (int i = 0; i < N; i += 4)
+                *reinterpret_cast<f4*>(a.part_o + at * D + channel + i) = f4{f[i], f[i + 1], f[i + 2], f[i + 3]};
+            if (channel == 0) reinterpret_cast<f2*>(a.part_ml)[at] = f2{top, sum};
+            continue;
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        uint16_t* to = a.out.p + orow * a.out.st + oh * a.out.sh + channel;
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const f4 y = f4{f[i], f[i + 1], f[i + 2], f[i + 3]} * inv;
+            *reinterpret_cast<uint2*>(to + i) = a.out_f16 ? make_uint2(pack_f16x2(y[0], y[1]), pack_f16x2(y[2], y[3]))
+                                                          : make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+        }
+    }
+}
+
+constexpr unsigned MOST_LDS = 40u << 10;  // of a unit's lists, beside the kernel's own: two workgroups a CU
+
+}  // namespace
+
+PickedPlan picked_plan(int head_dim, int batch, int rows, int heads, int kv_heads, int max_new, int max_pages,
+                       int page_tokens, int top) {
+    const int group = heads / kv_heads;
+    PickedPlan p{};
+    p.chunks = (long long)max_new * group > 16 && pick_lds_bytes(UCOLS, top, group, max_new, max_pages) <= MOST_LDS;
+    const int cols = p.chunks ? UCOLS : 16;
+    p.lds = pick_lds_bytes(cols, top, group, max_new, max_pages);
+    const long long units = ((long long)max_new * group + cols - 1) / cols * kv_heads * batch;
+    const long long steps = ((long long)pick_entries(cols, top, group, max_new, max_pages) * page_tokens + USTEP - 1) / USTEP;
+    const long long fill = head_dim == 64 && !p.chunks ? 768 : 512;
+    p.splits = (int)std::max(1ll, std::min({fill / std::max(units, 1ll), (steps + 1) / 2, (long long)MAX_SPLITS}));
+    p.part_rows = p.splits > 1 ? (uint64_t)p.splits * rows * heads : 0;
+    return p;
+}
+
+hipError_t launch_cache_attend_picked(int head_dim, const CacheAttnArgs& a, const PickedPlan& plan, hipStream_t s) {
+    hipError_t e;
+    if (plan.chunks) {
+        const unsigned tiles = (unsigned)(((long long)a.max_new * a.group + UCOLS - 1) / UCOLS);
+        const auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(tiles * a.splits * a.c.kv_heads, 1, a.c.batch), dim3(256), plan.lds, s, a);
+        };
+        if (head_dim == 64 && a.q_f16)
+            go(a.out_f16 ? picked_chunk<64, 2, true> : picked_chunk<64, 2, false>);
+        else if (head_dim == 64)
+            go(a.out_f16 ? picked_chunk<64, 1, true> : picked_chunk<64, 1, false>);
+        else if (a.q_f16)
+            go(a.out_f16 ? picked_chunk<128, 2, true> : picked_chunk<128, 2, false>);
+        else
+            go(a.out_f16 ? picked_chunk<128, 1, true> : picked_chunk<128, 1, false>);
+        e = hipGetLastError();
+    } else {
+        e = launch_cache_attend_few_picked(head_dim, a, plan.lds, s);
+    }
+    return e == hipSuccess && a.splits > 1 ? launch_cache_join_splits(head_dim, a, s) : e;
+}
+
+}  // namespace sage
