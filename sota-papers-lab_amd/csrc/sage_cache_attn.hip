@@ -58,13 +58,6 @@ struct Units {
     }
 };
 
-// A lane's value, scalar.
-__device__ __forceinline__ long long uniform(long long v, int lane) {
-    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, lane);
-    const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(v >> 32), lane);
-    return (long long)((uint64_t)hi << 32 | lo);
-}
-
 // The line as every wave sums it: each lane a run of sequences, `before` the
 // runs before the lane's.
 struct Line {

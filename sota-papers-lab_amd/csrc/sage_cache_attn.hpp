@@ -79,9 +79,11 @@ __device__ __forceinline__ void parts_of(const float* f, bf8 (&p)[PARTS]) {
 
 // Eight channels of a query, negated under a negative softmax scale (so that
 // the greatest logit is the greatest product).
-__device__ __forceinline__ uint4 load_q(const uint16_t* p, uint32_t sign) {
-    const uint4 x = *reinterpret_cast<const uint4*>(p);
+__device__ __forceinline__ uint4 signed_q(uint4 x, uint32_t sign) {
     return make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign);
+}
+__device__ __forceinline__ uint4 load_q(const uint16_t* p, uint32_t sign) {
+    return signed_q(*reinterpret_cast<const uint4*>(p), sign);
 }
 
 // Maximum and sum over the four lanes of a column (lanes 16 apart).
@@ -110,6 +112,13 @@ __device__ __forceinline__ uint32_t col_or(uint32_t v) {
     v = r[0] | r[1];
     r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
     return r[0] | r[1];
+}
+
+// A lane's value, scalar.
+__device__ __forceinline__ long long uniform(long long v, int lane) {
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, lane);
+    const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(v >> 32), lane);
+    return (long long)((uint64_t)hi << 32 | lo);
 }
 
 // A sequence's pages as a wave walks it: 64 columns of the page table, one a
@@ -317,12 +326,25 @@ __device__ __forceinline__ Entries entries_of(const CacheAttnArgs& a, const Sequ
         __syncthreads();
         e.count = 0;
     }
+    // A thread's first KEEP columns and their pages stay in registers from the first look to the last.
+    constexpr int KEEP = 2;
+    int kept[KEEP], ids[KEEP];
+#pragma unroll
+    for (int k = 0; k < KEEP; k++) {
+        const int i = threadIdx.x + k * 64 * W;
+        kept[k] = i < rows * a.top ? picked(i / a.top, i % a.top) : -1;
+    }
     for (int i = threadIdx.x; i < words; i += 64 * W) bits[i] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < rows * a.top; i += 64 * W) {
-        const int col = picked(i / a.top, i % a.top);
+    auto mark = [&](int col) {
         if (col >= 0) atomicOr(&bits[col >> 5], 1u << (col & 31));
+    };
+#pragma unroll
+    for (int k = 0; k < KEEP; k++) {
+        mark(kept[k]);
+        ids[k] = kept[k] >= 0 ? page_at(kept[k]) : -1;
     }
+    for (int i = threadIdx.x + KEEP * 64 * W; i < rows * a.top; i += 64 * W) mark(picked(i / a.top, i % a.top));
     __syncthreads();
     // A run of words a thread.
     const int run = (words + 64 * W - 1) / (64 * W), w0 = min(words, (int)threadIdx.x * run), w1 = min(words, w0 + run);
@@ -350,12 +372,17 @@ __device__ __forceinline__ Entries entries_of(const CacheAttnArgs& a, const Sequ
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < e.count; i += 64 * W) e.page[i] = page_at((int)e.col[i]);
-    for (int i = threadIdx.x; i < rows * a.top; i += 64 * W) {
-        const int r = i / a.top, col = picked(r, i - r * a.top);
-        if (col < 0) continue;
+    auto note = [&](int r, int col, int id) {
+        if (col < 0) return;
         const int place = before[col >> 5] + __builtin_popcount(bits[col >> 5] & ((1u << (col & 31)) - 1));
         atomicOr(&e.rows[place], 1u << r);
+        e.page[place] = id;  // (every row that picked it writes the same)
+    };
+#pragma unroll
+    for (int k = 0; k < KEEP; k++) note((threadIdx.x + k * 64 * W) / a.top, kept[k], ids[k]);
+    for (int i = threadIdx.x + KEEP * 64 * W; i < rows * a.top; i += 64 * W) {
+        const int col = picked(i / a.top, i % a.top);
+        note(i / a.top, col, col >= 0 ? page_at(col) : -1);
     }
     __syncthreads();
     return e;

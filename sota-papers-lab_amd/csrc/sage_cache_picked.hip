@@ -15,6 +15,71 @@ namespace {
 
 constexpr int UCOLS = 32;        // columns of a unit
 constexpr int USTEP = 4 * TOKENS;
+constexpr uint32_t SLOTS = 512;       // workgroups that the chip holds at once
+
+// The call's units in a line: sequence by sequence its tiles, KV heads fastest. As many
+// rounds of SLOTS as there are whole run a workgroup a unit; the units over, `rest`, are cut
+// into as many parts each as fill one more round, so that the chip does not wait for a
+// few (1563 rows behind 30000 tokens, 1568 units: 239 us with all of them whole, 227 so).
+struct Plot {
+    uint32_t whole, rest, parts;  // units that run whole, units over, parts of each of those
+    uint32_t cut;                 // the workgroup's: of which unit over,
+    int part;                     // which part, or -1: a whole unit;
+    int b, kvh, tile;             // its sequence (-1: none), KV head and tile
+    SequenceIndex seq;
+
+    // By every wave for itself; at: the place in the line of workgroups, or among the units over.
+    __device__ __forceinline__ Plot(const CacheAttnArgs& a, uint32_t at, bool over) {
+        const CacheDev& c = a.c;
+        const int lane = threadIdx.x & 63, run = (c.batch + 63) / 64;
+        const int b0 = min(c.batch, lane * run), b1 = min(c.batch, b0 + run);
+        uint32_t mine = 0;
+        for (int i = b0; i < b1; i++) mine += tiles_of(a, index_of(a, i));
+        uint32_t upto = mine;
+        for (int d = 1; d < min(64, c.batch); d *= 2) {
+            const uint32_t v = __shfl_up(upto, d);
+            if (lane >= d) upto += v;
+        }
+        const uint32_t units = __builtin_amdgcn_readlane(upto, (c.batch - 1) / run) * c.kv_heads;
+        whole = units / SLOTS * SLOTS;
+        rest = units - whole;
+        parts = rest ? min(SLOTS / rest, (uint32_t)a.splits) : 0;
+        if (parts == 1) whole = units, rest = 0;
+        b = -1, part = -1, cut = 0;
+        uint32_t unit = at;
+        if (over) {
+            if (at >= rest) return;
+            cut = at, unit = whole + at, part = 0;
+        } else if (at >= whole) {
+            if (at - whole >= rest * parts) return;
+            part = (int)((at - whole) / rest), cut = at - whole - part * rest, unit = whole + cut;
+        }
+        const uint32_t place = unit / c.kv_heads;  // among the tiles
+        kvh = (int)(unit - place * c.kv_heads);
+        const int from = 63 - __builtin_clzll(__ballot(upto - mine <= place && lane * run < c.batch));
+        uint32_t first = __builtin_amdgcn_readlane(upto - mine, from);
+        b = from * run;
+        while (true) {
+            seq = index_of(a, b);
+            const uint32_t n = tiles_of(a, seq);
+            tile = (int)(place - first);
+            if (place < first + n) return;
+            if (b >= c.batch - 1) break;
+            first += n;
+            b++;
+        }
+        b = -1;  // (starts that make no sense)
+    }
+    // Of the rows that the tensors have: their units are no more than the launch counts.
+    static __device__ __forceinline__ SequenceIndex index_of(const CacheAttnArgs& a, int b) {
+        SequenceIndex s = sequence_index(a.c, b, a.max_new);
+        s.n = (int)max(0ll, min((long long)s.n, a.c.rows - s.start));
+        return s;
+    }
+    static __device__ __forceinline__ uint32_t tiles_of(const CacheAttnArgs& a, const SequenceIndex& s) {
+        return ((uint32_t)s.n * a.group + UCOLS - 1) / UCOLS;
+    }
+};
 
 // Four waves take 64 tokens of the list each in turn; their outputs meet in LDS in the
 // end. K's codes go from memory to the MFMA's rows (a lane: a token, half of its channels)
@@ -36,39 +101,42 @@ __global__ __launch_bounds__(256, 2) void picked_chunk(CacheAttnArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     const CacheDev& c = a.c;
-    const int b = blockIdx.z, kvh = blockIdx.x % c.kv_heads, split = blockIdx.x / c.kv_heads % a.splits;
-    const int c0 = blockIdx.x / c.kv_heads / a.splits * UCOLS;
-    const SequenceIndex seq = sequence_index(c, b, a.max_new);
+    const Plot plot(a, blockIdx.x, false);
+    if (plot.b < 0) return;
+    const int b = plot.b, kvh = plot.kvh, c0 = plot.tile * UCOLS;
+    const SequenceIndex seq = plot.seq;
     const int cols = seq.n * a.group;
-    if (c0 >= cols) return;
     const int j0 = c0 / a.group, j1 = (min(c0 + UCOLS, cols) - 1) / a.group;
     const int j = (c0 + col) / a.group, head = kvh * a.group + (c0 + col) - j * a.group;
     const long long row = seq.start + j;
     const bool have = c0 + col < cols && row >= 0 && row < c.rows;
     const int limit = seq.limit(j, a.causal), least = seq.limit(j0, a.causal);
-    bf8 q[QP][KS];
+    uint4 raw[KS];  // the column's query, on its way while the list is made
     {
         const uint16_t* p = a.q.p + row * a.q.st + head * a.q.sh + half * (D / 2);
 #pragma unroll
-        for (int s = 0; s < KS; s++) {
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (have) x = load_q(p + 8 * s, a.q_sign);
-            if (QP == 2) {
-                float f[8];
-                unpack8(x, f, true);
-                bf8 two[2];
-                parts_of<2>(f, two);
-                q[0][s] = two[0], q[QP - 1][s] = two[1];
-            } else {
-                q[0][s] = __builtin_bit_cast(bf8, x);
-            }
-        }
+        for (int s = 0; s < KS; s++) raw[s] = have ? *reinterpret_cast<const uint4*>(p + 8 * s) : make_uint4(0, 0, 0, 0);
     }
     const int in_page = (1 << c.page_shift) - 1;
     const int pages = (seq.limit(j1, a.causal) + in_page) >> c.page_shift;
     const Entries entries = entries_of<4, UCOLS>(a, seq, b, kvh, j0, j1 - j0 + 1, pages, pick_lds);
+    bf8 q[QP][KS];
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+        const uint4 x = signed_q(raw[s], a.q_sign);
+        if (QP == 2) {
+            float f[8];
+            unpack8(x, f, true);
+            bf8 two[2];
+            parts_of<2>(f, two);
+            q[0][s] = two[0], q[QP - 1][s] = two[1];
+        } else {
+            q[0][s] = __builtin_bit_cast(bf8, x);
+        }
+    }
     const int tokens = entries.count << c.page_shift, steps = (tokens + USTEP - 1) / USTEP;
-    const int s0 = (int)((long long)steps * split / a.splits), s1 = (int)((long long)steps * (split + 1) / a.splits);
+    const int parts = (int)plot.parts;
+    const int s0 = plot.part < 0 ? 0 : steps * plot.part / parts, s1 = plot.part < 0 ? steps : steps * (plot.part + 1) / parts;
     const int t_first = s0 * USTEP + wave * TOKENS, end = min(s1 * USTEP, tokens);
 
     // A step's 16-token tiles: code row, slot of the first token, the rows that see it.
@@ -320,8 +388,8 @@ __global__ __launch_bounds__(256, 2) void picked_chunk(CacheAttnArgs a) {
             for (int i = 0; i < N; i++) f[i] += p[i] * s;
         }
         const int channel = pass * (D / 2) + ch;
-        if (a.splits > 1) {
-            const long long at = ((long long)split * c.rows + orow) * a.heads + oh;
+        if (plot.part >= 0) {
+            const long long at = (long long)(plot.part * plot.rest + plot.cut) * UCOLS + oc;
 #pragma unroll
             for (int i = 0; i < N; i += 4)
                 *reinterpret_cast<f4*>(a.part_o + at * D + channel + i) = f4{f[i], f[i + 1], f[i + 2], f[i + 3]};
@@ -339,6 +407,23 @@ __global__ __launch_bounds__(256, 2) void picked_chunk(CacheAttnArgs a) {
     }
 }
 
+// The parts of the units over joined: a group of D / 8 lanes a column. Grid: UCOLS columns
+// of SLOTS units.
+template <int D>
+__global__ __launch_bounds__(256) void picked_join(CacheAttnArgs a) {
+    constexpr int LANES = D / 8, GROUPS = 256 / LANES;
+    const int col = blockIdx.x * GROUPS % UCOLS + threadIdx.x / LANES, ch = (threadIdx.x % LANES) * 8;
+    const Plot plot(a, blockIdx.x * GROUPS / UCOLS, true);
+    if (plot.b < 0) return;
+    const int at = plot.tile * UCOLS + col, j = at / a.group;
+    const long long row = plot.seq.start + j;
+    if (at >= plot.seq.n * a.group || row < 0 || row >= a.c.rows) return;
+    float f[8];
+    const long long first = (long long)plot.cut * UCOLS + col, step = (long long)plot.rest * UCOLS;
+    const float l = join_parts<D, false>(a, (int)plot.parts, ch, [&](int p) { return first + p * step; }, f);
+    store_row(a, row, plot.kvh * a.group + at - j * a.group, ch, f, l);
+}
+
 constexpr unsigned MOST_LDS = 40u << 10;  // of a unit's lists, beside the kernel's own: two workgroups a CU
 
 }  // namespace
@@ -352,18 +437,27 @@ PickedPlan picked_plan(int head_dim, int batch, int rows, int heads, int kv_head
     p.lds = pick_lds_bytes(cols, top, group, max_new, max_pages);
     const long long units = ((long long)max_new * group + cols - 1) / cols * kv_heads * batch;
     const long long steps = ((long long)pick_entries(cols, top, group, max_new, max_pages) * page_tokens + USTEP - 1) / USTEP;
-    const long long fill = head_dim == 64 && !p.chunks ? 768 : 512;
-    p.splits = (int)std::max(1ll, std::min({fill / std::max(units, 1ll), (steps + 1) / 2, (long long)MAX_SPLITS}));
-    p.part_rows = p.splits > 1 ? (uint64_t)p.splits * rows * heads : 0;
+    if (p.chunks) {
+        // Of the units over whole rounds, at most; a part is two steps or more.
+        p.splits = (int)std::max(1ll, std::min((steps + 1) / 2, (long long)MAX_SPLITS));
+        p.part_rows = (uint64_t)SLOTS * UCOLS;
+    } else {
+        const long long fill = head_dim == 64 ? 768 : 512;
+        p.splits = (int)std::max(1ll, std::min({fill / std::max(units, 1ll), (steps + 1) / 2, (long long)MAX_SPLITS}));
+        p.part_rows = p.splits > 1 ? (uint64_t)p.splits * rows * heads : 0;
+    }
     return p;
 }
 
 hipError_t launch_cache_attend_picked(int head_dim, const CacheAttnArgs& a, const PickedPlan& plan, hipStream_t s) {
     hipError_t e;
     if (plan.chunks) {
-        const unsigned tiles = (unsigned)(((long long)a.max_new * a.group + UCOLS - 1) / UCOLS);
+        // Units at most: those of the longest rows that each sequence may have, of all rows together.
+        const long long each = ((long long)a.max_new * a.group + UCOLS - 1) / UCOLS;
+        const long long all = ((long long)a.c.rows * a.group + UCOLS - 1) / UCOLS + a.c.batch;
+        const unsigned wgs = (unsigned)(std::min(each * a.c.batch, all) * a.c.kv_heads + SLOTS);
         const auto go = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(tiles * a.splits * a.c.kv_heads, 1, a.c.batch), dim3(256), plan.lds, s, a);
+            hipLaunchKernelGGL(kernel, dim3(wgs), dim3(256), plan.lds, s, a);
         };
         if (head_dim == 64 && a.q_f16)
             go(a.out_f16 ? picked_chunk<64, 2, true> : picked_chunk<64, 2, false>);
@@ -374,9 +468,13 @@ hipError_t launch_cache_attend_picked(int head_dim, const CacheAttnArgs& a, cons
         else
             go(a.out_f16 ? picked_chunk<128, 1, true> : picked_chunk<128, 1, false>);
         e = hipGetLastError();
-    } else {
-        e = launch_cache_attend_few_picked(head_dim, a, plan.lds, s);
+        if (e != hipSuccess || a.splits == 1) return e;
+        const int groups = 256 / (head_dim / 8);
+        hipLaunchKernelGGL((head_dim == 64 ? picked_join<64> : picked_join<128>), dim3(SLOTS * UCOLS / groups), dim3(256), 0,
+                           s, a);
+        return hipGetLastError();
     }
+    e = launch_cache_attend_few_picked(head_dim, a, plan.lds, s);
     return e == hipSuccess && a.splits > 1 ? launch_cache_join_splits(head_dim, a, s) : e;
 }
 

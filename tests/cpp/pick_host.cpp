@@ -247,7 +247,8 @@ static void plans() {
                         const sage::PickedPlan p = sage::picked_plan(d, 3, rows, 2 * group, 2, rows, cols, 16, top);
                         CHECK(p.lds <= 64u << 10 && p.lds >= 4u * (2 + 3 * std::min(top, cols)));
                         CHECK(p.splits >= 1 && p.splits <= 256);
-                        CHECK(p.part_rows == (p.splits > 1 ? (uint64_t)p.splits * rows * 2 * group : 0));
+                        CHECK(p.part_rows == (p.chunks ? 512u * 32 : p.splits > 1 ? (uint64_t)p.splits * rows * 2 * group : 0));
+                        CHECK(p.chunks == (rows * group > 16 && p.lds <= 40u << 10) || !p.chunks);
                     }
     for (int cols : {1, 256, 32768})
         for (int kv : {1, 8, 100}) {
