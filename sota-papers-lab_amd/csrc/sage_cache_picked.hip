@@ -88,8 +88,9 @@ struct Plot {
 // logits, its values once the one before has its sums.
 // QP: bf16 parts of a query. OUT16: the output is fp16. For a bf16 one the weights
 // are fp16 while V's scales are within HALF_LEAST .. HALF_MOST, from the wave's first
-// step past them on two bf16 parts.
-template <int D, int QP, bool OUT16>
+// step past them on two bf16 parts. BIG: pages of 64 tokens or more, so that a step is of one
+// page, its place and rows scalar (PICKED_BIG).
+template <int D, int QP, bool OUT16, bool BIG>
 __global__ __launch_bounds__(256, 2) void picked_chunk(CacheAttnArgs a) {
     constexpr int G = D / 32, KS = D / 16, CT = D / 32;  // scale blocks, MFMA steps over the channels, channel tiles
     constexpr int VT = 64 / G, HALF = TOKENS / 2;        // tokens of a V load; of V in LDS at a time
@@ -140,33 +141,44 @@ __global__ __launch_bounds__(256, 2) void picked_chunk(CacheAttnArgs a) {
     const int t_first = s0 * USTEP + wave * TOKENS, end = min(s1 * USTEP, tokens);
 
     // A step's 16-token tiles: code row, slot of the first token, the rows that see it.
+    constexpr int TILES = BIG ? 1 : 4;
     struct Tiles {
-        long long at[4];
-        int slot[4];
-        uint32_t rows[4];
+        long long at[TILES];
+        int slot[TILES];
+        uint32_t rows[TILES];
     };
     Walk walk(entries, c.page_shift, lane, t_first);
     auto look_up = [&](int t, Tiles& x) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < TILES; i++) {
             const int page = walk.of(t + 16 * i, x.slot[i], x.rows[i]);
             if (page < 0) x.rows[i] = 0;
             x.at[i] = cache_row(c, max(page, 0), kvh, (t + 16 * i) & in_page);
         }
     };
+    // The code row of the lane's token k of the step, of its tiles i (and i + 1, for `second`): a scalar and an
+    // offset that never changes, where the step is of one page.
+    auto row_at = [&](const Tiles& x, int i, int second) {
+        if constexpr (BIG)
+            return x.at[0];
+        else
+            return x.at[i] + ((x.at[i + 1 < 4 ? i + 1 : i] - x.at[i]) & -(long long)second);
+    };
     uint32_t kw[2][KS], ks[2];
     auto load_k = [&](const Tiles& x) {
 #pragma unroll
         for (int sub = 0; sub < 2; sub++) {
-            const long long r = x.at[2 * sub] + ((x.at[2 * sub + 1] - x.at[2 * sub]) & -(long long)(col >> 4)) + (col & 15);
-            const uint8_t* p = c.k_codes + r * (D / 2) + half * (D / 4);
+            const long long r = row_at(x, 2 * sub, col >> 4);
+            const uint32_t k = BIG ? 32 * sub + col : col & 15;
+            const uint8_t* p = c.k_codes + r * (D / 2);
 #pragma unroll
             for (int n = 0; n < KS / 4; n++) {
-                const uint4 z = *reinterpret_cast<const uint4*>(p + 16 * n);
+                const uint4 z = *reinterpret_cast<const uint4*>(p + (k * (D / 2) + half * (D / 4) + 16 * n));
                 kw[sub][4 * n] = z.x, kw[sub][4 * n + 1] = z.y, kw[sub][4 * n + 2] = z.z, kw[sub][4 * n + 3] = z.w;
             }
-            const uint8_t* z = c.k_scales + r * G + half * (G / 2);
-            ks[sub] = D == 128 ? *reinterpret_cast<const uint16_t*>(z) : *z;
+            const uint8_t* z = c.k_scales + r * G;
+            const uint32_t at = k * G + half * (G / 2);
+            ks[sub] = D == 128 ? *reinterpret_cast<const uint16_t*>(z + at) : z[at];
         }
     };
     uint4 v[G];
@@ -174,11 +186,10 @@ __global__ __launch_bounds__(256, 2) void picked_chunk(CacheAttnArgs a) {
     auto load_v = [&](const Tiles& x) {
 #pragma unroll
         for (int i = 0; i < G; i++) {
-            long long r = x.at[i * VT / 16];
-            if (VT == 32 && lane >= 32) r = x.at[i * VT / 16 + 1];
-            r += lane / G & 15;
-            v[i] = *reinterpret_cast<const uint4*>(c.v_codes + r * (D / 2) + (lane % G) * 16);
-            vs[i] = c.v_scales[r * G + lane % G];
+            const long long r = row_at(x, i * VT / 16, VT == 32 && lane >= 32);
+            const uint32_t k = BIG ? i * VT + lane / G : lane / G & 15;
+            v[i] = *reinterpret_cast<const uint4*>(c.v_codes + r * (D / 2) + (k * (D / 2) + lane % G * 16));
+            vs[i] = (c.v_scales + r * G)[k * G + lane % G];
         }
     };
 
@@ -221,25 +232,29 @@ __global__ __launch_bounds__(256, 2) void picked_chunk(CacheAttnArgs a) {
                 load_k(next);
             }
             // Register i of sub is token 8 (i / 4) + 4 half + i % 4 of its 32: of 16-token tile 2 sub + i / 8.
+            auto slot_of = [&](int tile) { return BIG ? now.slot[0] + 16 * tile : now.slot[BIG ? 0 : tile]; };
+            auto picked = [&](int tile) { return (now.rows[BIG ? 0 : tile] >> (j - j0) & 1) != 0; };
             auto sees = [&](int sub, int i) {
-                const int tile = 2 * sub + i / 8, k = (8 * (i / 4) + i % 4) & 15;
-                return (now.rows[tile] >> (j - j0) & 1) && now.slot[tile] + k + 4 * half < limit;
+                const int tile = 2 * sub + i / 8;
+                return picked(tile) && slot_of(tile) + ((8 * (i / 4) + i % 4) & 15) + 4 * half < limit;
             };
             float mx = NEG_INF;
+            if (slot_of(0) + 16 > least || slot_of(1) + 16 > least || slot_of(2) + 16 > least || slot_of(3) + 16 > least) {
 #pragma unroll
-            for (int tile = 0; tile < 4; tile++) {
-                if (now.slot[tile] + 16 > least) {
+                for (int sub = 0; sub < 2; sub++)
 #pragma unroll
-                    for (int i = 8 * (tile & 1); i < 8 * (tile & 1) + 8; i++)
-                        if (!sees(tile / 2, i)) x[tile / 2][i] = NEG_INF;
-                } else {
-                    const bool in = now.rows[tile] >> (j - j0) & 1;
+                    for (int i = 0; i < 16; i++)
+                        if (!sees(sub, i)) x[sub][i] = NEG_INF;
+            } else {
 #pragma unroll
-                    for (int i = 8 * (tile & 1); i < 8 * (tile & 1) + 8; i++) x[tile / 2][i] = in ? x[tile / 2][i] : NEG_INF;
-                }
+                for (int sub = 0; sub < 2; sub++)
 #pragma unroll
-                for (int i = 8 * (tile & 1); i < 8 * (tile & 1) + 8; i++) mx = fmaxf(mx, x[tile / 2][i]);
+                    for (int i = 0; i < 16; i++) x[sub][i] = picked(2 * sub + i / 8) ? x[sub][i] : NEG_INF;
             }
+#pragma unroll
+            for (int sub = 0; sub < 2; sub++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) mx = fmaxf(mx, x[sub][i]);
             {
                 auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
                 mx = fmaxf(m, fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
@@ -459,14 +474,21 @@ hipError_t launch_cache_attend_picked(int head_dim, const CacheAttnArgs& a, cons
         const auto go = [&](auto kernel) {
             hipLaunchKernelGGL(kernel, dim3(wgs), dim3(256), plan.lds, s, a);
         };
-        if (head_dim == 64 && a.q_f16)
-            go(a.out_f16 ? picked_chunk<64, 2, true> : picked_chunk<64, 2, false>);
-        else if (head_dim == 64)
-            go(a.out_f16 ? picked_chunk<64, 1, true> : picked_chunk<64, 1, false>);
-        else if (a.q_f16)
-            go(a.out_f16 ? picked_chunk<128, 2, true> : picked_chunk<128, 2, false>);
+        const auto of = [&](auto big) {
+            constexpr bool BIG = decltype(big)::value;
+            if (head_dim == 64 && a.q_f16)
+                go(a.out_f16 ? picked_chunk<64, 2, true, BIG> : picked_chunk<64, 2, false, BIG>);
+            else if (head_dim == 64)
+                go(a.out_f16 ? picked_chunk<64, 1, true, BIG> : picked_chunk<64, 1, false, BIG>);
+            else if (a.q_f16)
+                go(a.out_f16 ? picked_chunk<128, 2, true, BIG> : picked_chunk<128, 2, false, BIG>);
+            else
+                go(a.out_f16 ? picked_chunk<128, 1, true, BIG> : picked_chunk<128, 1, false, BIG>);
+        };
+        if (a.c.page_shift >= 6)
+            of(std::true_type{});
         else
-            go(a.out_f16 ? picked_chunk<128, 1, true> : picked_chunk<128, 1, false>);
+            of(std::false_type{});
         e = hipGetLastError();
         if (e != hipSuccess || a.splits == 1) return e;
         const int groups = 256 / (head_dim / 8);
