@@ -38,6 +38,8 @@ COMMON = [
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
 SCHED = ["-mllvm", "--amdgpu-sched-strategy=iterative-maxocc", "-mllvm", "--misched-postra-direction=bottomup"]
+# Order for parallel instructions first: outputs bit-identical, 2.5% faster for chunks over picked pages.
+ILP = ["-mllvm", "--amdgpu-sched-strategy=max-ilp"]
 # (source, object, extra flags). The attention source is compiled twice: its
 # dense and causal kernels with LLVM's occupancy-keeping iterative pre-RA
 # scheduler and a bottom-up post-RA pass (SCHED: instruction order only,
@@ -53,7 +55,7 @@ UNITS = [
     ("sage_cache.hip", "sage_cache.hip.o", ["-ffp-contract=off"]),
     ("sage_cache_attn.hip", "sage_cache_attn.hip.o", []),
     ("sage_cache_step.hip", "sage_cache_step.hip.o", []),
-    ("sage_cache_picked.hip", "sage_cache_picked.hip.o", []),
+    ("sage_cache_picked.hip", "sage_cache_picked.hip.o", ILP),
     ("sage_cache_pick.hip", "sage_cache_pick.hip.o", ["-fno-honor-nans"]),
     ("sage_api.cpp", "sage_api.cpp.o", []),
     ("sage_cache_api.cpp", "sage_cache_api.cpp.o", []),

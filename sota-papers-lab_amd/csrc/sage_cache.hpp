@@ -138,10 +138,11 @@ struct PickedPlan {
     uint64_t part_rows;
     unsigned lds;
     bool chunks;
+    bool wide;  // units of 16 columns: of eight waves
 };
 PickedPlan picked_plan(int head_dim, int batch, int rows, int heads, int kv_heads, int max_new, int max_pages,
                        int page_tokens, int top);
-hipError_t launch_cache_attend_few_picked(int head_dim, const CacheAttnArgs& a, unsigned lds, hipStream_t s);
+hipError_t launch_cache_attend_few_picked(int head_dim, const CacheAttnArgs& a, const PickedPlan& plan, hipStream_t s);
 hipError_t launch_cache_join_splits(int head_dim, const CacheAttnArgs& a, hipStream_t s);
 hipError_t launch_cache_attend_picked(int head_dim, const CacheAttnArgs& a, const PickedPlan& plan, hipStream_t s);
 

@@ -913,15 +913,23 @@ hipError_t launch_cache_attend(int head_dim, const CacheAttnArgs& a, const Cache
     return head_dim == 64 ? launch<64>(a, plan, s) : launch<128>(a, plan, s);
 }
 
-hipError_t launch_cache_attend_few_picked(int head_dim, const CacheAttnArgs& a, unsigned lds, hipStream_t s) {
+hipError_t launch_cache_attend_few_picked(int head_dim, const CacheAttnArgs& a, const PickedPlan& plan, hipStream_t s) {
     const unsigned tiles = (unsigned)(((long long)a.max_new * a.group + COLS - 1) / COLS);
     const auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(tiles * a.splits * a.c.kv_heads, 1, a.c.batch), dim3(256), lds, s, a);
+        hipLaunchKernelGGL(kernel, dim3(tiles * a.splits * a.c.kv_heads, 1, a.c.batch), dim3(plan.wide ? 512 : 256),
+                           plan.lds, s, a);
     };
-    if (head_dim == 64)
-        go(a.q_f16 ? cache_attn<64, 2, 4, true> : cache_attn<64, 1, 4, true>);
+    const auto of = [&](auto waves) {
+        constexpr int W = decltype(waves)::value;
+        if (head_dim == 64)
+            go(a.q_f16 ? cache_attn<64, 2, W, true> : cache_attn<64, 1, W, true>);
+        else
+            go(a.q_f16 ? cache_attn<128, 2, W, true> : cache_attn<128, 1, W, true>);
+    };
+    if (plan.wide)
+        of(std::integral_constant<int, 8>{});
     else
-        go(a.q_f16 ? cache_attn<128, 2, 4, true> : cache_attn<128, 1, 4, true>);
+        of(std::integral_constant<int, 4>{});
     return hipGetLastError();
 }
 

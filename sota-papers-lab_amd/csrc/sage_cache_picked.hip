@@ -457,8 +457,16 @@ PickedPlan picked_plan(int head_dim, int batch, int rows, int heads, int kv_head
         p.splits = (int)std::max(1ll, std::min((steps + 1) / 2, (long long)MAX_SPLITS));
         p.part_rows = (uint64_t)SLOTS * UCOLS;
     } else {
-        const long long fill = head_dim == 64 ? 768 : 512;
-        p.splits = (int)std::max(1ll, std::min({fill / std::max(units, 1ll), (steps + 1) / 2, (long long)MAX_SPLITS}));
+        // Units that leave CUs free have eight waves and are cut into parts, one a CU, of two
+        // steps at least, but for the shortest, which a second kernel would not shorten. Replayed
+        // from a graph, us, 1, 8, 16 and 32 sequences of a row, 32/8 heads of 128:
+        //                                   1 part                  2                       4
+        //   32 pages of 64, eight waves     16.1 16.7 18.1 22.2     13.8 14.5 17.1 31.5     11.2 12.2 21.6 31.6
+        //   four waves                      21.2 22.0 23.5 25.1     15.7 16.8 18.5 24.6     11.7 12.6 17.4 24.8
+        //   128 pages of 64, eight waves    47.2 50.4 51.3 63.0     29.5 32.6 36.9 69.8     19.3 25.6 43.5 69.4
+        // and of 16 heads of 64, 64 pages of 16, eight waves: 9.5 9.7 10.6 16.5 and 10.0 10.7 17.2 16.5.
+        p.wide = units <= 256 && steps > 1;
+        p.splits = units > 256 || steps <= 4 ? 1 : (int)std::min(256 / std::max(units, 1ll), steps / 2);
         p.part_rows = p.splits > 1 ? (uint64_t)p.splits * rows * heads : 0;
     }
     return p;
@@ -496,7 +504,7 @@ hipError_t launch_cache_attend_picked(int head_dim, const CacheAttnArgs& a, cons
                            s, a);
         return hipGetLastError();
     }
-    e = launch_cache_attend_few_picked(head_dim, a, plan.lds, s);
+    e = launch_cache_attend_few_picked(head_dim, a, plan, s);
     return e == hipSuccess && a.splits > 1 ? launch_cache_join_splits(head_dim, a, s) : e;
 }
 

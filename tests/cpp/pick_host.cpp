@@ -159,7 +159,7 @@ static void picks() {
     const sage_cache_bounds bounds{reinterpret_cast<int8_t*>(mem), u, 5 * 2 * 256, 5 * 2};
     const sage_tensor q{mem, 4 * 512, {0, 512, 128}, SAGE_F16};
     const sage_tensor_mut o{mem, 4 * 512, {0, 512, 128}, SAGE_F16};
-    const Workspace made{H, 128, 2, 0, -2, 4, {1, 0, 0, false}, nullptr};
+    const Workspace made{H, 128, 2, 0, -2, 4, {1, 0, 0, false, false}, nullptr};
     auto update = [&](const sage_cache_shape& h, const sage_cache_bounds& b, const sage_cache_index& i) {
         return sage_cache_bounds_update(&ctx, &h, &cache, &i, &b);
     };

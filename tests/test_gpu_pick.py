@@ -266,7 +266,8 @@ def attend(p, qv, picked, causal, scale, out):
 
 
 class Plan(ctypes.Structure):
-    _fields_ = [("splits", ctypes.c_int), ("part_rows", ctypes.c_uint64), ("lds", ctypes.c_uint), ("chunks", ctypes.c_bool)]
+    _fields_ = [("splits", ctypes.c_int), ("part_rows", ctypes.c_uint64), ("lds", ctypes.c_uint), ("chunks", ctypes.c_bool),
+                ("wide", ctypes.c_bool)]
 
 
 def plan(shape, d, top):
