@@ -130,15 +130,15 @@ struct CachePlan {
 CachePlan cache_plan(int head_dim, int batch, int rows, int heads, int kv_heads, int max_new, int max_tokens);
 hipError_t launch_cache_attend(int head_dim, const CacheAttnArgs& a, const CachePlan& plan, hipStream_t s);
 
-// How a call over picked pages runs: in units of 32 columns (chunks) or of 16,
-// workgroups that a unit's pages are split over, the partial outputs that the workspace
-// holds, and the bytes of LDS of its lists.
+// How a call over picked pages runs: in units of 32 columns (chunks, unless the queries
+// are fp16 of 128 channels), those over whole rounds cut into `parts`, or in units of
+// 16, of eight waves (wide) or four, each cut into `splits`; the bytes of LDS of a unit's
+// lists either way, and the partial outputs that the workspace holds.
 struct PickedPlan {
-    int splits;
+    bool chunks, wide;
+    int splits, parts;
+    unsigned lds, chunk_lds;
     uint64_t part_rows;
-    unsigned lds;
-    bool chunks;
-    bool wide;  // units of 16 columns: of eight waves
 };
 PickedPlan picked_plan(int head_dim, int batch, int rows, int heads, int kv_heads, int max_new, int max_pages,
                        int page_tokens, int top);

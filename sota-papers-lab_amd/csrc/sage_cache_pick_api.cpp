@@ -201,7 +201,6 @@ sage_status sage_cache_attend_picked(const sage_attention* s, const sage_pick_wo
     if (h.rows == 0 || h.batch == 0 || h.max_new == 0) return succeeded();
     a.picked = picked;
     a.top = (int)ws->top;
-    a.splits = ws->plan.splits;
     a.part_o = static_cast<float*>(ws->buf);
     a.part_ml = ws->buf ? a.part_o + ws->plan.part_rows * s->head_dim : nullptr;
     return done(sage::launch_cache_attend_picked((int)s->head_dim, a, ws->plan, s->stream),

@@ -20,7 +20,8 @@ constexpr uint32_t SLOTS = 512;       // workgroups that the chip holds at once
 // The call's units in a line: sequence by sequence its tiles, KV heads fastest. As many
 // rounds of SLOTS as there are whole run a workgroup a unit; the units over, `rest`, are cut
 // into as many parts each as fill one more round, so that the chip does not wait for a
-// few (1563 rows behind 30000 tokens, 1568 units: 239 us with all of them whole, 227 so).
+// few (1563 rows behind 30000 tokens, 32/8 heads of 128, 32 pages of 64 each, 1568 units:
+// 239 us with all of them whole, 227 so).
 struct Plot {
     uint32_t whole, rest, parts;  // units that run whole, units over, parts of each of those
     uint32_t cut;                 // the workgroup's: of which unit over,
@@ -89,7 +90,7 @@ struct Plot {
 // QP: bf16 parts of a query. OUT16: the output is fp16. For a bf16 one the weights
 // are fp16 while V's scales are within HALF_LEAST .. HALF_MOST, from the wave's first
 // step past them on two bf16 parts. BIG: pages of 64 tokens or more, so that a step is of one
-// page, its place and rows scalar (PICKED_BIG).
+// page, its place and rows scalar (chunks of 1563 rows below: 226 us without it, 215 with).
 template <int D, int QP, bool OUT16, bool BIG>
 __global__ __launch_bounds__(256, 2) void picked_chunk(CacheAttnArgs a) {
     constexpr int G = D / 32, KS = D / 16, CT = D / 32;  // scale blocks, MFMA steps over the channels, channel tiles
@@ -443,44 +444,58 @@ constexpr unsigned MOST_LDS = 40u << 10;  // of a unit's lists, beside the kerne
 
 }  // namespace
 
+// Whether a call runs in units of 32 columns: up to 8 heads a KV head (of 16 and more a
+// unit of 16 columns is one row's, and does nothing twice), and from 64 units on. Replayed
+// from a graph, us, units of 16 columns and of 32, 32 pages of 64 of 16384 tokens, the
+// rows' picks half shared, bf16:
+//                       1 x 64 rows   1 x 200     1 x 1000     16 x 32 rows
+//   32/8 heads of 128   28   28       65   49     -            125  79
+//   16/8                22   25       46   37     156  94      88   61
+//   8/8                 19   26       36   31     104  65      60   47
+//   32/8 heads of 64    22   19       51   34     152  97      91   55
+// and under 64 units 20 and 25 (4 x 8 rows of 32/8 heads of 128). fp16 queries of 128
+// channels do not fit the larger unit's registers in two parts (8/8 heads, 1 x 1000: 160 and 182 us).
+static bool wide_units(int head_dim, bool q_f16, const PickedPlan& p) { return p.chunks && !(head_dim == 128 && q_f16); }
+
 PickedPlan picked_plan(int head_dim, int batch, int rows, int heads, int kv_heads, int max_new, int max_pages,
                        int page_tokens, int top) {
     const int group = heads / kv_heads;
     PickedPlan p{};
-    p.chunks = (long long)max_new * group > 16 && pick_lds_bytes(UCOLS, top, group, max_new, max_pages) <= MOST_LDS;
-    const int cols = p.chunks ? UCOLS : 16;
-    p.lds = pick_lds_bytes(cols, top, group, max_new, max_pages);
-    const long long units = ((long long)max_new * group + cols - 1) / cols * kv_heads * batch;
-    const long long steps = ((long long)pick_entries(cols, top, group, max_new, max_pages) * page_tokens + USTEP - 1) / USTEP;
-    if (p.chunks) {
-        // Of the units over whole rounds, at most; a part is two steps or more.
-        p.splits = (int)std::max(1ll, std::min((steps + 1) / 2, (long long)MAX_SPLITS));
-        p.part_rows = (uint64_t)SLOTS * UCOLS;
-    } else {
-        // Units that leave CUs free have eight waves and are cut into parts, one a CU, of two
-        // steps at least, but for the shortest, which a second kernel would not shorten. Replayed
-        // from a graph, us, 1, 8, 16 and 32 sequences of a row, 32/8 heads of 128:
-        //                                   1 part                  2                       4
-        //   32 pages of 64, eight waves     16.1 16.7 18.1 22.2     13.8 14.5 17.1 31.5     11.2 12.2 21.6 31.6
-        //   four waves                      21.2 22.0 23.5 25.1     15.7 16.8 18.5 24.6     11.7 12.6 17.4 24.8
-        //   128 pages of 64, eight waves    47.2 50.4 51.3 63.0     29.5 32.6 36.9 69.8     19.3 25.6 43.5 69.4
-        // and of 16 heads of 64, 64 pages of 16, eight waves: 9.5 9.7 10.6 16.5 and 10.0 10.7 17.2 16.5.
-        p.wide = units <= 256 && steps > 1;
-        p.splits = units > 256 || steps <= 4 ? 1 : (int)std::min(256 / std::max(units, 1ll), steps / 2);
-        p.part_rows = p.splits > 1 ? (uint64_t)p.splits * rows * heads : 0;
-    }
+    const auto units = [&](int cols) { return ((long long)max_new * group + cols - 1) / cols * kv_heads * batch; };
+    const auto steps = [&](int cols) {
+        return ((long long)pick_entries(cols, top, group, max_new, max_pages) * page_tokens + USTEP - 1) / USTEP;
+    };
+    p.lds = pick_lds_bytes(16, top, group, max_new, max_pages);
+    p.chunk_lds = pick_lds_bytes(UCOLS, top, group, max_new, max_pages);
+    p.chunks = group <= 8 && (long long)max_new * group > 16 && units(UCOLS) >= 64 && p.chunk_lds <= MOST_LDS;
+    // Of the units over whole rounds, at most; a part is two steps or more.
+    p.parts = (int)std::max(1ll, std::min((steps(UCOLS) + 1) / 2, (long long)MAX_SPLITS));
+    // Units that leave CUs free have eight waves and are cut into parts, one a CU, of two
+    // steps at least, but for the shortest, which a second kernel would not shorten. Replayed
+    // from a graph, us, 1, 8, 16 and 32 sequences of a row, 32/8 heads of 128:
+    //                                   1 part                  2                       4
+    //   32 pages of 64, eight waves     16.1 16.7 18.1 22.2     13.8 14.5 17.1 31.5     11.2 12.2 21.6 31.6
+    //   four waves                      21.2 22.0 23.5 25.1     15.7 16.8 18.5 24.6     11.7 12.6 17.4 24.8
+    //   128 pages of 64, eight waves    47.2 50.4 51.3 63.0     29.5 32.6 36.9 69.8     19.3 25.6 43.5 69.4
+    // and of 16 heads of 64, 64 pages of 16, eight waves: 9.5 9.7 10.6 16.5 and 10.0 10.7 17.2 16.5.
+    const long long few = units(16);
+    p.wide = few <= 256 && steps(16) > 1;
+    p.splits = few > 256 || steps(16) <= 4 ? 1 : (int)std::min(256 / std::max(few, 1ll), steps(16) / 2);
+    p.part_rows = std::max<uint64_t>(p.splits > 1 ? (uint64_t)p.splits * rows * heads : 0, p.chunks ? SLOTS * UCOLS : 0);
     return p;
 }
 
-hipError_t launch_cache_attend_picked(int head_dim, const CacheAttnArgs& a, const PickedPlan& plan, hipStream_t s) {
+hipError_t launch_cache_attend_picked(int head_dim, const CacheAttnArgs& args, const PickedPlan& plan, hipStream_t s) {
+    CacheAttnArgs a = args;
     hipError_t e;
-    if (plan.chunks) {
+    if (wide_units(head_dim, a.q_f16, plan)) {
+        a.splits = plan.parts;
         // Units at most: those of the longest rows that each sequence may have, of all rows together.
         const long long each = ((long long)a.max_new * a.group + UCOLS - 1) / UCOLS;
         const long long all = ((long long)a.c.rows * a.group + UCOLS - 1) / UCOLS + a.c.batch;
         const unsigned wgs = (unsigned)(std::min(each * a.c.batch, all) * a.c.kv_heads + SLOTS);
         const auto go = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(wgs), dim3(256), plan.lds, s, a);
+            hipLaunchKernelGGL(kernel, dim3(wgs), dim3(256), plan.chunk_lds, s, a);
         };
         const auto of = [&](auto big) {
             constexpr bool BIG = decltype(big)::value;
@@ -504,6 +519,7 @@ hipError_t launch_cache_attend_picked(int head_dim, const CacheAttnArgs& a, cons
                            s, a);
         return hipGetLastError();
     }
+    a.splits = plan.splits;
     e = launch_cache_attend_few_picked(head_dim, a, plan, s);
     return e == hipSuccess && a.splits > 1 ? launch_cache_join_splits(head_dim, a, s) : e;
 }

@@ -159,7 +159,7 @@ static void picks() {
     const sage_cache_bounds bounds{reinterpret_cast<int8_t*>(mem), u, 5 * 2 * 256, 5 * 2};
     const sage_tensor q{mem, 4 * 512, {0, 512, 128}, SAGE_F16};
     const sage_tensor_mut o{mem, 4 * 512, {0, 512, 128}, SAGE_F16};
-    const Workspace made{H, 128, 2, 0, -2, 4, {1, 0, 0, false, false}, nullptr};
+    const Workspace made{H, 128, 2, 0, -2, 4, {}, nullptr};
     auto update = [&](const sage_cache_shape& h, const sage_cache_bounds& b, const sage_cache_index& i) {
         return sage_cache_bounds_update(&ctx, &h, &cache, &i, &b);
     };
@@ -246,9 +246,10 @@ static void plans() {
                     for (int rows : {1, 2, 5, 1000}) {
                         const sage::PickedPlan p = sage::picked_plan(d, 3, rows, 2 * group, 2, rows, cols, 16, top);
                         CHECK(p.lds <= 64u << 10 && p.lds >= 4u * (2 + 3 * std::min(top, cols)));
-                        CHECK(p.splits >= 1 && p.splits <= 256);
-                        CHECK(p.part_rows == (p.chunks ? 512u * 32 : p.splits > 1 ? (uint64_t)p.splits * rows * 2 * group : 0));
-                        CHECK(p.chunks == (rows * group > 16 && p.lds <= 40u << 10) || !p.chunks);
+                        CHECK(p.splits >= 1 && p.splits <= 256 && p.parts >= 1 && p.parts <= 256);
+                        CHECK(!p.chunks || (rows * group > 16 && group <= 8 && p.chunk_lds <= 40u << 10));
+                        CHECK(p.part_rows >= (p.splits > 1 ? (uint64_t)p.splits * rows * 2 * group : 0));
+                        CHECK(p.part_rows >= (p.chunks ? 512u * 32 : 0));
                     }
     for (int cols : {1, 256, 32768})
         for (int kv : {1, 8, 100}) {

@@ -266,8 +266,8 @@ def attend(p, qv, picked, causal, scale, out):
 
 
 class Plan(ctypes.Structure):
-    _fields_ = [("splits", ctypes.c_int), ("part_rows", ctypes.c_uint64), ("lds", ctypes.c_uint), ("chunks", ctypes.c_bool),
-                ("wide", ctypes.c_bool)]
+    _fields_ = [("chunks", ctypes.c_bool), ("wide", ctypes.c_bool), ("splits", ctypes.c_int), ("parts", ctypes.c_int),
+                ("lds", ctypes.c_uint), ("chunk_lds", ctypes.c_uint), ("part_rows", ctypes.c_uint64)]
 
 
 def plan(shape, d, top):
@@ -279,9 +279,17 @@ def plan(shape, d, top):
     return f(d, shape.batch, shape.rows, shape.heads, shape.kv_heads, shape.max_new, shape.max_pages, shape.page_tokens, top)
 
 
-def fp16_weights(p, top, out_type):
+def in_chunks(p, top, q_type):
+    return plan(p.shape, p.d, top).chunks and not (p.d == 128 and q_type == "f16")
+
+
+def fp16_weights(p, top, q_type, out_type):
     """Chunks of rows with a bf16 output round their weights to fp16 (where V's scales allow)."""
-    return out_type == "bf16" and plan(p.shape, p.d, top).chunks
+    return out_type == "bf16" and in_chunks(p, top, q_type)
+
+
+def type_of(torch, x):
+    return "bf16" if x.dtype == torch.bfloat16 else "f16"
 
 
 def run_attend(torch, p, q, picked, out_type, causal=True, scale=None, out=None):
@@ -304,8 +312,12 @@ def check_attend(torch, p, q, qv, picked, out_type, causal=True, scale=None, out
     got = out[0].double().cpu().numpy()
     assert (np.isnan(got) == np.isnan(want)).all(), np.argwhere(np.isnan(got) != np.isnan(want))[:4]
     with np.errstate(invalid="ignore"):
-        tol = tolerance(want, size, reach, count, top, p.d, out_type, fp16_weights(p, picked.shape[2], out_type))
-        bad = ~(np.abs(got - want) <= tol) & ~np.isnan(want)
+        tol = tolerance(want, size, reach, count, top, p.d, out_type, fp16_weights(p, picked.shape[2], type_of(torch, q), out_type))
+        # From 65520 on, half a step past its greatest value, fp16 has infinity.
+        past = (np.abs(want) >= 65520 + tol) & (out_type == "f16")
+        assert (got[past] == np.sign(want[past]) * np.inf).all()
+        near = (np.abs(want) >= 65520 - tol) & (out_type == "f16")  # (either side of it)
+        bad = ~(np.abs(got - want) <= tol) & ~np.isnan(want) & ~near
     assert not bad.any(), (int(bad.sum()), bad.size, np.argwhere(bad)[:4], got[bad][:4], want[bad][:4], tol[bad][:4])
     return out
 
@@ -357,6 +369,55 @@ def test_attention(torch_gpu, d, name, group, q_type, out_type, causal):
     for top in (1, 7, 40):
         q, qv = queries(torch, rng, p, q_type)
         check_attend(torch, p, q, qv, some_columns(rng, p, top, causal), out_type, causal)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("page", [16, 32, 64, 256])
+@pytest.mark.parametrize("group", [1, 3, 8])
+@pytest.mark.parametrize("q_type,out_type,causal", [("bf16", "bf16", True), ("f16", "f16", False), ("f16", "bf16", True), ("bf16", "f16", True)])
+def test_attention_in_chunks(torch_gpu, d, page, group, q_type, out_type, causal):
+    """Units of 32 columns, of which the shape allows enough to choose them: ragged chunks, pages of part of a step and more."""
+    torch = torch_gpu
+    rng = np.random.default_rng(group + d)
+    p = Pool(torch, d, [0, 37, 38, 38, 103], [1300, 3, 100, 330], 2, page, 2 * group, 105, extra_cols=2, seed=group, max_new=1100)
+    spread(p, rng)
+    q, qv = queries(torch, rng, p, q_type)
+    for top in (3, 14):
+        assert plan(p.shape, d, top).chunks
+        check_attend(torch, p, q, qv, some_columns(rng, p, top, causal), out_type, causal)
+
+
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 64)])
+@pytest.mark.parametrize("rows", [258, 270, 512, 523])
+def test_units_past_whole_rounds(torch_gpu, d, page, rows):
+    """Just as many units as fill the chip, a few over, which are cut into parts, and hundreds."""
+    torch = torch_gpu
+    rng = np.random.default_rng(rows)
+    p = Pool(torch, d, [0, rows - 250, rows - 249, rows], [rows + 100, 5, 600], 16, page, 64, rows + 3, seed=rows)
+    spread(p, rng)
+    q, qv = queries(torch, rng, p, "bf16")
+    assert plan(p.shape, d, 8).chunks
+    check_attend(torch, p, q, qv, some_columns(rng, p, 8), "bf16")
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("d", [64, 128])
+def test_values_past_fp16_in_chunks(torch_gpu, d, page):
+    """A block of V past fp16, and one of NaN, behind pages that fp16 holds: the weights go on as bf16 parts."""
+    torch = torch_gpu
+    rng = np.random.default_rng(d + page)
+    p = Pool(torch, d, [0, 60, 100], [2000, 1500], 2, page, 8, extra_cols=0, seed=4, max_new=1100)
+    spread(p, rng)
+    for b, col in ((0, 1500 // page), (1, 700 // page)):
+        p.host["v_scales"][p.table[b, col], :, 3, 1] = 165
+        p.host["v_scales"][p.table[b, col], 1, 5, 0] = 90
+    p.host["v_scales"][p.table[1, 1000 // page], 0, 7, d // 32 - 1] = 255
+    p.upload()
+    q, qv = queries(torch, rng, p, "bf16")
+    picked = some_columns(rng, p, 40 if page == 16 else 14)
+    assert plan(p.shape, d, picked.shape[2]).chunks
+    check_attend(torch, p, q, qv, picked, "bf16")
+    check_attend(torch, p, q, qv, picked, "f16")
 
 
 @pytest.mark.parametrize("d", [64, 128])
@@ -423,7 +484,7 @@ def test_nan_missing_pages_and_shifts(torch_gpu, name, d):
     got = out[0].double().cpu().numpy()
     assert (np.isnan(got) == np.isnan(want)).all() and np.isnan(want).any() and not np.isnan(want).all()
     with np.errstate(invalid="ignore"):
-        tol = tolerance(want, size, reach, count, top, d, "bf16", fp16_weights(p, 12, "bf16"))
+        tol = tolerance(want, size, reach, count, top, d, "bf16", fp16_weights(p, 12, "bf16", "bf16"))
         assert ((np.abs(got - want) <= tol) | np.isnan(want)).all()
     p.host = host
 
