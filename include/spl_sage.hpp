@@ -556,6 +556,51 @@ struct Rotary {
     }
 };
 
+// Several axes: each pair of channels turns by the row's position on its own axis.
+enum class AxisLayout : int32_t {
+    Half = SAGE_ROTARY_AXES_HALF,
+    Pairs = SAGE_ROTARY_AXES_PAIRS,
+    AxisHalf = SAGE_ROTARY_AXES_AXIS_HALF
+};
+
+// The table of Axes: pairs of each axis, dealt in turn or in runs, frequencies of the whole head or of each axis.
+inline Table axes_table(const std::vector<uint64_t>& sections, std::size_t positions, double base = 10000.0,
+                        const Scaling& scaling = {}, bool dealt = false, bool per_axis = false) {
+    std::size_t rot = 0;
+    for (uint64_t n : sections) rot += 2 * n;
+    Table t{rot, positions, std::vector<float>(rot * positions)};
+    const sage_rotary_scaling sc = scaling.raw();
+    check(sage_rotary_axes_table(sections.data(), sections.size(), dealt, per_axis, positions, base, &sc, t.cos_sin.data(),
+                                 t.cos_sin.size()));
+    return t;
+}
+
+// The uploaded table, and the rows' positions on every axis: axis a's at a * positions_stride.
+struct Axes {
+    const float* table = nullptr;
+    std::size_t table_len = 0;
+    std::vector<uint64_t> sections;
+    AxisLayout layout = AxisLayout::Half;
+    bool dealt = false;
+    const int32_t* positions = nullptr;
+    std::size_t positions_len = 0, positions_stride = 0;
+    sage_rotary_axes raw() const {
+        sage_rotary_axes r{table, table_len, {}, sections.size(), static_cast<int32_t>(layout), dealt, positions,
+                           positions_len, positions_stride};
+        for (std::size_t i = 0; i < sections.size() && i < SAGE_ROTARY_AXES; i++) r.sections[i] = sections[i];
+        return r;
+    }
+};
+
+inline void apply(const SageAttention& sa, const Shape& shape, const Axes& r, const Tensor& x, const TensorMut& out,
+                  bool transpose = false) {
+    const sage_shape sh = shape.raw();
+    const sage_rotary_axes ro = r.raw();
+    const sage_tensor tx = x.raw();
+    const sage_tensor_mut to = out.raw();
+    check(sage_rotary_axes_apply(sa.handle(), &sh, &ro, &tx, &to, transpose));
+}
+
 inline void apply(const SageAttention& sa, const Shape& shape, const Rotary& r, const Tensor& x, const TensorMut& out,
                   bool transpose = false) {
     const sage_shape sh = shape.raw();
@@ -592,6 +637,16 @@ inline void append(const SageAttention& sa, const CacheShape& shape, const Pool&
     const sage_rotary r = rotary ? rotary->raw() : sage_rotary{};
     check(sage_cache_append(sa.handle(), &shape, &pool, &index, &tk, &tv, rotary ? &r : nullptr, q ? &tq : nullptr,
                             q_out ? &to : nullptr));
+}
+
+inline void append(const SageAttention& sa, const CacheShape& shape, const Pool& pool, const Index& index,
+                   const Tensor& k, const Tensor& v, const rotary::Axes& rotary, const Tensor* q = nullptr,
+                   const TensorMut* q_out = nullptr) {
+    const sage_tensor tk = k.raw(), tv = v.raw(), tq = q ? q->raw() : sage_tensor{};
+    const sage_tensor_mut to = q_out ? q_out->raw() : sage_tensor_mut{};
+    const sage_rotary_axes r = rotary.raw();
+    check(sage_cache_append_axes(sa.handle(), &shape, &pool, &index, &tk, &tv, &r, q ? &tq : nullptr,
+                                 q_out ? &to : nullptr));
 }
 
 inline void read(const SageAttention& sa, const CacheShape& shape, const Pool& pool, const Index& index,
@@ -631,6 +686,65 @@ inline void attend(const SageAttention& sa, const CacheWorkspace& ws, const Pool
     const sage_tensor_mut to = out.raw();
     const sage_cache_options o{opts.softmax_scale.value_or(0.0f), opts.softmax_scale.has_value(), opts.causal};
     check(sage_cache_attend(sa.handle(), ws.handle(), &pool, &index, &tq, &to, &o));
+}
+
+// A step's index from its requests' lengths.
+using Requests = sage_cache_requests;  // news, past, each with its count
+using FreePages = sage_cache_free;     // the ring of free pages and its state
+using Step = sage_cache_step;          // starts, lengths, page_table, positions, slots, sequences, state, scratch
+inline void tables(const SageAttention& sa, const CacheShape& shape, const Requests& requests, const FreePages& free,
+                   const Step& step) {
+    check(sage_cache_tables(sa.handle(), &shape, &requests, &free, &step));
+}
+inline Index index_of(const Step& s) {
+    return Index{s.starts, s.starts_len, s.lengths, s.lengths_len, s.page_table, s.page_table_len};
+}
+
+// Bounds of the pages' keys, the pick of pages by them, and the attention over those.
+using Bounds = sage_cache_bounds;  // codes, scales, each with its bytes
+inline void update_bounds(const SageAttention& sa, const CacheShape& shape, const Pool& pool, const Index& index,
+                          const Bounds& bounds) {
+    check(sage_cache_bounds_update(sa.handle(), &shape, &pool, &index, &bounds));
+}
+
+// pick's and attend_picked's workspace for one shape and number of pages a row; one call at a time uses it.
+class PickWorkspace {
+public:
+    PickWorkspace(const SageAttention& sa, const CacheShape& shape, std::size_t top) {
+        check(sage_pick_workspace_new(sa.handle(), &shape, top, &h_));
+    }
+    ~PickWorkspace() { sage_pick_workspace_destroy(h_); }
+    PickWorkspace(PickWorkspace&& o) noexcept : h_(std::exchange(o.h_, nullptr)) {}
+    PickWorkspace& operator=(PickWorkspace&& o) noexcept {
+        std::swap(h_, o.h_);
+        return *this;
+    }
+    PickWorkspace(const PickWorkspace&) = delete;
+    PickWorkspace& operator=(const PickWorkspace&) = delete;
+    std::size_t bytes() const { return sage_pick_workspace_bytes(h_); }
+    const sage_pick_workspace* handle() const { return h_; }
+
+private:
+    sage_pick_workspace* h_ = nullptr;
+};
+
+struct PickOptions {
+    std::size_t first = 1, last = 1;
+    bool causal = true;
+};
+inline void pick(const SageAttention& sa, const PickWorkspace& ws, const Bounds& bounds, const Index& index,
+                 const Tensor& q, int32_t* picked, std::size_t picked_len, const PickOptions& opts = {}) {
+    const sage_tensor tq = q.raw();
+    const sage_pick_options o{opts.first, opts.last, opts.causal};
+    check(sage_cache_pick(sa.handle(), ws.handle(), &bounds, &index, &tq, picked, picked_len, &o));
+}
+inline void attend_picked(const SageAttention& sa, const PickWorkspace& ws, const Pool& pool, const Index& index,
+                          const int32_t* picked, std::size_t picked_len, const Tensor& q, const TensorMut& out,
+                          const AttendOptions& opts = {}) {
+    const sage_tensor tq = q.raw();
+    const sage_tensor_mut to = out.raw();
+    const sage_cache_options o{opts.softmax_scale.value_or(0.0f), opts.softmax_scale.has_value(), opts.causal};
+    check(sage_cache_attend_picked(sa.handle(), ws.handle(), &pool, &index, picked, picked_len, &tq, &to, &o));
 }
 
 }  // namespace cache

@@ -112,6 +112,8 @@ struct PickArgs {
 };
 // Rows of a call that the scores are kept for at a time.
 int pick_window(int rows, int kv_heads, int max_pages);
+// Tiles of 16 columns a workgroup, where one launch serves the call, whose keys stay in LDS; else 0.
+int pick_tiles(int batch, int group, int kv_heads, int max_new, int max_pages);
 hipError_t launch_cache_pick(int head_dim, const PickArgs& a, hipStream_t s);
 
 hipError_t launch_rotary(int head_dim, const RotaryArgs& a, hipStream_t s);

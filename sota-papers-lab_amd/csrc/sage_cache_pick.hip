@@ -206,6 +206,12 @@ __global__ __launch_bounds__(256) void bounds_kernel(BoundsArgs a, int heads) {
 // (a maximum does not mind), so that a row's maximum over its heads stays in a lane's
 // four results or between lanes 16 and 32 apart. Groups over 16 take several
 // turns of one row. Pages run along the lanes, 16 a step.
+//
+// A step of a batch reads 2 D + 1 bytes a page once (63 rows over up to 256 pages each, 8 KV
+// heads of 128: 17 MB in 9.2 us), and is bound by a chain: index, page ids, bounds,
+// scores, list. Chunks meet the same pages again and again, in the L2: 20 GFLOP of
+// whole numbers for 1563 rows over up to 954 pages in 50 us; the VALU is 50% busy
+// with keys, codes and lists, the MFMA pipe 9%.
 
 // Eight channels' codes, a byte each: rint(x * up) of x kept within lo .. hi. The sum
 // with 1.5 * 2^23 has units of 1, so its low byte is the nearest whole number, ties to even.
@@ -251,7 +257,9 @@ __device__ __forceinline__ uint32_t key_of(float score) {
 
 constexpr float INF = __builtin_inff();
 
-// What a wave holds of 16 pages: lane (page, quarter of each 64 bytes of its bounds).
+// What a wave holds of 16 pages: lane (page, quarter of its bounds' bytes), so that a lane's loads
+// are of one line (1563 rows of 8 KV heads over up to 954 columns: 50 us; 58 where each
+// load took 64 bytes of every page).
 template <int D>
 struct PageStep {
     i4 w[2 * D / 64];
@@ -561,8 +569,8 @@ __device__ __forceinline__ void wave_sync() {
 
 // A row's list by one wave; key[i]: of column i * 64 + lane. For lists of at most
 // 64, the top-th greatest of the lanes' greatest keys is no more than the list's least, and
-// few keys reach it: the counts go over those, two a lane (954 columns, a list of 32:
-// PICKED_FEW). `few`: LDS of the wave.
+// few keys reach it: the counts go over those, two a lane (1563 rows of 8 KV heads over
+// up to 954 columns, lists of 32: 50 us, 61 with counts over all keys). `few`: LDS of the wave.
 struct Few {
     uint32_t key[128];
     int col[128];
@@ -714,16 +722,16 @@ hipError_t launch_cache_bounds(int head_dim, const BoundsArgs& a, hipStream_t s)
     return hipGetLastError();
 }
 
-int pick_window(int rows, int kv_heads, int max_pages) {
-    const long long most = 1 << 26;  // keys: 256 MB
-    return (int)std::min<long long>(rows, std::max(1ll, most / ((long long)kv_heads * max_pages)));
-}
-
 // Columns of a tile that a row takes, as a power of two.
 static int slots_of(int group) {
     int slots = 0;
     while (slots < 4 && 1 << slots < group) slots++;
     return slots;
+}
+
+int pick_window(int rows, int kv_heads, int max_pages) {
+    const long long most = 1 << 26;  // keys: 256 MB
+    return (int)std::min<long long>(rows, std::max(1ll, most / ((long long)kv_heads * max_pages)));
 }
 
 template <int D>
@@ -737,24 +745,34 @@ static void score(const PickArgs& a, hipStream_t s) {
                        dim3((unsigned)(row_tiles * parts * a.c.kv_heads), 1, a.c.batch), dim3(256), 0, s, a, slots, parts);
 }
 
-// One launch, where the keys of a workgroup's rows fit 64 KB of LDS and there are
-// workgroups enough, or few pages; the tiles of a workgroup, or 0.
-static int tiles_in_one(const PickArgs& a, int keys) {
-    const int slots = slots_of(a.group);
-    if (a.group > 16 || a.c.max_pages > keys * 64) return 0;
+// One launch, where the keys of a workgroup's rows fit 64 KB of LDS: as many tiles a
+// workgroup as leave 256 of them, but for single rows of few sequences over many pages,
+// which the two launches spread over more workgroups. Replayed from a graph, us, one launch
+// and two, 32/8 heads of 128, lists of 32:
+//                     256 columns  512        1024       2048
+//   1 row             6.7  8.1     9.0  8.3   13.7 9.4   23.5 13.0
+//   16 x 1            7.0  9.4     9.5  11.4  16.7 16.0  28.3 27.2
+//   64 x 1            10.7 14.1    17.3 20.6  29.0 32.7  58.4 69.6
+//   64                7.5  24.4    9.7  25.4  14.8 26.0  24.8 33.9
+//   500               14.0 27.4    17.4 32.7  23.1 41.4
+// (64 rows with four tiles a workgroup: 13.1, 16.8, 21.9). The tiles of a workgroup, or 0.
+int pick_tiles(int batch, int group, int kv_heads, int max_new, int max_pages) {
+    const int slots = slots_of(group);
+    if (group > 16 || max_pages > 2048) return 0;
     for (int tiles = 4; tiles; tiles /= 2) {
         const int rows = tiles << (4 - slots);
-        if (tiles > 1 && rows / 2 >= a.max_new) continue;  // half the tiles hold them
-        if (std::min(rows, a.max_new) * a.c.max_pages > 1 << 14) continue;
-        const long long units = ((long long)a.max_new + rows - 1) / rows * a.c.kv_heads * a.c.batch;
-        return units >= 128 || a.c.max_pages <= 512 ? tiles : 0;
+        if (std::min(rows, max_new) * max_pages > 1 << 14) continue;
+        const long long units = ((long long)max_new + rows - 1) / rows * kv_heads * batch;
+        if (tiles > 1 && (rows / 2 >= max_new || units < 256)) continue;  // fewer rows a workgroup
+        return units >= 128 || max_pages <= 512 || rows < max_new ? tiles : 0;
     }
     return 0;
 }
 
 template <int D, int KEYS>
 static bool row_pick(const PickArgs& a, hipStream_t s) {
-    const int tiles = tiles_in_one(a, KEYS), slots = slots_of(a.group), rows = tiles << (4 - slots);
+    const int tiles = pick_tiles(a.c.batch, a.group, a.c.kv_heads, a.max_new, a.c.max_pages);
+    const int slots = slots_of(a.group), rows = tiles << (4 - slots);
     if (!tiles) return false;
     const auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)((a.max_new + rows - 1) / rows * a.c.kv_heads), 1, a.c.batch), dim3(512),

@@ -23,8 +23,8 @@ struct sage_pick_workspace {
 
 namespace {
 
-// What the calls over picks ask of a shape beside shape_checked: columns that fit an
-// entry's bits and the kernels' LDS, and a workgroup a row and KV head in a grid's x.
+// What the calls over picks ask of a shape beside shape_checked: lists that fit the
+// kernels' LDS, and in a grid's x a workgroup a row and KV head, or 16 columns of one.
 sage_status pick_shape_checked(const sage_cache_shape& h, uint64_t top) {
     const sage_status st = shape_checked(h);
     if (st != SAGE_OK) return st;
@@ -33,9 +33,10 @@ sage_status pick_shape_checked(const sage_cache_shape& h, uint64_t top) {
     if (h.max_pages > SAGE_PICK_PAGES)
         return set_error(SAGE_ERR_INVALID, "pick: %llu columns in the page table (at most %d are supported)",
                          (u64)h.max_pages, SAGE_PICK_PAGES);
-    if (std::max(h.rows, h.max_new) * h.kv_heads >= 1ull << 22)
-        return set_error(SAGE_ERR_INVALID, "pick: %llu rows, %llu of a sequence, of %llu KV heads exceed the launch grid",
-                         (u64)h.rows, (u64)h.max_new, (u64)h.kv_heads);
+    if (std::max(h.rows, h.max_new) * h.kv_heads >= 1ull << 22 ||
+        (h.max_new * (h.heads / h.kv_heads) + 15) / 16 * h.kv_heads >= 1ull << 24)
+        return set_error(SAGE_ERR_INVALID, "pick: %llu rows, %llu of a sequence, of %llu and %llu heads exceed the launch grid",
+                         (u64)h.rows, (u64)h.max_new, (u64)h.heads, (u64)h.kv_heads);
     return SAGE_OK;
 }
 
@@ -123,8 +124,11 @@ sage_status sage_pick_workspace_new(const sage_attention* s, const sage_cache_sh
     const sage::PickedPlan plan =
         sage::picked_plan((int)s->head_dim, (int)h.batch, (int)h.rows, (int)h.heads, (int)h.kv_heads, (int)h.max_new,
                           (int)h.max_pages, (int)h.page_tokens, (int)top);
-    // A key is 4 bytes, where not every page is picked anyway; a partial row D floats, a maximum and a sum.
-    const uint64_t keys = h.max_pages > top ? 4ull * window * h.kv_heads * h.max_pages : 0;
+    // A key is 4 bytes, where memory keeps them and not every page is picked anyway; a partial
+    // row D floats, a maximum and a sum.
+    const bool in_memory = h.max_pages > top && !sage::pick_tiles((int)h.batch, (int)(h.heads / h.kv_heads), (int)h.kv_heads,
+                                                                  (int)h.max_new, (int)h.max_pages);
+    const uint64_t keys = in_memory ? 4ull * window * h.kv_heads * h.max_pages : 0;
     uint64_t bytes = 0;
     if (__builtin_mul_overflow(plan.part_rows, (s->head_dim + 2) * 4, &bytes) || bytes > 1ull << 62)
         return set_error(SAGE_ERR_INVALID, "pick workspace needs more than 2^62 bytes");

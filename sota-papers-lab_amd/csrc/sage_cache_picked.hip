@@ -444,6 +444,13 @@ constexpr unsigned MOST_LDS = 40u << 10;  // of a unit's lists, beside the kerne
 
 }  // namespace
 
+// Units at most: those of the longest rows that each sequence may have, of all rows together.
+static long long most_units(int batch, int rows, int group, int kv_heads, int max_new) {
+    const long long each = ((long long)max_new * group + UCOLS - 1) / UCOLS;
+    const long long all = ((long long)rows * group + UCOLS - 1) / UCOLS + batch;
+    return std::min(each * batch, all) * kv_heads;
+}
+
 // Whether a call runs in units of 32 columns: up to 8 heads a KV head (of 16 and more a
 // unit of 16 columns is one row's, and does nothing twice), and from 64 units on. Replayed
 // from a graph, us, units of 16 columns and of 32, 32 pages of 64 of 16384 tokens, the
@@ -467,7 +474,8 @@ PickedPlan picked_plan(int head_dim, int batch, int rows, int heads, int kv_head
     };
     p.lds = pick_lds_bytes(16, top, group, max_new, max_pages);
     p.chunk_lds = pick_lds_bytes(UCOLS, top, group, max_new, max_pages);
-    p.chunks = group <= 8 && (long long)max_new * group > 16 && units(UCOLS) >= 64 && p.chunk_lds <= MOST_LDS;
+    p.chunks = group <= 8 && (long long)max_new * group > 16 && units(UCOLS) >= 64 && p.chunk_lds <= MOST_LDS &&
+               most_units(batch, rows, group, kv_heads, max_new) < 1 << 23;  // (of a launch's 2^32 threads)
     // Of the units over whole rounds, at most; a part is two steps or more.
     p.parts = (int)std::max(1ll, std::min((steps(UCOLS) + 1) / 2, (long long)MAX_SPLITS));
     // Units that leave CUs free have eight waves and are cut into parts, one a CU, of two
@@ -490,10 +498,7 @@ hipError_t launch_cache_attend_picked(int head_dim, const CacheAttnArgs& args, c
     hipError_t e;
     if (wide_units(head_dim, a.q_f16, plan)) {
         a.splits = plan.parts;
-        // Units at most: those of the longest rows that each sequence may have, of all rows together.
-        const long long each = ((long long)a.max_new * a.group + UCOLS - 1) / UCOLS;
-        const long long all = ((long long)a.c.rows * a.group + UCOLS - 1) / UCOLS + a.c.batch;
-        const unsigned wgs = (unsigned)(std::min(each * a.c.batch, all) * a.c.kv_heads + SLOTS);
+        const unsigned wgs = (unsigned)most_units(a.c.batch, a.c.rows, a.group, a.c.kv_heads, a.max_new) + SLOTS;
         const auto go = [&](auto kernel) {
             hipLaunchKernelGGL(kernel, dim3(wgs), dim3(256), plan.chunk_lds, s, a);
         };

@@ -232,7 +232,8 @@ static void picks() {
     shaped(2, [](A h) { h.max_pages = 32769; }, "pick: 32769 columns");
     shaped(2, [](A h) { h.kv_heads = 3; }, "KV heads");
     shaped(2, [](A h) { h.rows = 1 << 21; }, "pick: 2097152 rows");
-    shaped(2, [](A h) { h.max_new = 1 << 21; }, "of a sequence, of 2 KV heads exceed the launch grid");
+    shaped(2, [](A h) { h.max_new = 1 << 21; }, "of a sequence, of 4 and 2 heads exceed the launch grid");
+    shaped(2, [](A h) { h.kv_heads = 1, h.heads = 1024, h.max_new = 1 << 18; }, "exceed the launch grid");
     CHECK(sage_pick_workspace_bytes(nullptr) == 0);
     sage_pick_workspace_destroy(nullptr);
 }
@@ -251,6 +252,19 @@ static void plans() {
                         CHECK(p.part_rows >= (p.splits > 1 ? (uint64_t)p.splits * rows * 2 * group : 0));
                         CHECK(p.part_rows >= (p.chunks ? 512u * 32 : 0));
                     }
+    CHECK(!sage::picked_plan(64, 65535, 100000, 8 * 4000, 4000, 9, 4, 16, 4).chunks);
+    CHECK(sage::picked_plan(64, 100, 100000, 8 * 40, 40, 1000, 4, 16, 4).chunks);
+    // One launch where it fits, and never more keys than LDS has.
+    CHECK(sage::pick_tiles(64, 4, 8, 1, 256) == 1 && sage::pick_tiles(1, 4, 8, 1, 1024) == 0);
+    CHECK(sage::pick_tiles(2, 4, 8, 1000, 954) == 4 && sage::pick_tiles(1, 17, 8, 1000, 954) == 0);
+    for (int group : {1, 2, 5, 16})
+        for (int rows : {1, 3, 40, 2000})
+            for (int cols : {1, 100, 1024, 2048, 2049}) {
+                const int tiles = sage::pick_tiles(9, group, 3, rows, cols);
+                int slots = 1;
+                while (slots < group) slots *= 2;
+                CHECK(tiles * std::min(tiles * 16 / slots, rows) * cols <= tiles << 14 && (tiles == 0 || cols <= 2048));
+            }
     for (int cols : {1, 256, 32768})
         for (int kv : {1, 8, 100}) {
             const int w = sage::pick_window(4000000, kv, cols);

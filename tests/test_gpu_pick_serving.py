@@ -3,6 +3,9 @@ them as one program runs them: requests that come, grow and end, eagerly, captur
 and replayed, on two streams, and graphs that share a workspace."""
 from __future__ import annotations
 
+import subprocess
+from pathlib import Path
+
 import numpy as np
 import pytest
 
@@ -230,3 +233,11 @@ def test_a_void_step_leaves_everything(torch_gpu):
     s.feed(rng, [1, 5, 30, -1])
     s.step()
     assert s.tables.state.tolist()[2:] == [0, 0] and s.tables.lengths.tolist() == [31, 45, 30, 0]
+
+
+def test_cpp_api(torch_gpu):
+    """The same calls through include/spl_sage.hpp (tests/cpp/gpu_pick.cpp)."""
+    exe = Path(__file__).resolve().parent / "cpp" / "bin" / "gpu_pick"
+    assert exe.exists(), f"{exe} is not built; run `python __graft_entry__.py` (build)"
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0 and "0 failure(s)" in r.stdout, r.stdout + r.stderr
