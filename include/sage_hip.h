@@ -620,7 +620,9 @@ sage_status sage_cache_attend(const sage_attention* s, const sage_cache_workspac
 /* ---- A step's index from the requests' lengths ----
  *
  * news [batch]: the rows that each request has in this step, below 0 for a request
- * that has ended; past [batch]: its tokens that are cached already (below 0: 0). */
+ * that has ended; past [batch]: its tokens that are cached already (below 0: 0;
+ * of an ended one those whose pages it still has: 0 once it gave them back, so that a
+ * place in the batch stays ended until a new request takes it). A page is one request's. */
 typedef struct sage_cache_requests {
     const int32_t* news;
     uint64_t news_len;

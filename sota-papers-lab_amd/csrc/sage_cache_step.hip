@@ -148,6 +148,7 @@ __global__ __launch_bounds__(N) void step_kernel(StepArgs a) {
     const int b0 = min(a.batch, (int)threadIdx.x * run), b1 = min(a.batch, b0 + run);
     Sums mine{0, 0, 0, 0};
     for (int b = b0; b < b1; b++) mine += Request(a, a.news[b], a.past[b]).s;
+    mine.back = min(mine.back, 1u << 31);  // past any ring: so that the sum before is too, where the sum with it stops
     Sums at = upto_lane(mine);
     if (lane == 63) waves[wave] = at;
     __syncthreads();  // (the inputs that may be outputs too are read)
