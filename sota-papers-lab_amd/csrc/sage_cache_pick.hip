@@ -37,27 +37,34 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
 //
 // A wave takes a page's KV heads one by one, `heads` of them, each head's bytes on
 // their way while the one before is at work: a lane has 16 channels of every
-// TOK-th token. With the greatest scale byte known, the codes become fp16
-// sixteenths of that scale (exact: 96 at most, what is under 2^-20 of the scale
-// counts as if it were that much), of which two take part in one maximum or
-// minimum. The VALU bounds it, so the lanes' meet by halves: of two registers, each
-// half of the lanes goes on with one.
-// Reads 17/32 of a byte a key's channel and writes two a page's.
-constexpr int BOUNDS_LOADS = 8;  // of a lane at a time: pages of 64 tokens (head dim 64: 128) at once
+// TOK-th token, LOADS of them at a time: the page's, eight at most. With the
+// greatest scale byte known, the codes become fp16 sixteenths of that scale (exact:
+// 96 at most, what is under 2^-20 of the scale counts as if it were that much),
+// of which two channels of two tokens take part in one maximum or minimum. The
+// VALU and the chain index -> page id -> codes bound it, so the lanes' meet by halves: of
+// two registers, each half of the lanes goes on with one.
+// Reads 17/32 of a byte a key's channel and writes two a page's: 44628 tokens of 16
+// heads of 64, pages of 32, 27 MB, in 11.3 us (13.8 with maxima of one token, and
+// eight loads' registers for pages of every size).
 
 constexpr uint32_t H2_INF = 0x7c007c00u, H2_SIGNS = 0x80008000u;
 __device__ __forceinline__ uint32_t pk_max(uint32_t a, uint32_t b) {
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(h2, a), __builtin_bit_cast(h2, b)));
 }
-__device__ __forceinline__ uint32_t pk_min(uint32_t a, uint32_t b) {
-    return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(h2, a), __builtin_bit_cast(h2, b)));
+__device__ __forceinline__ uint32_t pk_max3(uint32_t a, uint32_t b, uint32_t c) {
+    const h2 x = __builtin_elementwise_maximum(__builtin_bit_cast(h2, a), __builtin_bit_cast(h2, b));
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_maximum(x, __builtin_bit_cast(h2, c)));
+}
+__device__ __forceinline__ uint32_t pk_min3(uint32_t a, uint32_t b, uint32_t c) {
+    const h2 x = __builtin_elementwise_minimum(__builtin_bit_cast(h2, a), __builtin_bit_cast(h2, b));
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_minimum(x, __builtin_bit_cast(h2, c)));
 }
 
-template <int D>
+template <int D, int LOADS>
 struct BoundsPart {
     static constexpr int G = D / CACHE_BLOCK, LANES = D / 16, TOK = 64 / LANES;  // lanes a token, tokens a load
-    uint2 w[BOUNDS_LOADS];
-    uint32_t sc[BOUNDS_LOADS];
+    uint2 w[LOADS];
+    uint32_t sc[LOADS];
     // Tokens t0 .. of a page and head of code row `row`, `held` of which hold something;
     // the others count as the last of them.
     __device__ __forceinline__ void load(const CacheDev& c, long long row, int t0, int held) {
@@ -65,7 +72,7 @@ struct BoundsPart {
         const uint8_t* codes = c.k_codes + row * (D / 2);
         const uint8_t* scales = c.k_scales + row * G;
 #pragma unroll
-        for (int i = 0; i < BOUNDS_LOADS; i++) {
+        for (int i = 0; i < LOADS; i++) {
             if (t0 + i * TOK >= held) break;
             const uint32_t t = min(t0 + i * TOK + lane / LANES, held - 1);
             w[i] = *reinterpret_cast<const uint2*>(codes + t * (uint32_t)(D / 2) + part * 8);
@@ -76,7 +83,7 @@ struct BoundsPart {
     __device__ __forceinline__ uint32_t top(int t0, int held, bool& nan) const {
         uint32_t top = 1, most = 0;
 #pragma unroll
-        for (int i = 0; i < BOUNDS_LOADS; i++) {
+        for (int i = 0; i < LOADS; i++) {
             if (t0 + i * TOK >= held) break;
             most = max(most, sc[i]);
             top = max(top, sc[i] == SCALE_NAN ? 0u : sc[i]);
@@ -84,23 +91,30 @@ struct BoundsPart {
         nan = nan || __any(most == SCALE_NAN);
         return top;
     }
+    // Two loads at a time, whose codes take part in one maximum and minimum of three.
     __device__ __forceinline__ void take(int t0, int held, uint32_t top, bool nan, uint32_t (&hi)[8], uint32_t (&lo)[8]) const {
 #pragma unroll
-        for (int i = 0; i < BOUNDS_LOADS; i++) {
+        for (int i = 0; i < LOADS; i += 2) {
             if (t0 + i * TOK >= held) break;
-            const float s = __uint_as_float((uint32_t)(127 + max((int)sc[i] - (int)top + 4, -20)) << 23);
-            const uint2 c = w[i];
-            const h2 x[8] = {
-                __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.x, s, 0), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.x, s, 1),
-                __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.x, s, 2), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.x, s, 3),
-                __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.y, s, 0), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.y, s, 1),
-                __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.y, s, 2), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.y, s, 3)};
+            uint32_t x[2][8];
+            const bool both = LOADS > 1 && t0 + (i + 1) * TOK < held;
+            constexpr int NEXT = LOADS > 1 ? 1 : 0;
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const uint32_t u = __builtin_bit_cast(uint32_t, x[k]);
-                hi[k] = pk_max(hi[k], u), lo[k] = pk_min(lo[k], u);
+            for (int n = 0; n < 2; n++) {
+                const uint32_t scale = n && !both ? sc[i] : sc[i + n * NEXT];
+                const float s = __uint_as_float((uint32_t)(127 + max((int)scale - (int)top + 4, -20)) << 23);
+                const uint2 c = n && !both ? w[i] : w[i + n * NEXT];
+                const h2 y[8] = {
+                    __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.x, s, 0), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.x, s, 1),
+                    __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.x, s, 2), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.x, s, 3),
+                    __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.y, s, 0), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.y, s, 1),
+                    __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.y, s, 2), __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.y, s, 3)};
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[n][k] = __builtin_bit_cast(uint32_t, y[k]);
             }
-            if (nan && sc[i] == SCALE_NAN)
+#pragma unroll
+            for (int k = 0; k < 8; k++) hi[k] = pk_max3(hi[k], x[0][k], x[1][k]), lo[k] = pk_min3(lo[k], x[0][k], x[1][k]);
+            if (nan && (sc[i] == SCALE_NAN || (both && sc[i + NEXT] == SCALE_NAN)))
 #pragma unroll
                 for (int k = 0; k < 8; k++) hi[k] = H2_INF, lo[k] = H2_INF | H2_SIGNS;
         }
@@ -141,18 +155,19 @@ __device__ __forceinline__ void over_tokens(uint32_t (&hi)[8], uint32_t (&lo)[8]
     }
 }
 
-template <int D>
+template <int D, int LOADS>
 __global__ __launch_bounds__(256) void bounds_kernel(BoundsArgs a, int heads) {
-    using Part = BoundsPart<D>;
-    constexpr int SPAN = BOUNDS_LOADS * Part::TOK;
+    using Part = BoundsPart<D, LOADS>;
+    constexpr int SPAN = LOADS * Part::TOK;
     const CacheDev& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int b = blockIdx.y, runs = (c.kv_heads + heads - 1) / heads;
-    const long long unit = (long long)blockIdx.x * 4 + wave;
-    const int h0 = (int)(unit % runs) * heads, h1 = min(h0 + heads, c.kv_heads);
+    const uint32_t runs = (c.kv_heads + heads - 1) / heads;
+    const int b = blockIdx.y;
+    const uint32_t unit = blockIdx.x * 4 + wave, place = unit / runs;  // of the step's pages
+    const int h0 = (int)(unit - place * runs) * heads, h1 = min(h0 + heads, c.kv_heads);
     const SequenceIndex seq = sequence_index(c, b, a.max_new);
     if (seq.n == 0 || seq.diff + seq.n <= 0) return;
-    const long long col = (max(seq.diff, 0ll) >> c.page_shift) + unit / runs;
+    const long long col = (max(seq.diff, 0ll) >> c.page_shift) + place;
     if (col > (seq.diff + seq.n - 1) >> c.page_shift || col >= c.max_pages) return;
     const int page = __builtin_amdgcn_readfirstlane(cache_page(c, b, (int)col << c.page_shift));
     const int held = min(seq.len - ((int)col << c.page_shift), 1 << c.page_shift);
@@ -210,7 +225,7 @@ __global__ __launch_bounds__(256) void bounds_kernel(BoundsArgs a, int heads) {
 // A step of a batch reads 2 D + 1 bytes a page once (63 rows over up to 256 pages each, 8 KV
 // heads of 128: 17 MB in 9.2 us), and is bound by a chain: index, page ids, bounds,
 // scores, list. Chunks meet the same pages again and again, in the L2: 20 GFLOP of
-// whole numbers for 1563 rows over up to 954 pages in 50 us; the VALU is 50% busy
+// whole numbers for 1563 rows over up to 954 pages in 49 us; the VALU is 50% busy
 // with keys, codes and lists, the MFMA pipe 9%.
 
 // Eight channels' codes, a byte each: rint(x * up) of x kept within lo .. hi. The sum
@@ -258,7 +273,7 @@ __device__ __forceinline__ uint32_t key_of(float score) {
 constexpr float INF = __builtin_inff();
 
 // What a wave holds of 16 pages: lane (page, quarter of its bounds' bytes), so that a lane's loads
-// are of one line (1563 rows of 8 KV heads over up to 954 columns: 50 us; 58 where each
+// are of one line (1563 rows of 8 KV heads over up to 954 columns: 49 us; 58 where each
 // load took 64 bytes of every page).
 template <int D>
 struct PageStep {
@@ -352,39 +367,53 @@ struct TileLds {
     }
 };
 
-// By a wave for itself, eight channels a lane, a few columns at a time.
+// A tile's queries, eight channels a lane, a few columns a turn.
+template <int D>
+struct TileQueries {
+    static constexpr int PARTS = D / 8, COLS = 64 / PARTS, TURNS = 16 / COLS;  // columns a turn
+    uint4 raw[TURNS];
+    __device__ __forceinline__ TileQueries(const PickArgs& a, const SequenceIndex& seq, int kvh, int j0, int slots) {
+        const int lane = threadIdx.x & 63, n = lane / PARTS, part = lane % PARTS;
+#pragma unroll
+        for (int i = 0; i < TURNS; i++) {
+            const uint16_t* p = query_of(a, seq, kvh, j0, i * COLS + n, slots, 0);
+            raw[i] = p ? *reinterpret_cast<const uint4*>(p + 8 * part) : make_uint4(0, 0, 0, 0);
+        }
+    }
+    // The codes of turns first, first + step, ... into LDS.
+    __device__ __forceinline__ void encode(const PickArgs& a, int slots, TileLds<D>& lds, int first, int step) const {
+        const int lane = threadIdx.x & 63, n = lane / PARTS, part = lane % PARTS;
+        // Over a column's channels and a row's columns.
+        uint32_t top[TURNS];
+#pragma unroll
+        for (int i = 0; i < TURNS; i++) {
+            top[i] = greatest(raw[i]);
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2)
+                if (d < PARTS << slots) top[i] = max(top[i], (uint32_t)__shfl_xor((int)top[i], d));
+        }
+#pragma unroll
+        for (int d = 1; d < TURNS; d *= 2) {
+            if (1 << slots <= COLS * d) continue;
+            uint32_t other[TURNS];
+#pragma unroll
+            for (int i = 0; i < TURNS; i++) other[i] = top[i ^ d];
+#pragma unroll
+            for (int i = 0; i < TURNS; i++) top[i] = max(top[i], other[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < TURNS; i++)
+            if (i % step == first) lds.put(i * COLS + n, part, raw[i], a.q_f16, power_for(top[i], a.q_f16));
+    }
+};
+
+// By a wave for itself.
 template <int D>
 __device__ __forceinline__ void encode_tile(const PickArgs& a, const SequenceIndex& seq, int kvh, int j0, int slots,
                                             TileLds<D>& lds, i4 (&q)[2 * D / 64]) {
-    constexpr int PARTS = D / 8, COLS = 64 / PARTS, TURNS = 16 / COLS;  // columns at a time
-    const int lane = threadIdx.x & 63, n = lane / PARTS, part = lane % PARTS;
-    uint4 raw[TURNS];
-    uint32_t top[TURNS];
-#pragma unroll
-    for (int i = 0; i < TURNS; i++) {
-        const uint16_t* p = query_of(a, seq, kvh, j0, i * COLS + n, slots, 0);
-        raw[i] = p ? *reinterpret_cast<const uint4*>(p + 8 * part) : make_uint4(0, 0, 0, 0);
-    }
-    // Over a column's channels and a row's columns.
-#pragma unroll
-    for (int i = 0; i < TURNS; i++) {
-        top[i] = greatest(raw[i]);
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2)
-            if (d < PARTS << slots) top[i] = max(top[i], (uint32_t)__shfl_xor((int)top[i], d));
-    }
-#pragma unroll
-    for (int d = 1; d < TURNS; d *= 2) {
-        if (1 << slots <= COLS * d) continue;
-        uint32_t other[TURNS];
-#pragma unroll
-        for (int i = 0; i < TURNS; i++) other[i] = top[i ^ d];
-#pragma unroll
-        for (int i = 0; i < TURNS; i++) top[i] = max(top[i], other[i]);
-    }
+    const TileQueries<D> x(a, seq, kvh, j0, slots);
     __builtin_amdgcn_wave_barrier();  // the tile before is read
-#pragma unroll
-    for (int i = 0; i < TURNS; i++) lds.put(i * COLS + n, part, raw[i], a.q_f16, power_for(top[i], a.q_f16));
+    x.encode(a, slots, lds, 0, 1);
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -570,7 +599,7 @@ __device__ __forceinline__ void wave_sync() {
 // A row's list by one wave; key[i]: of column i * 64 + lane. For lists of at most
 // 64, the top-th greatest of the lanes' greatest keys is no more than the list's least, and
 // few keys reach it: the counts go over those, two a lane (1563 rows of 8 KV heads over
-// up to 954 columns, lists of 32: 50 us, 61 with counts over all keys). `few`: LDS of the wave.
+// up to 954 columns, lists of 32: 49 us, 61 with counts over all keys). `few`: LDS of the wave.
 struct Few {
     uint32_t key[128];
     int col[128];
@@ -669,23 +698,30 @@ __global__ __launch_bounds__(512, TILES == 1 ? 2 : 4) void row_pick_kernel(PickA
     if (count <= 0) return;
     auto pages_of = [&](int j) { return (seq.limit(j0 + j, a.causal) + (1 << c.page_shift) - 1) >> c.page_shift; };
     const int pages = pages_of(count - 1);
-    if (pages > a.top) {
-        uint4 raw;
-        if (TILES == 1) raw = raw_part<D>(a, seq, kvh, j0, slots, 0);
-        PageWalk<D> walk(a, b, kvh, wave * 16, 128, pages);
-        i4 q[TILES][2 * D / 64];
-        if constexpr (TILES == 1) {
-            encode_shared<D>(a, seq, kvh, j0, slots, 0, raw, lds.tile[0], q[0]);
-        } else {
-            if (wave < TILES) encode_tile<D>(a, seq, kvh, j0 + (wave << (4 - slots)), slots, lds.tile[wave], q[0]);
-            __syncthreads();
-#pragma unroll
-            for (int t = 0; t < TILES; t++) lds.tile[t].get(q[t]);
-        }
+    auto score = [&](PageWalk<D>& walk, const i4 (&q)[TILES][2 * D / 64]) {
         walk.template run<TILES>(a, kvh, slots, q, [&](int t, int r, int col, uint32_t key) {
             const int j = (t << (4 - slots)) + ((4 * g + r) >> slots);
             if (j < count) row_keys[j * a.key_cols + col] = key;
         });
+    };
+    if (pages > a.top) {
+        i4 q[TILES][2 * D / 64];
+        // (The queries are asked for in front of the pages, whose loads wait for their ids.)
+        if constexpr (TILES == 1) {
+            const uint4 raw = raw_part<D>(a, seq, kvh, j0, slots, 0);
+            PageWalk<D> walk(a, b, kvh, wave * 16, 128, pages);
+            encode_shared<D>(a, seq, kvh, j0, slots, 0, raw, lds.tile[0], q[0]);
+            score(walk, q);
+        } else {
+            const int t = wave % TILES;
+            const TileQueries<D> x(a, seq, kvh, j0 + (t << (4 - slots)), slots);
+            PageWalk<D> walk(a, b, kvh, wave * 16, 128, pages);
+            x.encode(a, slots, lds.tile[t], wave / TILES, 8 / TILES);
+            __syncthreads();
+#pragma unroll
+            for (int t = 0; t < TILES; t++) lds.tile[t].get(q[t]);
+            score(walk, q);
+        }
     }
     __syncthreads();  // (the tiles are read, too)
     for (int j = wave; j < count; j += 8) {
@@ -711,14 +747,22 @@ __global__ __launch_bounds__(512, TILES == 1 ? 2 : 4) void row_pick_kernel(PickA
 
 hipError_t launch_cache_bounds(int head_dim, const BoundsArgs& a, hipStream_t s) {
     const long long pages = std::min<long long>(((long long)a.max_new + (1 << a.c.page_shift) - 1) >> a.c.page_shift, a.c.max_pages) + 1;
-    // Heads of a page by one wave, where that leaves waves enough to fill the chip.
-    const int heads = (int)std::max(1ll, std::min<long long>({4, a.c.kv_heads, pages * a.c.batch * a.c.kv_heads / 4096}));
+    // Heads of a page by one wave, where that leaves waves enough to fill the chip. Replayed from a
+    // graph, us, 1, 2 and 4 heads, 3 x 15000 tokens:
+    //   16 heads of 64, pages of 16      19.5  15.7  14.0
+    //                   pages of 32      12.7  11.3  11.1 (ragged, 44628 tokens: 11.3 with 2, 11.9 with 4)
+    //   8 heads of 128, pages of 16      12.7  11.4  11.6
+    //                   pages of 64       8.3   8.5   8.3
+    //                   pages of 256      9.7   9.5  10.2
+    const int loads = (head_dim << a.c.page_shift) / 1024;  // of a page of one head, 1024 channels each
+    const int heads = (int)std::max(1ll, std::min<long long>({loads == 1 ? 4 : 2, a.c.kv_heads, pages * a.c.batch * a.c.kv_heads / 4096}));
     const long long units = pages * ((a.c.kv_heads + heads - 1) / heads);
     const dim3 grid((unsigned)((units + 3) / 4), a.c.batch);
+    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, heads); };
     if (head_dim == 64)
-        hipLaunchKernelGGL(bounds_kernel<64>, grid, dim3(256), 0, s, a, heads);
+        go(loads == 1 ? bounds_kernel<64, 1> : loads == 2 ? bounds_kernel<64, 2> : loads == 4 ? bounds_kernel<64, 4> : bounds_kernel<64, 8>);
     else
-        hipLaunchKernelGGL(bounds_kernel<128>, grid, dim3(256), 0, s, a, heads);
+        go(loads == 2 ? bounds_kernel<128, 2> : loads == 4 ? bounds_kernel<128, 4> : bounds_kernel<128, 8>);
     return hipGetLastError();
 }
 
