@@ -203,33 +203,40 @@ __global__ __launch_bounds__(N) void step_kernel(StepArgs a) {
 }
 
 // The request of a row below starts[batch] (another one's number for any other row), by
-// a wave: 64 starts at a time, so two loads in a row up to 4096 requests.
+// a wave: 512 starts at a time, so one round of loads up to 512 requests, two up to 32768.
+constexpr int AT_ONCE = 8;
 __device__ __forceinline__ int request_of_wave(const int* starts, int batch, int row) {
     const int lane = threadIdx.x & 63;
     int lo = 0, n = batch;  // starts[lo] <= row < starts[lo + n]
-    while (n > 1) {
+    while (n > 64 * AT_ONCE) {
         const int run = (n + 63) / 64, at = lo + lane * run;
         const int from = max(__builtin_popcountll(__ballot(at < lo + n && starts[at] <= row)) - 1, 0);
         n = min(run, n - from * run);
         lo += from * run;
     }
-    return lo;
+    int start[AT_ONCE], upto = 0;
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; i++) start[i] = starts[min(lo + i * 64 + lane, batch)];
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; i++) upto += __builtin_popcountll(__ballot(i * 64 + lane < n && start[i] <= row));
+    return lo + max(upto - 1, 0);
 }
 
 // The rows of a large step, four a thread, and behind their workgroups a
-// wave for each request that may have ended. A workgroup whose rows are all one
-// request's looks it up once; others look through the starts in LDS, row by row.
-constexpr int ROWS_WG = 1024, STARTS = 2048;
+// wave for each request that may have ended. A wave whose rows are all one
+// request's looks it up once; others look through the starts of the next 64, row by row.
+constexpr int ROWS_WG = 1024, ROWS_WAVE = ROWS_WG / 4;
 __global__ __launch_bounds__(256) void step_rows_kernel(StepArgs a, int row_wgs) {
     if ((int)blockIdx.x >= row_wgs) {
         const int b = ((int)blockIdx.x - row_wgs) * 4 + (threadIdx.x >> 6);
         if (b < a.batch && a.scratch[a.batch + b]) give_back(a, b, a.scratch[a.batch + b], a.scratch[b]);
         return;
     }
-    const int total = a.starts[a.batch], wg0 = blockIdx.x * ROWS_WG, row0 = wg0 + threadIdx.x * 4;
+    const int total = a.starts[a.batch], row0 = blockIdx.x * ROWS_WG + threadIdx.x * 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wave0 = __builtin_amdgcn_readfirstlane(row0);
     RowPlace p[4];
-    const int one = __builtin_amdgcn_readfirstlane(request_of_wave(a.starts, a.batch, wg0));
-    if (a.batch && wg0 + ROWS_WG <= a.starts[one + 1]) {
+    const int one = __builtin_amdgcn_readfirstlane(request_of_wave(a.starts, a.batch, wave0));
+    if (a.batch && wave0 + ROWS_WAVE <= a.starts[one + 1]) {
         const int start = a.starts[one], past = a.lengths[one] - (a.starts[one + 1] - start);
         const int held = (int)pages_of(past, a.page_shift), first = a.scratch[one];
         // Four tokens are of two pages at most: the first one's and the last one's.
@@ -251,13 +258,14 @@ __global__ __launch_bounds__(256) void step_rows_kernel(StepArgs a, int row_wgs)
             if ((unsigned)page < (unsigned)a.pages) p[i].slot = ((ll)page << a.page_shift) + ((t + i) & in_page);
         }
     } else {
-        __shared__ int lds[STARTS];
-        const int* starts = a.starts;
-        if (a.batch < STARTS) {
-            for (int i = threadIdx.x; i <= a.batch; i += 256) lds[i] = a.starts[i];
-            __syncthreads();
-            starts = lds;
-        }
+        __shared__ int lds[4][65];
+        int* next = lds[wave];
+        const int most = min(64, a.batch - one);  // starts[one] .. starts[one + most]
+        next[lane] = a.starts[min(one + lane, a.batch)];
+        if (lane == 0) next[64] = a.starts[min(one + 64, a.batch)];
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         int b = -1, start = 0, end = 0, past = 0, held = 0, first = 0;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -265,8 +273,8 @@ __global__ __launch_bounds__(256) void step_rows_kernel(StepArgs a, int row_wgs)
             p[i] = RowPlace{0, -1, -1};
             if (row >= total) continue;
             if (row >= end) {
-                b = request_of(starts, a.batch, row);
-                start = starts[b], end = starts[b + 1];
+                b = row < next[most] ? one + request_of(next, most, row) : request_of(a.starts, a.batch, row);
+                start = a.starts[b], end = a.starts[b + 1];
                 past = a.lengths[b] - (end - start), held = (int)pages_of(past, a.page_shift), first = a.scratch[b];
             }
             p[i] = place_row(a, b, past + row - start, held, first);
@@ -297,8 +305,10 @@ __global__ __launch_bounds__(256) void step_rows_kernel(StepArgs a, int row_wgs)
 //   one launch of 1024              3.4   3.7   3.9   4.8   6.7   10.3
 //   two launches                    7.2   5.9   6.0   6.6   6.6   6.7
 // (the eager call pays the host another 2 us for the second). A call that fills the
-// chip, 512 requests of 1380301 rows together: 13.0 us for 23 MB, of which the second
-// launch's chain start -> request -> page -> rows takes most; without the slots' 11 MB 11.1.
+// chip, 512 requests of 1380301 rows together: 12.2 us for 23 MB, of which the second
+// launch's chain start -> request -> page -> rows takes most; without the slots' 11 MB 10.0
+// (13.0 with 64 starts at a time and a look through LDS by every workgroup of two requests; 11.6 with
+// stores past the caches, which leave them to the next call's loads).
 hipError_t launch_cache_step(const StepArgs& a, hipStream_t s) {
     const bool one = a.batch <= THREADS && a.rows <= 4 * THREADS && (ll)a.batch * a.max_pages <= 1 << 18;
     if (one && a.batch <= 256 && a.rows <= 256) {
