@@ -445,6 +445,21 @@ def test_lists_in_any_order(torch_gpu, d, name):
     assert torch.equal(want, run_attend(torch, p, q, odd, "bf16"))
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("max_new,q_type", [(16, "bf16"), (16, "f16"), (2080, "bf16"), (2080, "f16")])
+def test_the_widest_table_and_the_longest_lists(torch_gpu, d, max_new, q_type):
+    """Lists of 256 pages that 16 rows share little of, under 32768 columns: the most that a unit's lists take of LDS, with
+    eight waves and, as the shape allows units enough, with four."""
+    torch = torch_gpu
+    rng = np.random.default_rng(max_new)
+    p = Pool(torch, d, [0, 16], [9000], 2, 16, 2, seed=3, extra_cols=32768 - 563, max_new=max_new)
+    assert p.table.shape[1] == 32768 and not plan(p.shape, d, 256).chunks
+    assert plan(p.shape, d, 256).wide == (max_new == 16)
+    spread(p, rng)
+    q, qv = queries(torch, rng, p, q_type)
+    check_attend(torch, p, q, qv, some_columns(rng, p, 256, shared=0.1), "bf16")
+
+
 @pytest.mark.parametrize("page", [16, 256])
 def test_every_page_is_the_whole_attention(torch_gpu, page):
     """Rows that pick all their pages, up to the most that a pick can hold."""
