@@ -90,7 +90,10 @@ struct Plot {
 // QP: bf16 parts of a query. OUT16: the output is fp16. For a bf16 one the weights
 // are fp16 while V's scales are within HALF_LEAST .. HALF_MOST, from the wave's first
 // step past them on two bf16 parts. BIG: pages of 64 tokens or more, so that a step is of one
-// page, its place and rows scalar (chunks of 1563 rows below: 226 us without it, 215 with).
+// page, its place and rows scalar (the chunks above: 226 us without it, 215 with).
+// They take 211 us now: 52 GFLOP of pairs that were picked, a third of those that the units
+// multiply. A wave's step of 64 tokens is 32 MFMAs and some 350 VALU instructions, of which 128
+// are conversions and 32 exponentials; two waves a SIMD is what the registers leave.
 template <int D, int QP, bool OUT16, bool BIG>
 __global__ __launch_bounds__(256, 2) void picked_chunk(CacheAttnArgs a) {
     constexpr int G = D / 32, KS = D / 16, CT = D / 32;  // scale blocks, MFMA steps over the channels, channel tiles
