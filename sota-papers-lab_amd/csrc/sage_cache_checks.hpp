@@ -20,6 +20,7 @@ constexpr uint64_t I32 = 2147483647ull;
 constexpr uint64_t ROWS = 1ull << 26;
 
 inline sage_status hip_failed(hipError_t e, const char* what) {
+    (void)hipGetLastError();  // reported here, not by the next launch as well
     return set_error(SAGE_ERR_DEVICE, "%s: %s (%s)", what, hipGetErrorName(e), hipGetErrorString(e));
 }
 

@@ -460,6 +460,23 @@ def test_the_widest_table_and_the_longest_lists(torch_gpu, d, max_new, q_type):
     check_attend(torch, p, q, qv, some_columns(rng, p, 256, shared=0.1), "bf16")
 
 
+def test_a_workspace_that_the_card_has_no_room_for(torch_gpu):
+    """8 TB of partial rows: refused, and the next calls do not report it again."""
+    import spl_sage as S
+    from spl_sage import cache as C
+
+    torch = torch_gpu
+    rng = np.random.default_rng(0)
+    sa = S.SageAttention(torch.cuda.current_stream(), 128)
+    large = C.CacheShape(1, 4000000, 1, 64, 1, 4, 256, 4000)
+    with pytest.raises(S.SageError, match="allocate pick workspace"):
+        sa.cache_pick_workspace(large, 256)
+    p = shaped(torch, "steps", 128, 2, 4)
+    spread(p, rng)
+    q, qv = queries(torch, rng, p, "bf16")
+    check_attend(torch, p, q, qv, some_columns(rng, p, 7), "bf16")
+
+
 @pytest.mark.parametrize("page", [16, 256])
 def test_every_page_is_the_whole_attention(torch_gpu, page):
     """Rows that pick all their pages, up to the most that a pick can hold."""
