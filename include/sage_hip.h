@@ -744,7 +744,8 @@ sage_status sage_cache_pick(const sage_attention* s, const sage_pick_workspace* 
                             const sage_pick_options* opts);
 
 /* sage_cache_attend over the slots of each row's picked columns alone, with its
- * masks, numerics and aliasing. picked [rows][kv_heads][top] may be a pick or the
+ * masks, numerics and aliasing; the probabilities are two bf16 parts in chunks of
+ * rows as well. picked [rows][kv_heads][top] may be a pick or the
  * caller's own, in any order; a column given twice counts once, one that the row does
  * not see, or outside the page table, not at all. */
 sage_status sage_cache_attend_picked(const sage_attention* s, const sage_pick_workspace* ws, const sage_cache* cache,

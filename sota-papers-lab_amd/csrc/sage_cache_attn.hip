@@ -454,6 +454,18 @@ __global__ __launch_bounds__(64 * W, D == 64 && W == 4 ? 3 : 2) void cache_attn(
 // Two parts everywhere took the chunks above from 427 us to 565, fp16 from 448
 // to 460 (another box).
 constexpr int CCOLS = 128;
+// V's scale bytes whose values, 0.5 to 6 times the scale, are normal fp16
+// numbers: 2^-13 to 2^13.
+constexpr uint32_t HALF_LEAST = 114, HALF_MOST = 140;
+// Weights of fp16 are 2^LIFT times those of bf16, from 2^-21 on normal numbers and
+// 2^15 at most; the reference that goes with their sums is as much lower.
+constexpr float LIFT = 7.0f;
+// Whether a scale byte is past HALF_LEAST .. HALF_MOST, and whether its block is
+// more than fp16 holds: NaN, or codes (its dwords or'ed) other than zeros.
+__device__ __forceinline__ bool past_half(uint32_t scale) { return scale - HALF_LEAST > HALF_MOST - HALF_LEAST; }
+__device__ __forceinline__ bool past_half(uint32_t scale, uint32_t codes) {
+    return past_half(scale) && (scale >= V_NAN || (codes & 0x77777777u));
+}
 template <int D>
 struct ChunkLds {
     uint8_t v[2][TOKENS * D * 2];

@@ -232,19 +232,6 @@ __device__ __forceinline__ float join_parts(const CacheAttnArgs& a, int parts, i
     return l;
 }
 
-// V's scale bytes whose values, 0.5 to 6 times the scale, are normal fp16
-// numbers: 2^-13 to 2^13.
-constexpr uint32_t HALF_LEAST = 114, HALF_MOST = 140;
-// Weights of fp16 are 2^LIFT times those of bf16, from 2^-21 on normal numbers and
-// 2^15 at most; the reference that goes with their sums is as much lower.
-constexpr float LIFT = 7.0f;
-// Whether a scale byte is past HALF_LEAST .. HALF_MOST, and whether its block is
-// more than fp16 holds: NaN, or codes (its dwords or'ed) other than zeros.
-__device__ __forceinline__ bool past_half(uint32_t scale) { return scale - HALF_LEAST > HALF_MOST - HALF_LEAST; }
-__device__ __forceinline__ bool past_half(uint32_t scale, uint32_t codes) {
-    return past_half(scale) && (scale >= V_NAN || (codes & 0x77777777u));
-}
-
 // ---- Picked pages ----
 //
 // The pages that a unit's rows have picked (sage_cache_attend_picked), one behind

@@ -87,14 +87,14 @@ struct Plot {
 // and are converted there; V's through the wave's own part of LDS, 32 tokens at a time,
 // for the transposing read. A step's keys are asked for once the one before has its
 // logits, its values once the one before has its sums.
-// QP: bf16 parts of a query. OUT16: the output is fp16. For a bf16 one the weights
-// are fp16 while V's scales are within HALF_LEAST .. HALF_MOST, from the wave's first
-// step past them on two bf16 parts. BIG: pages of 64 tokens or more, so that a step is of one
-// page, its place and rows scalar (the chunks above: 226 us without it, 215 with).
-// They take 211 us now: 52 GFLOP of pairs that were picked, a third of those that the units
-// multiply. A wave's step of 64 tokens is 32 MFMAs and some 350 VALU instructions, of which 128
-// are conversions and 32 exponentials; two waves a SIMD is what the registers leave.
-template <int D, int QP, bool OUT16, bool BIG>
+// QP: bf16 parts of a query. BIG: pages of 64 tokens or more, so that a step is of one
+// page, its place and rows scalar (1563 rows behind 30000 tokens: 226 us without it, 215 with, with
+// weights in fewer bits then). The weights are two bf16 parts (2^-16 of each), as in the
+// few-rows kernel, so that a row's output does not depend on how many rows share its
+// call: fp16 ones for bf16 outputs took those chunks 208 us where two parts take 248,
+// but are off by 2^-12 of each, which is more than the output's own rounding where values
+// cancel, and lose weights below 2^-32 of the row's greatest.
+template <int D, int QP, bool BIG>
 __global__ __launch_bounds__(256, 2) void picked_chunk(CacheAttnArgs a) {
     constexpr int G = D / 32, KS = D / 16, CT = D / 32;  // scale blocks, MFMA steps over the channels, channel tiles
     constexpr int VT = 64 / G, HALF = TOKENS / 2;        // tokens of a V load; of V in LDS at a time
@@ -202,171 +202,130 @@ __global__ __launch_bounds__(256, 2) void picked_chunk(CacheAttnArgs a) {
     for (int u = 0; u < CT; u++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[u][i] = 0.0f;
-    float m = NEG_INF, l = 0.0f, lift = OUT16 ? 0.0f : LIFT;
+    float m = NEG_INF, l = 0.0f;
     uint8_t* vl = lds + wave * PART;
     const int vtok = 4 * half + (lane >> 2 & 3), vunit = lane >> 4 & 1;
-    // The wave's steps from t on, with fp16 weights (H16) until a scale of V is past
-    // them; returns where they stopped.
-    auto pass = [&](int t, auto fp16) __attribute__((always_inline)) {
-        constexpr bool H16 = decltype(fp16)::value;
-        Tiles next;
-        if (t < end) {
-            look_up(t, next);
-            load_k(next);
-            load_v(next);
+    Tiles next;
+    if (t_first < end) {
+        look_up(t_first, next);
+        load_k(next);
+        load_v(next);
+    }
+    for (int t = t_first; t < end; t += USTEP) {
+        const Tiles now = next;
+        const bool more = t + USTEP < end;
+        f16v x[2];
+#pragma unroll
+        for (int sub = 0; sub < 2; sub++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[sub][i] = 0.0f;
+            const float sf[2] = {__uint_as_float((ks[sub] & 255) << 23), __uint_as_float((ks[sub] >> 8) << 23)};
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                const bf8 kk = __builtin_bit_cast(bf8, decode8(kw[sub][s], sf[s / 4]));
+#pragma unroll
+                for (int p = 0; p < QP; p++) x[sub] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kk, q[p][s], x[sub], 0, 0, 0);
+            }
         }
-        for (; t < end; t += USTEP) {
-            const Tiles now = next;
-            const bool more = t + USTEP < end;
-            f16v x[2];
-#pragma unroll
-            for (int sub = 0; sub < 2; sub++) {
-#pragma unroll
-                for (int i = 0; i < 16; i++) x[sub][i] = 0.0f;
-                const float sf[2] = {__uint_as_float((ks[sub] & 255) << 23), __uint_as_float((ks[sub] >> 8) << 23)};
-#pragma unroll
-                for (int s = 0; s < KS; s++) {
-                    const bf8 kk = __builtin_bit_cast(bf8, decode8(kw[sub][s], sf[s / 4]));
-#pragma unroll
-                    for (int p = 0; p < QP; p++) x[sub] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kk, q[p][s], x[sub], 0, 0, 0);
-                }
-            }
-            if (more) {
-                look_up(t + USTEP, next);
-                load_k(next);
-            }
-            // Register i of sub is token 8 (i / 4) + 4 half + i % 4 of its 32: of 16-token tile 2 sub + i / 8.
-            auto slot_of = [&](int tile) { return BIG ? now.slot[0] + 16 * tile : now.slot[BIG ? 0 : tile]; };
-            auto picked = [&](int tile) { return (now.rows[BIG ? 0 : tile] >> (j - j0) & 1) != 0; };
-            auto sees = [&](int sub, int i) {
-                const int tile = 2 * sub + i / 8;
-                return picked(tile) && slot_of(tile) + ((8 * (i / 4) + i % 4) & 15) + 4 * half < limit;
-            };
-            float mx = NEG_INF;
-            if (slot_of(0) + 16 > least || slot_of(1) + 16 > least || slot_of(2) + 16 > least || slot_of(3) + 16 > least) {
-#pragma unroll
-                for (int sub = 0; sub < 2; sub++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        if (!sees(sub, i)) x[sub][i] = NEG_INF;
-            } else {
-#pragma unroll
-                for (int sub = 0; sub < 2; sub++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) x[sub][i] = picked(2 * sub + i / 8) ? x[sub][i] : NEG_INF;
-            }
+        if (more) {
+            look_up(t + USTEP, next);
+            load_k(next);
+        }
+        // Register i of sub is token 8 (i / 4) + 4 half + i % 4 of its 32: of 16-token tile 2 sub + i / 8.
+        auto slot_of = [&](int tile) { return BIG ? now.slot[0] + 16 * tile : now.slot[BIG ? 0 : tile]; };
+        auto picked = [&](int tile) { return (now.rows[BIG ? 0 : tile] >> (j - j0) & 1) != 0; };
+        auto sees = [&](int sub, int i) {
+            const int tile = 2 * sub + i / 8;
+            return picked(tile) && slot_of(tile) + ((8 * (i / 4) + i % 4) & 15) + 4 * half < limit;
+        };
+        float mx = NEG_INF;
+        if (slot_of(0) + 16 > least || slot_of(1) + 16 > least || slot_of(2) + 16 > least || slot_of(3) + 16 > least) {
 #pragma unroll
             for (int sub = 0; sub < 2; sub++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) mx = fmaxf(mx, x[sub][i]);
-            {
-                auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-                mx = fmaxf(m, fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+                for (int i = 0; i < 16; i++)
+                    if (!sees(sub, i)) x[sub][i] = NEG_INF;
+        } else {
+#pragma unroll
+            for (int sub = 0; sub < 2; sub++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) x[sub][i] = picked(2 * sub + i / 8) ? x[sub][i] : NEG_INF;
+        }
+#pragma unroll
+        for (int sub = 0; sub < 2; sub++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) mx = fmaxf(mx, x[sub][i]);
+        {
+            auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+            mx = fmaxf(m, fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+        }
+        if (__any((mx - m) * a.qk_mul > SLACK)) {
+            const float scale = __builtin_amdgcn_exp2f((m - (mx == NEG_INF ? 0.0f : mx)) * a.qk_mul);
+            m = mx;
+            l *= scale;
+#pragma unroll
+            for (int u = 0; u < CT; u++) o[u] *= scale;
+        }
+        const float base = m == NEG_INF ? 0.0f : m * a.qk_mul;
+#pragma unroll
+        for (int sub = 0; sub < 2; sub++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                x[sub][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[sub][i], a.qk_mul, -base));
+                l += x[sub][i];
             }
-            if constexpr (H16) {
-                bool past = false;
+        // 32 tokens of V into LDS as bf16, then O^T += V^T P^T.
 #pragma unroll
-                for (int i = 0; i < G; i++) past = past || past_half(vs[i]);
-                if (__any(past)) {
-                    past = false;
+        for (int sub = 0; sub < 2; sub++) {
 #pragma unroll
-                    for (int i = 0; i < G; i++) past = past || past_half(vs[i], v[i].x | v[i].y | v[i].z | v[i].w);
-                    if (__any(past)) return t;
+            for (int n = sub * G / 2; n < (sub + 1) * G / 2; n++) {
+                const float s = __uint_as_float(vs[n] >= V_NAN ? 0 : vs[n] << 23);
+                const uint32_t w[4] = {v[n].x, v[n].y, v[n].z, v[n].w};
+#pragma unroll
+                for (int d = 0; d < 4; d++)
+                    *reinterpret_cast<uint4*>(vl + unit_at<D>((lane / G + n * VT) % HALF, (lane % G) * 2 + d / 2, d & 1)) =
+                        decode8(w[d], s);
+            }
+#pragma unroll
+            for (int st = 0; st < 2; st++) {
+                float e[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) e[i] = x[sub][8 * st + i];
+                bf8 p[2];
+                parts_of<2>(e, p);
+#pragma unroll
+                for (int u = 0; u < CT; u++) {
+                    const uint8_t* at = vl + 16 * st * (D * 2) + unit_at<D>(vtok, 2 * u + vunit, lane >> 1 & 1) + (lane & 1) * 8;
+                    const bf8 vv = read_v(at, 8 * (D * 2));
+#pragma unroll
+                    for (int k = 0; k < 2; k++)
+                        o[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv, p[k], o[u], 0, 0, 0);
                 }
             }
-            if (__any((mx - m) * a.qk_mul > SLACK)) {
-                const float scale = __builtin_amdgcn_exp2f((m - (mx == NEG_INF ? 0.0f : mx)) * a.qk_mul);
-                m = mx;
-                l *= scale;
+        }
+        // Blocks of NaN, bit (token % VT) * G + block of each load.
+        uint64_t bad[G], any_bad = 0;
 #pragma unroll
-                for (int u = 0; u < CT; u++) o[u] *= scale;
-            }
-            const float base = (m == NEG_INF ? 0.0f : m * a.qk_mul) - (H16 ? LIFT : 0.0f);
+        for (int i = 0; i < G; i++) bad[i] = __ballot(vs[i] >= V_NAN), any_bad |= bad[i];
+        if (any_bad) {
+            uint32_t hit = 0;  // blocks of NaN that this lane's tokens bring to its column
 #pragma unroll
             for (int sub = 0; sub < 2; sub++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    x[sub][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[sub][i], a.qk_mul, -base));
-                    l += x[sub][i];
+                    const int tok = 32 * sub + 8 * (i / 4) + 4 * half + i % 4;
+                    const uint32_t blocks = (uint32_t)(bad[(32 * sub + 8 * (i / 4)) / VT] >> (tok % VT * G)) & ((1u << G) - 1);
+                    if (sees(sub, i)) hit |= blocks;
                 }
-            // 32 tokens of V into LDS as 16-bit values, then O^T += V^T P^T.
+            auto r = __builtin_amdgcn_permlane32_swap(hit, hit, false, false);
+            hit = r[0] | r[1];
 #pragma unroll
-            for (int sub = 0; sub < 2; sub++) {
+            for (int u = 0; u < CT; u++)
+                if (hit >> u & 1)
 #pragma unroll
-                for (int n = sub * G / 2; n < (sub + 1) * G / 2; n++) {
-                    const float s = __uint_as_float(!H16 && vs[n] >= V_NAN ? 0 : vs[n] << 23);
-                    const uint32_t w[4] = {v[n].x, v[n].y, v[n].z, v[n].w};
-#pragma unroll
-                    for (int d = 0; d < 4; d++)
-                        *reinterpret_cast<uint4*>(vl + unit_at<D>((lane / G + n * VT) % HALF, (lane % G) * 2 + d / 2, d & 1)) =
-                            decode8<H16>(w[d], s);
-                }
-#pragma unroll
-                for (int st = 0; st < 2; st++) {
-                    float e[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) e[i] = x[sub][8 * st + i];
-                    bf8 p[2];
-                    if constexpr (H16)
-                        p[0] = __builtin_bit_cast(bf8, make_uint4(pack_f16x2(e[0], e[1]), pack_f16x2(e[2], e[3]),
-                                                                  pack_f16x2(e[4], e[5]), pack_f16x2(e[6], e[7])));
-                    else
-                        parts_of<2>(e, p);
-#pragma unroll
-                    for (int u = 0; u < CT; u++) {
-                        const uint8_t* at = vl + 16 * st * (D * 2) + unit_at<D>(vtok, 2 * u + vunit, lane >> 1 & 1) + (lane & 1) * 8;
-                        const bf8 vv = read_v(at, 8 * (D * 2));
-                        if constexpr (H16) {
-                            o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, vv),
-                                                                          __builtin_bit_cast(h8, p[0]), o[u], 0, 0, 0);
-                        } else {
-#pragma unroll
-                            for (int k = 0; k < 2; k++)
-                                o[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv, p[k], o[u], 0, 0, 0);
-                        }
-                    }
-                }
-            }
-            if constexpr (!H16) {
-                // Blocks of NaN, bit (token % VT) * G + block of each load.
-                uint64_t bad[G], any_bad = 0;
-#pragma unroll
-                for (int i = 0; i < G; i++) bad[i] = __ballot(vs[i] >= V_NAN), any_bad |= bad[i];
-                if (any_bad) {
-                    uint32_t hit = 0;  // blocks of NaN that this lane's tokens bring to its column
-#pragma unroll
-                    for (int sub = 0; sub < 2; sub++)
-#pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const int tok = 32 * sub + 8 * (i / 4) + 4 * half + i % 4;
-                            const uint32_t blocks = (uint32_t)(bad[(32 * sub + 8 * (i / 4)) / VT] >> (tok % VT * G)) & ((1u << G) - 1);
-                            if (sees(sub, i)) hit |= blocks;
-                        }
-                    auto r = __builtin_amdgcn_permlane32_swap(hit, hit, false, false);
-                    hit = r[0] | r[1];
-#pragma unroll
-                    for (int u = 0; u < CT; u++)
-                        if (hit >> u & 1)
-#pragma unroll
-                            for (int i = 0; i < 16; i++) o[u][i] = __builtin_nanf("");
-                }
-            }
-            if (more) load_v(next);
+                    for (int i = 0; i < 16; i++) o[u][i] = __builtin_nanf("");
         }
-        return t;
-    };
-    if constexpr (OUT16) {
-        pass(t_first, std::false_type{});
-    } else {
-        const int t = pass(t_first, std::true_type{});
-        if (t < end) {
-            lift = 0.0f;
-            l *= __builtin_amdgcn_exp2f(-LIFT);
-#pragma unroll
-            for (int u = 0; u < CT; u++) o[u] *= __builtin_amdgcn_exp2f(-LIFT);
-            walk.fill(t >> c.page_shift);
-            pass(t, std::false_type{});
-        }
+        if (more) load_v(next);
     }
     {
         auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
@@ -380,7 +339,7 @@ __global__ __launch_bounds__(256, 2) void picked_chunk(CacheAttnArgs a) {
     const int oj = (c0 + oc) / a.group, oh = kvh * a.group + (c0 + oc) - oj * a.group;
     const long long orow = seq.start + oj;
     const bool out = c0 + oc < cols && orow >= 0 && orow < c.rows;
-    if (half == 0) wm[wave][col] = m * a.qk_mul - lift, wl[wave][col] = l;
+    if (half == 0) wm[wave][col] = m * a.qk_mul, wl[wave][col] = l;
 #pragma unroll
     for (int pass = 0; pass < 2; pass++) {
         __syncthreads();
@@ -507,14 +466,10 @@ hipError_t launch_cache_attend_picked(int head_dim, const CacheAttnArgs& args, c
         };
         const auto of = [&](auto big) {
             constexpr bool BIG = decltype(big)::value;
-            if (head_dim == 64 && a.q_f16)
-                go(a.out_f16 ? picked_chunk<64, 2, true, BIG> : picked_chunk<64, 2, false, BIG>);
-            else if (head_dim == 64)
-                go(a.out_f16 ? picked_chunk<64, 1, true, BIG> : picked_chunk<64, 1, false, BIG>);
-            else if (a.q_f16)
-                go(a.out_f16 ? picked_chunk<128, 2, true, BIG> : picked_chunk<128, 2, false, BIG>);
+            if (head_dim == 64)
+                go(a.q_f16 ? picked_chunk<64, 2, BIG> : picked_chunk<64, 1, BIG>);
             else
-                go(a.out_f16 ? picked_chunk<128, 1, true, BIG> : picked_chunk<128, 1, false, BIG>);
+                go(a.q_f16 ? picked_chunk<128, 2, BIG> : picked_chunk<128, 1, BIG>);
         };
         if (a.c.page_shift >= 6)
             of(std::true_type{});
