@@ -160,6 +160,34 @@ def pick(q, hi, lo, scales, starts, lengths, page_table, page_tokens, pages, top
     return out
 
 
+def scores(q, hi, lo, scales, table, pages):
+    """Scores of some rows' queries [rows][heads][dim] for the pages of a sequence's table [columns]: [rows][kv_heads]
+    [columns], -inf where there is no page. All at once, in 32 bits, which hold them exactly."""
+    rows, kv = len(q), hi.shape[1]
+    x = q.reshape(rows, kv, -1, q.shape[2])
+    top = np.abs(x).max((2, 3), keepdims=True)
+    with np.errstate(divide="ignore"):
+        e = np.clip(np.floor(np.log2(127 / top)) + 1, -126, 126)
+    for _ in range(2):
+        e = np.where((top * 2.0 ** e > 127) & (e > -126), e - 1, e)
+    u = np.rint(x * 2.0 ** e).astype(np.float32)
+    there = (table >= 0) & (table < pages)
+    at = np.where(there, table, 0)
+    out = np.empty((rows, kv, len(table)))
+    for g in range(kv):
+        s = np.maximum(u[:, g], 0) @ hi[at, g].T.astype(np.float32) + np.minimum(u[:, g], 0) @ lo[at, g].T.astype(np.float32)
+        out[:, g] = s.max(1).astype(float) * 2.0 ** (np.clip(scales[at, g].astype(int), 1, 228) - 127.0)
+    return np.where(there, out, -np.inf)
+
+
+def greatest(score, top, first, last):
+    """The list of one row and KV head from the scores of the pages that it sees."""
+    col = np.arange(len(score))
+    score = np.where((col < first) | (col >= len(score) - last), np.inf, score)
+    best = np.sort(np.argsort(-score, kind="stable")[:top])
+    return np.concatenate([best, np.full(top - len(best), -1)])
+
+
 def seen_by(picked, limit, page_tokens, slots):
     """Which of `slots` slots a row sees under its picked columns."""
     seen = np.zeros(slots, bool)
