@@ -783,7 +783,7 @@ static void score(const PickArgs& a, hipStream_t s) {
     const int slots = slots_of(a.group);
     const bool chunks = a.group <= 16 && (long long)a.max_new << slots > 16;
     const long long rows = (chunks ? 4 * CHUNK_TILES : 1) << (4 - slots), row_tiles = (a.max_new + rows - 1) / rows;
-    const long long units = row_tiles * a.c.kv_heads * a.c.batch, most = chunks ? 512 : 1024, each = chunks ? 64 : 64;
+    const long long units = row_tiles * a.c.kv_heads * a.c.batch, most = chunks ? 512 : 1024, each = 64;
     const int parts = (int)std::max(1ll, std::min(most / units, (a.c.max_pages + each - 1) / each));
     hipLaunchKernelGGL((chunks ? score_kernel<D, CHUNK_TILES> : score_tile_kernel<D>),
                        dim3((unsigned)(row_tiles * parts * a.c.kv_heads), 1, a.c.batch), dim3(256), 0, s, a, slots, parts);

@@ -96,6 +96,7 @@ struct Plot {
 // cancel, and lose weights below 2^-32 of the row's greatest.
 template <int D, int QP, bool BIG>
 __global__ __launch_bounds__(256, 2) void picked_chunk(CacheAttnArgs a) {
+    static_assert(QP == 1 || D == 64, "two parts of 128 channels do not fit the registers");
     constexpr int G = D / 32, KS = D / 16, CT = D / 32;  // scale blocks, MFMA steps over the channels, channel tiles
     constexpr int VT = 64 / G, HALF = TOKENS / 2;        // tokens of a V load; of V in LDS at a time
     constexpr int PAD = D / 2 + 4;                       // floats of a column where half the outputs meet
@@ -418,12 +419,13 @@ static long long most_units(int batch, int rows, int group, int kv_heads, int ma
 // from a graph, us, units of 16 columns and of 32, 32 pages of 64 of 16384 tokens, the
 // rows' picks half shared, bf16:
 //                       1 x 64 rows   1 x 200     1 x 1000     16 x 32 rows
-//   32/8 heads of 128   28   28       65   49     -            125  79
-//   16/8                22   25       46   37     156  94      88   61
-//   8/8                 19   26       36   31     104  65      60   47
-//   32/8 heads of 64    22   19       51   34     152  97      91   55
-// and under 64 units 20 and 25 (4 x 8 rows of 32/8 heads of 128). fp16 queries of 128
-// channels do not fit the larger unit's registers in two parts (8/8 heads, 1 x 1000: 160 and 182 us).
+//   32/8 heads of 128   28   30       66   57     233  182     124  98
+//   16/8                22   26       46   42     155  115     86   72
+//   8/8                 19   27       36   33     103  78      60   52
+//   32/8 heads of 64    22   20       50   37     150  110     91   61
+// and under 64 units 21 and 26 (4 x 8 rows of 32/8 heads of 128). fp16 queries of 128
+// channels do not fit the larger unit's registers in two parts (in part in memory, 32/8 heads, 1 x 1000
+// rows: 238 and 245 us, 16 x 32: 127 and 149; 8/8 heads: 106 and 111, 62 and 79).
 static bool wide_units(int head_dim, bool q_f16, const PickedPlan& p) { return p.chunks && !(head_dim == 128 && q_f16); }
 
 PickedPlan picked_plan(int head_dim, int batch, int rows, int heads, int kv_heads, int max_new, int max_pages,
@@ -469,7 +471,7 @@ hipError_t launch_cache_attend_picked(int head_dim, const CacheAttnArgs& args, c
             if (head_dim == 64)
                 go(a.q_f16 ? picked_chunk<64, 2, BIG> : picked_chunk<64, 1, BIG>);
             else
-                go(a.q_f16 ? picked_chunk<128, 2, BIG> : picked_chunk<128, 1, BIG>);
+                go(picked_chunk<128, 1, BIG>);  // (wide_units)
         };
         if (a.c.page_shift >= 6)
             of(std::true_type{});
