@@ -415,17 +415,23 @@ static long long most_units(int batch, int rows, int group, int kv_heads, int ma
 }
 
 // Whether a call runs in units of 32 columns: up to 8 heads a KV head (of 16 and more a
-// unit of 16 columns is one row's, and does nothing twice), and from 64 units on. Replayed
-// from a graph, us, units of 16 columns and of 32, 32 pages of 64 of 16384 tokens, the
-// rows' picks half shared, bf16:
-//                       1 x 64 rows   1 x 200     1 x 1000     16 x 32 rows
-//   32/8 heads of 128   28   30       66   57     233  182     124  98
-//   16/8                22   26       46   42     155  115     86   72
-//   8/8                 19   27       36   33     103  78      60   52
-//   32/8 heads of 64    22   20       50   37     150  110     91   61
-// and under 64 units 21 and 26 (4 x 8 rows of 32/8 heads of 128). fp16 queries of 128
-// channels do not fit the larger unit's registers in two parts (in part in memory, 32/8 heads, 1 x 1000
-// rows: 238 and 245 us, 16 x 32: 127 and 149; 8/8 heads: 106 and 111, 62 and 79).
+// unit of 16 columns is one row's, and does nothing twice), and from 64 units on; from 256
+// where a wave's step is of several pages or 8 heads of 128 a KV head make a unit four
+// rows'. Replayed from a graph, us, units of 16 columns and of 32, 32 pages of 64 of 16384
+// tokens, the rows' picks half shared, bf16, rows of one sequence:
+//                          64       96       128      160      256      1000
+//   32/8 heads of 128      27 29    38 34    39 38    63 43    65 57    233 182
+//   16/8 (64 units at 128) 22 26    -        31 32    46 34    47 41    155 115
+//   64/8                   31 36    49 48    51 51    76 73    91 77    311 256
+//   32/8 heads of 64       22 20    30 23    30 26    49 30    51 39    150 110
+//   64/8                   24 23    38 32    39 33    45 47    68 50    -
+//   64 pages of 16:
+//   32/8 heads of 128      21 25    24 29    25 32    40 35    42 43    -
+//   64/8                   19 29    31 34    31 37    50 48    58 51    -
+//   32/8 heads of 64       17 18    20 20    20 22    32 25    33 31    -
+// fp16 queries of 128 channels do not fit the larger unit's registers in two parts (in part in
+// memory, 32/8 heads, 1000 rows: 238 and 245 us, 16 x 32: 127 and 149; 8/8 heads: 106 and 111,
+// 62 and 79).
 static bool wide_units(int head_dim, bool q_f16, const PickedPlan& p) { return p.chunks && !(head_dim == 128 && q_f16); }
 
 PickedPlan picked_plan(int head_dim, int batch, int rows, int heads, int kv_heads, int max_new, int max_pages,
@@ -438,7 +444,8 @@ PickedPlan picked_plan(int head_dim, int batch, int rows, int heads, int kv_head
     };
     p.lds = pick_lds_bytes(16, top, group, max_new, max_pages);
     p.chunk_lds = pick_lds_bytes(UCOLS, top, group, max_new, max_pages);
-    p.chunks = group <= 8 && (long long)max_new * group > 16 && units(UCOLS) >= 64 && p.chunk_lds <= MOST_LDS &&
+    const int least = page_tokens < TOKENS || (head_dim == 128 && group > 4) ? 256 : 64;
+    p.chunks = group <= 8 && (long long)max_new * group > 16 && units(UCOLS) >= least && p.chunk_lds <= MOST_LDS &&
                most_units(batch, rows, group, kv_heads, max_new) < 1 << 23;  // (of a launch's 2^32 threads)
     // Of the units over whole rounds, at most; a part is two steps or more.
     p.parts = (int)std::max(1ll, std::min((steps(UCOLS) + 1) / 2, (long long)MAX_SPLITS));

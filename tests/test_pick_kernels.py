@@ -7,6 +7,7 @@ import re
 import pytest
 
 from test_device_asm import assembly
+from test_gpu_pick import plan
 
 
 def kernels(unit, name):
@@ -46,3 +47,14 @@ def test_picks(name, want):
     assert set(got) == want
     for args, (vgprs, scratch) in got.items():
         assert scratch <= (12 if (name, args) == ("row_pick_kernel", (128, 4, 32)) else 0), (args, vgprs, scratch)
+
+
+@pytest.mark.parametrize("d,group,page,least", [(128, 4, 64, 64), (128, 4, 32, 256), (128, 4, 16, 256), (128, 8, 64, 256),
+                                                (64, 8, 64, 64), (64, 4, 128, 64), (64, 4, 16, 256)])
+def test_units_of_32_columns_where_there_are_many(d, group, page, least):
+    """On both sides of the number of units (rows * group / 32 * KV heads) from which a call runs in them."""
+    from spl_sage import cache as C
+
+    for rows, chunks in ((32 // group * (least // 8), True), (32 // group * (least // 8 - 1), False)):
+        shape = C.CacheShape(1, rows, rows, 8 * group, 8, 1024, page, 256)
+        assert plan(shape, d, 32).chunks == chunks, rows
