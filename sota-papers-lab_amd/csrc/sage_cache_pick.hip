@@ -682,6 +682,9 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void pick_kernel(Pic
 
 // Rows whose keys fit LDS: both in one launch, eight waves over the pages of TILES
 // tiles of rows, then over the rows. Grid: x = KV heads, row tiles; z = sequences.
+// The masks of 16 and 32 keys a lane are more than the scalar registers hold: 18 and some 91 of
+// them wait in lanes of a vector register (pick_kernel<16, 32>: 81), and <128, 4, 32> keeps two vector
+// registers in memory.
 template <int D, int TILES, int KEYS>
 __global__ __launch_bounds__(512, TILES == 1 ? 2 : 4) void row_pick_kernel(PickArgs a, int slots) {
     extern __shared__ uint32_t row_keys[];  // [rows][key_cols]
@@ -778,6 +781,10 @@ int pick_window(int rows, int kv_heads, int max_pages) {
     return (int)std::min<long long>(rows, std::max(1ll, most / ((long long)kv_heads * max_pages)));
 }
 
+// The pages are cut into as many parts as fill 512 workgroups with chunks and 1024 with single
+// tiles. Half of both, these and twice of both, us, 32/8 heads of 128: 1 x 1000 rows over 4096 columns
+// 207, 177, 188, over 8192 1068, 991, 964, 1 x 128 rows over 4096 49, 48, 60; 64/2 heads, 64 rows over
+// 1024 columns 24.5, 24.0, 27.4.
 template <int D>
 static void score(const PickArgs& a, hipStream_t s) {
     const int slots = slots_of(a.group);
@@ -790,16 +797,26 @@ static void score(const PickArgs& a, hipStream_t s) {
 }
 
 // One launch, where the keys of a workgroup's rows fit 64 KB of LDS: as many tiles a
-// workgroup as leave 256 of them, but for single rows of few sequences over many pages,
-// which the two launches spread over more workgroups. Replayed from a graph, us, one launch
-// and two, 32/8 heads of 128, lists of 32:
-//                     256 columns  512        1024       2048
-//   1 row             6.7  8.1     9.0  8.3   13.7 9.4   23.5 13.0
-//   16 x 1            7.0  9.4     9.5  11.4  16.7 16.0  28.3 27.2
-//   64 x 1            10.7 14.1    17.3 20.6  29.0 32.7  58.4 69.6
-//   64                7.5  24.4    9.7  25.4  14.8 26.0  24.8 33.9
-//   500               14.0 27.4    17.4 32.7  23.1 41.4
-// (64 rows with four tiles a workgroup: 13.1, 16.8, 21.9). The tiles of a workgroup, or 0.
+// workgroup as leave 256 of them. But where a sequence's rows are one tile, under 128 workgroups
+// and over 512 columns take two launches, which spread the pages over more workgroups; the
+// rows of several tiles do not, as their scores come from waves of four tiles each
+// (score_kernel). Replayed from a graph, us, one launch and two, lists of 32, pages of 16:
+//                           512 columns  1024       2048
+//   32/8 heads of 128
+//   1 row                   9.0  8.9     13.8 9.3   23.3 13.1
+//   4 rows                  10.3 8.6     14.3 9.4   24.2 13.9
+//   5 rows (two tiles)      9.5  22.2    14.2 22.6  24.0 27.0
+//   16                      9.6  23.3    14.5 24.4  24.3 28.7
+//   64                      9.8  25.6    17.1 26.3  24.8 32.8
+//   128                     10.2 25.8    15.4 28.2  25.5 41.8
+//   16 x 1                  9.5  11.4    16.7 16.0  28.3 27.2
+//   64 x 1                  17.3 20.6    29.0 32.7  58.4 69.6
+//   8/8 heads, 16 rows      12.7 9.2     18.4 9.9   14.5 13.8 (2048: in two launches both)
+//              32 (two)     12.3 22.3    18.4 23.1  28.6 27.5
+//   4/1 heads, 4 rows       8.9  8.3     14.0 9.2   23.3 13.1
+//              5 and 64     9.1  21.7    14.2 22.6  23.5 26.6;  9.3 24.7  14.1 25.3  23.9 31.5
+// and at 256 columns 6.7 and 8.1 for 1 row, 7.5 and 24.4 for 64 (with four tiles a workgroup
+// 13.1). The tiles of a workgroup, or 0.
 int pick_tiles(int batch, int group, int kv_heads, int max_new, int max_pages) {
     const int slots = slots_of(group);
     if (group > 16 || max_pages > 2048) return 0;
@@ -851,6 +868,9 @@ hipError_t launch_cache_pick(int head_dim, const PickArgs& a_, hipStream_t s) {
             const long long wgs = waves == 1 ? (units + 3) / 4 : units;
             hipLaunchKernelGGL(kernel, dim3((unsigned)wgs, 1, a.c.batch), dim3(waves == 1 ? 256 : waves * 64), 0, s, a);
         };
+        // As few waves a row as hold its keys, 16 a lane at most, but for the widest. With the next
+        // kernel one step earlier, us, both launches, 64/2 heads of 128, 1 and 1000 rows: 1024 columns
+        // 11.9 to 15.9 and 140 to 160; 4096 columns 16.7 to 32.8 and 538 to 716.
         if (a.c.max_pages <= 256)
             pick(pick_kernel<1, 4>, 1);
         else if (a.c.max_pages <= 512)
