@@ -15,7 +15,9 @@ GROUPS = [1, 2, 3, 4, 7, 8, 16]
 COLUMNS = [200, 500, 1000, 2000, 2100]
 # New rows of a sequence that the shape allows, columns of the page table, heads of a KV head.
 CASES = ([(1100, c, g) for c in COLUMNS for g in GROUPS] + [(130, c, g) for c in COLUMNS for g in (7, 16)] +
-         [(40, c, g) for c in COLUMNS for g in (1, 2, 4, 8, 16)] + [(12, 1000, 1), (12, 1000, 2)])
+         [(40, c, g) for c in COLUMNS for g in (1, 2, 4, 8, 16)] + [(12, 1000, 1), (12, 1000, 2)] +
+         # (all of the keys that 64 KB, and that a wave's lanes, hold)
+         [(1100, 1024, 4), (1100, 512, 2), (1100, 2048, 3), (1100, 2048, 8), (130, 2048, 16), (40, 1024, 1)])
 
 
 def tiles(batch, group, kv_heads, max_new, max_pages):
