@@ -735,7 +735,8 @@ typedef struct sage_pick_options {
  * them within 127, rounded to whole numbers (all 0 where one is not finite), a
  * page's score is 2^E times the greatest, over the heads, of the sum of u_c hi_c
  * where u_c > 0 and u_c lo_c elsewhere: what the group's greatest logit (of a
- * positive softmax scale) could be there. It is computed in whole numbers, exactly
+ * positive softmax scale) could be there, but for the rounding of u, to nearest: channels far
+ * below the group's greatest keep few bits or none. It is computed in whole numbers, exactly
  * (of E past 228 as of 228). A page that the pool does not have comes behind all
  * others. Rows of no sequence or past max_new keep what they have. q as in
  * sage_cache_attend. */

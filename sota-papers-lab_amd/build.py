@@ -38,7 +38,7 @@ COMMON = [
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
 SCHED = ["-mllvm", "--amdgpu-sched-strategy=iterative-maxocc", "-mllvm", "--misched-postra-direction=bottomup"]
-# Order for parallel instructions first: outputs bit-identical, 2.5% faster for chunks over picked pages.
+# Order for parallel instructions first: outputs bit-identical, 1 to 4% faster for chunks over picked pages.
 ILP = ["-mllvm", "--amdgpu-sched-strategy=max-ilp"]
 # (source, object, extra flags). The attention source is compiled twice: its
 # dense and causal kernels with LLVM's occupancy-keeping iterative pre-RA

@@ -4,8 +4,9 @@
 // so a query's product with any of them is at most unit * sum_c max(q_c lo_c, q_c hi_c):
 // a matrix product of [max(q, 0), min(q, 0)] with [hi, lo]. Both sides are
 // whole numbers of 8 bits, their products and sums exact in 32 on the int8 MFMA and
-// in fp32 (under 2^21), and a unit is a power of two, so the scores have no rounding, and their
-// order does not depend on how they are summed.
+// in fp32 (under 2^21), and a unit is a power of two, so the scores of a row's codes have no rounding, and
+// their order does not depend on how they are summed. The codes do: a query has 8 bits beside the
+// greatest channel of its group.
 #include <algorithm>
 
 #include "sage_cache.hpp"
@@ -41,8 +42,10 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
 // greatest scale byte known, the codes become fp16 sixteenths of that scale (exact:
 // 96 at most, what is under 2^-20 of the scale counts as if it were that much),
 // of which two channels of two tokens take part in one maximum or minimum. The
-// VALU and the chain index -> page id -> codes bound it, so the lanes' meet by halves: of
-// two registers, each half of the lanes goes on with one.
+// chain index -> page id -> codes bounds it, and the work of a (page, head) that does not
+// depend on its tokens (190 VALU instructions at pages of 32 and 64 channels, of which 32 are
+// conversions, maxima and minima of codes; the VALU is 39% busy), so the lanes' meet by
+// halves: of two registers, each half of the lanes goes on with one.
 // Reads 17/32 of a byte a key's channel and writes two a page's: 44628 tokens of 16
 // heads of 64, pages of 32, 27 MB, in 11.3 us (13.8 with maxima of one token, and
 // eight loads' registers for pages of every size).
@@ -225,8 +228,8 @@ __global__ __launch_bounds__(256) void bounds_kernel(BoundsArgs a, int heads) {
 // A step of a batch reads 2 D + 1 bytes a page once (63 rows over up to 256 pages each, 8 KV
 // heads of 128: 17 MB in 9.2 us), and is bound by a chain: index, page ids, bounds,
 // scores, list. Chunks meet the same pages again and again, in the L2: 20 GFLOP of
-// whole numbers for 1563 rows over up to 954 pages in 49 us; the VALU is 50% busy
-// with keys, codes and lists, the MFMA pipe 9%.
+// whole numbers for 1563 rows over up to 954 pages in 49 us; the VALU is 42% busy
+// with keys, codes and lists, the MFMA pipe 7%.
 
 // Eight channels' codes, a byte each: rint(x * up) of x kept within lo .. hi. The sum
 // with 1.5 * 2^23 has units of 1, so its low byte is the nearest whole number, ties to even.

@@ -21,7 +21,7 @@ constexpr uint32_t SLOTS = 512;       // workgroups that the chip holds at once
 // rounds of SLOTS as there are whole run a workgroup a unit; the units over, `rest`, are cut
 // into as many parts each as fill one more round, so that the chip does not wait for a
 // few (1563 rows behind 30000 tokens, 32/8 heads of 128, 32 pages of 64 each, 1568 units:
-// 239 us with all of them whole, 227 so).
+// 267 us with all of them whole, 252 so).
 struct Plot {
     uint32_t whole, rest, parts;  // units that run whole, units over, parts of each of those
     uint32_t cut;                 // the workgroup's: of which unit over,
@@ -88,12 +88,15 @@ struct Plot {
 // for the transposing read. A step's keys are asked for once the one before has its
 // logits, its values once the one before has its sums.
 // QP: bf16 parts of a query. BIG: pages of 64 tokens or more, so that a step is of one
-// page, its place and rows scalar (1563 rows behind 30000 tokens: 226 us without it, 215 with, with
-// weights in fewer bits then). The weights are two bf16 parts (2^-16 of each), as in the
-// few-rows kernel, so that a row's output does not depend on how many rows share its
-// call: fp16 ones for bf16 outputs took those chunks 208 us where two parts take 248,
-// but are off by 2^-12 of each, which is more than the output's own rounding where values
-// cancel, and lose weights below 2^-32 of the row's greatest.
+// page, its place and rows scalar (the chunks above: 264 us without it, 252 with). The
+// weights are two bf16 parts (2^-16 of each), as in the few-rows kernel, so that a row's
+// bits do not depend on how many rows share its call: fp16 ones for bf16 outputs took those
+// chunks 208 us, but are off by up to 2^-11 of each, which is more than the output's own rounding
+// where values cancel, and lose weights below 2^-32 of the row's greatest.
+// They are 52 GFLOP of pairs that were picked, a third of those that the units multiply. A wave's step
+// of 64 tokens is 48 MFMAs and 486 other VALU instructions, of which 128 are conversions, 32
+// exponentials and some 100 the weights' parts; the VALU is 56% busy, the MFMA pipe 38%. Two waves a
+// SIMD is what 256 registers leave, which they need (255, none in memory).
 template <int D, int QP, bool BIG>
 __global__ __launch_bounds__(256, 2) void picked_chunk(CacheAttnArgs a) {
     static_assert(QP == 1 || D == 64, "two parts of 128 channels do not fit the registers");
